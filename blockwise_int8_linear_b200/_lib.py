@@ -30,10 +30,19 @@ EXPORTS = [
     "bi8_peer_allreduce_large_partial_offset", "bi8_peer_allreduce_large_out_offset", "bi8_rope_cache_append",
     "bi8_gemm_dequant_residual", "bi8_quantize_rowwise_pitched", "bi8_quantize_colwise_pitched", "bi8_quantize_dual_pitched",
     "bi8_quantize_rowwise_pre_pitched", "bi8_dequantize_rowwise_pitched", "bi8_column_sum", "bi8_column_sum_workspace_bytes",
-    "bi8_copy_rows",
+    "bi8_copy_rows", "bi8_quantize_int4", "bi8_dequantize_int4", "bi8_matmul_int4", "bi8_rope_cache_append_int4", "bi8_attention_int4",
+    "bi8_attention_int4_workspace_bytes",
 ]
 ADDEND_FULL = 0x100
 PRE_NONE, PRE_RMSNORM, PRE_SILU_MUL = 0, 1, 2
+
+
+
+class Int4Cache(ctypes.Structure):
+    """``bi8_int4_cache``: a key/value cache in 4-bit blocks."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_state", "v_state")]
+                + [(n, ctypes.c_int64) for n in ("k_batch", "k_head", "v_batch", "v_head", "ks_batch", "ks_head", "vs_batch", "vs_head", "max_len")])
+
 
 _lib = None
 _native = None
@@ -104,11 +113,19 @@ def lib() -> ctypes.CDLL:
         L.bi8_gemm_wait_selftest.argtypes = [vp, i64, vp, i64, vp, vp, vp, i64, i32, i64, i64, i64, i32, c.c_uint, i32, vp]
         L.bi8_stream_capture_id.argtypes = [vp, c.POINTER(c.c_ulonglong)]
         L.bi8_mma_peak_probe.argtypes = [i32, c.POINTER(c.c_float), c.POINTER(i32)]
+        L.bi8_quantize_int4.argtypes = [vp, i32, i64, vp, i64, vp, i64, i64, i32, vp]
+        L.bi8_dequantize_int4.argtypes = [vp, i64, vp, i32, vp, i32, i64, i64, i32, vp]
+        L.bi8_matmul_int4.argtypes = [vp, i32, i64, vp, i64, vp, vp, i32, vp, i64, vp, i64, i32, i64, i64, i64, i32, vp]
+        L.bi8_rope_cache_append_int4.argtypes = [vp, i32, vp, i64, vp, i64, vp, c.POINTER(Int4Cache), i64, i64, i64, i64, i64, vp]
+        L.bi8_attention_int4_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
+        L.bi8_attention_int4_workspace_bytes.restype = sz
+        L.bi8_attention_int4.argtypes = [vp, i32, i64, i64, i64, c.POINTER(Int4Cache), vp, i64, vp, i64, c.c_float, vp, i64, i64, i64, i64, i64,
+                                         vp, sz, vp]
         for name in EXPORTS:
             fn = getattr(L, name)
             if name not in ("bi8_last_error_string", "bi8_gemm_workspace_bytes", "bi8_gemm_workspace_used", "bi8_quantize_dual_sum_workspace_bytes", "bi8_gemm_static_scratch_bytes",
                             "bi8_peer_allreduce_buffer_bytes", "bi8_peer_allreduce_large_buffer_bytes", "bi8_column_sum_workspace_bytes",
-                            "bi8_peer_allreduce_large_partial_offset", "bi8_peer_allreduce_large_out_offset"):
+                            "bi8_peer_allreduce_large_partial_offset", "bi8_peer_allreduce_large_out_offset", "bi8_attention_int4_workspace_bytes"):
                 fn.restype = i32
         _lib = L
     return _lib

@@ -12,6 +12,7 @@ from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from . import block_linear_config
+from .int4_functions import dequantize_block_int4, int4_matmul, quantize_block_int4
 from .triton_functions import (
     dequantize_block_rowwise,
     int8_matmul_block64_rowwise_dequantize,
@@ -23,7 +24,7 @@ from .triton_functions import _block, _pre_code, _scale_dtype
 
 __all__ = [
     "replace_linear_with_blockwise_int8", "fast_matmul", "blockwise_int8_linear", "BlockInt8Linear", "BlockLinear",
-    "BlockLinearConfig",
+    "BlockLinearConfig", "BlockInt4Linear", "replace_linear_with_blockwise_int4",
 ]
 
 
@@ -31,12 +32,20 @@ def replace_linear_with_blockwise_int8(model: nn.Module) -> nn.Module:
     """Swap every direct-child ``nn.Linear`` of ``model`` for a ``BlockInt8Linear`` sharing its weight and
     bias storage (``block_linear.py:16-32``).  Not recursive: use ``model.apply(replace_linear_with_blockwise_int8)``
     to patch a whole tree, as with the reference."""
+    return _replace_linears(model, BlockInt8Linear)
+
+
+def replace_linear_with_blockwise_int4(model: nn.Module) -> nn.Module:
+    """The same with ``BlockInt4Linear``, for inference.  Layers that either function has swapped stay what they are."""
+    return _replace_linears(model, BlockInt4Linear)
+
+
+def _replace_linears(model, cls):
     names = [name for name, child in model.named_children() if type(child) is nn.Linear or
-             (isinstance(child, nn.Linear) and not isinstance(child, BlockInt8Linear))]
+             (isinstance(child, nn.Linear) and not isinstance(child, (BlockInt8Linear, BlockInt4Linear)))]
     for name in names:
         old = model._modules[name]
-        new = BlockInt8Linear(old.in_features, old.out_features, old.bias is not None, old.weight.device,
-                              old.weight.dtype, _skip_init=True)
+        new = cls(old.in_features, old.out_features, old.bias is not None, old.weight.device, old.weight.dtype, _skip_init=True)
         new.weight.data = old.weight.data
         if old.bias is not None:
             new.bias.data = old.bias.data
@@ -127,6 +136,34 @@ class blockwise_int8_linear(torch.autograd.Function):
         return grad_X, grad_W, grad_bias
 
 
+def _init_linear(layer, in_features, out_features, bias, device, dtype, skip_init):
+    if not skip_init:
+        nn.Linear.__init__(layer, in_features, out_features, bias, device, dtype)
+        return
+    # the caller rebinds weight/bias storage right away: skip the random init of nn.Linear
+    nn.Module.__init__(layer)
+    layer.in_features, layer.out_features = in_features, out_features
+    kw = {"device": device, "dtype": dtype}
+    layer.weight = nn.Parameter(torch.empty((0,), **kw))
+    if bias:
+        layer.bias = nn.Parameter(torch.empty((0,), **kw))
+    else:
+        layer.register_parameter("bias", None)
+
+
+def _make_room_for_buffers(layer, names, state_dict, prefix):
+    # a checkpoint saved after the first eval forward carries the quantized weight: make room for it
+    for name in names:
+        key = prefix + name
+        if key in state_dict and not hasattr(layer, name):
+            layer.register_buffer(name, torch.empty_like(state_dict[key], device=layer.weight.device))
+    # a checkpoint saved after the floating-point weight was dropped carries an empty `weight` (and the other way
+    # round): take the shape the checkpoint has
+    key = prefix + "weight"
+    if key in state_dict and state_dict[key].shape != layer.weight.shape:
+        layer.weight.data = torch.empty_like(state_dict[key], device=layer.weight.device, dtype=layer.weight.dtype)
+
+
 class BlockInt8Linear(nn.Linear):
     """Drop-in ``nn.Linear`` (``block_linear.py:114-152``).
 
@@ -136,18 +173,7 @@ class BlockInt8Linear(nn.Linear):
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None,
                  _skip_init: bool = False):
-        if _skip_init:
-            # the caller rebinds weight/bias storage right away: skip the random init of nn.Linear
-            nn.Module.__init__(self)
-            self.in_features, self.out_features = in_features, out_features
-            kw = {"device": device, "dtype": dtype}
-            self.weight = nn.Parameter(torch.empty((0,), **kw))
-            if bias:
-                self.bias = nn.Parameter(torch.empty((0,), **kw))
-            else:
-                self.register_parameter("bias", None)
-        else:
-            super().__init__(in_features, out_features, bias, device, dtype)
+        _init_linear(self, in_features, out_features, bias, device, dtype, _skip_init)
 
     def prepare_for_eval(self, drop_weight: bool = None):
         """Quantizes the weight into the buffers ``W_int8`` / ``state_W`` (``block_linear.py:125-128``).  With
@@ -208,20 +234,65 @@ class BlockInt8Linear(nn.Linear):
         return blockwise_int8_linear.apply(x, weight, self.bias)
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
-        # a checkpoint saved after the first eval forward carries W_int8/state_W: make room for them
-        for name in ("W_int8", "state_W"):
-            key = prefix + name
-            if key in state_dict and not hasattr(self, name):
-                self.register_buffer(name, torch.empty_like(state_dict[key], device=self.weight.device))
-        # a checkpoint saved after the floating-point weight was dropped carries an empty `weight` (and the other way
-        # round): take the shape the checkpoint has
-        key = prefix + "weight"
-        if key in state_dict and state_dict[key].shape != self.weight.shape:
-            self.weight.data = torch.empty_like(state_dict[key], device=self.weight.device, dtype=self.weight.dtype)
+        _make_room_for_buffers(self, ("W_int8", "state_W"), state_dict, prefix)
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
 
 BlockLinear = BlockInt8Linear
+
+
+class BlockInt4Linear(nn.Linear):
+    """``nn.Linear`` for inference with its weight in 4-bit blocks (no counterpart in the reference): half the bytes of
+    ``BlockInt8Linear``'s, which is what a decode step of a few rows is bound by.  Activations are not quantized.
+
+    The weight is quantized on the first forward in eval mode (buffers ``W_int4`` uint8 ``[out, ceil(in/2)]`` and ``state_W4``
+    ``[out, ceil(in/block)]``, part of ``state_dict()``); a float32 weight is rounded to ``INPUT_OUTPUT_TORCH_TYPE`` first (to bfloat16
+    where that is float32 too), and activations have the type of the scales.  Training mode refuses to run."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None,
+                 _skip_init: bool = False):
+        _init_linear(self, in_features, out_features, bias, device, dtype, _skip_init)
+
+    def prepare_for_eval(self, drop_weight: bool = None):
+        """Quantizes the weight into the buffers; ``drop_weight`` (default: ``block_linear_config.DROP_WEIGHT_IN_EVAL``) releases the
+        floating-point weight as ``BlockInt8Linear.prepare_for_eval`` does."""
+        if self.weight.numel() == 0:
+            if not hasattr(self, "W_int4"):
+                raise RuntimeError("BlockInt4Linear has neither a floating-point weight nor 4-bit buffers")
+            return
+        weight = self.weight.detach()
+        if weight.dtype == torch.float32:
+            io = block_linear_config.INPUT_OUTPUT_TORCH_TYPE
+            weight = weight.to(torch.bfloat16 if io == torch.float32 else io)
+        W_int4, state_W4 = quantize_block_int4(weight)
+        self.register_buffer("W_int4", W_int4)
+        self.register_buffer("state_W4", state_W4)
+        if drop_weight is None:
+            drop_weight = getattr(block_linear_config, "DROP_WEIGHT_IN_EVAL", False)
+        if drop_weight:
+            self.weight.data = torch.empty(0, device=self.weight.device, dtype=self.weight.dtype)
+
+    def dequantized_weight(self):
+        """What the 4-bit weight stands for, in ``INPUT_OUTPUT_TORCH_TYPE``."""
+        if not hasattr(self, "W_int4"):
+            self.prepare_for_eval()
+        return dequantize_block_int4(self.W_int4, self.state_W4, features=self.in_features)
+
+    def infer(self, x, residual=None):
+        """``x @ W^T (+ bias) (+ residual)``; ``residual`` has the output's shape and type."""
+        if self._buffers.get("W_int4") is None:
+            self.prepare_for_eval()
+        bias = self.bias
+        return int4_matmul(x, self._buffers["W_int4"], self._buffers["state_W4"], None if bias is None else bias.detach(), residual=residual)
+
+    def forward(self, x):
+        if self.training:
+            raise RuntimeError("BlockInt4Linear is for inference: call eval() first")
+        return self.infer(x)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        _make_room_for_buffers(self, ("W_int4", "state_W4"), state_dict, prefix)
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
 
 class BlockLinearConfig:

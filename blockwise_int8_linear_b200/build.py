@@ -21,7 +21,8 @@ OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libbi8.so")
 NATIVE = os.path.join(HERE, "_native.so")
 NATIVE_SOURCE = "torch_ops.cpp"
-SOURCES = ["api.cu", "quantize.cu", "quantize_tile.cu", "gemm_generic.cu", "gemm_tc.cu", "gemm_tc_skinny.cu", "gemm_smallm.cu", "no_alloc.cu", "peer_reduce.cu", "peer_reduce_large.cu", "quantize_pre.cu", "column_sum.cu", "rope_cache.cu", "copy_rows.cu"]
+SOURCES = ["api.cu", "quantize.cu", "quantize_tile.cu", "gemm_generic.cu", "gemm_tc.cu", "gemm_tc_skinny.cu", "gemm_smallm.cu", "no_alloc.cu", "peer_reduce.cu", "peer_reduce_large.cu", "quantize_pre.cu", "column_sum.cu", "rope_cache.cu", "copy_rows.cu",
+           "int4_quantize.cu", "int4_matmul.cu", "int4_cache.cu", "int4_attention.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -99,7 +100,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
             print(log)
         return obj
 
-    with ThreadPoolExecutor(max_workers=6) as ex:
+    with ThreadPoolExecutor(max_workers=8) as ex:
         objs = list(ex.map(compile_one, [NATIVE_SOURCE] + sources()))
     _run([nvcc, "-shared", "-o", LIB, *objs[1:], "-cudart", "static"], "link failed")
     _link_native(objs[0])

@@ -574,6 +574,118 @@ int bi8_rope_cache_append(const void* qkv, int dtype, const float* cis, const lo
     return launch_rope_cache_append(qkv, dtype, cis, pos, q_out, kcache, vcache, B, H, D, max_len, static_cast<cudaStream_t>(stream));
 }
 
+// ---- weights and key/value caches in 4-bit blocks ---------------------------------------------------------------------------
+namespace {
+
+int check_int4(const char* what, int dtype, int64_t rows, int64_t K, int block) {
+    if (dtype != BI8_BF16 && dtype != BI8_F16) return fail(BI8_ERR_DTYPE, "%s: bf16 or fp16 values and scales (got code %d)", what, dtype);
+    if (block != 32 && block != 64 && block != 128) return fail(BI8_ERR_BLOCK, "%s: block size %d, expected 32, 64 or 128", what, block);
+    if (rows < 0 || K < 0) return fail(BI8_ERR_SHAPE, "%s: negative dimension (%lld x %lld)", what, (long long)rows, (long long)K);
+    return BI8_OK;
+}
+
+// The shape of a step with a 4-bit cache, and the cache's own layout.
+int check_int4_cache(const char* what, int dtype, const bi8_int4_cache* c, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D) {
+    if (dtype != BI8_BF16 && dtype != BI8_F16) return fail(BI8_ERR_DTYPE, "%s: bf16 or fp16 activations (got code %d)", what, dtype);
+    if (!c) return fail(BI8_ERR_NULL, "%s: null cache", what);
+    if (B < 0 || T < 0 || Hq < 0 || Hkv < 0 || c->max_len < 0 || B > 0x7fffffff || T > 0x7fffffff || Hq > 0xffff || Hkv > 0xffff ||
+        c->max_len > 0x7fff0000)
+        return fail(BI8_ERR_SHAPE, "%s: bad shape B %lld T %lld Hq %lld Hkv %lld max_len %lld", what, (long long)B, (long long)T, (long long)Hq,
+                    (long long)Hkv, (long long)c->max_len);
+    if (D != 64 && D != 128 && D != 256) return fail(BI8_ERR_SHAPE, "%s: head size %lld, expected 64, 128 or 256", what, (long long)D);
+    if (Hkv == 0 ? Hq != 0 : Hq % Hkv != 0)
+        return fail(BI8_ERR_SHAPE, "%s: %lld query heads do not divide over %lld cache heads", what, (long long)Hq, (long long)Hkv);
+    if (B == 0 || T == 0 || Hq == 0) return BI8_OK;
+    if (Hq / Hkv * T > 0x7fffffff) return fail(BI8_ERR_LIMIT, "%s: too many queries per cache head", what);
+    if (c->max_len > 0 && (!c->k || !c->v || !c->k_state || !c->v_state)) return fail(BI8_ERR_NULL, "%s: null cache tensor", what);
+    const int64_t n = D / 64;
+    if (!aligned(c->k, 8) || !aligned(c->v, 8) || c->k_batch % 8 || c->k_head % 8 || c->v_batch % 8 || c->v_head % 8)
+        return fail(BI8_ERR_ALIGN, "%s: codes of the cache not on 8-byte boundaries", what);
+    if (!aligned(c->k_state, 2 * n) || !aligned(c->v_state, 2 * n) || c->ks_batch % n || c->ks_head % n || c->vs_batch % n || c->vs_head % n)
+        return fail(BI8_ERR_ALIGN, "%s: scales of the cache not on boundaries of a row's scales", what);
+    return BI8_OK;
+}
+
+}  // namespace
+
+int bi8_quantize_int4(const void* x, int dtype, int64_t ldx, uint8_t* q, int64_t ldq, void* s, int64_t M, int64_t K, int block, void* stream) {
+    DeviceOfCall call;
+    if (int rc = check_int4("quantize_int4", dtype, M, K, block)) return rc;
+    if (M == 0 || K == 0) return BI8_OK;
+    if (!x || !q || !s) return fail(BI8_ERR_NULL, "quantize_int4: null pointer");
+    if (M > 1 && (ldx < K || ldq < (K + 1) / 2)) return fail(BI8_ERR_SHAPE, "quantize_int4: row pitch smaller than a row");
+    if (!aligned(x, 2) || !aligned(s, 2)) return fail(BI8_ERR_ALIGN, "quantize_int4: pointer not element aligned");
+    return launch_quantize_int4(x, dtype, ldx, q, ldq, s, M, K, block, static_cast<cudaStream_t>(stream));
+}
+
+int bi8_dequantize_int4(const uint8_t* q, int64_t ldq, const void* s, int s_dtype, void* out, int out_dtype, int64_t M, int64_t K, int block,
+                        void* stream) {
+    DeviceOfCall call;
+    if (int rc = check_int4("dequantize_int4", s_dtype, M, K, block)) return rc;
+    if (!dtype_ok(out_dtype)) return fail(BI8_ERR_DTYPE, "dequantize_int4: unknown output dtype code %d", out_dtype);
+    if (M == 0 || K == 0) return BI8_OK;
+    if (!q || !s || !out) return fail(BI8_ERR_NULL, "dequantize_int4: null pointer");
+    if (M > 1 && ldq < (K + 1) / 2) return fail(BI8_ERR_SHAPE, "dequantize_int4: row pitch smaller than a row");
+    if (!aligned(s, 2) || !aligned(out, dtype_size(out_dtype))) return fail(BI8_ERR_ALIGN, "dequantize_int4: pointer not element aligned");
+    return launch_dequantize_int4(q, ldq, s, s_dtype, out, out_dtype, M, K, block, static_cast<cudaStream_t>(stream));
+}
+
+int bi8_matmul_int4(const void* x, int x_dtype, int64_t ldx, const uint8_t* Wq, int64_t ldw, const void* sW, const void* bias, int bias_dtype,
+                    const void* residual, int64_t ldr, void* C, int64_t ldc, int out_dtype, int64_t M, int64_t N, int64_t K, int block,
+                    void* stream) {
+    DeviceOfCall call;
+    if (int rc = check_int4("matmul_int4", x_dtype, M, K, block)) return rc;
+    if (N < 0 || M > 0x400000 || N > 0x7fffff00 || K > 0x7fffff00)
+        return fail(BI8_ERR_SHAPE, "matmul_int4: bad shape M %lld N %lld K %lld", (long long)M, (long long)N, (long long)K);
+    if (!dtype_ok(out_dtype) || (bias && !dtype_ok(bias_dtype))) return fail(BI8_ERR_DTYPE, "matmul_int4: unknown dtype code");
+    if (M == 0 || N == 0) return BI8_OK;
+    if (!C || (K > 0 && (!x || !Wq || !sW))) return fail(BI8_ERR_NULL, "matmul_int4: null operand");
+    if ((M > 1 && (ldx < K || ldc < N || (residual && ldr < N))) || (N > 1 && ldw < (K + 1) / 2))
+        return fail(BI8_ERR_SHAPE, "matmul_int4: row pitch smaller than a row");
+    if (!aligned(x, 2) || !aligned(sW, 2) || !aligned(C, dtype_size(out_dtype)) || !aligned(residual, dtype_size(out_dtype)) ||
+        (bias && !aligned(bias, dtype_size(bias_dtype))))
+        return fail(BI8_ERR_ALIGN, "matmul_int4: pointer not element aligned");
+    if (residual && !(residual == C && ldr == ldc) && overlaps_output(residual, ldr, C, ldc, out_dtype, M, N))
+        return fail(BI8_ERR_SHAPE, "matmul_int4: residual overlaps the output without being it");
+    return launch_matmul_int4(x, x_dtype, ldx, Wq, ldw, sW, bias, bias_dtype, residual, ldr, C, ldc, out_dtype, M, N, K, block,
+                              static_cast<cudaStream_t>(stream));
+}
+
+int bi8_rope_cache_append_int4(const void* qkv, int dtype, const float* cis, int64_t cis_rows, const long long* pos, int64_t pos_step, void* q_out,
+                               const bi8_int4_cache* cache, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, void* stream) {
+    DeviceOfCall call;
+    if (int rc = check_int4_cache("rope_cache_append_int4", dtype, cache, B, T, Hq, Hkv, D)) return rc;
+    if (cis_rows < 0 || pos_step < 0) return fail(BI8_ERR_SHAPE, "rope_cache_append_int4: negative size");
+    if (B == 0 || T == 0 || Hq == 0) return BI8_OK;
+    if (!qkv || !pos || !q_out || (cis_rows > 0 && !cis)) return fail(BI8_ERR_NULL, "rope_cache_append_int4: null pointer");
+    if (!aligned(qkv, 16) || !aligned(q_out, 16) || !aligned(cis, 16) || !aligned(pos, 8))
+        return fail(BI8_ERR_ALIGN, "rope_cache_append_int4: pointer not aligned");
+    return launch_rope_cache_append_int4(qkv, dtype, cis, cis_rows, pos, pos_step, q_out, cache, B, T, Hq, Hkv, D, static_cast<cudaStream_t>(stream));
+}
+
+size_t bi8_attention_int4_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len) {
+    if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128 && D != 256) || max_len <= 0) return 0;
+    DeviceOfCall call;
+    return attention_int4_workspace_bytes(B, T, Hq, Hkv, D, max_len);
+}
+
+int bi8_attention_int4(const void* q, int dtype, int64_t q_batch, int64_t q_head, int64_t q_tok, const bi8_int4_cache* cache,
+                       const long long* lengths, int64_t lengths_step, const long long* starts, int64_t starts_step, float scale, void* out,
+                       int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, void* workspace, size_t workspace_bytes, void* stream) {
+    DeviceOfCall call;
+    if (int rc = check_int4_cache("attention_int4", dtype, cache, B, T, Hq, Hkv, D)) return rc;
+    if (lengths_step < 0 || starts_step < 0) return fail(BI8_ERR_SHAPE, "attention_int4: negative step");
+    if (B == 0 || T == 0 || Hq == 0) return BI8_OK;
+    if (!q || !lengths || !out) return fail(BI8_ERR_NULL, "attention_int4: null pointer");
+    if (!aligned(q, 16) || q_batch % 8 || q_head % 8 || q_tok % 8 || !aligned(out, 16) || !aligned(lengths, 8) || !aligned(starts, 8))
+        return fail(BI8_ERR_ALIGN, "attention_int4: pointer or step not aligned");
+    const size_t want = attention_int4_workspace_bytes(B, T, Hq, Hkv, D, cache->max_len);
+    if (want > 0 && (!workspace || workspace_bytes < want || !aligned(workspace, 16)))
+        return fail(BI8_ERR_WORKSPACE, "attention_int4: %zu bytes of workspace needed, got %zu", want, workspace ? workspace_bytes : (size_t)0);
+    return launch_attention_int4(q, dtype, q_batch, q_head, q_tok, cache, lengths, lengths_step, starts, starts_step, scale, out, B, T, Hq, Hkv, D,
+                                 workspace, static_cast<cudaStream_t>(stream));
+}
+
 int bi8_stream_capture_id(void* stream, unsigned long long* id) {
     if (!id) return fail(BI8_ERR_NULL, "stream_capture_id: null output");
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;

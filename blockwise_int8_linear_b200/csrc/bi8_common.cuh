@@ -156,6 +156,19 @@ int launch_peer_allreduce_large(void* const* peer_bufs, int rank, int world, int
 // rotary embedding of q and k and the append of k and v to the caches for one decode step (rope_cache.cu)
 int launch_rope_cache_append(const void* qkv, int dt, const float* cis, const long long* pos, void* q_out, void* kcache, void* vcache,
                              int64_t B, int64_t H, int64_t D, int64_t max_len, cudaStream_t st);
+// weights and key/value caches in 4-bit blocks (int4_quantize.cu, int4_matmul.cu, int4_cache.cu, int4_attention.cu)
+int launch_quantize_int4(const void* x, int dt, int64_t ldx, uint8_t* q, int64_t ldq, void* s, int64_t M, int64_t K, int block, cudaStream_t st);
+int launch_dequantize_int4(const uint8_t* q, int64_t ldq, const void* s, int s_dt, void* out, int out_dt, int64_t M, int64_t K, int block,
+                           cudaStream_t st);
+int launch_matmul_int4(const void* x, int x_dt, int64_t ldx, const uint8_t* W, int64_t ldw, const void* sW, const void* bias, int bias_dt,
+                       const void* residual, int64_t ldr, void* C, int64_t ldc, int out_dt, int64_t M, int64_t N, int64_t K, int block,
+                       cudaStream_t st);
+int launch_rope_cache_append_int4(const void* qkv, int dt, const float* cis, int64_t cis_rows, const long long* pos, int64_t pos_step, void* q_out,
+                                  const bi8_int4_cache* cache, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, cudaStream_t st);
+size_t attention_int4_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len);
+int launch_attention_int4(const void* q, int dt, int64_t q_batch, int64_t q_head, int64_t q_tok, const bi8_int4_cache* cache, const long long* lengths,
+                          int64_t lengths_step, const long long* starts, int64_t starts_step, float scale, void* out, int64_t B, int64_t T, int64_t Hq,
+                          int64_t Hkv, int64_t D, void* workspace, cudaStream_t st);
 // int8 rows of any alignment to rows on 16-byte boundaries (copy_rows.cu)
 int launch_copy_rows(const int8_t* src, int64_t lds, int8_t* dst, int64_t ldd, int64_t rows, int64_t cols, cudaStream_t st);
 // column sums in fp32 (column_sum.cu)

@@ -1,0 +1,130 @@
+// What the kernels for 4-bit blocks share: the format, its arithmetic and the operand layouts of the tensor cores.
+//
+// Format: `block` consecutive values of a row have the scale s = max|x|, held exactly in x's own 16-bit type; a value's code is
+// q = rint(7 x / s), -7 to 7, and stands for s q / 7.  A byte holds two neighbouring codes, offset by 8, the even one in its low half;
+// a row of odd length ends in a code 0.  A block that holds an infinity or a NaN has the scale NaN: all of it reads as NaN.
+#pragma once
+
+#include "bi8_common.cuh"
+
+namespace bi8 {
+
+constexpr float kInv7 = 1.0f / 7.0f;
+constexpr int kCacheBlock = 64;          // values per block of a key/value cache
+
+template <typename T>
+struct F16Bits;
+template <>
+struct F16Bits<__nv_bfloat16> {
+    static constexpr uint32_t kInf = 0x7f80u, kNaN = 0x7fc0u;
+    __device__ static float lo(uint32_t w) { return bf16lo(w); }
+    __device__ static float hi(uint32_t w) { return bf16hi(w); }
+    __device__ static float one(uint32_t bits) { return __uint_as_float(bits << 16); }
+    __device__ static uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+};
+template <>
+struct F16Bits<__half> {
+    static constexpr uint32_t kInf = 0x7c00u, kNaN = 0x7e00u;
+    __device__ static float lo(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w & 0xffffu))); }
+    __device__ static float hi(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
+    __device__ static float one(uint32_t bits) { return lo(bits); }
+    __device__ static uint32_t pack(float a, float b) { return pack_f16x2(a, b); }
+};
+
+// Largest |value| among eight 16-bit values, as the bits of that type: without the sign they order like integers, NaN above infinity.
+__device__ __forceinline__ uint32_t absmax8(const uint4& v) {
+    const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
+}
+
+// The codes of eight values under the scale `s` (finite): 32 bits, the first value's code in the lowest four.
+//
+// fma(x, 7/s, 56) lies between 49 and 63, where fp32 has steps of 2^-18: a quotient 7x/s that is a tie k + 1/2 is off by at most
+// 7 * 2^-24 before that rounding and lands on the tie, and any other is 2^-15 or more away from one (14x - (2k+1)s is a multiple of
+// the smaller one's last place, for x >= s/14 and 11 significant bits), so it stays on its side.  Adding 1.5 * 2^23 then rounds to an
+// integer, ties to even, whose low four bits are q + 8 because 56 = 3 * 16 + 8.  Two operations a value instead of a division.
+// Scales below 2^-60 are lifted first, so that 7/s stays finite.
+template <typename T>
+__device__ __forceinline__ uint32_t codes8(const uint4& v, float s) {
+    const float up = s < 0x1p-60f ? 0x1p100f : 1.0f;
+    const float r = s > 0.0f ? __fdiv_rn(7.0f, s * up) : 0.0f;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t a = __float_as_uint(__fadd_rn(__fmaf_rn(F16Bits<T>::lo(w[i]) * up, r, 56.0f), 12582912.0f));
+        const uint32_t b = __float_as_uint(__fadd_rn(__fmaf_rn(F16Bits<T>::hi(w[i]) * up, r, 56.0f), 12582912.0f));
+        out |= ((a & 15u) | ((b & 15u) << 4)) << (8 * i);
+    }
+    return out;
+}
+constexpr uint32_t kZeroCodes = 0x88888888u;
+
+// Quantizes a block that lies in `lanes` neighbouring lanes, eight values each: codes of this lane, the scale's bits in all of them.
+template <typename T>
+__device__ __forceinline__ uint32_t quantize8(const uint4& v, int lanes, uint32_t* scale_bits) {
+    uint32_t m = absmax8(v);
+    for (int d = lanes / 2; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const bool bad = m >= F16Bits<T>::kInf;
+    *scale_bits = bad ? F16Bits<T>::kNaN : m;
+    return bad ? kZeroCodes : codes8<T>(v, F16Bits<T>::one(m));
+}
+
+// s q / 7 in fp32, rounded once: s q is exact (14 bits), and the quotient is corrected by its remainder (Markstein's division by a
+// constant).  Scales outside the range in which the remainder is exact take the division itself, the largest of them a factor of
+// 2^20 lower, where 7 s does not overflow.
+__device__ __forceinline__ float value_of(float s, uint32_t code, bool plain) {
+    const float q = (float)((int)code - 8);
+    if (!plain) return s > 1.0f ? __fdiv_rn(s * 0x1p-20f * q, 7.0f) * 0x1p20f : __fdiv_rn(s * q, 7.0f);
+    const float m = s * q;
+    const float y = m * kInv7;
+    return __fmaf_rn(__fmaf_rn(-7.0f, y, m), kInv7, y);
+}
+__device__ __forceinline__ bool plain_scale(float s) { return (s > 0x1p-100f && s < 0x1p120f) || s == 0.0f; }
+
+// ---- tensor-core operands -----------------------------------------------------------------------------------------------------
+// Codes become fp16 operands in pairs: four bits c + 8 under the exponent of 1024 are 1024 + 8 + c, four bits further up 1024 + 16 (8 + c);
+// less 1032 and 1152 that is c and 16 c, exactly.  Eight codes are one shift, four AND-ORs and four packed subtractions.  (The four bits
+// alone are fp16 denormals, (8 + c) 2^-24, which need neither the OR nor the subtraction; but the matrix instruction aligns its sums by the
+// operands' exponent fields, and ten leading zeros in one operand cost the sum as many bits: measured 2^-16 of the largest term.)  The
+// other operand is scaled by a power of two to fit fp16, which keeps everything of a bf16 value that is 2^-28 or more of the largest
+// one, and the values that meet the higher codes by 1/16.
+//
+// Order of a word's eight codes in the contraction: pairs (0,4), (1,5), (2,6), (3,7); 1, 3, 5 and 7 sit four bits higher.
+__device__ __forceinline__ uint32_t minus2(uint32_t v, uint32_t k) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&k));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t codes_low(uint32_t w) { return minus2((w & 0x000f000fu) | 0x64006400u, 0x64086408u); }
+__device__ __forceinline__ uint32_t codes_high(uint32_t w) { return minus2((w & 0x00f000f0u) | 0x64006400u, 0x64806480u); }
+struct Codes4 {
+    uint32_t p04, p15, p26, p37;
+};
+__device__ __forceinline__ Codes4 unpack8(uint32_t w) { return {codes_low(w), codes_high(w), codes_low(w >> 8), codes_high(w >> 8)}; }
+// 2^e with |x| < 2^15 for x = max / 2^e (m: the bits of max in T), as the pair (2^e, 2^-e)
+template <typename T>
+__device__ __forceinline__ float2 fit_fp16(uint32_t m) {
+    if (m == 0u || m >= F16Bits<T>::kInf) return make_float2(1.0f, 1.0f);
+    const float a = F16Bits<T>::one(m);
+    // a bf16 denormal is an fp32 denormal: exponent field 0, treated as 2^-126
+    int e = max((int)(__float_as_uint(a) >> 23), 1) - 127 - 14;
+    e = max(e, -126 + 14);
+    return make_float2(__uint_as_float((uint32_t)(e + 127) << 23), __uint_as_float((uint32_t)(127 - e) << 23));
+}
+// Eight values as the operand that meets a word of codes: scaled, in the pairs above, odd ones by 1/16.
+template <typename T>
+__device__ __forceinline__ uint4 operand8(const uint4& v, float inv) {
+    using H = F16Bits<T>;
+    const float odd = inv * 0.0625f;
+    return make_uint4(pack_f16x2(H::lo(v.x) * inv, H::lo(v.z) * inv), pack_f16x2(H::hi(v.x) * odd, H::hi(v.z) * odd),
+                      pack_f16x2(H::lo(v.y) * inv, H::lo(v.w) * inv), pack_f16x2(H::hi(v.y) * odd, H::hi(v.w) * odd));
+}
+
+// D += A B, A 16 x 16 (rows g and g + 8 of lane 4 g + c, columns 2c, 2c+1 and 2c+8, 2c+9), B 16 x 8 (column g), D 16 x 8 (columns 2c, 2c+1)
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+}  // namespace bi8

@@ -849,6 +849,213 @@ Tensor rope_cache_append(const Tensor& qkv_in, const Tensor& cis_in, const Tenso
     return q;
 }
 
+// ---- weights and key/value caches in 4-bit blocks ---------------------------------------------------------------------------
+// These have no backward pass: a tensor that wants a gradient would lose it silently.
+void no_gradient(const Tensor& t, const char* what) {
+    if (t.defined() && at::GradMode::is_enabled() && t.requires_grad())
+        throw PyFail{PyExc_RuntimeError, std::string(what) + " has no backward pass: call it under torch.no_grad() or on detached tensors"};
+}
+int dtype_code16(at::ScalarType t, const char* what) {
+    if (t != at::kBFloat16 && t != at::kHalf) value_error(std::string(what) + " must be bfloat16 or float16, got " + c10::toString(t));
+    return dtype_code(t);
+}
+void same_device(const Tensor& t, const Tensor& like, const char* what) {
+    if (t.defined() && t.device() != like.device()) value_error(std::string(what) + " must be on " + like.device().str() + ", got " + t.device().str());
+}
+void check_block4(int64_t block) {
+    if (block != 32 && block != 64 && block != 128) value_error("4-bit blocks have 32, 64 or 128 values, got " + std::to_string(block));
+}
+using Sizes = c10::SmallVector<int64_t, 6>;
+Sizes with_last(const Tensor& t, int64_t last) {
+    Sizes s(t.sizes().begin(), t.sizes().end());
+    s.back() = last;
+    return s;
+}
+
+Quantized quantize_int4(const Tensor& x, int64_t block) {
+    need_cuda(x);
+    no_gradient(x, "quantize_block_int4");
+    if (x.dim() == 0) value_error("expected a tensor with a feature dimension, got a scalar");
+    const int code = dtype_code16(x.scalar_type(), "values");
+    check_block4(block);
+    OnDevice on(x);
+    const int64_t k = x.size(-1);
+    Quantized r{empty_on(x, with_last(x, ceil_div(k, 2)), at::kByte), empty_on(x, with_last(x, ceil_div(k, block)), x.scalar_type())};
+    if (x.numel() == 0) return r;
+    const Mat m = mat_rows(x);
+    check(bi8_quantize_int4(m.ptr, code, m.ld, r.q.mutable_data_ptr<uint8_t>(), ceil_div(k, 2), r.s.data_ptr(), m.rows, k, (int)block, on.raw()),
+          "bi8_quantize_int4");
+    return r;
+}
+
+// scales [..., blocks] of codes [..., bytes]
+void check_scales4(const Tensor& state, const Tensor& codes, int64_t blocks, int64_t block) {
+    const Sizes want = with_last(codes, blocks);
+    if (state.sizes() != at::IntArrayRef(want))
+        value_error("state must have " + std::to_string(blocks) + " scales per row for block " + std::to_string(block) + ", got " + shape_of(state) +
+                    " for codes " + shape_of(codes));
+    same_device(state, codes, "state");
+}
+
+Tensor dequantize_int4(const Tensor& codes, const Tensor& state, int64_t block, int64_t features, at::ScalarType out_type) {
+    need_cuda(codes);
+    if (codes.dim() == 0 || codes.scalar_type() != at::kByte) value_error(std::string("codes must be uint8 with a feature dimension, got ") + c10::toString(codes.scalar_type()));
+    const int code = dtype_code16(state.scalar_type(), "state");
+    check_block4(block);
+    const int64_t k = features < 0 ? 2 * codes.size(-1) : features;
+    if (ceil_div(k, 2) != codes.size(-1)) value_error(std::to_string(k) + " features do not have " + std::to_string(codes.size(-1)) + " bytes of codes");
+    check_scales4(state, codes, ceil_div(k, block), block);
+    OnDevice on(codes);
+    Tensor out = empty_on(codes, with_last(codes, k), out_type);
+    if (out.numel() == 0) return out;
+    const Mat m = mat_rows(codes);
+    const Tensor s = state.contiguous();
+    check(bi8_dequantize_int4(static_cast<const uint8_t*>(m.ptr), m.ld, s.data_ptr(), code, out.data_ptr(), dtype_code(out_type), m.rows, k, (int)block, on.raw()),
+          "bi8_dequantize_int4");
+    return out;
+}
+
+Tensor matmul_int4(const Tensor& x_in, const Tensor& codes, const Tensor& state, const Tensor& bias_in, const Tensor& residual, int64_t block,
+                   at::ScalarType out_type) {
+    need_cuda(x_in);
+    no_gradient(x_in, "int4_matmul");
+    no_gradient(residual, "int4_matmul");
+    if (x_in.dim() == 0) value_error("expected a tensor with a feature dimension, got a scalar");
+    const int code = dtype_code16(x_in.scalar_type(), "activations");
+    check_block4(block);
+    const int64_t k = x_in.size(-1);
+    if (codes.dim() != 2 || codes.scalar_type() != at::kByte || codes.size(1) != ceil_div(k, 2))
+        value_error("codes must be uint8 [N, " + std::to_string(ceil_div(k, 2)) + "] for " + std::to_string(k) + " features, got " +
+                    c10::toString(codes.scalar_type()) + " " + shape_of(codes));
+    same_device(codes, x_in, "codes");
+    check_scales4(state, codes, ceil_div(k, block), block);
+    if (state.scalar_type() != x_in.scalar_type())
+        value_error(std::string("activations and scales must have one type, got ") + c10::toString(x_in.scalar_type()) + " and " + c10::toString(state.scalar_type()));
+    same_device(bias_in, x_in, "bias");
+    OnDevice on(x_in);
+    const int64_t n = codes.size(0), m = k ? x_in.numel() / k : c10::multiply_integers(x_in.sizes().begin(), x_in.sizes().end() - 1);
+    const Bias bias(bias_in, n);
+    Tensor out = empty_on(x_in, with_last(x_in, n), out_type);
+    Mat res;
+    if (residual.defined()) {
+        if (residual.sizes() != out.sizes() || residual.scalar_type() != out_type)
+            value_error(std::string("residual must be ") + c10::toString(out_type) + " " + shape_of(out) + ", got " + c10::toString(residual.scalar_type()) + " " +
+                        shape_of(residual));
+        same_device(residual, x_in, "residual");
+        if (out.numel() > 0) res = mat_rows(residual);
+    }
+    if (out.numel() == 0) return out;
+    const Mat x = k ? mat_rows(x_in) : Mat{}, w = mat2d(codes);
+    const Tensor s = state.contiguous();
+    check(bi8_matmul_int4(x.ptr, code, std::max(x.ld, k), static_cast<const uint8_t*>(w.ptr), w.ld, s.data_ptr(), bias.ptr, bias.code, res.ptr, res.ld,
+                          out.data_ptr(), n, dtype_code(out_type), m, n, k, (int)block, on.raw()),
+          "bi8_matmul_int4");
+    return out;
+}
+
+// The cache's tensors as the library takes them.  `written`: heads and sequences must not share memory.
+bi8_int4_cache cache4(const Tensor& k, const Tensor& k_state, const Tensor& v, const Tensor& v_state, const Tensor& like, int64_t b, int64_t d, bool written) {
+    if (k.dim() != 4) value_error("cache codes must be 4-D, got " + shape_of(k));
+    const int64_t h = k.size(1), rows = k.size(2);
+    int64_t steps[8];
+    int at = 0;
+    for (const Tensor* t : {&k, &v, &k_state, &v_state}) {
+        const bool codes = t == &k || t == &v;
+        const int64_t width = codes ? d / 2 : d / 64;
+        const at::ScalarType type = codes ? at::kByte : like.scalar_type();
+        const bool dense = t->dim() == 4 && (width <= 1 || t->stride(3) == 1) && (rows <= 1 || t->stride(2) == width);
+        if (t->dim() != 4 || t->size(0) != b || t->size(1) != h || t->size(2) != rows || t->size(3) != width || t->scalar_type() != type || !dense ||
+            t->device() != like.device())
+            value_error(std::string("cache ") + (codes ? "codes" : "scales") + " must be " + c10::toString(type) + " [" + std::to_string(b) + ", " +
+                        std::to_string(h) + ", " + std::to_string(rows) + ", " + std::to_string(width) + "] with dense rows on " + like.device().str() + ", got " +
+                        c10::toString(t->scalar_type()) + " " + shape_of(*t));
+        for (int dim = 0; dim < 2; ++dim) {
+            steps[at++] = t->size(dim) > 1 ? t->stride(dim) : 0;
+            if (written && t->size(dim) > 1 && t->stride(dim) < rows * width) value_error("a cache that is written must not share memory between sequences or heads");
+        }
+    }
+    return {static_cast<uint8_t*>(k.data_ptr()), static_cast<uint8_t*>(v.data_ptr()), k_state.data_ptr(), v_state.data_ptr(),
+            steps[0], steps[1], steps[2], steps[3], steps[4], steps[5], steps[6], steps[7], rows};
+}
+
+// One int64 for all sequences or one for each: its address and step.
+struct PerSequence {
+    const long long* ptr = nullptr;
+    int64_t step = 0;
+    PerSequence(const Tensor& t, const Tensor& like, int64_t b, const char* what) {
+        if (!t.defined()) return;
+        if (t.scalar_type() != at::kLong || t.device() != like.device() || !(t.numel() == 1 || (t.dim() == 1 && t.size(0) == b)))
+            value_error(std::string(what) + " must be an int64 tensor with one element or " + std::to_string(b) + " on the activations' device");
+        ptr = static_cast<const long long*>(t.data_ptr());
+        step = t.numel() == 1 ? 0 : t.stride(0);
+    }
+};
+
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+Tensor rope_cache_append_int4(const Tensor& qkv_in, const Tensor& cis_in, const Tensor& pos, const Tensor& k, const Tensor& k_state, const Tensor& v,
+                              const Tensor& v_state) {
+    need_cuda(qkv_in);
+    no_gradient(qkv_in, "rope_cache_append_int4");
+    if (qkv_in.dim() != 4) value_error("expected [B, T, Hq + 2 Hkv, D], got " + shape_of(qkv_in));
+    const int code = dtype_code16(qkv_in.scalar_type(), "activations");
+    const int64_t b = qkv_in.size(0), t = qkv_in.size(1), d = qkv_in.size(3);
+    if (d != 64 && d != 128 && d != 256) value_error("head size must be 64, 128 or 256, got " + std::to_string(d));
+    const bi8_int4_cache cache = cache4(k, k_state, v, v_state, qkv_in, b, d, true);
+    const int64_t hkv = k.size(1), hq = qkv_in.size(2) - 2 * hkv;
+    if (hkv < 1 || hq < hkv || hq % hkv != 0) value_error(std::to_string(qkv_in.size(2)) + " heads are not Hq + 2 * " + std::to_string(hkv) + " with Hq a multiple of " + std::to_string(hkv));
+    OnDevice on(qkv_in);
+    Tensor qkv = qkv_in.contiguous();
+    if (qkv.numel() > 0 && !aligned16(qkv)) qkv = qkv.clone();
+    // complex64 [rows, D/2] or float32 (cos, sin) pairs: the same bytes
+    const bool cplx = cis_in.scalar_type() == at::kComplexFloat;
+    if ((!cplx && cis_in.scalar_type() != at::kFloat) || cis_in.dim() != (cplx ? 2 : 3) || cis_in.size(1) != d / 2 || (!cplx && cis_in.size(2) != 2) ||
+        cis_in.device() != qkv.device())
+        value_error("cis must hold [rows, " + std::to_string(d / 2) + "] (cos, sin) float32 pairs on the activations' device");
+    Tensor cis = cis_in.is_conj() ? cis_in.resolve_conj().contiguous() : cis_in.contiguous();
+    if (cis.numel() > 0 && !aligned16(cis)) cis = cis.clone();
+    const PerSequence p(pos, qkv, b, "pos");
+    Tensor q = empty_on(qkv, {b, hq, t, d}, qkv.scalar_type());
+    check(bi8_rope_cache_append_int4(qkv.data_ptr(), code, static_cast<const float*>(cis.data_ptr()), cis.size(0), p.ptr, p.step, q.data_ptr(), &cache, b, t, hq,
+                                     hkv, d, on.raw()),
+          "bi8_rope_cache_append_int4");
+    return q;
+}
+
+Tensor attention_int4(const Tensor& q_in, const Tensor& k, const Tensor& k_state, const Tensor& v, const Tensor& v_state, const Tensor& lengths,
+                      const Tensor& starts, double scale) {
+    need_cuda(q_in);
+    no_gradient(q_in, "attention_int4_cache");
+    if (q_in.dim() != 4) value_error("expected queries [B, Hq, T, D], got " + shape_of(q_in));
+    const int code = dtype_code16(q_in.scalar_type(), "queries");
+    const int64_t b = q_in.size(0), hq = q_in.size(1), t = q_in.size(2), d = q_in.size(3);
+    if (d != 64 && d != 128 && d != 256) value_error("head size must be 64, 128 or 256, got " + std::to_string(d));
+    const bi8_int4_cache cache = cache4(k, k_state, v, v_state, q_in, b, d, false);
+    const int64_t hkv = k.size(1);
+    if (hkv < 1 || hq < 1 || hq % hkv != 0) value_error(std::to_string(hq) + " query heads do not divide over " + std::to_string(hkv) + " cache heads");
+    OnDevice on(q_in);
+    const PerSequence len(lengths, q_in, b, "lengths"), start(starts, q_in, b, "starts");
+    Tensor out = empty_on(q_in, {b, hq, t, d}, q_in.scalar_type());
+    if (out.numel() == 0) return out;
+    Tensor q = q_in;
+    int64_t steps[3];
+    bool ok = q.stride(3) == 1 && aligned16(q);
+    for (int i = 0; i < 3; ++i) {
+        steps[i] = q.size(i) > 1 ? q.stride(i) : 0;
+        ok = ok && steps[i] % 8 == 0;
+    }
+    if (!ok) {
+        q = q.clone(at::MemoryFormat::Contiguous);
+        steps[0] = hq * t * d, steps[1] = t * d, steps[2] = d;
+    }
+    const size_t bytes = bi8_attention_int4_workspace_bytes(b, t, hq, hkv, d, cache.max_len);
+    const Tensor ws = scratch(q, (int64_t)bytes);
+    check(bi8_attention_int4(q.data_ptr(), code, steps[0], steps[1], steps[2], &cache, len.ptr, len.step, start.ptr, start.step, (float)scale, out.data_ptr(), b, t,
+                             hq, hkv, d, ws.defined() ? ws.data_ptr() : nullptr, bytes, on.raw()),
+          "bi8_attention_int4");
+    return out;
+}
+
 // ---- bindings -----------------------------------------------------------------------------------------------------------
 struct Args {
     PyObject* const* a;
@@ -991,6 +1198,34 @@ BI8_METHOD(rope_cache_append) {  // qkv, cis, pos, kcache, vcache
         return [q = g.tensor(0), c = g.tensor(1), p = g.tensor(2), k = g.tensor(3), v = g.tensor(4)] { return rope_cache_append(q, c, p, k, v); };
     });
 }
+BI8_METHOD(quantize_int4) {      // x, block
+    return call("quantize_int4", {a, n}, 2, [](const Args& g) { return [x = g.tensor(0), b = g.block(1)] { return quantize_int4(x, b); }; });
+}
+BI8_METHOD(dequantize_int4) {    // codes, state, block, features or -1, dtype
+    return call("dequantize_int4", {a, n}, 5, [](const Args& g) {
+        return [q = g.tensor(0), s = g.tensor(1), b = g.block(2), k = g.integer(3), t = g.dtype(4)] { return dequantize_int4(q, s, b, k, t); };
+    });
+}
+BI8_METHOD(matmul_int4) {        // x, codes, state, bias, residual, block, dtype
+    return call("matmul_int4", {a, n}, 7, [](const Args& g) {
+        return [x = g.tensor(0), q = g.tensor(1), s = g.tensor(2), bias = g.optional(3), res = g.optional(4), b = g.block(5), t = g.dtype(6)] {
+            return matmul_int4(x, q, s, bias, res, b, t);
+        };
+    });
+}
+BI8_METHOD(rope_cache_append_int4) {  // qkv, cis, pos, k, k_state, v, v_state
+    return call("rope_cache_append_int4", {a, n}, 7, [](const Args& g) {
+        return [x = g.tensor(0), c = g.tensor(1), p = g.tensor(2), k = g.tensor(3), ks = g.tensor(4), v = g.tensor(5), vs = g.tensor(6)] {
+            return rope_cache_append_int4(x, c, p, k, ks, v, vs);
+        };
+    });
+}
+BI8_METHOD(attention_int4) {     // q, k, k_state, v, v_state, lengths, starts, scale
+    return call("attention_int4", {a, n}, 8, [](const Args& g) {
+        return [q = g.tensor(0), k = g.tensor(1), ks = g.tensor(2), v = g.tensor(3), vs = g.tensor(4), len = g.tensor(5), start = g.optional(6),
+                scale = g.number(7)] { return attention_int4(q, k, ks, v, vs, len, start, scale); };
+    });
+}
 BI8_METHOD(bind) {               // the exception class of failed library calls, the configuration module
     if (n != 2) {
         PyErr_SetString(PyExc_TypeError, "bind takes 2 arguments");
@@ -1004,7 +1239,8 @@ BI8_METHOD(bind) {               // the exception class of failed library calls,
 #define BI8_ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name##_py)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {BI8_ENTRY(quantize_rowwise), BI8_ENTRY(quantize_colwise), BI8_ENTRY(quantize_dual), BI8_ENTRY(quantize_pre),
                          BI8_ENTRY(dequantize), BI8_ENTRY(gemm), BI8_ENTRY(block_partials), BI8_ENTRY(matmul), BI8_ENTRY(linear),
-                         BI8_ENTRY(train_linear), BI8_ENTRY(rope_cache_append), BI8_ENTRY(bind),
+                         BI8_ENTRY(train_linear), BI8_ENTRY(rope_cache_append), BI8_ENTRY(quantize_int4), BI8_ENTRY(dequantize_int4),
+                         BI8_ENTRY(matmul_int4), BI8_ENTRY(rope_cache_append_int4), BI8_ENTRY(attention_int4), BI8_ENTRY(bind),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Host path of the blockwise-int8 operations.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

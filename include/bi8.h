@@ -265,6 +265,68 @@ BI8_API int bi8_gemm_dequant_fused_pre(int op, const void* x, const void* x2, in
 BI8_API int bi8_rope_cache_append(const void* qkv, int dtype, const float* cis, const long long* pos, void* q_out, void* kcache,
                           void* vcache, int64_t B, int64_t H, int64_t D, int64_t max_len, void* stream);
 
+/* ---- weights and caches in 4 bits (no counterpart in the reference, whose values have 8) -------------------------------------
+ * Format: `block` consecutive values of a row have the scale s = max|x|, held exactly in x's own type (bf16 or fp16); a value's code is
+ * rint(7 x / s), -7 to 7 (the quotient in exact arithmetic, ties to even), and stands for s * code / 7.  Codes lie two to a byte,
+ * offset by 8, the even one in the low half; a row of K values has ceil(K/2) bytes (an odd one ends in a code 0) and
+ * ceil(K/block) scales.  Scales lie row by row, [rows, ceil(K/block)]: not transposed as the int8 ones are, because a kernel that
+ * streams weights or a cache takes several scales of one row at a time.  An all-zero block has scale 0 and codes 0; one that
+ * holds an infinity or a NaN has the scale NaN, so that all of it reads as NaN. */
+
+/* x [M,K] of dtype (BI8_BF16 or BI8_F16), row stride ldx: codes q [M, ceil(K/2)] with row pitch ldq bytes, scales s dense, of x's type.
+ * block 32, 64 or 128. */
+BI8_API int bi8_quantize_int4(const void* x, int dtype, int64_t ldx, uint8_t* q, int64_t ldq, void* s, int64_t M, int64_t K, int block,
+                              void* stream);
+/* out [M,K] contiguous of out_dtype = cast(s * code / 7), the quotient rounded to fp32 once. */
+BI8_API int bi8_dequantize_int4(const uint8_t* q, int64_t ldq, const void* s, int s_dtype, void* out, int out_dtype, int64_t M, int64_t K,
+                                int block, void* stream);
+/* C[m,n] = cast( sum_k x[m,k] * value(W[n,k]) (+ bias[n]) (+ residual[m,n]) ): fp32 sums in a fixed order, one rounding.
+ * x [M,K] of x_dtype (BI8_BF16 or BI8_F16), row stride ldx.  Wq / sW as bi8_quantize_int4 gives them, row pitch ldw bytes, scales of
+ * x_dtype.  bias [N] of bias_dtype or NULL.  residual [M,N] of out_dtype, row stride ldr, or NULL; C may be the residual itself.
+ * Made for few rows of x, for which the weights are read once (up to 64; more rows are taken 64 at a time).  Code rows that begin
+ * on 8-byte boundaries are read faster than others.  A row of x with an infinity or a NaN gives nothing finite. */
+BI8_API int bi8_matmul_int4(const void* x, int x_dtype, int64_t ldx, const uint8_t* Wq, int64_t ldw, const void* sW, const void* bias,
+                            int bias_dtype, const void* residual, int64_t ldr, void* C, int64_t ldc, int out_dtype, int64_t M, int64_t N,
+                            int64_t K, int block, void* stream);
+
+/* A key/value cache in 4 bits: codes [batch, head, max_len, D/2] and scales [batch, head, max_len, D/64] (blocks of 64) of k and of v.  Rows
+ * of a head are dense; steps between batches and heads are free: bytes for the codes (multiples of 8), elements for the scales
+ * (multiples of D/64).  Codes begin on 8-byte boundaries, scales on boundaries of a row's scales. */
+typedef struct {
+    uint8_t* k;
+    uint8_t* v;
+    void* k_state;
+    void* v_state;
+    int64_t k_batch, k_head, v_batch, v_head;
+    int64_t ks_batch, ks_head, vs_batch, vs_head;
+    int64_t max_len;
+} bi8_int4_cache;
+
+/* bi8_rope_cache_append for a cache in 4 bits, any number of new tokens and fewer heads of k and v than of q.
+ *   qkv      [B, T, Hq + 2 Hkv, D] of dtype, contiguous, 16-byte aligned: q, k, v of T new tokens per sequence; D 64, 128 or 256
+ *   cis      [cis_rows, D/2] pairs (cos, sin) fp32, 16-byte aligned: the rotation of every position
+ *   pos      device address of the first token's position (int64), of sequence b at pos[b * pos_step] (pos_step 0: one for all).
+ *            Token t goes to position and cache row pos + t.  Outside the cache or the table its key and value are not written and its
+ *            query is zero
+ *   q_out    [B, Hq, T, D] contiguous, 16-byte aligned: the rotated queries
+ * k is quantized after its rotation has been rounded to dtype. */
+BI8_API int bi8_rope_cache_append_int4(const void* qkv, int dtype, const float* cis, int64_t cis_rows, const long long* pos, int64_t pos_step,
+                                       void* q_out, const bi8_int4_cache* cache, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                       void* stream);
+
+/* Attention of T queries per sequence over such a cache: out [B, Hq, T, D] contiguous = softmax(scale * q k^T) v.
+ *   q        [B, Hq, T, D] of dtype: steps q_batch, q_head, q_tok in elements (multiples of 8), features contiguous, 16-byte aligned
+ *   lengths  device address (int64): sequence b has lengths[b * lengths_step] rows, the last T of which are the queries' own: query t sees
+ *            rows up to lengths - T + t.  Lengths beyond max_len see max_len rows
+ *   starts   the first row that is seen (rows before it belong to nobody, as in a batch padded on the left), or NULL for 0
+ * A query that sees no row gives zeros.  Rows that no query sees are not read.  Hq is a multiple of Hkv; query head h reads cache head
+ * h / (Hq / Hkv).  workspace: bi8_attention_int4_workspace_bytes bytes, 16-byte aligned, scratch of this call. */
+BI8_API size_t bi8_attention_int4_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len);
+BI8_API int bi8_attention_int4(const void* q, int dtype, int64_t q_batch, int64_t q_head, int64_t q_tok, const bi8_int4_cache* cache,
+                               const long long* lengths, int64_t lengths_step, const long long* starts, int64_t starts_step, float scale,
+                               void* out, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
 /* Capture sequence number of `stream` if it is being captured into a CUDA graph, 0 otherwise (no counterpart in the
  * reference).  A host layer that caches workspaces uses it to give every captured graph a scratch buffer of its own:
  * an address baked into a graph must not be shared with another graph that may be replayed on a different stream. */
