@@ -599,8 +599,8 @@ int check_int4_cache(const char* what, int dtype, const bi8_int4_cache* c, int64
     if (Hq / Hkv * T > 0x7fffffff) return fail(BI8_ERR_LIMIT, "%s: too many queries per cache head", what);
     if (c->max_len > 0 && (!c->k || !c->v || !c->k_state || !c->v_state)) return fail(BI8_ERR_NULL, "%s: null cache tensor", what);
     const int64_t n = D / 64;
-    if (!aligned(c->k, 8) || !aligned(c->v, 8) || c->k_batch % 8 || c->k_head % 8 || c->v_batch % 8 || c->v_head % 8)
-        return fail(BI8_ERR_ALIGN, "%s: codes of the cache not on 8-byte boundaries", what);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->k_batch % 16 || c->k_head % 16 || c->v_batch % 16 || c->v_head % 16)
+        return fail(BI8_ERR_ALIGN, "%s: codes of the cache not on 16-byte boundaries", what);
     if (!aligned(c->k_state, 2 * n) || !aligned(c->v_state, 2 * n) || c->ks_batch % n || c->ks_head % n || c->vs_batch % n || c->vs_head % n)
         return fail(BI8_ERR_ALIGN, "%s: scales of the cache not on boundaries of a row's scales", what);
     return BI8_OK;

@@ -9,12 +9,11 @@
 // them, the eight columns:
 //   S[row, query]  = sum_d k[row, d] q[query, d]
 //   O[d, query]    = sum_row v[row, d] P[row, query]  two rows' words interleaved by byte permutes
-// v's scales differ by row, so they go into P: p * vs as a sum of two fp16 numbers (22 bits), normalised by a power of two that
-// follows the largest scale met, like the running maximum of the softmax.  P leaves the first product with its rows along the lanes and
+// v's scales differ by row, so they go into P: p * vs in fp16 (11 bits, for bf16 results of 8) or, for fp16 results, as a sum of two fp16
+// numbers, normalised by a power of two that follows the largest scale met, like the running maximum of the softmax.  P leaves the first product with its rows along the lanes and
 // enters the second transposed (movmatrix).  Sums, statistics and scales are fp32.
 //
-// A warp takes steps of 16, 32 or 64 rows (4 KB) with the next step's loads in flight, straight into the registers that the matrix
-// instructions read: no shared memory for the cache.  The warps of a CTA and the CTAs of a cluster divide the rows of one cache head
+// A warp takes steps of 16, 32 or 64 rows (4 KB), the next one on its way into shared memory while this one is multiplied.  The warps of a CTA and the CTAs of a cluster divide the rows of one cache head
 // (each reads the lengths and takes its share of what there really is) and are joined over distributed shared memory; more than eight
 // shares go through a workspace and a second kernel.  Every sum has a fixed order.
 #include "int4_common.cuh"
@@ -44,7 +43,24 @@ struct AttnArgs {
     int B, Hq, Hkv, T, G;
     int col_tiles, shares;
     float scale_log2;        // scale * log2(e)
+    bool s_vec;              // pairs of scales begin on 4-byte boundaries
 };
+
+// 2^e with |x| < 2^15 for x = max / 2^e (m: the bits of max in T), as the pair (2^e, 2^-e): what fits queries to fp16, which keeps
+// everything of a bf16 value that is 2^-28 or more of the largest one.  Infinities and NaN stay what they are.
+template <typename T>
+__device__ __forceinline__ float2 fit_fp16(uint32_t m) {
+    if (m == 0u || m >= F16Bits<T>::kInf) return make_float2(1.0f, 1.0f);
+    int e = max((int)(__float_as_uint(F16Bits<T>::one(m)) >> 23), 1) - 127 - 14;          // denormals have the exponent -126
+    e = max(e, -126 + 14);
+    return make_float2(__uint_as_float((uint32_t)(e + 127) << 23), __uint_as_float((uint32_t)(127 - e) << 23));
+}
+template <typename T>
+__device__ __forceinline__ uint4 scaled8(const uint4& v, float f) {
+    using H = F16Bits<T>;
+    return make_uint4(pack_f16x2(H::lo(v.x) * f, H::hi(v.x) * f), pack_f16x2(H::lo(v.y) * f, H::hi(v.y) * f), pack_f16x2(H::lo(v.z) * f, H::hi(v.z) * f),
+                      pack_f16x2(H::lo(v.w) * f, H::hi(v.w) * f));
+}
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -57,53 +73,40 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
-// the scales of one row: U 16-bit values
-template <int U>
-struct RowScales {
-    uint32_t w[(U + 1) / 2];
-    __device__ __forceinline__ void load(const unsigned short* p) {
-        if (U == 1) w[0] = __ldg(p);
-        else if (U == 2) w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-        else {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-            w[0] = v.x;
-            w[(U + 1) / 2 - 1] = v.y;
-        }
-    }
-    template <typename T>
-    __device__ __forceinline__ float get(int u) const { return u & 1 ? F16Bits<T>::hi(w[u / 2]) : F16Bits<T>::lo(w[u / 2]); }
-};
-
-template <int U, int TT>
-struct Step {
-    uint2 k[TT][2][U];           // rows g and g + 8 of each 16: eight bytes of every 64 values
-    uint32_t v[TT][4][U];        // rows 2c, 2c + 1, 2c + 8, 2c + 9: four bytes of every 64 values
-    RowScales<U> ks[TT][2], vs[TT][2];
-};
-
 template <int D>
 constexpr int kStepTiles = D == 64 ? 4 : D == 128 ? 2 : 1;       // 16 rows each
 
+// A warp's rows of one step in shared memory: k, v (16 more or less than a multiple of 32 or 64 bytes apart, so that what the lanes read at a
+// time lies in different banks), their scales.  A warp has two steps there: one in use, one on its way.
+template <int D>
+struct Ring {
+    static constexpr int kRows = 16 * kStepTiles<D>, kPitchK = D / 2 + (D == 64 ? 0 : 32), kPitchV = D / 2 + 16, kRowScales = D / 64 * 2;
+    static constexpr int kV = kRows * kPitchK, kScalesK = kV + kRows * kPitchV, kScalesV = kScalesK + kRows * kRowScales, kBytes = kScalesV + kRows * kRowScales;
+    static constexpr int kSteps = 2;
+};
+
 template <int D, int NT>
 constexpr int attn_smem() {
-    // queries, the warps' sums (eight columns at a time), the CTA's sums, statistics
-    return 8 * NT * (2 * D + 16) + kWarps * 8 * (D + 4) * 4 + 8 * NT * D * 4 + (kWarps * 2 + 2 + kClusterShares) * 8 * NT * 4 +
-           8 * NT * 4;
+    // queries; the warps' rings, and afterwards the warps' sums (eight columns at a time) and the CTA's; statistics
+    constexpr int rings = kWarps * Ring<D>::kSteps * Ring<D>::kBytes, sums = kWarps * 8 * (D + 4) * 4 + 8 * NT * D * 4;
+    return 8 * NT * (2 * D + 16) + (rings > sums ? rings : sums) + (kWarps * 2 + 2 + kClusterShares) * 8 * NT * 4 + 8 * NT * 4;
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attention_int4_kernel(const AttnArgs a) {
+    constexpr bool FINE = std::is_same<T, __half>::value;
     constexpr int U = D / 64, TT = kStepTiles<D>, STEP = 16 * TT, COLS = 8 * NT, PITCH = 2 * D + 16, BUF = D + 4;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* const xs = smem;                                                    // [COLS] rows of PITCH bytes
-    float* const buf = reinterpret_cast<float*>(xs + COLS * PITCH);              // [kWarps][8][BUF]
-    float* const sums = buf + kWarps * 8 * BUF;                                  // [COLS][D]
-    float* const warp_m = sums + COLS * D;                                       // [kWarps][COLS]
+    float* const warp_m = reinterpret_cast<float*>(xs + COLS * PITCH);           // [kWarps][COLS]
     float* const warp_l = warp_m + kWarps * COLS;                                // [kWarps][COLS]
     float* const cta_m = warp_l + kWarps * COLS;                                 // [COLS]
     float* const cta_l = cta_m + COLS;                                           // [COLS]
     float* const weight = cta_l + COLS;                                          // [kClusterShares][COLS]
     float* const factor = weight + kClusterShares * COLS;                        // [COLS]
+    uint8_t* const rings = reinterpret_cast<uint8_t*>(factor + COLS);
+    float* const buf = reinterpret_cast<float*>(rings);                          // [kWarps][8][BUF], when the rings are done with
+    float* const sums = buf + kWarps * 8 * BUF;                                  // [COLS][D]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int share = blockIdx.x % a.shares, tile = blockIdx.x / a.shares;
@@ -121,8 +124,8 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
 #pragma unroll
         for (int d = 1; d < D / 8; d <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, d));
         const float2 f = fit_fp16<T>(big);
-        *reinterpret_cast<uint4*>(xs + col * PITCH + p * 16) = operand8<T>(v, f.y);
-        if (p == 0) factor[col] = a.scale_log2 * f.x * (1.0f / 7.0f);
+        *reinterpret_cast<uint4*>(xs + col * PITCH + p * 16) = paired8(scaled8<T>(v, a.scale_log2 < 0.0f ? -f.y : a.scale_log2 > 0.0f ? f.y : 0.0f));
+        if (p == 0) factor[col] = fabsf(a.scale_log2) * f.x * (1.0f / 7.0f);
     }
     __syncthreads();
 
@@ -140,9 +143,10 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
     }
     const bool one_head = col0 / a.T == (col0 + cols - 1) / a.T;
     const int fewest = rows_seen(one_head ? col0 % a.T : 0), most = rows_seen(one_head ? (col0 + cols - 1) % a.T : a.T - 1);
-    const int n_rows = max(0, most - start);
+    // shares begin at multiples of 16 rows, which is what aligned copies of scales need; rows before `start` are masked
+    const int origin = start & ~15, n_rows = most > start ? most - origin : 0;
     const int chunk = (n_rows + a.shares * STEP - 1) / (a.shares * STEP) * STEP;
-    const int first = start + min(n_rows, share * chunk), last = min(most, first + chunk);
+    const int first = origin + min(n_rows, share * chunk), last = min(origin + n_rows, first + chunk);
     int limit[NT][2];
     float m[NT][2], l[NT][2], fac[NT][2];
 #pragma unroll
@@ -157,58 +161,85 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
         }
     const int unmasked = min(last, fewest);
     float o[NT][4 * U][4] = {};
-    float vmax = 0x1p-110f;                               // power of two, no smaller than the scales of v so far (up to 2^127)
+    float vmax = 0x1p-110f, vscale = 0x1p124f;            // power of two, no smaller than the scales of v so far (up to 2^127); 2^14 over it
 
-    const uint8_t* const kp = a.cache.k + b * a.cache.k_batch + h * a.cache.k_head + 8 * c;
-    const uint8_t* const vp = a.cache.v + b * a.cache.v_batch + h * a.cache.v_head + 4 * g;
+    const uint8_t* const kp = a.cache.k + b * a.cache.k_batch + h * a.cache.k_head;
+    const uint8_t* const vp = a.cache.v + b * a.cache.v_batch + h * a.cache.v_head;
     const unsigned short* const ksp = static_cast<const unsigned short*>(a.cache.k_state) + b * a.cache.ks_batch + h * a.cache.ks_head;
     const unsigned short* const vsp = static_cast<const unsigned short*>(a.cache.v_state) + b * a.cache.vs_batch + h * a.cache.vs_head;
-    auto load = [&](Step<U, TT>& s, int base) {           // rows behind the last one read that one again; they are masked
+    using Slot = Ring<D>;
+    uint8_t* const ring = rings + warp * (Slot::kSteps * Slot::kBytes);
+    // One step's rows into a slot.  Rows behind the last one are that one again; they are masked.
+    auto fill = [&](uint8_t* slot, int base) {
+        constexpr int CH = D / 32;                         // 16-byte pieces of a row; 32 lanes take 32 / CH rows at a time
+        const bool whole = base + STEP <= last;
+        const int row0 = lane / CH, piece = lane % CH * 16;
+        const uint32_t to_k = (uint32_t)__cvta_generic_to_shared(slot + row0 * Slot::kPitchK + piece), to_v = (uint32_t)__cvta_generic_to_shared(slot + Slot::kV + row0 * Slot::kPitchV + piece);
+        const uint8_t *from_k = kp + (int64_t)base * (D / 2) + piece, *from_v = vp + (int64_t)base * (D / 2) + piece;
 #pragma unroll
-        for (int i = 0; i < TT; ++i) {
+        for (int i = 0; i < STEP * CH / 32; ++i) {
+            const int row = whole ? row0 + i * (32 / CH) : min(row0 + i * (32 / CH), last - 1 - base);
+            copy16(to_k + i * (32 / CH) * Slot::kPitchK, from_k + row * (D / 2));
+            copy16(to_v + i * (32 / CH) * Slot::kPitchV, from_v + row * (D / 2));
+        }
+        if (U >= 2 || (a.s_vec && whole)) {                // a row's scales (two rows' where they have one) per lane, k and v in turn
+            constexpr int BYTES = U == 4 ? 8 : 4, ROWS = BYTES / (2 * U), LANES = STEP / ROWS;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int64_t row = min(base + 16 * i + g + 8 * r, last - 1);
-#pragma unroll
-                for (int u = 0; u < U; ++u) s.k[i][r][u] = __ldg(reinterpret_cast<const uint2*>(kp + row * (D / 2) + 32 * u));
-                s.ks[i][r].load(ksp + row * U);
-                s.vs[i][r].load(vsp + row * U);
+            for (int i = lane; i < 2 * LANES; i += 32) {
+                const bool key = i < LANES;
+                const int r = (key ? i : i - LANES) * ROWS, row = whole ? r : min(r, last - 1 - base);
+                copy_some<BYTES>((uint32_t)__cvta_generic_to_shared(slot + (key ? Slot::kScalesK : Slot::kScalesV) + r * (2 * U)),
+                                 (key ? ksp : vsp) + (int64_t)(base + row) * U);
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t row = min(base + 16 * i + 2 * c + (r & 1) + 8 * (r >> 1), last - 1);
-#pragma unroll
-                for (int u = 0; u < U; ++u) s.v[i][r][u] = __ldg(reinterpret_cast<const uint32_t*>(vp + row * (D / 2) + 32 * u));
+        } else {
+            for (int r = lane; r < STEP; r += 32) {
+                const int64_t row = min(base + r, last - 1);
+                reinterpret_cast<unsigned short*>(slot + Slot::kScalesK)[r] = __ldg(ksp + row);
+                reinterpret_cast<unsigned short*>(slot + Slot::kScalesV)[r] = __ldg(vsp + row);
             }
         }
     };
+    // the scales of a row as floats
+    auto scales_of = [&](const uint8_t* at, int row, float (&out)[U]) {
+        if (U == 1) out[0] = F16Bits<T>::one(reinterpret_cast<const unsigned short*>(at)[row]);
+#pragma unroll
+        for (int i = 0; i < U / 2; ++i) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(at)[row * (U / 2) + i];
+            out[2 * i] = F16Bits<T>::lo(w);
+            out[(2 * i + 1) % U] = F16Bits<T>::hi(w);
+        }
+    };
 
-    auto multiply = [&](const Step<U, TT>& s, int base, auto masked) {
+    auto multiply = [&](const uint8_t* slot, int base, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         // ---- scores
         float p[TT][NT][4] = {};
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int i = 0; i < TT; ++i) {
+            float s0[U], s1[U];
+            scales_of(slot + Slot::kScalesK, 16 * i + g, s0);
+            scales_of(slot + Slot::kScalesK, 16 * i + g + 8, s1);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint4* x = reinterpret_cast<const uint4*>(xs + (8 * t + g) * PITCH + u * 128 + c * 32);
-                const uint4 xa = x[0], xb = x[1];
+            for (int u = 0; u < U; ++u) {
+                const uint8_t* const k = slot + (16 * i + g) * Slot::kPitchK + 32 * u + 8 * c;
+                const uint2 w0 = *reinterpret_cast<const uint2*>(k), w1 = *reinterpret_cast<const uint2*>(k + 8 * Slot::kPitchK);
+                const Codes4 r0a = unpack8<__half>(w0.x), r0b = unpack8<__half>(w0.y), r1a = unpack8<__half>(w1.x), r1b = unpack8<__half>(w1.y);
 #pragma unroll
-                for (int i = 0; i < TT; ++i) {
-                    const Codes4 r0a = unpack8(s.k[i][0][u].x), r0b = unpack8(s.k[i][0][u].y);
-                    const Codes4 r1a = unpack8(s.k[i][1][u].x), r1b = unpack8(s.k[i][1][u].y);
-                    float d[4] = {};
-                    mma_f16(d, r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa.x, xa.y);
-                    mma_f16(d, r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa.z, xa.w);
-                    mma_f16(d, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
-                    mma_f16(d, r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb.z, xb.w);
-                    const float s0 = s.ks[i][0].template get<T>(u), s1 = s.ks[i][1].template get<T>(u);
-                    p[i][t][0] = fmaf(d[0], s0, p[i][t][0]);
-                    p[i][t][1] = fmaf(d[1], s0, p[i][t][1]);
-                    p[i][t][2] = fmaf(d[2], s1, p[i][t][2]);
-                    p[i][t][3] = fmaf(d[3], s1, p[i][t][3]);
+                for (int t = 0; t < NT; ++t) {
+                    const uint4* x = reinterpret_cast<const uint4*>(xs + (8 * t + g) * PITCH + u * 128 + c * 32);
+                    const uint4 xa = x[0], xb = x[1];
+                    float d[4];
+                    mma16_first<__half>(d, r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa.x, xa.y);
+                    mma16<__half>(d, r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa.z, xa.w);
+                    mma16<__half>(d, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
+                    mma16<__half>(d, r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb.z, xb.w);
+                    p[i][t][0] = fmaf(d[0], s0[u], p[i][t][0]);
+                    p[i][t][1] = fmaf(d[1], s0[u], p[i][t][1]);
+                    p[i][t][2] = fmaf(d[2], s1[u], p[i][t][2]);
+                    p[i][t][3] = fmaf(d[3], s1[u], p[i][t][3]);
                 }
             }
+        }
         // ---- softmax: running maximum and sum of every column
         bool grown = false;
         float alpha[NT][2];
@@ -222,15 +253,15 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         float& x = p[i][t][2 * r + j];
-                        x *= fac[t][j];
-                        if (MASKED && base + 16 * i + g + 8 * r >= limit[t][j]) x = -INFINITY;
+                        if (MASKED && (base + 16 * i + g + 8 * r >= limit[t][j] || base + 16 * i + g + 8 * r < start)) x = -INFINITY;
                         top = fmaxf(top, x);
                     }
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                 const float now = fmaxf(m[t][j], top);
-                const float ref = MASKED && now == -INFINITY ? 0.0f : now;      // a column that has seen nothing yet
-                alpha[t][j] = exp2_fast(m[t][j] - ref);
+                // scores are the products without the column's factor, which is not negative; a column may have seen nothing yet
+                const float ref = MASKED && now == -INFINITY ? 0.0f : now * fac[t][j];
+                alpha[t][j] = exp2_fast(fmaf(m[t][j], fac[t][j], -ref));
                 grown = grown || now != m[t][j];
                 m[t][j] = now;
                 float sum = 0.0f;
@@ -239,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         float& x = p[i][t][2 * r + j];
-                        x = exp2_fast(x - ref);
+                        x = exp2_fast(fmaf(x, fac[t][j], -ref));
                         sum += x;
                     }
                 l[t][j] = fmaf(l[t][j], alpha[t][j], sum);
@@ -249,23 +280,23 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
 #pragma unroll
         for (int i = 0; i < TT; ++i)
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < 2; ++r) {
+                scales_of(slot + Slot::kScalesV, 16 * i + g + 8 * r, vs[i][r]);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    vs[i][r][u] = s.vs[i][r].template get<T>(u);
-                    big = fmaxf(big, vs[i][r][u]);
-                }
-        float shrink = 1.0f;
-        if (__any_sync(0xffffffffu, big > vmax && vmax < 0x1p127f)) {
+                for (int u = 0; u < U; ++u) big = fmaxf(big, vs[i][r][u]);       // passes over the NaN of blocks that hold one
+            }
+        if (__any_sync(0xffffffffu, grown || big > vmax)) {
+            float top = big;
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-            const uint32_t e = min((__float_as_uint(big) >> 23) + 1u, 254u);
-            const float next = __uint_as_float(e << 23);
-            shrink = vmax / next;
-            vmax = next;
-            grown = true;
-        }
-        if (__any_sync(0xffffffffu, grown)) {
+            for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            float shrink = 1.0f;
+            if (top > vmax && vmax < 0x1p127f) {
+                const uint32_t e = min((__float_as_uint(top) >> 23) + 1u, 254u);
+                const float next = __uint_as_float(e << 23);
+                shrink = vmax / next;
+                vmax = next;
+                vscale = 0x1p14f / next;
+            }
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -273,7 +304,6 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[t][w][j] *= alpha[t][j & 1] * shrink;
         }
-        const float vscale = 0x1p14f / vmax;
         // ---- O += V^T P
 #pragma unroll
         for (int i = 0; i < TT; ++i)
@@ -289,44 +319,52 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
                         float x0 = p[i][t][2 * r] * sc, x1 = p[i][t][2 * r + 1] * sc;
                         if (MASKED) {                     // a masked row's scale may be anything
                             const int row = base + 16 * i + g + 8 * r;
-                            if (row >= limit[t][0]) x0 = 0.0f;
-                            if (row >= limit[t][1]) x1 = 0.0f;
+                            if (row >= limit[t][0] || row < start) x0 = 0.0f;
+                            if (row >= limit[t][1] || row < start) x1 = 0.0f;
                         }
                         const uint32_t hi = pack_f16x2(x0, x1);
                         using H = F16Bits<__half>;
                         bh[t][r] = transpose8x8(hi);
-                        bl[t][r] = transpose8x8(pack_f16x2(x0 - H::lo(hi), x1 - H::hi(hi)));
+                        if (FINE) bl[t][r] = transpose8x8(pack_f16x2(x0 - H::lo(hi), x1 - H::hi(hi)));
                     }
+                const uint8_t* const v = slot + Slot::kV + (16 * i + 2 * c) * Slot::kPitchV + 32 * u + 4 * g;
+                uint32_t w[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) w[r] = *reinterpret_cast<const uint32_t*>(v + ((r & 1) + 8 * (r >> 1)) * Slot::kPitchV);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     // four codes of two rows: nibble n of both in bits 4n and 16 + 4n
-                    const uint32_t w01 = __byte_perm(s.v[i][0][u], s.v[i][1][u], half ? 0x7632 : 0x5410);
-                    const uint32_t w23 = __byte_perm(s.v[i][2][u], s.v[i][3][u], half ? 0x7632 : 0x5410);
+                    const uint32_t w01 = __byte_perm(w[0], w[1], half ? 0x7632 : 0x5410);
+                    const uint32_t w23 = __byte_perm(w[2], w[3], half ? 0x7632 : 0x5410);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const uint32_t x = w01 >> (8 * j), y = w23 >> (8 * j);
-                        const uint32_t a0 = codes_low(x), a1 = codes_high(x), a2 = codes_low(y), a3 = codes_high(y);
+                        const uint32_t a0 = half2_low(x), a1 = half2_high(x), a2 = half2_low(y), a3 = half2_high(y);
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            mma_f16(o[t][4 * u + 2 * half + j], a0, a1, a2, a3, bh[t][0], bh[t][1]);
-                            mma_f16(o[t][4 * u + 2 * half + j], a0, a1, a2, a3, bl[t][0], bl[t][1]);
+                            mma16<__half>(o[t][4 * u + 2 * half + j], a0, a1, a2, a3, bh[t][0], bh[t][1]);
+                            if (FINE) mma16<__half>(o[t][4 * u + 2 * half + j], a0, a1, a2, a3, bl[t][0], bl[t][1]);
                         }
                     }
                 }
             }
     };
 
-    {
-        Step<U, TT> cur, nxt;
-        int base = first + warp * STEP;
-        if (base < last) load(cur, base);
-        for (; base < last; base += kWarps * STEP) {
-            if (base + kWarps * STEP < last) load(nxt, base + kWarps * STEP);
-            if (base + STEP <= unmasked) multiply(cur, base, std::false_type{});
-            else multiply(cur, base, std::true_type{});
-            cur = nxt;
-        }
+    int slot = 0;
+    if (first + warp * STEP < last) fill(ring, first + warp * STEP);
+    commit_copies();
+    for (int base = first + warp * STEP; base < last; base += kWarps * STEP) {
+        const int next = base + kWarps * STEP;
+        if (next < last) fill(ring + (slot ^ 1) * Slot::kBytes, next);
+        commit_copies();
+        wait_copies<1>();
+        __syncwarp();
+        if (base >= start && base + STEP <= unmasked) multiply(ring + slot * Slot::kBytes, base, std::false_type{});
+        else multiply(ring + slot * Slot::kBytes, base, std::true_type{});
+        __syncwarp();
+        slot ^= 1;
     }
+    wait_copies<0>();
 
     // ---- the warps' results into one
 #pragma unroll
@@ -336,7 +374,7 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l[t][j] += __shfl_xor_sync(0xffffffffu, l[t][j], d);
             if (g == 0) {
-                warp_m[warp * COLS + 8 * t + 2 * c + j] = m[t][j];
+                warp_m[warp * COLS + 8 * t + 2 * c + j] = m[t][j] == -INFINITY ? -INFINITY : m[t][j] * fac[t][j];      // log2 units
                 warp_l[warp * COLS + 8 * t + 2 * c + j] = l[t][j];
             }
         }
@@ -350,20 +388,19 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
         cta_l[col] = total;
     }
     __syncthreads();
-    const float unit = vmax * (0x1p-14f / 7.0f);
+    const float unit = vmax * (0x1p-14f / 7.0f);          // (every warp has left its ring)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int col = 2 * c + j;
-            const float w = m[t][j] == -INFINITY ? 0.0f : exp2_fast(m[t][j] - cta_m[8 * t + col]) * unit;
+            const float w = m[t][j] == -INFINITY ? 0.0f : exp2_fast(m[t][j] * fac[t][j] - cta_m[8 * t + col]) * unit;
             float* dst = buf + (warp * 8 + col) * BUF + 8 * g;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float x = w, y = w * 0.0625f;                  // the odd ones are 16 times too large
-                *reinterpret_cast<float4*>(dst + 64 * u) = make_float4(o[t][4 * u][j] * x, o[t][4 * u][2 + j] * y, o[t][4 * u + 1][j] * x, o[t][4 * u + 1][2 + j] * y);
+                *reinterpret_cast<float4*>(dst + 64 * u) = make_float4(o[t][4 * u][j] * w, o[t][4 * u][2 + j] * w, o[t][4 * u + 1][j] * w, o[t][4 * u + 1][2 + j] * w);
                 *reinterpret_cast<float4*>(dst + 64 * u + 4) =
-                    make_float4(o[t][4 * u + 2][j] * x, o[t][4 * u + 2][2 + j] * y, o[t][4 * u + 3][j] * x, o[t][4 * u + 3][2 + j] * y);
+                    make_float4(o[t][4 * u + 2][j] * w, o[t][4 * u + 2][2 + j] * w, o[t][4 * u + 3][j] * w, o[t][4 * u + 3][2 + j] * w);
             }
         }
         __syncthreads();
@@ -425,12 +462,16 @@ __global__ void __launch_bounds__(kThreads) attention_int4_kernel(const AttnArgs
     for (int i = share * part + threadIdx.x; i < min(pairs, (share + 1) * part); i += kThreads) {
         const int col = i / (D / 2), d = i % (D / 2) * 2;
         float x = 0.0f, y = 0.0f;
-        for (int r = 0; r < a.shares; ++r) {
-            const float w = weight[r * COLS + col];
-            const float2 v = *reinterpret_cast<const float2*>(cluster.map_shared_rank(sums, r) + col * D + d);
-            x = fmaf(v.x, w, x);
-            y = fmaf(v.y, w, y);
-        }
+        float2 v[kClusterShares];
+#pragma unroll
+        for (int r = 0; r < kClusterShares; ++r)
+            if (r < a.shares) v[r] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(sums, r) + col * D + d);
+#pragma unroll
+        for (int r = 0; r < kClusterShares; ++r)
+            if (r < a.shares) {
+                x = fmaf(v[r].x, weight[r * COLS + col], x);
+                y = fmaf(v[r].y, weight[r * COLS + col], y);
+            }
         store(col, d, x, y);
     }
     cluster.sync();                                       // the others read this CTA's sums
@@ -471,21 +512,16 @@ __global__ void __launch_bounds__(D) attention_int4_join_kernel(const AttnArgs a
     __syncthreads();
     const float* src = a.ws + (cta0 * COLS + col) * D + threadIdx.x;
     float x = 0.0f;
-    for (int k = 0; k < a.shares; ++k) x = fmaf(src[(int64_t)k * COLS * D], weight[k], x);
+    for (int k0 = 0; k0 < a.shares; k0 += 16) {
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = k0 + k < a.shares ? src[(int64_t)(k0 + k) * COLS * D] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            if (k0 + k < a.shares) x = fmaf(v[k], weight[k0 + k], x);
+    }
     const int64_t at = (((int64_t)b * a.Hq + h * a.G + r / a.T) * a.T + r % a.T) * D + threadIdx.x;
     static_cast<unsigned short*>(a.out)[at] = (unsigned short)F16Bits<T>::pack(x, 0.0f);
-}
-
-int sm_count() {
-    static int sms[64] = {0};
-    int dev = 0;
-    if (current_device(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (sms[dev] == 0) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
-        sms[dev] = n;
-    }
-    return sms[dev];
 }
 
 struct Plan {
@@ -500,7 +536,8 @@ Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     p.tiles = B * Hkv * p.col_tiles;
     // Three CTAs an SM, as long as a warp of a full cache has two steps; the clusters' sizes are powers of two.
     const int64_t step = 16 * (D == 64 ? kStepTiles<64> : D == 128 ? kStepTiles<128> : kStepTiles<256>);
-    const int64_t useful = (max_len + 2 * kWarps * step - 1) / (2 * kWarps * step), want = (3 * sm_count() + p.tiles - 1) / p.tiles;
+    const int64_t useful = (max_len + 2 * kWarps * step - 1) / (2 * kWarps * step);
+    int64_t want = (p.nt == 1 && D <= 128 ? 4 : 2) * sm_count() / p.tiles;
     int64_t s = useful < want ? useful : want;
     if (s > kMaxShares) s = kMaxShares;
     if (s <= kClusterShares) {
@@ -569,6 +606,8 @@ int launch_attention_int4(const void* q, int dt, int64_t q_batch, int64_t q_head
     a.G = (int)(Hq / Hkv);
     a.col_tiles = p.col_tiles;
     a.shares = p.shares;
+    a.s_vec = aligned(cache->k_state, 4) && aligned(cache->v_state, 4) && cache->ks_batch % 2 == 0 && cache->ks_head % 2 == 0 && cache->vs_batch % 2 == 0 &&
+              cache->vs_head % 2 == 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     auto go = [&](auto* tag) {
         using E = std::remove_pointer_t<decltype(tag)>;

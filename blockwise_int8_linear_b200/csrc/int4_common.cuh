@@ -7,6 +7,8 @@
 
 #include "bi8_common.cuh"
 
+#include <type_traits>
+
 namespace bi8 {
 
 constexpr float kInv7 = 1.0f / 7.0f;
@@ -83,48 +85,103 @@ __device__ __forceinline__ float value_of(float s, uint32_t code, bool plain) {
 __device__ __forceinline__ bool plain_scale(float s) { return (s > 0x1p-100f && s < 0x1p120f) || s == 0.0f; }
 
 // ---- tensor-core operands -----------------------------------------------------------------------------------------------------
-// Codes become fp16 operands in pairs: four bits c + 8 under the exponent of 1024 are 1024 + 8 + c, four bits further up 1024 + 16 (8 + c);
-// less 1032 and 1152 that is c and 16 c, exactly.  Eight codes are one shift, four AND-ORs and four packed subtractions.  (The four bits
-// alone are fp16 denormals, (8 + c) 2^-24, which need neither the OR nor the subtraction; but the matrix instruction aligns its sums by the
-// operands' exponent fields, and ten leading zeros in one operand cost the sum as many bits: measured 2^-16 of the largest term.)  The
-// other operand is scaled by a power of two to fit fp16, which keeps everything of a bf16 value that is 2^-28 or more of the largest
-// one, and the values that meet the higher codes by 1/16.
+// Codes become the matrix instruction's operands in pairs, as the numbers -7 to 7 in the other operand's type.  Four bits c + 8 under the
+// exponent of 1024 are the fp16 number 1024 + 8 + c, four bits further up 1024 + 16 (8 + c); a packed subtraction or multiply-add
+// makes c of them, exactly: eight codes are one shift, four AND-ORs and four packed operations.  bf16 has 128 + 8 + c, and no room for four
+// bits further up: two shifts more.  (The four bits alone are fp16 denormals, (8 + c) 2^-24, and the offset could be left to the
+// accumulator's start value, which saves half of that.  But the instruction aligns its sums by the operands' exponent fields, and ten
+// leading zeros in one operand cost the sum as many bits: measured, 2^-16 of the largest term.)
 //
-// Order of a word's eight codes in the contraction: pairs (0,4), (1,5), (2,6), (3,7); 1, 3, 5 and 7 sit four bits higher.
-__device__ __forceinline__ uint32_t minus2(uint32_t v, uint32_t k) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&k));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t codes_low(uint32_t w) { return minus2((w & 0x000f000fu) | 0x64006400u, 0x64086408u); }
-__device__ __forceinline__ uint32_t codes_high(uint32_t w) { return minus2((w & 0x00f000f0u) | 0x64006400u, 0x64806480u); }
+// Order of a word's eight codes in the contraction: pairs (0,4), (1,5), (2,6), (3,7).
 struct Codes4 {
     uint32_t p04, p15, p26, p37;
 };
-__device__ __forceinline__ Codes4 unpack8(uint32_t w) { return {codes_low(w), codes_high(w), codes_low(w >> 8), codes_high(w >> 8)}; }
-// 2^e with |x| < 2^15 for x = max / 2^e (m: the bits of max in T), as the pair (2^e, 2^-e)
-template <typename T>
-__device__ __forceinline__ float2 fit_fp16(uint32_t m) {
-    if (m == 0u || m >= F16Bits<T>::kInf) return make_float2(1.0f, 1.0f);
-    const float a = F16Bits<T>::one(m);
-    // a bf16 denormal is an fp32 denormal: exponent field 0, treated as 2^-126
-    int e = max((int)(__float_as_uint(a) >> 23), 1) - 127 - 14;
-    e = max(e, -126 + 14);
-    return make_float2(__uint_as_float((uint32_t)(e + 127) << 23), __uint_as_float((uint32_t)(127 - e) << 23));
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t set) {      // (w & mask) | set, as one instruction
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(set));
+    return r;
 }
-// Eight values as the operand that meets a word of codes: scaled, in the pairs above, odd ones by 1/16.
+__device__ __forceinline__ uint32_t half2_low(uint32_t w) {
+    const uint32_t v = and_or(w, 0x000f000fu, 0x64006400u), k = 0x64086408u;             // 1024 + 8 + c, 1032
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&k));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t half2_high(uint32_t w) {
+    const uint32_t v = and_or(w, 0x00f000f0u, 0x64006400u), m = 0x2c002c00u, k = 0xd480d480u;  // 1024 + 16 (8 + c), 1/16, -72
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&k));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t bf162_low(uint32_t w) {
+    const uint32_t v = and_or(w, 0x000f000fu, 0x43004300u), k = 0x43084308u;             // 128 + 8 + c, 136
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&k));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 template <typename T>
-__device__ __forceinline__ uint4 operand8(const uint4& v, float inv) {
-    using H = F16Bits<T>;
-    const float odd = inv * 0.0625f;
-    return make_uint4(pack_f16x2(H::lo(v.x) * inv, H::lo(v.z) * inv), pack_f16x2(H::hi(v.x) * odd, H::hi(v.z) * odd),
-                      pack_f16x2(H::lo(v.y) * inv, H::lo(v.w) * inv), pack_f16x2(H::hi(v.y) * odd, H::hi(v.w) * odd));
+__device__ __forceinline__ Codes4 unpack8(uint32_t w);
+template <>
+__device__ __forceinline__ Codes4 unpack8<__half>(uint32_t w) {
+    return {half2_low(w), half2_high(w), half2_low(w >> 8), half2_high(w >> 8)};
+}
+template <>
+__device__ __forceinline__ Codes4 unpack8<__nv_bfloat16>(uint32_t w) {
+    return {bf162_low(w), bf162_low(w >> 4), bf162_low(w >> 8), bf162_low(w >> 12)};
+}
+// Eight neighbouring 16-bit values in that order.
+__device__ __forceinline__ uint4 paired8(const uint4& v) {
+    return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
 }
 
-// D += A B, A 16 x 16 (rows g and g + 8 of lane 4 g + c, columns 2c, 2c+1 and 2c+8, 2c+9), B 16 x 8 (column g), D 16 x 8 (columns 2c, 2c+1)
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// D = C + A B, A 16 x 16 (rows g and g + 8 of lane 4 g + c, columns 2c, 2c+1 and 2c+8, 2c+9), B 16 x 8 (column g), C and D 16 x 8 (columns
+// 2c, 2c+1)
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1,
+                                      float c2, float c3) {
+    if (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {      // D += A B
+    mma16<T>(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
+}
+template <typename T>
+__device__ __forceinline__ void mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {      // D = A B
+    mma16<T>(d, a0, a1, a2, a3, b0, b1, 0.0f, 0.0f, 0.0f, 0.0f);
+}
+
+// ---- asynchronous copies into shared memory ----------------------------------------------------------------------------------
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {      // bytes read; the rest of the 16 is zero
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_some(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+// SMs of the current device.
+inline int sm_count() {
+    static int sms[64] = {0};
+    int dev = 0;
+    if (current_device(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (sms[dev] == 0) {
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
+        sms[dev] = n;
+    }
+    return sms[dev];
 }
 
 }  // namespace bi8

@@ -9,12 +9,12 @@
 // A warp takes 16 rows of W and strides over K in pieces of 256 (128 bytes a row; lane 4g + c reads 8 bytes of rows g and g + 8 for every 64
 // values), the next piece's loads in flight while this one is multiplied.  A CTA is eight warps, over rows and over K; CTAs of a
 // cluster share the rows and divide K once more, and add what they have over distributed shared memory in rank order: no
-// workspace, no atomics, the same bits on every call.  x comes through shared memory as fp16 with a power of two
-// per row and 64 (32) values.
+// workspace, no atomics, the same bits on every call.  x comes through shared memory, in the order of the codes.
 #include "int4_common.cuh"
 
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <type_traits>
 
 namespace bi8 {
@@ -22,9 +22,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kPiece = 256;                  // values of K that a warp takes at a time
-constexpr int kMaxStage = 160 * 1024;        // shared memory for x
+constexpr int kSmemSM = 227 * 1024;          // shared memory that an SM's CTAs have
 
 struct MatmulArgs {
     const void* x;
@@ -39,12 +39,12 @@ struct MatmulArgs {
     void* C;
     int64_t ldc;
     int bias_dtype, out_dtype;
-    int M, N;
-    int64_t K;
-    int shift;               // log2 of the block
+    int M, N, K;
+    int tiles;               // of 16 * warps_n rows of W
     int warps_n;             // warps of a CTA over rows of W; the others divide K
     int pieces;              // of K
-    int pieces_cta;          // a cluster rank's share
+    int ranks;               // CTAs of a cluster
+    int pieces_cta;          // a CTA's share
     int pieces_stage;        // as many of them as x has room for
     bool x_vec, w_vec, s_vec;
 };
@@ -70,262 +70,364 @@ __device__ __forceinline__ uint32_t load_word(const uint8_t* p, const uint8_t* e
     return __funnelshift_r(lo, hi, (uint32_t)(a & 3u) * 8u);
 }
 
-// One piece of 16 rows as a lane holds it: for each 64 values two words of row g and two of row g + 8, and the rows' scales.
-struct Piece {
-    uint2 w[2][4];
-    uint32_t s[2][4];        // bits of the scale of each 64 values (SHORT: of both halves)
-};
+// A warp's ring of pieces in shared memory: 16 rows of 128 bytes of codes, 32 bytes apart modulo 128 (the eight bytes that the lanes of
+// four rows read are in different banks), then the rows' scales.
+constexpr int kCodePitch = kPiece / 2 + 32;
+template <int BLOCK>
+constexpr int kPieceBytes = 16 * kCodePitch + 16 * (kPiece / BLOCK) * 2;
 
-// SHORT: blocks of 32, a lane's two words of 64 values lie in the two blocks; else the eight bytes lie in one.
-// VEC: code rows begin on 8-byte boundaries.
-template <bool SHORT, bool VEC>
-__device__ __forceinline__ void load_piece(Piece& p, const MatmulArgs& a, const uint8_t* const (&row)[2], const unsigned short* const (&srow)[2],
-                                           int piece, int c) {
-    const int64_t kb = (a.K + 1) / 2, at = (int64_t)piece * (kPiece / 2);
-    const bool full = at + kPiece / 2 <= kb;
+// One piece of 16 rows from `n0` on into shared memory.  Rows behind the last one are read as the last one (and not stored); codes behind a
+// row's end are zero bytes, scales whatever (x is zero there).
+template <int BLOCK>
+__device__ __forceinline__ void fill(uint8_t* dst, const MatmulArgs& a, int n0, int piece, int lane) {
+    constexpr int PER = kPiece / BLOCK;
+    const int64_t at = (int64_t)piece * (kPiece / 2) + 16 * (lane & 7), kb = ((int64_t)a.K + 1) / 2;
+    const int room = (int)max((int64_t)0, min((int64_t)16, kb - at));
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int64_t o = at + 32 * u + (SHORT ? 4 : 8) * c;
-            if (VEC && !SHORT) {
-                p.w[r][u] = make_uint2(0u, 0u);
-                if (full || o < kb) p.w[r][u] = __ldg(reinterpret_cast<const uint2*>(row[r] + o));
-            } else if (VEC) {
-                p.w[r][u] = make_uint2(0u, 0u);
-                if (full || o < kb) p.w[r][u].x = __ldg(reinterpret_cast<const uint32_t*>(row[r] + o));
-                if (full || o + 16 < kb) p.w[r][u].y = __ldg(reinterpret_cast<const uint32_t*>(row[r] + o + 16));
-            } else {
-                p.w[r][u] = make_uint2(load_word(row[r] + o, row[r] + kb), load_word(row[r] + o + (SHORT ? 16 : 4), row[r] + kb));
-            }
+    for (int i = 0; i < 4; ++i) {
+        const int row = (lane >> 3) + 4 * i;
+        const uint8_t* src = a.W + (int64_t)min(n0 + row, a.N - 1) * a.ldw;
+        uint8_t* to = dst + row * kCodePitch + 16 * (lane & 7);
+        if (a.w_vec) {
+            copy16((uint32_t)__cvta_generic_to_shared(to), room > 0 ? src + at : src, room);
+        } else {
+            const uint8_t *from = src + at, *end = src + kb;
+            *reinterpret_cast<uint4*>(to) = make_uint4(load_word(from, end), load_word(from + 4, end), load_word(from + 8, end), load_word(from + 12, end));
         }
-        // scales: four, two or eight neighbouring ones
-        const int64_t j = (int64_t)piece * kPiece >> a.shift;
-        if (a.s_vec && full) {
-            if (SHORT) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(srow[r] + j));
-                p.s[r][0] = v.x, p.s[r][1] = v.y, p.s[r][2] = v.z, p.s[r][3] = v.w;
-            } else if (a.shift == 6) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(srow[r] + j));
-                p.s[r][0] = v.x & 0xffffu, p.s[r][1] = v.x >> 16, p.s[r][2] = v.y & 0xffffu, p.s[r][3] = v.y >> 16;
-            } else {
-                const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(srow[r] + j));
-                p.s[r][0] = p.s[r][1] = v & 0xffffu, p.s[r][2] = p.s[r][3] = v >> 16;
-            }
+    }
+    if (lane < 16) {
+        const int64_t j = (int64_t)piece * PER;
+        const unsigned short* src = a.sW + (int64_t)min(n0 + lane, a.N - 1) * a.blocks + j;
+        uint8_t* to = dst + 16 * kCodePitch + lane * (2 * PER);
+        if (a.s_vec && j + PER <= a.blocks) {
+            copy_some<2 * PER>((uint32_t)__cvta_generic_to_shared(to), src);
         } else {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int64_t i = ((int64_t)piece * kPiece + 64 * u) >> a.shift;
-                uint32_t v = i < a.blocks ? (uint32_t)__ldg(srow[r] + i) : 0u;
-                if (SHORT && i + 1 < a.blocks) v |= (uint32_t)__ldg(srow[r] + i + 1) << 16;
-                p.s[r][u] = v;
-            }
+            for (int i = 0; i < PER; ++i) reinterpret_cast<unsigned short*>(to)[i] = j + i < a.blocks ? __ldg(src + i) : (unsigned short)0;
         }
     }
 }
 
-template <typename T, bool SHORT, int NT, bool VEC>
-__global__ void __launch_bounds__(kThreads) matmul_int4_kernel(const MatmulArgs a) {
-    constexpr int SEG = SHORT ? 32 : 64;     // values under one power of two of x
-    constexpr int COLS = 8 * NT;
+// Pieces of a warp in shared memory: one in use, the others on their way.
+template <int NT>
+constexpr int kRing = NT <= 2 ? 3 : 2;
+
+// Sizes in shared memory: the warps' rings, x, and the sums of the warps that share rows with the CTA's own behind them.  Up to 16 columns
+// have those twice: one tile's are read while the next one's are written.
+template <int BLOCK, int NT>
+constexpr int kRingBytes = kWarps * kRing<NT> * kPieceBytes<BLOCK>;
+template <int NT>
+constexpr int kSumBuffers = NT <= 2 ? 2 : 1;
+inline __host__ __device__ int x_pitch(int pieces) { return pieces * kPiece * 2 + 16; }
+inline __host__ __device__ int sum_parts(int warps_k) { return warps_k == 1 ? 1 : warps_k + 1; }
+
+template <typename T, int BLOCK, int NT>
+__global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulArgs a) {
+    constexpr int COLS = 8 * NT, PER = kPiece / BLOCK, RING = kRing<NT>;
     extern __shared__ __align__(16) uint8_t smem[];
     const cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int ranks = a.ranks, rank = (int)(blockIdx.x % ranks);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int warps_k = kWarps / a.warps_n, wn = warp % a.warps_n, wk = warp / a.warps_n;
+    const int warps_k = kWarps / a.warps_n, wn = warp % a.warps_n, wk = warp / a.warps_n, rows_cta = 16 * a.warps_n;
     const int m0 = blockIdx.y * COLS, rows_x = min(COLS, a.M - m0);
-    const int n0 = (int)(blockIdx.x / ranks) * 16 * a.warps_n + 16 * wn;
     const int first = rank * a.pieces_cta, last = min(a.pieces, first + a.pieces_cta);
-    const int stage = a.pieces_stage;
-    // x: rows of `stage` pieces, 16 bytes apart modulo 128, so that the lanes of two rows read different banks; then the power of two of
-    // every segment and column
-    const int pitch = stage * kPiece * 2 + 16;
-    uint8_t* const xs = smem;
-    float* const seg = reinterpret_cast<float*>(smem + (size_t)rows_x * pitch);
+    const int tile_step = (int)(gridDim.x / ranks), tile0 = (int)(blockIdx.x / ranks);
+    uint8_t* const ring = smem + warp * (RING * kPieceBytes<BLOCK>);
+    // x: rows 16 bytes apart modulo 128, so that the lanes of two rows read different banks
+    const int pitch = x_pitch(a.pieces_stage);
+    uint8_t* const xs = smem + kRingBytes<BLOCK, NT>;
+    const int sums = rows_x * rows_cta;
+    float* const part = reinterpret_cast<float*>(xs + rows_x * pitch);       // [buffer][part][rows_x][rows_cta]
 
-    after_predecessor();
-    const uint8_t* row[2];
-    const unsigned short* srow[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int64_t n = min(n0 + g + 8 * r, a.N - 1);       // rows behind the last one read it again and are not stored
-        row[r] = a.W + n * a.ldw;
-        srow[r] = a.sW + n * a.blocks;
-    }
-    float y[NT][4] = {};
-    Piece cur, nxt;
-    int piece = first + wk;
-    if (piece < last) load_piece<SHORT, VEC>(cur, a, row, srow, piece, c);
-
-    for (int base = first; base < last; base += stage) {
-        const int end = min(last, base + stage);
-        if (base > first) __syncthreads();
-        // ---- x into shared memory: a thread takes eight values, SEG / 8 lanes a segment
+    // x of pieces base to end: as copies into the slots that the lanes read (lane c reads 32 bytes of every 64 values: what meets its two
+    // words of codes; with blocks of 32, of both halves), then, by the thread that copied them, into the order of the codes.
+    auto each_eight = [&](int base, int end, auto body) {
+        if (base >= end) return;                              // a rank behind the last piece
         const int per_row = (end - base) * (kPiece / 8);
-        for (int i = threadIdx.x; i < rows_x * per_row; i += kThreads) {       // per_row is a multiple of 32: whole warps
-            const int m = i / per_row, p = i - m * per_row;
-            const int64_t k = (int64_t)base * kPiece + 8 * p;
-            const unsigned short* src = static_cast<const unsigned short*>(a.x) + (int64_t)(m0 + m) * a.ldx + k;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (a.x_vec && k + 8 <= a.K) {
-                v = __ldg(reinterpret_cast<const uint4*>(src));
-            } else if (k < a.K) {
+        int m = 0, p = threadIdx.x;
+        while (true) {
+            while (p >= per_row) p -= per_row, ++m;
+            if (m >= rows_x) break;
+            const int i = p & 7, slot = BLOCK == 32 ? (i & 3) * 2 + (i >> 2) : i;
+            body(m, base * kPiece + 8 * p, xs + m * pitch + (p >> 3) * 128 + slot * 16);
+            p += kThreads;
+        }
+    };
+    auto fetch_x = [&](int base, int end) {
+        each_eight(base, end, [&](int m, int k, uint8_t* to) {
+            const unsigned short* src = static_cast<const unsigned short*>(a.x) + (int64_t)(m0 + m) * a.ldx;
+            const int room = max(0, min(8, a.K - k));
+            if (a.x_vec) {
+                copy16((uint32_t)__cvta_generic_to_shared(to), room > 0 ? src + k : src, 2 * room);
+            } else {
                 uint32_t e[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) e[j] = k + j < a.K ? __ldg(src + j) : 0u;
-                v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+                for (int j = 0; j < 8; ++j) e[j] = j < room ? __ldg(src + k + j) : 0u;
+                *reinterpret_cast<uint4*>(to) = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
             }
-            uint32_t big = absmax8(v);
-#pragma unroll
-            for (int d = 1; d < SEG / 8; d <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, d));
-            const float2 f = fit_fp16<T>(big);
-            const uint4 o = operand8<T>(v, f.y);
-            // lane c of a warp reads 32 bytes of every 64 values: what meets its two words of codes
-            const int in = p & 7, slot = SHORT ? (in & 3) * 2 + (in >> 2) : in;
-            *reinterpret_cast<uint4*>(xs + (size_t)m * pitch + (p >> 3) * 128 + slot * 16) = o;
-            if ((p & (SEG / 8 - 1)) == 0) seg[(p / (SEG / 8)) * COLS + m] = f.x;
-        }
-        const int segs = (end - base) * (kPiece / SEG);
-        if (rows_x < COLS)
-            for (int i = threadIdx.x; i < segs * (COLS - rows_x); i += kThreads)
-                seg[i / (COLS - rows_x) * COLS + rows_x + i % (COLS - rows_x)] = 0.0f;
-        __syncthreads();
+        });
+    };
+    auto order_x = [&](int base, int end) {
+        each_eight(base, end, [&](int, int, uint8_t* at) {
+            uint4* p = reinterpret_cast<uint4*>(at);
+            *p = paired8(*p);
+        });
+    };
 
-        // ---- this warp's pieces
-        for (; piece < end; piece += warps_k) {
-            const int next = piece + warps_k;
-            if (next < last) load_piece<SHORT, VEC>(nxt, a, row, srow, next, c);
-            const int u0 = (piece - base) * 4;
+    after_predecessor();
+    const bool once = a.pieces_cta <= a.pieces_stage;         // all of this CTA's x fits
+    if (once) fetch_x(first, last);
+    commit_copies();
+    int f_tile = tile0, f_piece = first + wk, in = 0, out = 0;          // what is filled next, and where
+    // this lane's part of a piece of whole rows: 16 bytes of every fourth row, a row's scales
+    const int64_t lane_codes = (int64_t)(lane >> 3) * a.ldw + 16 * (lane & 7), lane_scales = (int64_t)(lane & 15) * a.blocks;
+    const int inside = a.w_vec && a.s_vec ? a.K / kPiece : 0;          // pieces below are whole and aligned
+    auto fill_next = [&] {
+        if (f_piece >= last) f_piece = first + wk, f_tile += tile_step;
+        if (f_tile < a.tiles && f_piece < last) {
+            const int n0 = f_tile * rows_cta + 16 * wn;
+            uint8_t* const dst = ring + in * kPieceBytes<BLOCK>;
+            if (f_piece < inside && n0 + 16 <= a.N) {
+                const uint8_t* src = a.W + ((int64_t)n0 * a.ldw + (int64_t)f_piece * (kPiece / 2)) + lane_codes;
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + (lane >> 3) * kCodePitch + 16 * (lane & 7));
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const Codes4 r0a = unpack8(cur.w[0][u].x), r0b = unpack8(cur.w[0][u].y);
-                const Codes4 r1a = unpack8(cur.w[1][u].x), r1b = unpack8(cur.w[1][u].y);
+                for (int i = 0; i < 4; ++i) copy16(to + 4 * i * kCodePitch, src + (int64_t)(4 * i) * a.ldw);
+                if (lane < 16)
+                    copy_some<2 * PER>((uint32_t)__cvta_generic_to_shared(dst + 16 * kCodePitch + lane * (2 * PER)),
+                                       a.sW + ((int64_t)n0 * a.blocks + (int64_t)f_piece * PER) + lane_scales);
+            } else {
+                fill<BLOCK>(dst, a, n0, f_piece, lane);
+            }
+        }
+        commit_copies();
+        f_piece += warps_k;
+        in = in + 1 == RING ? 0 : in + 1;
+    };
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    uint4 xa = make_uint4(0u, 0u, 0u, 0u), xb = xa;
-                    if (8 * t + g < rows_x) {
-                        const uint4* p = reinterpret_cast<const uint4*>(xs + (size_t)(8 * t + g) * pitch + (u0 + u) * 128 + c * 32);
-                        xa = p[0];
-                        xb = p[1];
-                    }
-                    const float* sp = seg + (size_t)(u0 + u) * (64 / SEG) * COLS + 8 * t + 2 * c;
-                    const float2 f = *reinterpret_cast<const float2*>(sp);
-                    float d[4] = {};
-                    mma_f16(d, r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa.x, xa.y);
-                    mma_f16(d, r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa.z, xa.w);
-                    if (SHORT) {
-                        const float s0 = F16Bits<T>::one(cur.s[0][u] & 0xffffu), s1 = F16Bits<T>::one(cur.s[1][u] & 0xffffu);
-                        y[t][0] = fmaf(d[0], s0 * f.x, y[t][0]);
-                        y[t][1] = fmaf(d[1], s0 * f.y, y[t][1]);
-                        y[t][2] = fmaf(d[2], s1 * f.x, y[t][2]);
-                        y[t][3] = fmaf(d[3], s1 * f.y, y[t][3]);
-                        const float2 h = *reinterpret_cast<const float2*>(sp + COLS);
-                        float e[4] = {};
-                        mma_f16(e, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
-                        mma_f16(e, r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb.z, xb.w);
-                        const float t0 = F16Bits<T>::one(cur.s[0][u] >> 16), t1 = F16Bits<T>::one(cur.s[1][u] >> 16);
-                        y[t][0] = fmaf(e[0], t0 * h.x, y[t][0]);
-                        y[t][1] = fmaf(e[1], t0 * h.y, y[t][1]);
-                        y[t][2] = fmaf(e[2], t1 * h.x, y[t][2]);
-                        y[t][3] = fmaf(e[3], t1 * h.y, y[t][3]);
+    for (int i = 0; i < RING - 1; ++i) fill_next();
+    if (once) {
+        wait_copies<RING - 1>();
+        order_x(first, last);
+        __syncthreads();
+    }
+
+    int parity = 0;
+    for (int tile = tile0; tile < a.tiles; tile += tile_step, parity = kSumBuffers<NT> - 1 - parity) {
+        float y[NT][4] = {};
+        for (int base = first, piece = first + wk; base < last; base += a.pieces_stage) {
+            const int end = min(last, base + a.pieces_stage);
+            if (!once) {
+                __syncthreads();
+                fetch_x(base, end);
+                commit_copies();
+                wait_copies<0>();
+                order_x(base, end);
+                __syncthreads();
+            }
+            for (; piece < end; piece += warps_k) {
+                fill_next();                                  // into the slot that every lane left at the end of the piece before
+                wait_copies<RING - 1>();
+                __syncwarp();
+                const uint8_t* const lo = ring + out * kPieceBytes<BLOCK> + g * kCodePitch + (BLOCK == 32 ? 4 : 8) * c;
+                const uint8_t* const hi = lo + 8 * kCodePitch;
+                const uint32_t* const sp = reinterpret_cast<const uint32_t*>(ring + out * kPieceBytes<BLOCK> + 16 * kCodePitch + g * (2 * PER));
+                uint32_t sw[2][PER / 2];
+#pragma unroll
+                for (int i = 0; i < PER / 2; ++i) sw[0][i] = sp[i], sw[1][i] = sp[4 * PER + i];
+                auto scale = [&](int r, int i) { return i & 1 ? F16Bits<T>::hi(sw[r][i / 2]) : F16Bits<T>::lo(sw[r][i / 2]); };
+                const uint8_t* const xp = xs + (piece - base) * (kPiece * 2) + c * 32;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    uint2 w0, w1;
+                    if (BLOCK == 32) {
+                        w0 = make_uint2(*reinterpret_cast<const uint32_t*>(lo + 32 * u), *reinterpret_cast<const uint32_t*>(lo + 32 * u + 16));
+                        w1 = make_uint2(*reinterpret_cast<const uint32_t*>(hi + 32 * u), *reinterpret_cast<const uint32_t*>(hi + 32 * u + 16));
                     } else {
-                        mma_f16(d, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
-                        mma_f16(d, r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb.z, xb.w);
-                        const float s0 = F16Bits<T>::one(cur.s[0][u]), s1 = F16Bits<T>::one(cur.s[1][u]);
-                        y[t][0] = fmaf(d[0], s0 * f.x, y[t][0]);
-                        y[t][1] = fmaf(d[1], s0 * f.y, y[t][1]);
-                        y[t][2] = fmaf(d[2], s1 * f.x, y[t][2]);
-                        y[t][3] = fmaf(d[3], s1 * f.y, y[t][3]);
+                        w0 = *reinterpret_cast<const uint2*>(lo + 32 * u);
+                        w1 = *reinterpret_cast<const uint2*>(hi + 32 * u);
+                    }
+                    const Codes4 r0a = unpack8<T>(w0.x), r0b = unpack8<T>(w0.y), r1a = unpack8<T>(w1.x), r1b = unpack8<T>(w1.y);
+                    const int AFTER = BLOCK == 32 ? 2 * u + 1 : u * PER / 4;         // the scale of (the second half of) these 64 values
+                    // eight columns, or twice eight, whose sums do not wait for one another
+                    constexpr int PAIR = NT == 1 ? 1 : 2;
+#pragma unroll
+                    for (int t = 0; t < NT; t += PAIR) {
+                        uint4 xa[PAIR], xb[PAIR];
+                        float d[PAIR][4];
+#pragma unroll
+                        for (int h = 0; h < PAIR; ++h) {
+                            // columns behind the last row of x read that row again and are not stored
+                            const uint4* p = reinterpret_cast<const uint4*>(xp + min(8 * (t + h) + g, rows_x - 1) * pitch + u * 128);
+                            xa[h] = p[0];
+                            xb[h] = p[1];
+                        }
+                        auto scaled = [&](int h, int i) {
+                            float (&y4)[4] = y[t + h];
+                            y4[0] = fmaf(d[h][0], scale(0, i), y4[0]);
+                            y4[1] = fmaf(d[h][1], scale(0, i), y4[1]);
+                            y4[2] = fmaf(d[h][2], scale(1, i), y4[2]);
+                            y4[3] = fmaf(d[h][3], scale(1, i), y4[3]);
+                        };
+#pragma unroll
+                        for (int h = 0; h < PAIR; ++h) mma16_first<T>(d[h], r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa[h].x, xa[h].y);
+#pragma unroll
+                        for (int h = 0; h < PAIR; ++h) mma16<T>(d[h], r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa[h].z, xa[h].w);
+#pragma unroll
+                        for (int h = 0; h < PAIR; ++h) {
+                            if (BLOCK == 32) {
+                                scaled(h, 2 * u);
+                                mma16_first<T>(d[h], r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb[h].x, xb[h].y);
+                            } else {
+                                mma16<T>(d[h], r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb[h].x, xb[h].y);
+                            }
+                        }
+#pragma unroll
+                        for (int h = 0; h < PAIR; ++h) mma16<T>(d[h], r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb[h].z, xb[h].w);
+#pragma unroll
+                        for (int h = 0; h < PAIR; ++h) scaled(h, AFTER);
                     }
                 }
+                out = out + 1 == RING ? 0 : out + 1;
+                __syncwarp();
             }
-            cur = nxt;
+        }
+        // ---- sums over the warps that share rows, then over the cluster: both in a fixed order
+        float* const mine = part + (size_t)parity * sum_parts(warps_k) * sums;
+        float* const total = warps_k == 1 ? mine : mine + (size_t)warps_k * sums;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int col = 8 * t + 2 * c + (i & 1);
+                if (col < rows_x) mine[(size_t)wk * sums + col * rows_cta + 16 * wn + g + 8 * (i >> 1)] = y[t][i];
+            }
+        __syncthreads();
+        // Four rows at a time; every load is under way before the first sum.
+        auto add = [](float4& s, const float4& v) { s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w; };
+        auto warps_sum = [&](int i) {
+            float4 s = *reinterpret_cast<const float4*>(mine + i);
+            for (int w0 = 1; w0 < warps_k; w0 += 3) {             // 2, 4, 8 or 16 warps: 1, 3, 7 or 15 more
+                float4 v[3];
+#pragma unroll
+                for (int w = 0; w < 3; ++w)
+                    if (w0 + w < warps_k) v[w] = *reinterpret_cast<const float4*>(mine + (size_t)(w0 + w) * sums + i);
+#pragma unroll
+                for (int w = 0; w < 3; ++w)
+                    if (w0 + w < warps_k) add(s, v[w]);
+            }
+            return s;
+        };
+        auto store = [&](int i, const float4& s) {
+            const int m = m0 + i / rows_cta, n = tile * rows_cta + i % rows_cta;
+            const float y[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (n + j >= a.N) return;
+                float v = y[j] * (1.0f / 7.0f);
+                if (a.bias) v += load_as_float(a.bias, a.bias_dtype, n + j);
+                if (a.residual) v += load_as_float(a.residual, a.out_dtype, (int64_t)m * a.ldr + n + j);
+                store_from_float(a.C, a.out_dtype, (int64_t)m * a.ldc + n + j, v);
+            }
+        };
+        if (ranks == 1) {
+            for (int i = 4 * threadIdx.x; i < sums; i += 4 * kThreads) store(i, warps_sum(i));
+        } else {
+            if (warps_k > 1)
+                for (int i = 4 * threadIdx.x; i < sums; i += 4 * kThreads) *reinterpret_cast<float4*>(total + i) = warps_sum(i);
+            cluster.sync();
+            const int share = (sums / 4 + ranks - 1) / ranks * 4;
+            for (int i = rank * share + 4 * threadIdx.x; i < min(sums, (rank + 1) * share); i += 4 * kThreads) {
+                float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int r0 = 0; r0 < ranks; r0 += 4) {
+                    float4 v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (r0 + r < ranks) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(total, r0 + r) + i);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (r0 + r < ranks) add(s, v[r]);
+                }
+                store(i, s);
+            }
+        }
+        if (kSumBuffers<NT> == 1 && tile + tile_step < a.tiles) {
+            if (ranks > 1) cluster.sync();
+            else __syncthreads();
         }
     }
-
-    // ---- sums over the warps that share rows, then over the cluster: both in a fixed order
-    __syncthreads();
-    const int rows_cta = 16 * a.warps_n;
-    float* const part = reinterpret_cast<float*>(smem);                      // [warps_k][COLS][rows_cta]
-    float* const total = part + (size_t)warps_k * COLS * rows_cta;           // [COLS][rows_cta]
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            part[((size_t)wk * COLS + 8 * t + 2 * c + (i & 1)) * rows_cta + 16 * wn + g + 8 * (i >> 1)] = y[t][i];
-    __syncthreads();
-    const int values = rows_x * rows_cta;
-    for (int i = threadIdx.x; i < values; i += kThreads) {
-        float s = part[i];
-        for (int w = 1; w < warps_k; ++w) s += part[(size_t)w * COLS * rows_cta + i];
-        total[i] = s;
-    }
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
-    const int tile0 = (int)(blockIdx.x / ranks) * rows_cta;
-    const int share = (values + ranks - 1) / ranks;
-    for (int i = rank * share + threadIdx.x; i < min(values, (rank + 1) * share); i += kThreads) {
-        float s = 0.0f;
-        if (ranks == 1) s = total[i];
-        else
-            for (int r = 0; r < ranks; ++r) s += cluster.map_shared_rank(total, r)[i];
-        const int m = m0 + i / rows_cta, n = tile0 + i % rows_cta;
-        if (n >= a.N) continue;
-        float out = s * (1.0f / 7.0f);
-        if (a.bias) out += load_as_float(a.bias, a.bias_dtype, n);
-        if (a.residual) out += load_as_float(a.residual, a.out_dtype, (int64_t)m * a.ldr + n);
-        store_from_float(a.C, a.out_dtype, (int64_t)m * a.ldc + n, out);
-    }
+    wait_copies<0>();
     if (ranks > 1) cluster.sync();           // the others read this CTA's sums
 }
 
-int sm_count() {
-    static int sms[64] = {0};
-    int dev = 0;
-    if (current_device(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (sms[dev] == 0) {
-        int n = 0;
-        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
-        sms[dev] = n;
-    }
-    return sms[dev];
-}
+// How a product is divided: a CTA's warps over rows of W (the others divide its K), the CTAs of a cluster over K.
+struct Division {
+    int warps_n, ranks, pieces_cta, pieces_stage, tiles, grid;
+    size_t smem;
+    double cost;
+};
 
-template <typename T, bool SHORT, int NT, bool VEC>
+template <typename T, int BLOCK, int NT>
 int launch(MatmulArgs a, cudaStream_t st) {
     constexpr int COLS = 8 * NT;
     static SmemOptIn opt_in;
-    // Rows of W per CTA grow with the rows of x, which every CTA reads.
-    a.warps_n = a.M <= 2 ? 1 : a.M <= 8 ? 2 : a.M <= 16 ? 4 : 8;
-    const int tiles = (a.N + 16 * a.warps_n - 1) / (16 * a.warps_n), warps_k = kWarps / a.warps_n;
-    const int m_tiles = (a.M + COLS - 1) / COLS;
-    a.pieces = (int)((a.K + kPiece - 1) / kPiece);
-    // CTAs of a cluster divide K until there are two CTAs an SM, as long as every warp keeps a piece.
-    int ranks = 1;
-    while (ranks < 8 && (int64_t)tiles * m_tiles * ranks < 2 * sm_count() && a.pieces >= 2 * ranks * warps_k) ranks *= 2;
-    a.pieces_cta = (a.pieces + ranks - 1) / ranks;
-    const int rows_x = a.M < COLS ? a.M : COLS;
-    const int per_piece = rows_x * kPiece * 2 + (kPiece / (SHORT ? 32 : 64)) * COLS * 4;
-    a.pieces_stage = a.pieces_cta;
-    if ((int64_t)a.pieces_stage * per_piece + rows_x * 16 > kMaxStage) a.pieces_stage = (kMaxStage - rows_x * 16) / per_piece;
-    size_t smem = (size_t)a.pieces_stage * per_piece + rows_x * 16;
-    const size_t sums = (size_t)(warps_k + 1) * COLS * 16 * a.warps_n * 4;
-    if (smem < sums) smem = sums;
-    if (int rc = opt_in.ensure(matmul_int4_kernel<T, SHORT, NT, VEC>, smem)) return rc;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(tiles * ranks), (unsigned)m_tiles);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
+    const int m_tiles = (a.M + COLS - 1) / COLS, rows_x = a.M < COLS ? a.M : COLS, sms = sm_count();
+    a.pieces = (a.K + kPiece - 1) / kPiece;
+    // The division with the shortest estimate, in cycles.  An SM has one CTA, which goes through its tiles one after the other: its warps
+    // take a piece in the time that their matrix and other instructions need, or, if it is their only one, in one piece's latency.
+    // clusters of 1, 2, 4 and 8 such CTAs that the device runs at once: fewer than its SMs would hold, which come in groups
+    static std::atomic<int> at_once[64][4];
+    int dev = 0;
+    BI8_CUDA_TRY(current_device(&dev));
+    if (dev < 0 || dev >= 64) return fail(BI8_ERR_CUDA, "device ordinal %d out of range", dev);
+    if (int rc = opt_in.ensure(matmul_int4_kernel<T, BLOCK, NT>, kSmemSM - 1024)) return rc;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)ranks;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.blockDim = dim3(kThreads);
     cfg.attrs = attr;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    for (int r = 0; r < 4; ++r) {
+        if (at_once[dev][r].load(std::memory_order_relaxed) > 0) continue;
+        int n = 0;
+        attr[0].val.clusterDim.x = 1u << r;
+        cfg.gridDim = dim3((unsigned)sms / 8 * 8);
+        cfg.dynamicSmemBytes = kSmemSM - 1024;
+        cfg.numAttrs = 1;
+        BI8_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, matmul_int4_kernel<T, BLOCK, NT>, &cfg));
+        at_once[dev][r].store(n > 0 ? n : 1, std::memory_order_relaxed);
+    }
+    Division best{};
+    best.cost = 1e30;
+    auto consider = [&](int wn, int ranks) {
+        const int wk = kWarps / wn, cta = (a.pieces + ranks - 1) / ranks, tiles = (a.N + 16 * wn - 1) / (16 * wn);
+        const size_t fixed = kRingBytes<BLOCK, NT> + (size_t)kSumBuffers<NT> * sum_parts(wk) * rows_x * 16 * wn * 4, limit = kSmemSM - 1024;
+        if (fixed + (size_t)rows_x * x_pitch(1) > limit) return;
+        int stage = cta;
+        if (fixed + (size_t)rows_x * x_pitch(stage) > limit) stage = ((int)((limit - fixed) / rows_x) - 16) / (kPiece * 2);
+        const int room = at_once[dev][ranks == 1 ? 0 : ranks == 2 ? 1 : ranks == 4 ? 2 : 3].load(std::memory_order_relaxed);
+        int clusters = room / m_tiles;
+        if (clusters < 1) clusters = 1;
+        if (clusters > tiles) clusters = tiles;
+        const int rounds = (tiles + clusters - 1) / clusters;
+        clusters = (tiles + rounds - 1) / rounds;
+        const double waves = ((int64_t)clusters * m_tiles + room - 1) / room, pieces = (cta + wk - 1) / wk;
+        const double round = pieces * kWarps * (60.0 + 40.0 * NT) + 400.0 + (ranks > 1 ? 700.0 : 0.0) + rows_x * wn * (4.0 + ranks) +
+                             (stage < cta ? 3000.0 * ((cta + stage - 1) / stage) : 0.0);
+        const double cost = waves * (3000.0 + rows_x * cta + rounds * round);
+        if (cost < best.cost) best = {wn, ranks, cta, stage, tiles, clusters * ranks, fixed + (size_t)rows_x * x_pitch(stage), cost};
+    };
+    for (int wn = 1; wn <= kWarps; wn *= 2)
+        for (int ranks = 1; ranks <= 8; ranks *= 2)
+            if (ranks == 1 || a.pieces >= ranks) consider(wn, ranks);
+    a.warps_n = best.warps_n, a.ranks = best.ranks, a.pieces_cta = best.pieces_cta, a.pieces_stage = best.pieces_stage, a.tiles = best.tiles;
+    cfg.gridDim = dim3((unsigned)best.grid, (unsigned)m_tiles);
+    cfg.dynamicSmemBytes = best.smem;
+    cfg.stream = st;
+    attr[0].val.clusterDim.x = (unsigned)best.ranks;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 2;
-    BI8_CUDA_TRY(cudaLaunchKernelEx(&cfg, matmul_int4_kernel<T, SHORT, NT, VEC>, a));
+    BI8_CUDA_TRY(cudaLaunchKernelEx(&cfg, matmul_int4_kernel<T, BLOCK, NT>, a));
     return BI8_OK;
 }
 
@@ -350,22 +452,24 @@ int launch_matmul_int4(const void* x, int x_dt, int64_t ldx, const uint8_t* W, i
     a.out_dtype = out_dt;
     a.M = (int)M;
     a.N = (int)N;
-    a.K = K;
-    a.shift = block == 32 ? 5 : block == 64 ? 6 : 7;
+    a.K = (int)K;
     a.x_vec = aligned(x, 16) && (M == 1 || ldx % 8 == 0);
-    a.w_vec = aligned(W, 8) && (N == 1 || ldw % 8 == 0);
+    a.w_vec = aligned(W, 16) && (N == 1 || ldw % 16 == 0);
     const int scale_bytes = 2 * kPiece / block;
     a.s_vec = aligned(sW, scale_bytes) && (N == 1 || a.blocks % (kPiece / block) == 0);
-    auto by_columns = [&](auto* tag, auto is_short, auto vec) {
+    auto by_columns = [&](auto* tag, auto blk) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        constexpr bool S = decltype(is_short)::value, V = decltype(vec)::value;
-        if (M <= 8) return launch<T, S, 1, V>(a, st);
-        if (M <= 16) return launch<T, S, 2, V>(a, st);
-        if (M <= 32) return launch<T, S, 4, V>(a, st);
-        return launch<T, S, 8, V>(a, st);
+        constexpr int B = decltype(blk)::value;
+        if (M <= 8) return launch<T, B, 1>(a, st);
+        if (M <= 16) return launch<T, B, 2>(a, st);
+        if (M <= 32) return launch<T, B, 4>(a, st);
+        return launch<T, B, 8>(a, st);
     };
-    auto by_layout = [&](auto* tag, auto is_short) { return a.w_vec ? by_columns(tag, is_short, std::true_type{}) : by_columns(tag, is_short, std::false_type{}); };
-    auto by_block = [&](auto* tag) { return block == 32 ? by_layout(tag, std::true_type{}) : by_layout(tag, std::false_type{}); };
+    auto by_block = [&](auto* tag) {
+        if (block == 32) return by_columns(tag, std::integral_constant<int, 32>{});
+        if (block == 64) return by_columns(tag, std::integral_constant<int, 64>{});
+        return by_columns(tag, std::integral_constant<int, 128>{});
+    };
     return x_dt == BI8_BF16 ? by_block(static_cast<__nv_bfloat16*>(nullptr)) : by_block(static_cast<__half*>(nullptr));
 }
 

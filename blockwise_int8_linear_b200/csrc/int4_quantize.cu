@@ -1,7 +1,8 @@
 // Block quantizer and dequantizer of the 4-bit format.
 //
-// Both stream: a thread takes eight values (16 bytes of the 16-bit side, 4 bytes of codes).  The quantizer's blocks of 32, 64 or 128
-// values are 4, 8 or 16 neighbouring lanes, which find the block's largest value by shuffles over the bits of |x|.
+// Both stream: a thread takes eight values at a time (16 bytes of the 16-bit side, 4 bytes of codes), and where the matrix is one long
+// row, four times eight with all loads under way at once.  The quantizer's blocks of 32, 64 or 128 values are 4, 8 or 16 neighbouring
+// lanes, which find the block's largest value by shuffles over the bits of |x|.
 #include "int4_common.cuh"
 
 #include <type_traits>
@@ -35,35 +36,49 @@ struct Rows {
 };
 
 // FLAT: K is a multiple of the block, rows and code rows are dense and aligned; the matrix is one long row.
+template <bool FLAT>
+constexpr int kUnits = FLAT ? 4 : 1;                 // of a thread
+
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(kThreads) quantize_int4_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq,
                                                                  T* __restrict__ s, int64_t K, Rows rows) {
+    constexpr int N = kUnits<FLAT>;
     after_predecessor();
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const bool live = i < rows.units;
-    const Unit u = live ? rows.unit<FLAT>(i) : Unit{0, 0};
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (FLAT) {
-        if (live) v = ld_nc_v4(x + u.k);
-    } else if (live) {
-        const unsigned short* p = reinterpret_cast<const unsigned short*>(x) + u.row * ldx + u.k;
-        uint32_t e[8];
+    const int64_t first = (int64_t)blockIdx.x * (N * kThreads) + threadIdx.x;
+    uint4 v[N];
+    Unit u[N];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = u.k + j < K ? p[j] : 0u;
-        v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-    }
-    uint32_t bits;
-    const uint32_t w = quantize8<T>(v, 1 << rows.shift, &bits);
-    if (!live) return;
-    if (FLAT) {
-        *reinterpret_cast<uint32_t*>(q + u.k / 2) = w;
-    } else {
-        uint8_t* p = q + u.row * ldq + u.k / 2;
+    for (int n = 0; n < N; ++n) {
+        const int64_t i = first + n * kThreads;
+        const bool live = i < rows.units;
+        u[n] = live ? rows.unit<FLAT>(i) : Unit{0, 0};
+        v[n] = make_uint4(0u, 0u, 0u, 0u);
+        if (FLAT) {
+            if (live) v[n] = ld_nc_v4(x + u[n].k);
+        } else if (live) {
+            const unsigned short* p = reinterpret_cast<const unsigned short*>(x) + u[n].row * ldx + u[n].k;
+            uint32_t e[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (u.k + 2 * j < K) p[j] = (uint8_t)(w >> (8 * j));
+            for (int j = 0; j < 8; ++j) e[j] = u[n].k + j < K ? p[j] : 0u;
+            v[n] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        }
     }
-    if ((threadIdx.x & ((1 << rows.shift) - 1)) == 0) reinterpret_cast<unsigned short*>(s)[i >> rows.shift] = (unsigned short)bits;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int64_t i = first + n * kThreads;
+        uint32_t bits;
+        const uint32_t w = quantize8<T>(v[n], 1 << rows.shift, &bits);
+        if (i >= rows.units) continue;
+        if (FLAT) {
+            *reinterpret_cast<uint32_t*>(q + u[n].k / 2) = w;
+        } else {
+            uint8_t* p = q + u[n].row * ldq + u[n].k / 2;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (u[n].k + 2 * j < K) p[j] = (uint8_t)(w >> (8 * j));
+        }
+        if ((threadIdx.x & ((1 << rows.shift) - 1)) == 0) reinterpret_cast<unsigned short*>(s)[i >> rows.shift] = (unsigned short)bits;
+    }
 }
 
 template <typename O>
@@ -93,38 +108,50 @@ __device__ __forceinline__ __nv_bfloat16 to_out<__nv_bfloat16>(float y) { return
 template <typename T, typename O, bool FLAT>
 __global__ void __launch_bounds__(kThreads) dequantize_int4_kernel(const uint8_t* __restrict__ q, int64_t ldq, const T* __restrict__ s,
                                                                    O* __restrict__ out, int64_t K, Rows rows) {
+    constexpr int N = kUnits<FLAT>;
     after_predecessor();
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= rows.units) return;
-    const Unit u = rows.unit<FLAT>(i);
-    if (!FLAT && u.k >= K) return;
-    const float sc = F16Bits<T>::one(reinterpret_cast<const unsigned short*>(s)[i >> rows.shift]);
-    const bool plain = plain_scale(sc);
-    uint32_t w = kZeroCodes;
-    if (FLAT) {
-        w = *reinterpret_cast<const uint32_t*>(q + u.k / 2);
-    } else {
-        const uint8_t* p = q + u.row * ldq + u.k / 2;
-        w = 0;
+    const int64_t first = (int64_t)blockIdx.x * (N * kThreads) + threadIdx.x;
+    uint32_t w[N];
+    float sc[N];
+    Unit u[N];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (u.k + 2 * j < K) w |= (uint32_t)p[j] << (8 * j);
+    for (int n = 0; n < N; ++n) {
+        const int64_t i = first + n * kThreads;
+        w[n] = kZeroCodes;
+        sc[n] = 0.0f;
+        if (i >= rows.units) continue;
+        u[n] = rows.unit<FLAT>(i);
+        sc[n] = F16Bits<T>::one(__ldg(reinterpret_cast<const unsigned short*>(s) + (i >> rows.shift)));
+        if (FLAT) {
+            w[n] = __ldg(reinterpret_cast<const uint32_t*>(q + u[n].k / 2));
+        } else {
+            const uint8_t* p = q + u[n].row * ldq + u[n].k / 2;
+            w[n] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (u[n].k + 2 * j < K) w[n] |= (uint32_t)p[j] << (8 * j);
+        }
     }
-    float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = value_of(sc, (w >> (4 * j)) & 15u, plain);
-    if (FLAT) {
-        store8(out + u.k, y);
-    } else {
-        O* p = out + u.row * K + u.k;
+    for (int n = 0; n < N; ++n) {
+        if (first + n * kThreads >= rows.units) continue;
+        const bool plain = plain_scale(sc[n]);
+        float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (u.k + j < K) p[j] = to_out<O>(y[j]);
+        for (int j = 0; j < 8; ++j) y[j] = value_of(sc[n], (w[n] >> (4 * j)) & 15u, plain);
+        if (FLAT) {
+            store8(out + u[n].k, y);
+        } else {
+            O* p = out + u[n].row * K + u[n].k;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (u[n].k + j < K) p[j] = to_out<O>(y[j]);
+        }
     }
 }
 
-int grid_of(int64_t units, unsigned* grid) {
-    const int64_t g = (units + kThreads - 1) / kThreads;
+int grid_of(int64_t units, bool flat, unsigned* grid) {
+    const int64_t per = (int64_t)kThreads * (flat ? kUnits<true> : kUnits<false>), g = (units + per - 1) / per;
     if (g > 0x7fffffff) return fail(BI8_ERR_LIMIT, "int4: %lld values exceed one launch", (long long)units * 8);
     *grid = (unsigned)g;
     return BI8_OK;
@@ -137,7 +164,7 @@ int launch_quantize_int4(const void* x, int dt, int64_t ldx, uint8_t* q, int64_t
     const Rows rows(M, K, block);
     const bool flat = K % block == 0 && (M == 1 || (ldx == K && ldq == K / 2)) && aligned(x, 16) && aligned(q, 4);
     unsigned grid;
-    if (int rc = grid_of(rows.units, &grid)) return rc;
+    if (int rc = grid_of(rows.units, flat, &grid)) return rc;
     auto go = [&](auto* tag, auto is_flat) {
         using T = std::remove_pointer_t<decltype(tag)>;
         return launch_chained(quantize_int4_kernel<T, decltype(is_flat)::value>, grid, kThreads, 0, st, static_cast<const T*>(x), ldx, q, ldq,
@@ -153,7 +180,7 @@ int launch_dequantize_int4(const uint8_t* q, int64_t ldq, const void* s, int s_d
     const Rows rows(M, K, block);
     const bool flat = K % block == 0 && (M == 1 || ldq == K / 2) && aligned(q, 4) && aligned(out, 16);
     unsigned grid;
-    if (int rc = grid_of(rows.units, &grid)) return rc;
+    if (int rc = grid_of(rows.units, flat, &grid)) return rc;
     auto go = [&](auto* tag, auto* out_tag, auto is_flat) {
         using T = std::remove_pointer_t<decltype(tag)>;
         using O = std::remove_pointer_t<decltype(out_tag)>;

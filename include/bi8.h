@@ -284,14 +284,14 @@ BI8_API int bi8_dequantize_int4(const uint8_t* q, int64_t ldq, const void* s, in
  * x [M,K] of x_dtype (BI8_BF16 or BI8_F16), row stride ldx.  Wq / sW as bi8_quantize_int4 gives them, row pitch ldw bytes, scales of
  * x_dtype.  bias [N] of bias_dtype or NULL.  residual [M,N] of out_dtype, row stride ldr, or NULL; C may be the residual itself.
  * Made for few rows of x, for which the weights are read once (up to 64; more rows are taken 64 at a time).  Code rows that begin
- * on 8-byte boundaries are read faster than others.  A row of x with an infinity or a NaN gives nothing finite. */
+ * on 16-byte boundaries are read faster than others.  A row of x with an infinity or a NaN gives nothing finite. */
 BI8_API int bi8_matmul_int4(const void* x, int x_dtype, int64_t ldx, const uint8_t* Wq, int64_t ldw, const void* sW, const void* bias,
                             int bias_dtype, const void* residual, int64_t ldr, void* C, int64_t ldc, int out_dtype, int64_t M, int64_t N,
                             int64_t K, int block, void* stream);
 
 /* A key/value cache in 4 bits: codes [batch, head, max_len, D/2] and scales [batch, head, max_len, D/64] (blocks of 64) of k and of v.  Rows
- * of a head are dense; steps between batches and heads are free: bytes for the codes (multiples of 8), elements for the scales
- * (multiples of D/64).  Codes begin on 8-byte boundaries, scales on boundaries of a row's scales. */
+ * of a head are dense; steps between batches and heads are free: bytes for the codes (multiples of 16), elements for the scales
+ * (multiples of D/64).  Codes begin on 16-byte boundaries, scales on boundaries of a row's scales. */
 typedef struct {
     uint8_t* k;
     uint8_t* v;
