@@ -6,7 +6,7 @@
 // What bounds one new token per sequence is the cache: D codes and D / 64 scales of k and of v for each row, read once for all G heads
 // (0.53 bytes a value; at 6.5 TB/s 12 values per ns, three instructions of the SMs for each).  So the products are the tensor cores',
 // with the codes as the 16-row operand of both (unpacked by one instruction a value, int4_common.cuh) and the queries, G * T of
-// them, the eight columns:
+// them, eight at a time, the columns:
 //   S[row, query]  = sum_d k[row, d] q[query, d]
 //   O[d, query]    = sum_row v[row, d] P[row, query]  two rows' words interleaved by byte permutes
 // v's scales differ by row, so they go into P: p * vs in fp16 (11 bits, for bf16 results of 8) or, for fp16 results, as a sum of two fp16
@@ -28,8 +28,9 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kCols = 8;                 // queries of a CTA
 constexpr int kClusterShares = 8;        // shares that a cluster joins
-constexpr int kMaxShares = 64;
+constexpr int kMaxShares = 128;
 
 struct AttnArgs {
     const void* q;
@@ -39,7 +40,7 @@ struct AttnArgs {
     const long long* starts;
     int64_t lengths_step, starts_step;
     void* out;
-    float* ws;               // [tile][share][8 NT][D] sums, then [tile][share][8 NT] pairs (maximum, total)
+    float* ws;               // [tile][share][kCols][D] sums, then [tile][share][kCols] pairs (maximum, total)
     int B, Hq, Hkv, T, G;
     int col_tiles, shares;
     float scale_log2;        // scale * log2(e)
@@ -76,6 +77,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 template <int D>
 constexpr int kStepTiles = D == 64 ? 4 : D == 128 ? 2 : 1;       // 16 rows each
 
+template <int D>
+constexpr int kResident = D == 256 ? 3 : 4;                     // CTAs of an SM
+
 // A warp's rows of one step in shared memory: k, v (16 more or less than a multiple of 32 or 64 bytes apart, so that what the lanes read at a
 // time lies in different banks), their scales.  A warp has two steps there: one in use, one on its way.
 template <int D>
@@ -85,17 +89,17 @@ struct Ring {
     static constexpr int kSteps = 2;
 };
 
-template <int D, int NT>
+template <int D>
 constexpr int attn_smem() {
     // queries; the warps' rings, and afterwards the warps' sums (eight columns at a time) and the CTA's; statistics
-    constexpr int rings = kWarps * Ring<D>::kSteps * Ring<D>::kBytes, sums = kWarps * 8 * (D + 4) * 4 + 8 * NT * D * 4;
-    return 8 * NT * (2 * D + 16) + (rings > sums ? rings : sums) + (kWarps * 2 + 2 + kClusterShares) * 8 * NT * 4 + 8 * NT * 4;
+    constexpr int rings = kWarps * Ring<D>::kSteps * Ring<D>::kBytes, sums = kWarps * 8 * (D + 4) * 4 + kCols * D * 4;
+    return kCols * (2 * D + 16) + (rings > sums ? rings : sums) + (kWarps * 2 + 2 + kClusterShares) * kCols * 4 + kCols * 4;
 }
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attention_int4_kernel(const AttnArgs a) {
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(const AttnArgs a) {
     constexpr bool FINE = std::is_same<T, __half>::value;
-    constexpr int U = D / 64, TT = kStepTiles<D>, STEP = 16 * TT, COLS = 8 * NT, PITCH = 2 * D + 16, BUF = D + 4;
+    constexpr int U = D / 64, TT = kStepTiles<D>, STEP = 16 * TT, COLS = kCols, PITCH = 2 * D + 16, BUF = D + 4;
     extern __shared__ __align__(16) uint8_t smem[];
     uint8_t* const xs = smem;                                                    // [COLS] rows of PITCH bytes
     float* const warp_m = reinterpret_cast<float*>(xs + COLS * PITCH);           // [kWarps][COLS]
@@ -113,21 +117,6 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
     const int ct = tile % a.col_tiles, bh = tile / a.col_tiles, h = bh % a.Hkv, b = bh / a.Hkv;
     const int R = a.G * a.T, col0 = ct * COLS, cols = min(COLS, R - col0);
     after_predecessor();
-
-    // ---- queries: fp16 with a power of two per query; D / 8 lanes a query
-    for (int i = threadIdx.x; i < COLS * (D / 8); i += kThreads) {
-        const int col = i / (D / 8), p = i % (D / 8), r = col0 + col;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (col < cols)
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_batch + (int64_t)(h * a.G + r / a.T) * a.q_head + (r % a.T) * a.q_tok + 8 * p);
-        uint32_t big = absmax8(v);
-#pragma unroll
-        for (int d = 1; d < D / 8; d <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, d));
-        const float2 f = fit_fp16<T>(big);
-        *reinterpret_cast<uint4*>(xs + col * PITCH + p * 16) = paired8(scaled8<T>(v, a.scale_log2 < 0.0f ? -f.y : a.scale_log2 > 0.0f ? f.y : 0.0f));
-        if (p == 0) factor[col] = fabsf(a.scale_log2) * f.x * (1.0f / 7.0f);
-    }
-    __syncthreads();
 
     // ---- rows of this share
     const long long len = a.lengths[b * a.lengths_step];
@@ -147,20 +136,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
     const int origin = start & ~15, n_rows = most > start ? most - origin : 0;
     const int chunk = (n_rows + a.shares * STEP - 1) / (a.shares * STEP) * STEP;
     const int first = origin + min(n_rows, share * chunk), last = min(origin + n_rows, first + chunk);
-    int limit[NT][2];
-    float m[NT][2], l[NT][2], fac[NT][2];
+    int limit[2];
+    float m[2], l[2], fac[2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int col = 8 * t + 2 * c + j;
-            limit[t][j] = col < cols ? min(last, rows_seen((col0 + col) % a.T)) : last;
-            m[t][j] = -INFINITY;
-            l[t][j] = 0.0f;
-            fac[t][j] = factor[col];
-        }
+    for (int j = 0; j < 2; ++j) {
+        const int col = 2 * c + j;
+        limit[j] = col < cols ? min(last, rows_seen((col0 + col) % a.T)) : last;
+        m[j] = -INFINITY;
+        l[j] = 0.0f;
+    }
     const int unmasked = min(last, fewest);
-    float o[NT][4 * U][4] = {};
+    float o[4 * U][4] = {};
     float vmax = 0x1p-110f, vscale = 0x1p124f;            // power of two, no smaller than the scales of v so far (up to 2^127); 2^14 over it
 
     const uint8_t* const kp = a.cache.k + b * a.cache.k_batch + h * a.cache.k_head;
@@ -213,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
     auto multiply = [&](const uint8_t* slot, int base, auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         // ---- scores
-        float p[TT][NT][4] = {};
+        float p[TT][4] = {};
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
             float s0[U], s1[U];
@@ -224,57 +210,52 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
                 const uint8_t* const k = slot + (16 * i + g) * Slot::kPitchK + 32 * u + 8 * c;
                 const uint2 w0 = *reinterpret_cast<const uint2*>(k), w1 = *reinterpret_cast<const uint2*>(k + 8 * Slot::kPitchK);
                 const Codes4 r0a = unpack8<__half>(w0.x), r0b = unpack8<__half>(w0.y), r1a = unpack8<__half>(w1.x), r1b = unpack8<__half>(w1.y);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const uint4* x = reinterpret_cast<const uint4*>(xs + (8 * t + g) * PITCH + u * 128 + c * 32);
-                    const uint4 xa = x[0], xb = x[1];
-                    float d[4];
-                    mma16_first<__half>(d, r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa.x, xa.y);
-                    mma16<__half>(d, r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa.z, xa.w);
-                    mma16<__half>(d, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
-                    mma16<__half>(d, r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb.z, xb.w);
-                    p[i][t][0] = fmaf(d[0], s0[u], p[i][t][0]);
-                    p[i][t][1] = fmaf(d[1], s0[u], p[i][t][1]);
-                    p[i][t][2] = fmaf(d[2], s1[u], p[i][t][2]);
-                    p[i][t][3] = fmaf(d[3], s1[u], p[i][t][3]);
-                }
+                const uint4* x = reinterpret_cast<const uint4*>(xs + g * PITCH + u * 128 + c * 32);
+                const uint4 xa = x[0], xb = x[1];
+                float d[4];
+                mma16_first<__half>(d, r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa.x, xa.y);
+                mma16<__half>(d, r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa.z, xa.w);
+                mma16<__half>(d, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
+                mma16<__half>(d, r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb.z, xb.w);
+                p[i][0] = fmaf(d[0], s0[u], p[i][0]);
+                p[i][1] = fmaf(d[1], s0[u], p[i][1]);
+                p[i][2] = fmaf(d[2], s1[u], p[i][2]);
+                p[i][3] = fmaf(d[3], s1[u], p[i][3]);
             }
         }
         // ---- softmax: running maximum and sum of every column
         bool grown = false;
-        float alpha[NT][2];
+        float alpha[2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int j = 0; j < 2; ++j) {
+            float top = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float top = -INFINITY;
+            for (int i = 0; i < TT; ++i)
 #pragma unroll
-                for (int i = 0; i < TT; ++i)
+                for (int r = 0; r < 2; ++r) {
+                    float& x = p[i][2 * r + j];
+                    if (MASKED && (base + 16 * i + g + 8 * r >= limit[j] || base + 16 * i + g + 8 * r < start)) x = -INFINITY;
+                    top = fmaxf(top, x);
+                }
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float& x = p[i][t][2 * r + j];
-                        if (MASKED && (base + 16 * i + g + 8 * r >= limit[t][j] || base + 16 * i + g + 8 * r < start)) x = -INFINITY;
-                        top = fmaxf(top, x);
-                    }
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float now = fmaxf(m[j], top);
+            // scores are the products without the column's factor, which is not negative; a column may have seen nothing yet
+            const float ref = MASKED && now == -INFINITY ? 0.0f : now * fac[j];
+            alpha[j] = exp2_fast(fmaf(m[j], fac[j], -ref));
+            grown = grown || now != m[j];
+            m[j] = now;
+            float sum = 0.0f;
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                const float now = fmaxf(m[t][j], top);
-                // scores are the products without the column's factor, which is not negative; a column may have seen nothing yet
-                const float ref = MASKED && now == -INFINITY ? 0.0f : now * fac[t][j];
-                alpha[t][j] = exp2_fast(fmaf(m[t][j], fac[t][j], -ref));
-                grown = grown || now != m[t][j];
-                m[t][j] = now;
-                float sum = 0.0f;
+            for (int i = 0; i < TT; ++i)
 #pragma unroll
-                for (int i = 0; i < TT; ++i)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float& x = p[i][t][2 * r + j];
-                        x = exp2_fast(fmaf(x, fac[t][j], -ref));
-                        sum += x;
-                    }
-                l[t][j] = fmaf(l[t][j], alpha[t][j], sum);
-            }
+                for (int r = 0; r < 2; ++r) {
+                    float& x = p[i][2 * r + j];
+                    x = exp2_fast(fmaf(x, fac[j], -ref));
+                    sum += x;
+                }
+            l[j] = fmaf(l[j], alpha[j], sum);
+        }
         // ---- v's scales: a larger one than any before moves the normalisation
         float vs[TT][2][U], big = 0.0f;
 #pragma unroll
@@ -298,11 +279,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
                 vscale = 0x1p14f / next;
             }
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int w = 0; w < 4 * U; ++w)
 #pragma unroll
-                for (int w = 0; w < 4 * U; ++w)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[t][w][j] *= alpha[t][j & 1] * shrink;
+                for (int j = 0; j < 4; ++j) o[w][j] *= alpha[j & 1] * shrink;
         }
         // ---- O += V^T P
 #pragma unroll
@@ -310,23 +289,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const float s0 = vs[i][0][u] * vscale, s1 = vs[i][1][u] * vscale;
-                uint32_t bh[NT][2], bl[NT][2];
+                uint32_t bh[2], bl[2];
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float sc = r ? s1 : s0;
-                        float x0 = p[i][t][2 * r] * sc, x1 = p[i][t][2 * r + 1] * sc;
-                        if (MASKED) {                     // a masked row's scale may be anything
-                            const int row = base + 16 * i + g + 8 * r;
-                            if (row >= limit[t][0] || row < start) x0 = 0.0f;
-                            if (row >= limit[t][1] || row < start) x1 = 0.0f;
-                        }
-                        const uint32_t hi = pack_f16x2(x0, x1);
-                        using H = F16Bits<__half>;
-                        bh[t][r] = transpose8x8(hi);
-                        if (FINE) bl[t][r] = transpose8x8(pack_f16x2(x0 - H::lo(hi), x1 - H::hi(hi)));
+                for (int r = 0; r < 2; ++r) {
+                    const float sc = r ? s1 : s0;
+                    float x0 = p[i][2 * r] * sc, x1 = p[i][2 * r + 1] * sc;
+                    if (MASKED) {                     // a masked row's scale may be anything
+                        const int row = base + 16 * i + g + 8 * r;
+                        if (row >= limit[0] || row < start) x0 = 0.0f;
+                        if (row >= limit[1] || row < start) x1 = 0.0f;
                     }
+                    const uint32_t hi = pack_f16x2(x0, x1);
+                    using H = F16Bits<__half>;
+                    bh[r] = transpose8x8(hi);
+                    if (FINE) bl[r] = transpose8x8(pack_f16x2(x0 - H::lo(hi), x1 - H::hi(hi)));
+                }
                 const uint8_t* const v = slot + Slot::kV + (16 * i + 2 * c) * Slot::kPitchV + 32 * u + 4 * g;
                 uint32_t w[4];
 #pragma unroll
@@ -340,11 +317,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
                     for (int j = 0; j < 2; ++j) {
                         const uint32_t x = w01 >> (8 * j), y = w23 >> (8 * j);
                         const uint32_t a0 = half2_low(x), a1 = half2_high(x), a2 = half2_low(y), a3 = half2_high(y);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            mma16<__half>(o[t][4 * u + 2 * half + j], a0, a1, a2, a3, bh[t][0], bh[t][1]);
-                            if (FINE) mma16<__half>(o[t][4 * u + 2 * half + j], a0, a1, a2, a3, bl[t][0], bl[t][1]);
-                        }
+                        mma16<__half>(o[4 * u + 2 * half + j], a0, a1, a2, a3, bh[0], bh[1]);
+                        if (FINE) mma16<__half>(o[4 * u + 2 * half + j], a0, a1, a2, a3, bl[0], bl[1]);
                     }
                 }
             }
@@ -353,6 +327,26 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
     int slot = 0;
     if (first + warp * STEP < last) fill(ring, first + warp * STEP);
     commit_copies();
+
+    // ---- queries: fp16 with a power of two per query; D / 8 lanes a query
+    for (int i = threadIdx.x; i < COLS * (D / 8); i += kThreads) {
+        const int col = i / (D / 8), p = i % (D / 8), r = col0 + col;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (col < cols)
+            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_batch + (int64_t)(h * a.G + r / a.T) * a.q_head + (r % a.T) * a.q_tok + 8 * p);
+        uint32_t big = absmax8(v);
+#pragma unroll
+        for (int d = 1; d < D / 8; d <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, d));
+        const float2 f = fit_fp16<T>(big);
+        *reinterpret_cast<uint4*>(xs + col * PITCH + p * 16) = paired8(scaled8<T>(v, a.scale_log2 < 0.0f ? -f.y : a.scale_log2 > 0.0f ? f.y : 0.0f));
+        // never 0, which the infinities of unseen rows do not bear (a scale of 0 makes the queries 0)
+        if (p == 0) factor[col] = a.scale_log2 == 0.0f ? 1.0f : fmaxf(fabsf(a.scale_log2) * f.x * (1.0f / 7.0f), 0x1p-126f);
+    }
+    __syncthreads();
+
+#pragma unroll
+    for (int j = 0; j < 2; ++j) fac[j] = factor[2 * c + j];
+
     for (int base = first + warp * STEP; base < last; base += kWarps * STEP) {
         const int next = base + kWarps * STEP;
         if (next < last) fill(ring + (slot ^ 1) * Slot::kBytes, next);
@@ -368,16 +362,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
 
     // ---- the warps' results into one
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) l[t][j] += __shfl_xor_sync(0xffffffffu, l[t][j], d);
-            if (g == 0) {
-                warp_m[warp * COLS + 8 * t + 2 * c + j] = m[t][j] == -INFINITY ? -INFINITY : m[t][j] * fac[t][j];      // log2 units
-                warp_l[warp * COLS + 8 * t + 2 * c + j] = l[t][j];
-            }
+        for (int d = 4; d < 32; d <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], d);
+        if (g == 0) {
+            warp_m[warp * COLS + 2 * c + j] = m[j] == -INFINITY ? -INFINITY : m[j] * fac[j];      // log2 units
+            warp_l[warp * COLS + 2 * c + j] = l[j];
         }
+    }
     __syncthreads();
     for (int col = threadIdx.x; col < COLS; col += kThreads) {
         float top = -INFINITY, total = 0.0f;
@@ -390,29 +382,26 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
     __syncthreads();
     const float unit = vmax * (0x1p-14f / 7.0f);          // (every warp has left its ring)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int j = 0; j < 2; ++j) {
+        const int col = 2 * c + j;
+        const float w = m[j] == -INFINITY ? 0.0f : exp2_fast(m[j] * fac[j] - cta_m[col]) * unit;
+        float* dst = buf + (warp * 8 + col) * BUF + 8 * g;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int col = 2 * c + j;
-            const float w = m[t][j] == -INFINITY ? 0.0f : exp2_fast(m[t][j] * fac[t][j] - cta_m[8 * t + col]) * unit;
-            float* dst = buf + (warp * 8 + col) * BUF + 8 * g;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                *reinterpret_cast<float4*>(dst + 64 * u) = make_float4(o[t][4 * u][j] * w, o[t][4 * u][2 + j] * w, o[t][4 * u + 1][j] * w, o[t][4 * u + 1][2 + j] * w);
-                *reinterpret_cast<float4*>(dst + 64 * u + 4) =
-                    make_float4(o[t][4 * u + 2][j] * w, o[t][4 * u + 2][2 + j] * w, o[t][4 * u + 3][j] * w, o[t][4 * u + 3][2 + j] * w);
-            }
+        for (int u = 0; u < U; ++u) {
+            *reinterpret_cast<float4*>(dst + 64 * u) = make_float4(o[4 * u][j] * w, o[4 * u][2 + j] * w, o[4 * u + 1][j] * w, o[4 * u + 1][2 + j] * w);
+            *reinterpret_cast<float4*>(dst + 64 * u + 4) =
+                make_float4(o[4 * u + 2][j] * w, o[4 * u + 2][2 + j] * w, o[4 * u + 3][j] * w, o[4 * u + 3][2 + j] * w);
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 8 * D; i += kThreads) {
-            const int col = i / D, d = i % D;
-            float s = buf[col * BUF + d];
-#pragma unroll
-            for (int w = 1; w < kWarps; ++w) s += buf[(w * 8 + col) * BUF + d];
-            sums[(8 * t + col) * D + d] = s;
-        }
-        __syncthreads();
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * D; i += kThreads) {
+        const int col = i / D, d = i % D;
+        float s = buf[col * BUF + d];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) s += buf[(w * 8 + col) * BUF + d];
+        sums[col * D + d] = s;
+    }
+    __syncthreads();
 
     auto store = [&](int col, int d, float x, float y) {
         const int r = col0 + col;
@@ -477,15 +466,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 && D <= 128 ? 4 : 2) attenti
     cluster.sync();                                       // the others read this CTA's sums
 }
 
-// Joins the shares of one query: a CTA of D threads.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(D) attention_int4_join_kernel(const AttnArgs a, int64_t ctas) {
-    constexpr int COLS = 8 * NT;
+// Joins the shares of one query: a CTA of four times D threads, a quarter of the shares each.
+template <typename T, int D>
+__global__ void __launch_bounds__(4 * D) attention_int4_join_kernel(const AttnArgs a, int64_t ctas) {
+    constexpr int COLS = kCols;
     __shared__ float weight[kMaxShares];
+    __shared__ float sum[4][D];
     after_predecessor();
     const int R = a.G * a.T, r = blockIdx.x % R, bh = blockIdx.x / R, h = bh % a.Hkv, b = bh / a.Hkv;
     const int64_t cta0 = ((int64_t)bh * a.col_tiles + r / COLS) * a.shares;
-    const int col = r % COLS;
+    const int col = r % COLS, d = threadIdx.x % D, part = threadIdx.x / D;
+    const int per = (a.shares + 3) / 4, first = part * per, last = min(a.shares, first + per);
+    const float* src = a.ws + (cta0 * COLS + col) * D + d;
+    float v[8];                                           // on their way before the weights are known
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = first + k < last ? src[(int64_t)(first + k) * COLS * D] : 0.0f;
     const float2* stat = reinterpret_cast<const float2*>(a.ws + ctas * COLS * D) + cta0 * COLS + col;
     if (threadIdx.x < 32) {
         float top = -INFINITY, total = 0.0f;
@@ -510,34 +505,37 @@ __global__ void __launch_bounds__(D) attention_int4_join_kernel(const AttnArgs a
         for (int i = 0; i < kMaxShares / 32; ++i) weight[threadIdx.x + 32 * i] = s[i].x * inv;
     }
     __syncthreads();
-    const float* src = a.ws + (cta0 * COLS + col) * D + threadIdx.x;
     float x = 0.0f;
-    for (int k0 = 0; k0 < a.shares; k0 += 16) {
-        float v[16];
+    for (int k0 = first; k0 < last; k0 += 8) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = k0 + k < a.shares ? src[(int64_t)(k0 + k) * COLS * D] : 0.0f;
+        for (int k = 0; k < 8; ++k)
+            if (k0 + k < last) x = fmaf(v[k], weight[k0 + k], x);
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-            if (k0 + k < a.shares) x = fmaf(v[k], weight[k0 + k], x);
+        for (int k = 0; k < 8; ++k) v[k] = k0 + 8 + k < last ? src[(int64_t)(k0 + 8 + k) * COLS * D] : 0.0f;
     }
-    const int64_t at = (((int64_t)b * a.Hq + h * a.G + r / a.T) * a.T + r % a.T) * D + threadIdx.x;
-    static_cast<unsigned short*>(a.out)[at] = (unsigned short)F16Bits<T>::pack(x, 0.0f);
+    sum[part][d] = x;
+    __syncthreads();
+    if (part > 0) return;
+    const int64_t at = (((int64_t)b * a.Hq + h * a.G + r / a.T) * a.T + r % a.T) * D + d;
+    static_cast<unsigned short*>(a.out)[at] = (unsigned short)F16Bits<T>::pack((sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d]), 0.0f);
 }
 
 struct Plan {
-    int nt, col_tiles, shares;
+    int col_tiles, shares;
     int64_t tiles;
 };
 Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len) {
     const int64_t R = Hq / Hkv * T;
     Plan p;
-    p.nt = R <= 8 ? 1 : R <= 16 || D == 256 ? 2 : 4;
-    p.col_tiles = (int)((R + 8 * p.nt - 1) / (8 * p.nt));
+    p.col_tiles = (int)((R + kCols - 1) / kCols);
     p.tiles = B * Hkv * p.col_tiles;
-    // Three CTAs an SM, as long as a warp of a full cache has two steps; the clusters' sizes are powers of two.
-    const int64_t step = 16 * (D == 64 ? kStepTiles<64> : D == 128 ? kStepTiles<128> : kStepTiles<256>);
-    const int64_t useful = (max_len + 2 * kWarps * step - 1) / (2 * kWarps * step);
-    int64_t want = (p.nt == 1 && D <= 128 ? 4 : 2) * sm_count() / p.tiles;
+    // As many CTAs as the device holds at once, as long as a warp of a full cache has two steps; and shares of 2048 rows in long caches, whose
+    // sequences may differ much in length (32 sequences of 1 to 8192 rows, 8 heads: 65 us in 2 shares, 55 in 4, 61 in 8; 64 of 4096 rows
+    // each: 71 us in 1, 68 in 2, 82 in 4).  The clusters' sizes are powers of two.
+    const int64_t step = 16 * (D == 64 ? kStepTiles<64> : D == 128 ? kStepTiles<128> : kStepTiles<256>), resident = (D == 256 ? kResident<256> : kResident<128>) * sm_count();
+    const int64_t useful = (max_len + 2 * kWarps * step - 1) / (2 * kWarps * step), long_ones = max_len / 2048;
+    int64_t want = resident / p.tiles;
+    if (want < kClusterShares && want < long_ones) want = long_ones < kClusterShares ? long_ones : kClusterShares;
     int64_t s = useful < want ? useful : want;
     if (s > kMaxShares) s = kMaxShares;
     if (s <= kClusterShares) {
@@ -549,11 +547,11 @@ Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     return p;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D>
 int launch(const AttnArgs& a, int64_t tiles, cudaStream_t st) {
-    constexpr int smem = attn_smem<D, NT>();
+    constexpr int smem = attn_smem<D>();
     static SmemOptIn opt_in;
-    if (int rc = opt_in.ensure(attention_int4_kernel<T, D, NT>, smem)) return rc;
+    if (int rc = opt_in.ensure(attention_int4_kernel<T, D>, smem)) return rc;
     const unsigned grid = (unsigned)(tiles * a.shares);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
@@ -568,9 +566,9 @@ int launch(const AttnArgs& a, int64_t tiles, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    BI8_CUDA_TRY(cudaLaunchKernelEx(&cfg, attention_int4_kernel<T, D, NT>, a));
+    BI8_CUDA_TRY(cudaLaunchKernelEx(&cfg, attention_int4_kernel<T, D>, a));
     if (a.shares <= kClusterShares) return BI8_OK;
-    return launch_chained(attention_int4_join_kernel<T, D, NT>, (unsigned)((int64_t)a.B * a.Hq * a.T), D, 0, st, a, (int64_t)grid);
+    return launch_chained(attention_int4_join_kernel<T, D>, (unsigned)((int64_t)a.B * a.Hq * a.T), 4 * D, 0, st, a, (int64_t)grid);
 }
 
 }  // namespace
@@ -578,7 +576,7 @@ int launch(const AttnArgs& a, int64_t tiles, cudaStream_t st) {
 size_t attention_int4_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len) {
     const Plan p = plan_of(B, T, Hq, Hkv, D, max_len);
     if (p.shares <= kClusterShares) return 0;
-    return (size_t)(p.tiles * p.shares) * 8 * p.nt * (D + 2) * 4;
+    return (size_t)(p.tiles * p.shares) * kCols * (D + 2) * 4;
 }
 
 int launch_attention_int4(const void* q, int dt, int64_t q_batch, int64_t q_head, int64_t q_tok, const bi8_int4_cache* cache, const long long* lengths,
@@ -611,9 +609,9 @@ int launch_attention_int4(const void* q, int dt, int64_t q_batch, int64_t q_head
     a.scale_log2 = scale * 1.4426950408889634f;
     auto go = [&](auto* tag) {
         using E = std::remove_pointer_t<decltype(tag)>;
-        if (D == 64) return p.nt == 1 ? launch<E, 64, 1>(a, p.tiles, st) : p.nt == 2 ? launch<E, 64, 2>(a, p.tiles, st) : launch<E, 64, 4>(a, p.tiles, st);
-        if (D == 128) return p.nt == 1 ? launch<E, 128, 1>(a, p.tiles, st) : p.nt == 2 ? launch<E, 128, 2>(a, p.tiles, st) : launch<E, 128, 4>(a, p.tiles, st);
-        return p.nt == 1 ? launch<E, 256, 1>(a, p.tiles, st) : launch<E, 256, 2>(a, p.tiles, st);
+        if (D == 64) return launch<E, 64>(a, p.tiles, st);
+        if (D == 128) return launch<E, 128>(a, p.tiles, st);
+        return launch<E, 256>(a, p.tiles, st);
     };
     return dt == BI8_BF16 ? go(static_cast<__nv_bfloat16*>(nullptr)) : go(static_cast<__half*>(nullptr));
 }

@@ -11,7 +11,6 @@
 
 namespace bi8 {
 
-constexpr float kInv7 = 1.0f / 7.0f;
 constexpr int kCacheBlock = 64;          // values per block of a key/value cache
 
 template <typename T>
@@ -41,24 +40,30 @@ __device__ __forceinline__ uint32_t absmax8(const uint4& v) {
 
 // The codes of eight values under the scale `s` (finite): 32 bits, the first value's code in the lowest four.
 //
-// fma(x, 7/s, 56) lies between 49 and 63, where fp32 has steps of 2^-18: a quotient 7x/s that is a tie k + 1/2 is off by at most
-// 7 * 2^-24 before that rounding and lands on the tie, and any other is 2^-15 or more away from one (14x - (2k+1)s is a multiple of
-// the smaller one's last place, for x >= s/14 and 11 significant bits), so it stays on its side.  Adding 1.5 * 2^23 then rounds to an
-// integer, ties to even, whose low four bits are q + 8 because 56 = 3 * 16 + 8.  Two operations a value instead of a division.
-// Scales below 2^-60 are lifted first, so that 7/s stays finite.
+// fma(x, 7/s, 56) lies between 49 and 63, where fp32 has steps of 2^-18: with 7/s good to 2^-23, a quotient 7x/s that is a tie k + 1/2 is
+// off by at most 7 * 2^-23 before that rounding and lands on the tie, and any other is 2^-15 or more away from one (14x - (2k+1)s is a
+// multiple of the smaller one's last place, for x >= s/14 and 11 significant bits), so it stays on its side.  Adding 1.5 * 2^23 then
+// rounds to an integer, ties to even, whose bits are 0x4b400000 + 56 + q; eight of those times the powers of 16, less what is not q + 8,
+// are the word.  Three operations a value, no division: 1/s is the hardware's estimate after one Newton step.  Very small and very
+// large scales, whose reciprocal may leave the normal numbers, are moved to the middle first.
 template <typename T>
 __device__ __forceinline__ uint32_t codes8(const uint4& v, float s) {
-    const float up = s < 0x1p-60f ? 0x1p100f : 1.0f;
-    const float r = s > 0.0f ? __fdiv_rn(7.0f, s * up) : 0.0f;
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t out = 0;
+    auto word = [&](float r, auto value) {
+        uint32_t out = 0u - 0x11111111u * (0x4b400000u + 56u - 8u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t a = __float_as_uint(__fadd_rn(__fmaf_rn(F16Bits<T>::lo(w[i]) * up, r, 56.0f), 12582912.0f));
-        const uint32_t b = __float_as_uint(__fadd_rn(__fmaf_rn(F16Bits<T>::hi(w[i]) * up, r, 56.0f), 12582912.0f));
-        out |= ((a & 15u) | ((b & 15u) << 4)) << (8 * i);
+        for (int i = 0; i < 8; ++i)
+            out += __float_as_uint(__fadd_rn(__fmaf_rn(value(i & 1 ? F16Bits<T>::hi(w[i / 2]) : F16Bits<T>::lo(w[i / 2])), r, 56.0f), 12582912.0f)) << (4 * i);
+        return out;
+    };
+    if (s >= 0x1p-60f && s <= 0x1p100f) {
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+        r = __fmaf_rn(r, __fmaf_rn(-s, r, 1.0f), r);
+        return word(7.0f * r, [](float x) { return x; });
     }
-    return out;
+    const float lift = s < 1.0f ? 0x1p100f : 0x1p-100f;
+    return word(s > 0.0f ? __fdiv_rn(7.0f, s * lift) : 0.0f, [lift](float x) { return x * lift; });
 }
 constexpr uint32_t kZeroCodes = 0x88888888u;
 
@@ -72,18 +77,10 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& v, int lanes, uint32_
     return bad ? kZeroCodes : codes8<T>(v, F16Bits<T>::one(m));
 }
 
-// s q / 7 in fp32, rounded once: s q is exact (14 bits), and the quotient is corrected by its remainder (Markstein's division by a
-// constant).  Scales outside the range in which the remainder is exact take the division itself, the largest of them a factor of
-// 2^20 lower, where 7 s does not overflow.
-__device__ __forceinline__ float value_of(float s, uint32_t code, bool plain) {
-    const float q = (float)((int)code - 8);
-    if (!plain) return s > 1.0f ? __fdiv_rn(s * 0x1p-20f * q, 7.0f) * 0x1p20f : __fdiv_rn(s * q, 7.0f);
-    const float m = s * q;
-    const float y = m * kInv7;
-    return __fmaf_rn(__fmaf_rn(-7.0f, y, m), kInv7, y);
-}
-__device__ __forceinline__ bool plain_scale(float s) { return (s > 0x1p-100f && s < 0x1p120f) || s == 0.0f; }
-
+// s q / 7 in fp32, rounded once, for the codes q of a word under one scale.  With 1/7 = h + l and s h = a + e exactly (a rounded, e its error),
+// s q / 7 = q a + q (e + s l): the first product is exact inside a multiply-add, the second is 2^-24 of it and its rounding harmless.
+// Scales outside the range in which e is exact take the division itself, the largest a factor of 2^20 lower, where 7 s does not overflow.
+__device__ __forceinline__ void values8(float s, uint32_t w, float (&y)[8]);
 // ---- tensor-core operands -----------------------------------------------------------------------------------------------------
 // Codes become the matrix instruction's operands in pairs, as the numbers -7 to 7 in the other operand's type.  Four bits c + 8 under the
 // exponent of 1024 are the fp16 number 1024 + 8 + c, four bits further up 1024 + 16 (8 + c); a packed subtraction or multiply-add
@@ -125,6 +122,23 @@ __device__ __forceinline__ Codes4 unpack8<__half>(uint32_t w) {
 template <>
 __device__ __forceinline__ Codes4 unpack8<__nv_bfloat16>(uint32_t w) {
     return {bf162_low(w), bf162_low(w >> 4), bf162_low(w >> 8), bf162_low(w >> 12)};
+}
+__device__ __forceinline__ void values8(float s, uint32_t w, float (&y)[8]) {
+    constexpr float H = 1.0f / 7.0f, L = (float)(1.0 / 7.0 - (double)H);
+    const Codes4 c = unpack8<__half>(w);
+    const uint32_t pairs[4] = {c.p04, c.p15, c.p26, c.p37};
+    if ((s > 0x1p-90f && s < 0x1p127f) || s == 0.0f) {
+        const float a = s * H, b = __fmaf_rn(s, L, __fmaf_rn(s, H, -a));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q = i < 4 ? F16Bits<__half>::lo(pairs[i]) : F16Bits<__half>::hi(pairs[i - 4]);
+            y[i] = __fmaf_rn(q, a, q * b);
+        }
+    } else {
+        const float up = s > 1.0f ? 0x1p20f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(s / up * (i < 4 ? F16Bits<__half>::lo(pairs[i]) : F16Bits<__half>::hi(pairs[i - 4])), 7.0f) * up;
+    }
 }
 // Eight neighbouring 16-bit values in that order.
 __device__ __forceinline__ uint4 paired8(const uint4& v) {

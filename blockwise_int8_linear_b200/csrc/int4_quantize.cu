@@ -135,10 +135,8 @@ __global__ void __launch_bounds__(kThreads) dequantize_int4_kernel(const uint8_t
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         if (first + n * kThreads >= rows.units) continue;
-        const bool plain = plain_scale(sc[n]);
         float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = value_of(sc[n], (w[n] >> (4 * j)) & 15u, plain);
+        values8(sc[n], w[n], y);
         if (FLAT) {
             store8(out + u[n].k, y);
         } else {

@@ -10,9 +10,10 @@ from oracle import int4_oracle as O
 F32 = np.float32
 
 
-def _codes_as_the_kernel(x, s):
-    """fma(x, 7/s, 56) + 1.5 * 2^23 in fp32 (the product of a 16-bit value and an fp32 one is exact in 64 bits)."""
+def _codes_as_the_kernel(x, s, off=0):
+    """fma(x, r, 56) + 1.5 * 2^23 in fp32 (the product of a 16-bit value and an fp32 one is exact in 64 bits), r = 7/s and `off` steps."""
     r = F32(7) / s.astype(F32)
+    r = (r.view(np.int32) + off).view(F32)
     v = (x.astype(np.float64) * r.astype(np.float64) + 56.0).astype(F32)
     u = v + F32(12582912.0)
     return (u.view(np.uint32) & 15).astype(np.int64) - 8
@@ -31,19 +32,23 @@ def test_quantizer_arithmetic_gives_the_definition(bits):
             q, rest = num // den, num % den
             q = q + ((2 * rest > den) | ((2 * rest == den) & (q % 2 == 1)))
             x = xm.astype(F32) * F32(2.0 ** -e)
-            assert np.array_equal(_codes_as_the_kernel(x, np.full(x.shape, sm, F32)), q)
-            assert np.array_equal(_codes_as_the_kernel(-x, np.full(x.shape, sm, F32)), -q)
+            for off in (-1, 0, 1):                         # a reciprocal that is not the nearest one
+                assert np.array_equal(_codes_as_the_kernel(x, np.full(x.shape, sm, F32), off), q)
+                assert np.array_equal(_codes_as_the_kernel(-x, np.full(x.shape, sm, F32), off), -q)
 
 
 def test_dequantizer_arithmetic_is_the_division():
-    """m / 7 by fp32 multiplication with one correction, m = s q of up to 14 bits: the fp32 number nearest to the quotient."""
-    m = np.arange(1, 1 << 14, dtype=np.float64)
-    inv = float(F32(1.0) / F32(7.0))
-    y = (m * inv).astype(F32).astype(np.float64)
-    r = m - 7.0 * y                                       # exact in 64 bits, and an fp32 number
-    assert np.array_equal(r.astype(F32).astype(np.float64), r)
-    got = (r * inv + y).astype(F32)
-    assert np.array_equal(got, (m.astype(F32) / F32(7.0)))
+    """fma(q, a, q b) with a = s h, b = (s h - a) + s l and 1/7 = h + l, in fp32: the fp32 number nearest to s q / 7, for every significand of a
+    16-bit scale (11 bits) and every code."""
+    s = np.arange(1 << 10, 1 << 11, dtype=np.float64)[:, None]
+    q = np.arange(-7, 8, dtype=np.float64)[None]
+    h = float(F32(1.0) / F32(7.0))
+    low = float(F32(1.0 / 7.0 - h))
+    f = lambda t: t.astype(F32).astype(np.float64)
+    a = f(s * h)
+    b = f(s * low + f(s * h - a))                         # both products are exact in 64 bits
+    got = (q * a + f(q * b)).astype(F32)
+    assert np.array_equal(got, (s * q).astype(F32) / F32(7.0))
 
 
 def test_packing_order():
