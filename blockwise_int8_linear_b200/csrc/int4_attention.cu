@@ -13,7 +13,7 @@
 // numbers, normalised by a power of two that follows the largest scale met, like the running maximum of the softmax.  P leaves the first product with its rows along the lanes and
 // enters the second transposed (movmatrix).  Sums, statistics and scales are fp32.
 //
-// A warp takes steps of 16, 32 or 64 rows (4 KB), the next one on its way into shared memory while this one is multiplied.  The warps of a CTA and the CTAs of a cluster divide the rows of one cache head
+// A warp takes steps of 16, 32 or 64 rows (4 KB), the next one on its way into shared memory while one is multiplied.  The warps of a CTA and the CTAs of a cluster divide the rows of one cache head
 // (each reads the lengths and takes its share of what there really is) and are joined over distributed shared memory; more than eight
 // shares go through a workspace and a second kernel.  Every sum has a fixed order.
 #include "int4_common.cuh"
@@ -41,6 +41,7 @@ struct AttnArgs {
     int64_t lengths_step, starts_step;
     void* out;
     float* ws;               // [tile][share][kCols][D] sums, then [tile][share][kCols] pairs (maximum, total)
+    CodeBits bits;
     int B, Hq, Hkv, T, G;
     int col_tiles, shares;
     float scale_log2;        // scale * log2(e)
@@ -80,35 +81,47 @@ constexpr int kStepTiles = D == 64 ? 4 : D == 128 ? 2 : 1;       // 16 rows each
 template <int D>
 constexpr int kResident = D == 256 ? 3 : 4;                     // CTAs of an SM
 
-// A warp's rows of one step in shared memory: k, v (16 more or less than a multiple of 32 or 64 bytes apart, so that what the lanes read at a
-// time lies in different banks), their scales.  A warp has two steps there: one in use, one on its way.
+// A warp's rows of one step in shared memory: k, v, their scales.  A warp has two steps there: one in use, one on its way.
+//
+// Rows lie one behind the other without padding; the 16-byte pieces of every 128 bytes are permuted so that what the lanes read at a time
+// lies in different banks: of k eight bytes (piece 2u + c / 2) of rows g, of v four bytes (piece 2u + g / 4) of every other row.  The
+// permutation is an exclusive or with a number that is the same for rows eight apart, and so are its effects: a lane's address for the
+// next 64 values or the next row is its first one with some bits flipped.
 template <int D>
 struct Ring {
-    static constexpr int kRows = 16 * kStepTiles<D>, kPitchK = D / 2 + (D == 64 ? 0 : 32), kPitchV = D / 2 + 16, kRowScales = D / 64 * 2;
-    static constexpr int kV = kRows * kPitchK, kScalesK = kV + kRows * kPitchV, kScalesV = kScalesK + kRows * kRowScales, kBytes = kScalesV + kRows * kRowScales;
+    static constexpr int kRows = 16 * kStepTiles<D>, kRowScales = D / 64 * 2;
+    static constexpr int kV = kRows * (D / 2), kScalesK = 2 * kV, kScalesV = kScalesK + kRows * kRowScales, kBytes = kScalesV + kRows * kRowScales;
     static constexpr int kSteps = 2;
+    static __device__ __forceinline__ int at(int row, int piece) {
+        if (D == 64) return (row >> 2) * 128 + ((((row & 3) << 1) | piece) ^ (((row >> 2) & 1) << 1)) * 16;
+        if (D == 128) return (row >> 1) * 128 + ((((row & 1) << 2) | piece) ^ (((row >> 1) & 3) << 1)) * 16;
+        return row * 128 + (piece ^ (((row ^ (row >> 1)) & 3) << 1)) * 16;
+    }
+    static constexpr int kOdd = D == 128 ? 64 : 32, kOddAdd = D == 256 ? 128 : 0;        // from an even row to the next: bits to flip, bytes to add
 };
 
+// Shared memory: queries; the warps' rings, afterwards the warps' sums and the CTA's; statistics.
 template <int D>
-constexpr int attn_smem() {
-    // queries; the warps' rings, and afterwards the warps' sums (eight columns at a time) and the CTA's; statistics
-    constexpr int rings = kWarps * Ring<D>::kSteps * Ring<D>::kBytes, sums = kWarps * 8 * (D + 4) * 4 + kCols * D * 4;
-    return kCols * (2 * D + 16) + (rings > sums ? rings : sums) + (kWarps * 2 + 2 + kClusterShares) * kCols * 4 + kCols * 4;
-}
+struct Smem {
+    static constexpr int kPitch = 2 * D + 16, kRings = kCols * kPitch, kBuf = D + 4;         // a query's row in bytes, a sum's in floats
+    static constexpr int kRingBytes = kWarps * Ring<D>::kSteps * Ring<D>::kBytes, kSumBytes = (kWarps * kCols * kBuf + kCols * D) * 4;
+    static constexpr int kStats = kRings + (kRingBytes > kSumBytes ? kRingBytes : kSumBytes);
+    static constexpr int kBytes = kStats + (2 * kWarps + 3 + kClusterShares) * kCols * 4;
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(const AttnArgs a) {
     constexpr bool FINE = std::is_same<T, __half>::value;
-    constexpr int U = D / 64, TT = kStepTiles<D>, STEP = 16 * TT, COLS = kCols, PITCH = 2 * D + 16, BUF = D + 4;
-    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int U = D / 64, TT = kStepTiles<D>, STEP = 16 * TT, COLS = kCols, PITCH = Smem<D>::kPitch, BUF = Smem<D>::kBuf;
+    extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* const xs = smem;                                                    // [COLS] rows of PITCH bytes
-    float* const warp_m = reinterpret_cast<float*>(xs + COLS * PITCH);           // [kWarps][COLS]
+    uint8_t* const rings = smem + Smem<D>::kRings;                               // on a 128-byte boundary
+    float* const warp_m = reinterpret_cast<float*>(smem + Smem<D>::kStats);      // [kWarps][COLS]
     float* const warp_l = warp_m + kWarps * COLS;                                // [kWarps][COLS]
     float* const cta_m = warp_l + kWarps * COLS;                                 // [COLS]
     float* const cta_l = cta_m + COLS;                                           // [COLS]
     float* const weight = cta_l + COLS;                                          // [kClusterShares][COLS]
     float* const factor = weight + kClusterShares * COLS;                        // [COLS]
-    uint8_t* const rings = reinterpret_cast<uint8_t*>(factor + COLS);
     float* const buf = reinterpret_cast<float*>(rings);                          // [kWarps][8][BUF], when the rings are done with
     float* const sums = buf + kWarps * 8 * BUF;                                  // [COLS][D]
 
@@ -154,19 +167,24 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
     const unsigned short* const ksp = static_cast<const unsigned short*>(a.cache.k_state) + b * a.cache.ks_batch + h * a.cache.ks_head;
     const unsigned short* const vsp = static_cast<const unsigned short*>(a.cache.v_state) + b * a.cache.vs_batch + h * a.cache.vs_head;
     using Slot = Ring<D>;
+    const CodeBits bits = a.bits;
     uint8_t* const ring = rings + warp * (Slot::kSteps * Slot::kBytes);
+    const int at_k = Slot::at(g, c >> 1) + 8 * (c & 1), at_v = Slot::at(2 * c, g >> 2) + 4 * (g & 3);       // this lane's first codes
     // One step's rows into a slot.  Rows behind the last one are that one again; they are masked.
     auto fill = [&](uint8_t* slot, int base) {
         constexpr int CH = D / 32;                         // 16-byte pieces of a row; 32 lanes take 32 / CH rows at a time
         const bool whole = base + STEP <= last;
         const int row0 = lane / CH, piece = lane % CH * 16;
-        const uint32_t to_k = (uint32_t)__cvta_generic_to_shared(slot + row0 * Slot::kPitchK + piece), to_v = (uint32_t)__cvta_generic_to_shared(slot + Slot::kV + row0 * Slot::kPitchV + piece);
+        constexpr int AT_ONCE = 32 / CH;
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(slot) + Slot::at(row0, lane % CH);
         const uint8_t *from_k = kp + (int64_t)base * (D / 2) + piece, *from_v = vp + (int64_t)base * (D / 2) + piece;
 #pragma unroll
-        for (int i = 0; i < STEP * CH / 32; ++i) {
-            const int row = whole ? row0 + i * (32 / CH) : min(row0 + i * (32 / CH), last - 1 - base);
-            copy16(to_k + i * (32 / CH) * Slot::kPitchK, from_k + row * (D / 2));
-            copy16(to_v + i * (32 / CH) * Slot::kPitchV, from_v + row * (D / 2));
+        for (int i = 0; i < STEP / AT_ONCE; ++i) {
+            const int row = whole ? row0 + i * AT_ONCE : min(row0 + i * AT_ONCE, last - 1 - base);
+            // rows that are not eight apart are permuted differently
+            const uint32_t dst = AT_ONCE % 8 == 0 ? to + i * AT_ONCE * (D / 2) : (uint32_t)__cvta_generic_to_shared(slot) + Slot::at(row0 + i * AT_ONCE, lane % CH);
+            copy16(dst, from_k + row * (D / 2));
+            copy16(dst + Slot::kV, from_v + row * (D / 2));
         }
         if (U >= 2 || (a.s_vec && whole)) {                // a row's scales (two rows' where they have one) per lane, k and v in turn
             constexpr int BYTES = U == 4 ? 8 : 4, ROWS = BYTES / (2 * U), LANES = STEP / ROWS;
@@ -207,9 +225,9 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
             scales_of(slot + Slot::kScalesK, 16 * i + g + 8, s1);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint8_t* const k = slot + (16 * i + g) * Slot::kPitchK + 32 * u + 8 * c;
-                const uint2 w0 = *reinterpret_cast<const uint2*>(k), w1 = *reinterpret_cast<const uint2*>(k + 8 * Slot::kPitchK);
-                const Codes4 r0a = unpack8<__half>(w0.x), r0b = unpack8<__half>(w0.y), r1a = unpack8<__half>(w1.x), r1b = unpack8<__half>(w1.y);
+                const uint8_t* const k = slot + (at_k ^ (32 * u)) + 16 * i * (D / 2);
+                const uint2 w0 = *reinterpret_cast<const uint2*>(k), w1 = *reinterpret_cast<const uint2*>(k + 8 * (D / 2));
+                const Codes4 r0a = unpack8<__half>(w0.x, bits), r0b = unpack8<__half>(w0.y, bits), r1a = unpack8<__half>(w1.x, bits), r1b = unpack8<__half>(w1.y, bits);
                 const uint4* x = reinterpret_cast<const uint4*>(xs + g * PITCH + u * 128 + c * 32);
                 const uint4 xa = x[0], xb = x[1];
                 float d[4];
@@ -304,10 +322,11 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
                     bh[r] = transpose8x8(hi);
                     if (FINE) bl[r] = transpose8x8(pack_f16x2(x0 - H::lo(hi), x1 - H::hi(hi)));
                 }
-                const uint8_t* const v = slot + Slot::kV + (16 * i + 2 * c) * Slot::kPitchV + 32 * u + 4 * g;
+                const uint8_t* const even = slot + (at_v ^ (32 * u)) + Slot::kV + 16 * i * (D / 2);
+                const uint8_t* const odd = slot + ((at_v ^ (32 * u)) ^ Slot::kOdd) + Slot::kOddAdd + Slot::kV + 16 * i * (D / 2);
                 uint32_t w[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) w[r] = *reinterpret_cast<const uint32_t*>(v + ((r & 1) + 8 * (r >> 1)) * Slot::kPitchV);
+                for (int r = 0; r < 4; ++r) w[r] = *reinterpret_cast<const uint32_t*>((r & 1 ? odd : even) + 8 * (r >> 1) * (D / 2));
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     // four codes of two rows: nibble n of both in bits 4n and 16 + 4n
@@ -316,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const uint32_t x = w01 >> (8 * j), y = w23 >> (8 * j);
-                        const uint32_t a0 = half2_low(x), a1 = half2_high(x), a2 = half2_low(y), a3 = half2_high(y);
+                        const uint32_t a0 = half2_low(x, bits), a1 = half2_high(x, bits), a2 = half2_low(y, bits), a3 = half2_high(y, bits);
                         mma16<__half>(o[4 * u + 2 * half + j], a0, a1, a2, a3, bh[0], bh[1]);
                         if (FINE) mma16<__half>(o[4 * u + 2 * half + j], a0, a1, a2, a3, bl[0], bl[1]);
                     }
@@ -324,9 +343,14 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
             }
     };
 
-    int slot = 0;
-    if (first + warp * STEP < last) fill(ring, first + warp * STEP);
-    commit_copies();
+    int in = 0, out = 0;                                  // slots of the ring
+    auto fill_next = [&](int base) {
+        if (base < last) fill(ring + in * Slot::kBytes, base);
+        commit_copies();
+        in = in + 1 == Slot::kSteps ? 0 : in + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < Slot::kSteps - 1; ++i) fill_next(first + (warp + i * kWarps) * STEP);
 
     // ---- queries: fp16 with a power of two per query; D / 8 lanes a query
     for (int i = threadIdx.x; i < COLS * (D / 8); i += kThreads) {
@@ -348,15 +372,13 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
     for (int j = 0; j < 2; ++j) fac[j] = factor[2 * c + j];
 
     for (int base = first + warp * STEP; base < last; base += kWarps * STEP) {
-        const int next = base + kWarps * STEP;
-        if (next < last) fill(ring + (slot ^ 1) * Slot::kBytes, next);
-        commit_copies();
-        wait_copies<1>();
+        fill_next(base + (Slot::kSteps - 1) * kWarps * STEP);         // into the slot that every lane left at the end of the step before
+        wait_copies<Slot::kSteps - 1>();
         __syncwarp();
-        if (base >= start && base + STEP <= unmasked) multiply(ring + slot * Slot::kBytes, base, std::false_type{});
-        else multiply(ring + slot * Slot::kBytes, base, std::true_type{});
+        if (base >= start && base + STEP <= unmasked) multiply(ring + out * Slot::kBytes, base, std::false_type{});
+        else multiply(ring + out * Slot::kBytes, base, std::true_type{});
         __syncwarp();
-        slot ^= 1;
+        out = out + 1 == Slot::kSteps ? 0 : out + 1;
     }
     wait_copies<0>();
 
@@ -529,12 +551,16 @@ Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     Plan p;
     p.col_tiles = (int)((R + kCols - 1) / kCols);
     p.tiles = B * Hkv * p.col_tiles;
-    // As many CTAs as the device holds at once, as long as a warp of a full cache has two steps; and shares of 2048 rows in long caches, whose
-    // sequences may differ much in length (32 sequences of 1 to 8192 rows, 8 heads: 65 us in 2 shares, 55 in 4, 61 in 8; 64 of 4096 rows
-    // each: 71 us in 1, 68 in 2, 82 in 4).  The clusters' sizes are powers of two.
-    const int64_t step = 16 * (D == 64 ? kStepTiles<64> : D == 128 ? kStepTiles<128> : kStepTiles<256>), resident = (D == 256 ? kResident<256> : kResident<128>) * sm_count();
-    const int64_t useful = (max_len + 2 * kWarps * step - 1) / (2 * kWarps * step), long_ones = max_len / 2048;
-    int64_t want = resident / p.tiles;
+    // As many CTAs as the device holds at once.  Few tiles are divided down to a step for each warp (one sequence of 2048 rows, 8 heads: 16 us in
+    // 1 share, 8 in 4, 6 in 16), beyond two CTAs an SM into 512 rows and more (16384 rows: 13.1 us in 16 shares, 11.5 in 32, 13.5 in 74), more
+    // tiles than SMs only into 1024 rows and more (256 tiles of 576 rows: 10.6 us in 1, 11.7 in 2).  Long
+    // caches, whose sequences may differ much in length, have shares of 2048 rows (32 sequences of 1 to 8192 rows, 8 heads: 65 us in 2, 55
+    // in 4, 61 in 8; 64 of 4096 rows each: 71 us in 1, 68 in 2, 82 in 4).  The clusters' sizes are powers of two.
+    const int64_t step = 16 * (D == 64 ? kStepTiles<64> : D == 128 ? kStepTiles<128> : kStepTiles<256>), sms = sm_count();
+    const int64_t useful = p.tiles < sms ? (max_len + kWarps * step - 1) / (kWarps * step) : max_len / 1024, long_ones = max_len / 2048;
+    int64_t want = (D == 256 ? kResident<256> : kResident<128>) * sms / p.tiles;
+    const int64_t two = 2 * sms / p.tiles, half = max_len / 512;
+    if (want > two && want > half) want = two > half ? two : half;
     if (want < kClusterShares && want < long_ones) want = long_ones < kClusterShares ? long_ones : kClusterShares;
     int64_t s = useful < want ? useful : want;
     if (s > kMaxShares) s = kMaxShares;
@@ -549,7 +575,7 @@ Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
 
 template <typename T, int D>
 int launch(const AttnArgs& a, int64_t tiles, cudaStream_t st) {
-    constexpr int smem = attn_smem<D>();
+    constexpr int smem = Smem<D>::kBytes;
     static SmemOptIn opt_in;
     if (int rc = opt_in.ensure(attention_int4_kernel<T, D>, smem)) return rc;
     const unsigned grid = (unsigned)(tiles * a.shares);
@@ -597,6 +623,7 @@ int launch_attention_int4(const void* q, int dt, int64_t q_batch, int64_t q_head
     a.starts_step = starts_step;
     a.out = out;
     a.ws = static_cast<float*>(workspace);
+    a.bits = code_bits<__half>();
     a.B = (int)B;
     a.Hq = (int)Hq;
     a.Hkv = (int)Hkv;

@@ -40,7 +40,9 @@ struct MatmulArgs {
     int64_t ldc;
     int bias_dtype, out_dtype;
     int M, N, K;
+    CodeBits bits;
     int tiles;               // of 16 * warps_n rows of W
+    int group;               // tiles whose sums a CTA collects before they are added
     int warps_n;             // warps of a CTA over rows of W; the others divide K
     int pieces;              // of K
     int ranks;               // CTAs of a cluster
@@ -112,14 +114,12 @@ __device__ __forceinline__ void fill(uint8_t* dst, const MatmulArgs& a, int n0, 
 template <int NT>
 constexpr int kRing = NT <= 2 ? 3 : 2;
 
-// Sizes in shared memory: the warps' rings, x, and the sums of the warps that share rows with the CTA's own behind them.  Up to 16 columns
-// have those twice: one tile's are read while the next one's are written.
+// Sizes in shared memory: the warps' rings, x, and for a group of tiles the sums of the warps that share rows, with the CTA's own behind
+// them where a cluster adds them.
 template <int BLOCK, int NT>
 constexpr int kRingBytes = kWarps * kRing<NT> * kPieceBytes<BLOCK>;
-template <int NT>
-constexpr int kSumBuffers = NT <= 2 ? 2 : 1;
 inline __host__ __device__ int x_pitch(int pieces) { return pieces * kPiece * 2 + 16; }
-inline __host__ __device__ int sum_parts(int warps_k) { return warps_k == 1 ? 1 : warps_k + 1; }
+inline __host__ __device__ int sum_parts(int warps_k, int ranks) { return warps_k == 1 || ranks == 1 ? warps_k : warps_k + 1; }
 
 template <typename T, int BLOCK, int NT>
 __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulArgs a) {
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
     const int pitch = x_pitch(a.pieces_stage);
     uint8_t* const xs = smem + kRingBytes<BLOCK, NT>;
     const int sums = rows_x * rows_cta;
-    float* const part = reinterpret_cast<float*>(xs + rows_x * pitch);       // [buffer][part][rows_x][rows_cta]
+    float* const part = reinterpret_cast<float*>(xs + rows_x * pitch);       // [tile of the group][part][rows_x][rows_cta]
 
     // x of pieces base to end: as copies into the slots that the lanes read (lane c reads 32 bytes of every 64 values: what meets its two
     // words of codes; with blocks of 32, of both halves), then, by the thread that copied them, into the order of the codes.
@@ -174,33 +174,44 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
         });
     };
 
+    const CodeBits bits = a.bits;
     after_predecessor();
     const bool once = a.pieces_cta <= a.pieces_stage;         // all of this CTA's x fits
     if (once) fetch_x(first, last);
     commit_copies();
-    int f_tile = tile0, f_piece = first + wk, in = 0, out = 0;          // what is filled next, and where
-    // this lane's part of a piece of whole rows: 16 bytes of every fourth row, a row's scales
-    const int64_t lane_codes = (int64_t)(lane >> 3) * a.ldw + 16 * (lane & 7), lane_scales = (int64_t)(lane & 15) * a.blocks;
-    const int inside = a.w_vec && a.s_vec ? a.K / kPiece : 0;          // pieces below are whole and aligned
+    // What is filled next: a tile and a piece of it, and this lane's part: 16 bytes of every fourth row, a row's scales.  The addresses move
+    // on by constants; they are used where the piece is whole and aligned and all of its rows exist.
+    int f_tile = tile0, f_piece = first + wk, in = 0, out = 0;
+    const int aligned_pieces = a.w_vec && a.s_vec ? a.K / kPiece : 0, whole_tiles = a.N / rows_cta;
+    const int64_t row0 = (int64_t)tile0 * rows_cta + 16 * wn;
+    const uint8_t* w_tile = a.W + (row0 + (lane >> 3)) * a.ldw + (int64_t)f_piece * (kPiece / 2) + 16 * (lane & 7);
+    const unsigned short* s_tile = a.sW + (row0 + (lane & 15)) * a.blocks + (int64_t)f_piece * PER;
+    const int64_t w_tile_step = (int64_t)tile_step * rows_cta * a.ldw, s_tile_step = (int64_t)tile_step * rows_cta * a.blocks, w_rows = 4 * a.ldw;
+    const uint8_t* w_at = w_tile;
+    const unsigned short* s_at = s_tile;
+    const uint32_t w_slot = (uint32_t)__cvta_generic_to_shared(ring + (lane >> 3) * kCodePitch + 16 * (lane & 7));
+    const uint32_t s_slot = (uint32_t)__cvta_generic_to_shared(ring + 16 * kCodePitch + (lane & 15) * (2 * PER));
     auto fill_next = [&] {
-        if (f_piece >= last) f_piece = first + wk, f_tile += tile_step;
+        if (f_piece >= last) {
+            f_piece = first + wk, f_tile += tile_step;
+            w_at = w_tile += w_tile_step;
+            s_at = s_tile += s_tile_step;
+        }
         if (f_tile < a.tiles && f_piece < last) {
-            const int n0 = f_tile * rows_cta + 16 * wn;
-            uint8_t* const dst = ring + in * kPieceBytes<BLOCK>;
-            if (f_piece < inside && n0 + 16 <= a.N) {
-                const uint8_t* src = a.W + ((int64_t)n0 * a.ldw + (int64_t)f_piece * (kPiece / 2)) + lane_codes;
-                const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + (lane >> 3) * kCodePitch + 16 * (lane & 7));
+            if (f_piece < aligned_pieces && f_tile < whole_tiles) {
+                const uint32_t to = w_slot + in * kPieceBytes<BLOCK>;
+                const uint8_t* src = w_at;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) copy16(to + 4 * i * kCodePitch, src + (int64_t)(4 * i) * a.ldw);
-                if (lane < 16)
-                    copy_some<2 * PER>((uint32_t)__cvta_generic_to_shared(dst + 16 * kCodePitch + lane * (2 * PER)),
-                                       a.sW + ((int64_t)n0 * a.blocks + (int64_t)f_piece * PER) + lane_scales);
+                for (int i = 0; i < 4; ++i, src += w_rows) copy16(to + 4 * i * kCodePitch, src);
+                if (lane < 16) copy_some<2 * PER>(s_slot + in * kPieceBytes<BLOCK>, s_at);
             } else {
-                fill<BLOCK>(dst, a, n0, f_piece, lane);
+                fill<BLOCK>(ring + in * kPieceBytes<BLOCK>, a, f_tile * rows_cta + 16 * wn, f_piece, lane);
             }
         }
         commit_copies();
         f_piece += warps_k;
+        w_at += warps_k * (kPiece / 2);
+        s_at += warps_k * PER;
         in = in + 1 == RING ? 0 : in + 1;
     };
 #pragma unroll
@@ -211,113 +222,116 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
         __syncthreads();
     }
 
-    int parity = 0;
-    for (int tile = tile0; tile < a.tiles; tile += tile_step, parity = kSumBuffers<NT> - 1 - parity) {
-        float y[NT][4] = {};
-        for (int base = first, piece = first + wk; base < last; base += a.pieces_stage) {
-            const int end = min(last, base + a.pieces_stage);
-            if (!once) {
-                __syncthreads();
-                fetch_x(base, end);
-                commit_copies();
-                wait_copies<0>();
-                order_x(base, end);
-                __syncthreads();
-            }
-            for (; piece < end; piece += warps_k) {
-                fill_next();                                  // into the slot that every lane left at the end of the piece before
-                wait_copies<RING - 1>();
-                __syncwarp();
-                const uint8_t* const lo = ring + out * kPieceBytes<BLOCK> + g * kCodePitch + (BLOCK == 32 ? 4 : 8) * c;
-                const uint8_t* const hi = lo + 8 * kCodePitch;
-                const uint32_t* const sp = reinterpret_cast<const uint32_t*>(ring + out * kPieceBytes<BLOCK> + 16 * kCodePitch + g * (2 * PER));
-                uint32_t sw[2][PER / 2];
-#pragma unroll
-                for (int i = 0; i < PER / 2; ++i) sw[0][i] = sp[i], sw[1][i] = sp[4 * PER + i];
-                auto scale = [&](int r, int i) { return i & 1 ? F16Bits<T>::hi(sw[r][i / 2]) : F16Bits<T>::lo(sw[r][i / 2]); };
-                const uint8_t* const xp = xs + (piece - base) * (kPiece * 2) + c * 32;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    uint2 w0, w1;
-                    if (BLOCK == 32) {
-                        w0 = make_uint2(*reinterpret_cast<const uint32_t*>(lo + 32 * u), *reinterpret_cast<const uint32_t*>(lo + 32 * u + 16));
-                        w1 = make_uint2(*reinterpret_cast<const uint32_t*>(hi + 32 * u), *reinterpret_cast<const uint32_t*>(hi + 32 * u + 16));
-                    } else {
-                        w0 = *reinterpret_cast<const uint2*>(lo + 32 * u);
-                        w1 = *reinterpret_cast<const uint2*>(hi + 32 * u);
-                    }
-                    const Codes4 r0a = unpack8<T>(w0.x), r0b = unpack8<T>(w0.y), r1a = unpack8<T>(w1.x), r1b = unpack8<T>(w1.y);
-                    const int AFTER = BLOCK == 32 ? 2 * u + 1 : u * PER / 4;         // the scale of (the second half of) these 64 values
-                    // eight columns, or twice eight, whose sums do not wait for one another
-                    constexpr int PAIR = NT == 1 ? 1 : 2;
-#pragma unroll
-                    for (int t = 0; t < NT; t += PAIR) {
-                        uint4 xa[PAIR], xb[PAIR];
-                        float d[PAIR][4];
-#pragma unroll
-                        for (int h = 0; h < PAIR; ++h) {
-                            // columns behind the last row of x read that row again and are not stored
-                            const uint4* p = reinterpret_cast<const uint4*>(xp + min(8 * (t + h) + g, rows_x - 1) * pitch + u * 128);
-                            xa[h] = p[0];
-                            xb[h] = p[1];
-                        }
-                        auto scaled = [&](int h, int i) {
-                            float (&y4)[4] = y[t + h];
-                            y4[0] = fmaf(d[h][0], scale(0, i), y4[0]);
-                            y4[1] = fmaf(d[h][1], scale(0, i), y4[1]);
-                            y4[2] = fmaf(d[h][2], scale(1, i), y4[2]);
-                            y4[3] = fmaf(d[h][3], scale(1, i), y4[3]);
-                        };
-#pragma unroll
-                        for (int h = 0; h < PAIR; ++h) mma16_first<T>(d[h], r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa[h].x, xa[h].y);
-#pragma unroll
-                        for (int h = 0; h < PAIR; ++h) mma16<T>(d[h], r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa[h].z, xa[h].w);
-#pragma unroll
-                        for (int h = 0; h < PAIR; ++h) {
-                            if (BLOCK == 32) {
-                                scaled(h, 2 * u);
-                                mma16_first<T>(d[h], r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb[h].x, xb[h].y);
-                            } else {
-                                mma16<T>(d[h], r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb[h].x, xb[h].y);
-                            }
-                        }
-#pragma unroll
-                        for (int h = 0; h < PAIR; ++h) mma16<T>(d[h], r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb[h].z, xb[h].w);
-#pragma unroll
-                        for (int h = 0; h < PAIR; ++h) scaled(h, AFTER);
-                    }
+    const int parts = sum_parts(warps_k, ranks);
+    for (int group = tile0; group < a.tiles; group += a.group * tile_step) {
+        // ---- the group's tiles one after the other; no warp waits for another one in between
+        const int count = min(a.group, (a.tiles - group + tile_step - 1) / tile_step);
+        for (int in_group = 0; in_group < count; ++in_group) {
+            float y[NT][4] = {};
+            for (int base = first, piece = first + wk; base < last; base += a.pieces_stage) {
+                const int end = min(last, base + a.pieces_stage);
+                if (!once) {
+                    __syncthreads();
+                    fetch_x(base, end);
+                    commit_copies();
+                    wait_copies<0>();
+                    order_x(base, end);
+                    __syncthreads();
                 }
-                out = out + 1 == RING ? 0 : out + 1;
-                __syncwarp();
+                for (; piece < end; piece += warps_k) {
+                    fill_next();                                  // into the slot that every lane left at the end of the piece before
+                    wait_copies<RING - 1>();
+                    __syncwarp();
+                    const uint8_t* const lo = ring + out * kPieceBytes<BLOCK> + g * kCodePitch + (BLOCK == 32 ? 4 : 8) * c;
+                    const uint8_t* const hi = lo + 8 * kCodePitch;
+                    const uint32_t* const sp = reinterpret_cast<const uint32_t*>(ring + out * kPieceBytes<BLOCK> + 16 * kCodePitch + g * (2 * PER));
+                    uint32_t sw[2][PER / 2];
+#pragma unroll
+                    for (int i = 0; i < PER / 2; ++i) sw[0][i] = sp[i], sw[1][i] = sp[4 * PER + i];
+                    auto scale = [&](int r, int i) { return i & 1 ? F16Bits<T>::hi(sw[r][i / 2]) : F16Bits<T>::lo(sw[r][i / 2]); };
+                    const uint8_t* const xp = xs + (piece - base) * (kPiece * 2) + c * 32;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        uint2 w0, w1;
+                        if (BLOCK == 32) {
+                            w0 = make_uint2(*reinterpret_cast<const uint32_t*>(lo + 32 * u), *reinterpret_cast<const uint32_t*>(lo + 32 * u + 16));
+                            w1 = make_uint2(*reinterpret_cast<const uint32_t*>(hi + 32 * u), *reinterpret_cast<const uint32_t*>(hi + 32 * u + 16));
+                        } else {
+                            w0 = *reinterpret_cast<const uint2*>(lo + 32 * u);
+                            w1 = *reinterpret_cast<const uint2*>(hi + 32 * u);
+                        }
+                        const Codes4 r0a = unpack8<T>(w0.x, bits), r0b = unpack8<T>(w0.y, bits), r1a = unpack8<T>(w1.x, bits), r1b = unpack8<T>(w1.y, bits);
+                        const int AFTER = BLOCK == 32 ? 2 * u + 1 : u * PER / 4;         // the scale of (the second half of) these 64 values
+                        // eight columns, or twice eight, whose sums do not wait for one another
+                        constexpr int PAIR = NT == 1 ? 1 : 2;
+#pragma unroll
+                        for (int t = 0; t < NT; t += PAIR) {
+                            uint4 xa[PAIR], xb[PAIR];
+                            float d[PAIR][4];
+#pragma unroll
+                            for (int h = 0; h < PAIR; ++h) {
+                                // columns behind the last row of x read that row again and are not stored
+                                const uint4* p = reinterpret_cast<const uint4*>(xp + min(8 * (t + h) + g, rows_x - 1) * pitch + u * 128);
+                                xa[h] = p[0];
+                                xb[h] = p[1];
+                            }
+                            auto scaled = [&](int h, int i) {
+                                float (&y4)[4] = y[t + h];
+                                y4[0] = fmaf(d[h][0], scale(0, i), y4[0]);
+                                y4[1] = fmaf(d[h][1], scale(0, i), y4[1]);
+                                y4[2] = fmaf(d[h][2], scale(1, i), y4[2]);
+                                y4[3] = fmaf(d[h][3], scale(1, i), y4[3]);
+                            };
+#pragma unroll
+                            for (int h = 0; h < PAIR; ++h) mma16_first<T>(d[h], r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa[h].x, xa[h].y);
+#pragma unroll
+                            for (int h = 0; h < PAIR; ++h) mma16<T>(d[h], r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa[h].z, xa[h].w);
+#pragma unroll
+                            for (int h = 0; h < PAIR; ++h) {
+                                if (BLOCK == 32) {
+                                    scaled(h, 2 * u);
+                                    mma16_first<T>(d[h], r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb[h].x, xb[h].y);
+                                } else {
+                                    mma16<T>(d[h], r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb[h].x, xb[h].y);
+                                }
+                            }
+#pragma unroll
+                            for (int h = 0; h < PAIR; ++h) mma16<T>(d[h], r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb[h].z, xb[h].w);
+#pragma unroll
+                            for (int h = 0; h < PAIR; ++h) scaled(h, AFTER);
+                        }
+                    }
+                    out = out + 1 == RING ? 0 : out + 1;
+                    __syncwarp();
+                }
             }
+            float* const mine = part + (size_t)(in_group * parts + wk) * sums;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int col = 8 * t + 2 * c + (i & 1);
+                    if (col < rows_x) mine[col * rows_cta + 16 * wn + g + 8 * (i >> 1)] = y[t][i];
+                }
         }
-        // ---- sums over the warps that share rows, then over the cluster: both in a fixed order
-        float* const mine = part + (size_t)parity * sum_parts(warps_k) * sums;
-        float* const total = warps_k == 1 ? mine : mine + (size_t)warps_k * sums;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int col = 8 * t + 2 * c + (i & 1);
-                if (col < rows_x) mine[(size_t)wk * sums + col * rows_cta + 16 * wn + g + 8 * (i >> 1)] = y[t][i];
-            }
         __syncthreads();
-        // Four rows at a time; every load is under way before the first sum.
+        // ---- sums over the warps that share rows, then over the cluster: both in a fixed order.  Four rows at a time; loads are under way
+        // before the first sum.
         auto add = [](float4& s, const float4& v) { s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w; };
-        auto warps_sum = [&](int i) {
-            float4 s = *reinterpret_cast<const float4*>(mine + i);
+        auto warps_sum = [&](const float* p) {
+            float4 s = *reinterpret_cast<const float4*>(p);
             for (int w0 = 1; w0 < warps_k; w0 += 3) {             // 2, 4, 8 or 16 warps: 1, 3, 7 or 15 more
                 float4 v[3];
 #pragma unroll
                 for (int w = 0; w < 3; ++w)
-                    if (w0 + w < warps_k) v[w] = *reinterpret_cast<const float4*>(mine + (size_t)(w0 + w) * sums + i);
+                    if (w0 + w < warps_k) v[w] = *reinterpret_cast<const float4*>(p + (size_t)(w0 + w) * sums);
 #pragma unroll
                 for (int w = 0; w < 3; ++w)
                     if (w0 + w < warps_k) add(s, v[w]);
             }
             return s;
         };
-        auto store = [&](int i, const float4& s) {
+        auto store = [&](int tile, int i, const float4& s) {
             const int m = m0 + i / rows_cta, n = tile * rows_cta + i % rows_cta;
             const float y[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
@@ -329,28 +343,38 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
                 store_from_float(a.C, a.out_dtype, (int64_t)m * a.ldc + n + j, v);
             }
         };
+        const int values = count * sums;
         if (ranks == 1) {
-            for (int i = 4 * threadIdx.x; i < sums; i += 4 * kThreads) store(i, warps_sum(i));
+            for (int i = 4 * threadIdx.x; i < values; i += 4 * kThreads) {
+                const int k = i / sums, e = i - k * sums;
+                store(group + k * tile_step, e, warps_sum(part + (size_t)k * parts * sums + e));
+            }
         } else {
             if (warps_k > 1)
-                for (int i = 4 * threadIdx.x; i < sums; i += 4 * kThreads) *reinterpret_cast<float4*>(total + i) = warps_sum(i);
+                for (int i = 4 * threadIdx.x; i < values; i += 4 * kThreads) {
+                    const int k = i / sums, e = i - k * sums;
+                    float* const p = part + (size_t)k * parts * sums + e;
+                    *reinterpret_cast<float4*>(p + (size_t)warps_k * sums) = warps_sum(p);
+                }
             cluster.sync();
-            const int share = (sums / 4 + ranks - 1) / ranks * 4;
-            for (int i = rank * share + 4 * threadIdx.x; i < min(sums, (rank + 1) * share); i += 4 * kThreads) {
+            const int share = (values / 4 + ranks - 1) / ranks * 4;
+            for (int i = rank * share + 4 * threadIdx.x; i < min(values, (rank + 1) * share); i += 4 * kThreads) {
+                const int k = i / sums, e = i - k * sums;
+                float* const p = part + (size_t)(k * parts + parts - 1) * sums + e;
                 float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 for (int r0 = 0; r0 < ranks; r0 += 4) {
                     float4 v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (r0 + r < ranks) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(total, r0 + r) + i);
+                        if (r0 + r < ranks) v[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(p, r0 + r));
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (r0 + r < ranks) add(s, v[r]);
                 }
-                store(i, s);
+                store(group + k * tile_step, e, s);
             }
         }
-        if (kSumBuffers<NT> == 1 && tile + tile_step < a.tiles) {
+        if (group + a.group * tile_step < a.tiles) {              // the next group overwrites what the others read
             if (ranks > 1) cluster.sync();
             else __syncthreads();
         }
@@ -361,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
 
 // How a product is divided: a CTA's warps over rows of W (the others divide its K), the CTAs of a cluster over K.
 struct Division {
-    int warps_n, ranks, pieces_cta, pieces_stage, tiles, grid;
+    int warps_n, ranks, pieces_cta, pieces_stage, tiles, group, grid;
     size_t smem;
     double cost;
 };
@@ -372,6 +396,7 @@ int launch(MatmulArgs a, cudaStream_t st) {
     static SmemOptIn opt_in;
     const int m_tiles = (a.M + COLS - 1) / COLS, rows_x = a.M < COLS ? a.M : COLS, sms = sm_count();
     a.pieces = (a.K + kPiece - 1) / kPiece;
+    a.bits = code_bits<T>();
     // The division with the shortest estimate, in cycles.  An SM has one CTA, which goes through its tiles one after the other: its warps
     // take a piece in the time that their matrix and other instructions need, or, if it is their only one, in one piece's latency.
     // clusters of 1, 2, 4 and 8 such CTAs that the device runs at once: fewer than its SMs would hold, which come in groups
@@ -400,7 +425,7 @@ int launch(MatmulArgs a, cudaStream_t st) {
     best.cost = 1e30;
     auto consider = [&](int wn, int ranks) {
         const int wk = kWarps / wn, cta = (a.pieces + ranks - 1) / ranks, tiles = (a.N + 16 * wn - 1) / (16 * wn);
-        const size_t fixed = kRingBytes<BLOCK, NT> + (size_t)kSumBuffers<NT> * sum_parts(wk) * rows_x * 16 * wn * 4, limit = kSmemSM - 1024;
+        const size_t sums = (size_t)sum_parts(wk, ranks) * rows_x * 16 * wn * 4, fixed = kRingBytes<BLOCK, NT> + sums, limit = kSmemSM - 1024;
         if (fixed + (size_t)rows_x * x_pitch(1) > limit) return;
         int stage = cta;
         if (fixed + (size_t)rows_x * x_pitch(stage) > limit) stage = ((int)((limit - fixed) / rows_x) - 16) / (kPiece * 2);
@@ -410,16 +435,23 @@ int launch(MatmulArgs a, cudaStream_t st) {
         if (clusters > tiles) clusters = tiles;
         const int rounds = (tiles + clusters - 1) / clusters;
         clusters = (tiles + rounds - 1) / rounds;
+        size_t bytes = fixed + (size_t)rows_x * x_pitch(stage);
+        int group = (int)((limit - bytes) / sums) + 1;
+        if (group > rounds) group = rounds;
+        group = (rounds + (rounds + group - 1) / group - 1) / ((rounds + group - 1) / group);
+        bytes += (group - 1) * sums;
         const double waves = ((int64_t)clusters * m_tiles + room - 1) / room, pieces = (cta + wk - 1) / wk;
-        const double round = pieces * kWarps * (60.0 + 40.0 * NT) + 400.0 + (ranks > 1 ? 700.0 : 0.0) + rows_x * wn * (4.0 + ranks) +
-                             (stage < cta ? 3000.0 * ((cta + stage - 1) / stage) : 0.0);
-        const double cost = waves * (3000.0 + rows_x * cta + rounds * round);
-        if (cost < best.cost) best = {wn, ranks, cta, stage, tiles, clusters * ranks, fixed + (size_t)rows_x * x_pitch(stage), cost};
+        // a tile: its pieces on all warps, x again where it does not stay, what is left of the loop; a group's sums; x, once
+        const double tile = pieces * kWarps * (110.0 + 50.0 * NT) + (stage < cta ? 30.0 * rows_x * cta + 2000.0 * ((cta + stage - 1) / stage) : 0.0) + 450.0;
+        const double quads = (double)group * rows_x * wn * 4 / kThreads;
+        const double reduction = 600.0 + quads * (1800.0 + 80.0 * wk) + (ranks > 1 ? 1800.0 : 0.0);
+        const double cost = waves * (4000.0 + 30.0 * rows_x * cta + rounds * tile + (rounds + group - 1) / group * reduction);
+        if (cost < best.cost) best = {wn, ranks, cta, stage, tiles, group, clusters * ranks, bytes, cost};
     };
     for (int wn = 1; wn <= kWarps; wn *= 2)
         for (int ranks = 1; ranks <= 8; ranks *= 2)
             if (ranks == 1 || a.pieces >= ranks) consider(wn, ranks);
-    a.warps_n = best.warps_n, a.ranks = best.ranks, a.pieces_cta = best.pieces_cta, a.pieces_stage = best.pieces_stage, a.tiles = best.tiles;
+    a.warps_n = best.warps_n, a.ranks = best.ranks, a.pieces_cta = best.pieces_cta, a.pieces_stage = best.pieces_stage, a.tiles = best.tiles, a.group = best.group;
     cfg.gridDim = dim3((unsigned)best.grid, (unsigned)m_tiles);
     cfg.dynamicSmemBytes = best.smem;
     cfg.stream = st;

@@ -17,6 +17,9 @@ by peer loads and an all-gather by peer stores) or by NCCL (``--reduce nccl``).
 The elementwise steps between the layer's kernels run inside the library's calls (``BlockInt8Linear.infer_pre``: RMSNorm and
 ``silu(gate) * up`` in the quantizer, the residual sum in the kernel that writes the GEMM's result; rotary embedding and
 cache append of a decode step in one kernel); ``--no-fuse`` runs them as torch kernels, for comparison.
+
+``--weights int4`` holds every weight in 4-bit blocks instead (``BlockInt4Linear``), ``--cache int4`` the keys and values
+(``rope_cache_append_int4`` and ``attention_int4_cache`` for the prompt and for every step): half the bytes that a decode step reads.
 """
 from __future__ import annotations
 
@@ -37,8 +40,9 @@ if ROOT not in sys.path:
     sys.path.insert(0, ROOT)
 
 import block_linear_config as cfg  # noqa: E402
-from block_linear import BlockInt8Linear  # noqa: E402
-from blockwise_int8_linear_b200.decode_ops import rope_cache_append  # noqa: E402
+from block_linear import BlockInt4Linear, BlockInt8Linear  # noqa: E402
+from blockwise_int8_linear_b200.decode_ops import (attention_int4_cache, int4_kv_cache, rope_cache_append,  # noqa: E402
+                                                   rope_cache_append_int4)
 from blockwise_int8_linear_b200.parallel import block_aligned_bounds  # noqa: E402
 from triton_functions import pre_quantize_matmul_block_rowwise_dequantize  # noqa: E402
 
@@ -61,7 +65,7 @@ class Int8Linear(nn.Module):
     GEMM for them; each part keeps its own seed, so the model is the same function as with separate layers), local output.
     mode 'row': columns [lo,hi), fp32 partial output summed over the group."""
 
-    def __init__(self, in_f, out_fs, seeds, dev, mode, rank, world, block, ops=None):
+    def __init__(self, in_f, out_fs, seeds, dev, mode, rank, world, block, ops=None, weights="int8"):
         super().__init__()
         self.mode, self.world, self.ops = mode, world, ops
         if mode == "col":
@@ -83,10 +87,11 @@ class Int8Linear(nn.Module):
             self.lin = None
             self.W_int8, self.state_W = ops.quantize_block_rowwise(w)
             return
-        self.lin = BlockInt8Linear(w.shape[1], w.shape[0], bias=False, device=dev, dtype=torch.bfloat16)
+        cls = BlockInt4Linear if weights == "int4" else BlockInt8Linear
+        self.lin = cls(w.shape[1], w.shape[0], bias=False, device=dev, dtype=torch.bfloat16)
         self.lin.weight.data = w
         self.lin.eval()
-        self.lin.prepare_for_eval(drop_weight=True)                                  # keep only the int8 copy resident
+        self.lin.prepare_for_eval(drop_weight=True)                                  # keep only the quantized copy resident
 
     def _infer(self, x):
         if self.lin is not None:
@@ -115,8 +120,8 @@ class Int8Linear(nn.Module):
         return part.to(cfg.INPUT_OUTPUT_TORCH_TYPE)
 
     def fusable(self):
-        """Whether `fused` runs as one library call: a layer whose output needs no sum over ranks."""
-        return FUSE and self.lin is not None and (self.mode == "col" or self.world == 1)
+        """Whether `fused` runs as one library call: an int8 layer whose output needs no sum over ranks."""
+        return FUSE and isinstance(self.lin, BlockInt8Linear) and (self.mode == "col" or self.world == 1)
 
     def fused(self, x, op="none", x2=None, residual=None):
         """``residual + self(pre(x))`` with pre = rms_norm ('rmsnorm'), silu(x) * x2 ('silu_mul') or nothing ('none'):
@@ -125,6 +130,8 @@ class Int8Linear(nn.Module):
         if self.fusable():
             return self.lin.infer_pre(x, op, x2=x2, eps=NORM_EPS, residual=residual)
         inp = rms_norm(x) if op == "rmsnorm" else (F.silu(x) * x2 if op == "silu_mul" else x)
+        if isinstance(self.lin, BlockInt4Linear) and (self.mode == "col" or self.world == 1):
+            return self.lin.infer(inp, residual=residual)
         y = self.forward(inp)
         return y if residual is None else residual + y
 
@@ -132,14 +139,14 @@ class Int8Linear(nn.Module):
         """``residual + sum over the group of this row-parallel layer applied to pre(x)``, cast to the activation type: for
         decode-sized inputs with the peer-memory reduction installed, one library call whose first kernel applies `op` and
         quantizes and whose last kernel adds the ranks' partial results and the residual."""
-        peer = self.world > 1 and self.mode == "row" and PEER is not None and self.lin is not None
+        peer = self.world > 1 and self.mode == "row" and PEER is not None and isinstance(self.lin, BlockInt8Linear)
         if peer:
             rows = x.numel() // x.shape[-1]
             peer = rows <= 64 and rows * self.widths[0] <= PEER.capacity
         if peer and FUSE:
             return PEER.row_parallel_linear(x, self.lin.W_int8, self.lin.state_W, op=op, x2=x2, residual=residual)
         rows = x.numel() // x.shape[-1]
-        if (not peer and self.world > 1 and self.mode == "row" and PEER_LARGE is not None and self.lin is not None
+        if (not peer and self.world > 1 and self.mode == "row" and PEER_LARGE is not None and isinstance(self.lin, BlockInt8Linear)
                 and rows * self.widths[0] <= PEER_LARGE.capacity and self.widths[0] % 4 == 0):
             # prefill: the GEMM writes its fp32 partial result into the exchange buffer, one kernel per rank sums the ranks
             # (reduce-scatter by peer loads, all-gather by peer stores), casts and adds the residual
@@ -190,7 +197,8 @@ class Layer(nn.Module):
     def __init__(self, i, a, dev, rank, world, ops=None):
         super().__init__()
         d, f, blk = a.hidden, a.ffn, a.block
-        mk = lambda in_f, out_fs, seeds, mode: Int8Linear(in_f, out_fs, [1000 * i + s for s in seeds], dev, mode, rank, world, blk, ops)
+        mk = lambda in_f, out_fs, seeds, mode: Int8Linear(in_f, out_fs, [1000 * i + s for s in seeds], dev, mode, rank, world, blk, ops,
+                                                              getattr(a, "weights", "int8"))
         self.qkv = mk(d, (d, d, d), (1, 2, 3), "col")
         self.o = mk(d, (d,), (4,), "row")
         self.gate_up = mk(d, (f, f), (5, 6), "col")
@@ -198,6 +206,7 @@ class Layer(nn.Module):
         self.heads_local = self.qkv.widths[0] // a.head_dim
         self.head_dim = a.head_dim
         self.kcache = self.vcache = None
+        self.int4_cache, self.cache = getattr(a, "cache", "bf16") == "int4", None
 
     def attn_partial(self, x, pos0, max_len, cis, mask=None, pos_dev=None, summed=False, residual=None):
         """Attention half of the layer up to the output projection; without `residual` also without the sum over ranks
@@ -208,16 +217,20 @@ class Layer(nn.Module):
         B, T, _ = x.shape
         hl, hd = self.heads_local, self.head_dim
         qkv = self.qkv.fused(x, "rmsnorm").view(B, T, 3, hl, hd)
+        if self.int4_cache:
+            # prompt and decode alike: rotation, quantization and append in one launch, attention over what the cache then has; `cis`
+            # holds the factors of all positions
+            if self.cache is None:
+                self.cache = int4_kv_cache(B, hl, max_len, hd, x.dtype, x.device)
+            pos = torch.full((1,), pos0, device=x.device, dtype=torch.long) if pos_dev is None else pos_dev
+            q = rope_cache_append_int4(qkv.view(B, T, 3 * hl, hd), cis, pos, self.cache)
+            att = attention_int4_cache(q, self.cache, pos + T).transpose(1, 2).reshape(B, T, hl * hd)
+            return self.project(att, summed, residual)
         if pos_dev is not None and T == 1 and FUSE and self.qkv.lin is not None and self.kcache is not None:
             # decode: rotation of q and k and the append of k and v to the caches in one launch
             q = rope_cache_append(qkv.view(B, 3, hl, hd), cis, pos_dev, self.kcache, self.vcache)
             att = F.scaled_dot_product_attention(q, self.kcache, self.vcache, attn_mask=mask)
-            att = att.transpose(1, 2).reshape(B, T, hl * hd)
-            if residual is not None and self.o.fusable():
-                return self.o.fused(att, "none", residual=residual)
-            if residual is not None:
-                return self.o.summed(att, residual=residual)
-            return self.o.summed(att) if summed else self.o.partial(att)
+            return self.project(att.transpose(1, 2).reshape(B, T, hl * hd), summed, residual)
         qk = rope(qkv[:, :, :2], cis)                                   # q and k in one pass: [B, T, 2, H, D]
         q, k, v = qk[:, :, 0].transpose(1, 2), qk[:, :, 1].transpose(1, 2), qkv[:, :, 2].transpose(1, 2)
         if self.kcache is None:
@@ -232,8 +245,11 @@ class Layer(nn.Module):
             self.kcache.index_copy_(2, pos_dev, k)
             self.vcache.index_copy_(2, pos_dev, v)
             att = F.scaled_dot_product_attention(q, self.kcache, self.vcache, attn_mask=mask)
-        att = att.transpose(1, 2).reshape(B, T, hl * hd)
-        if residual is not None and self.o.fusable():
+        return self.project(att.transpose(1, 2).reshape(B, T, hl * hd), summed, residual)
+
+    def project(self, att, summed, residual):
+        """The output projection of the attention half, as `attn_partial` returns it."""
+        if residual is not None and (self.o.fusable() or self.o.world == 1):
             return self.o.fused(att, "none", residual=residual)
         if residual is not None:
             return self.o.summed(att, residual=residual)
@@ -276,12 +292,15 @@ class Llama(nn.Module):
         g = torch.Generator(device=dev).manual_seed(7)
         self.emb = (torch.randn((a.vocab, a.hidden), device=dev, generator=g) * 0.02).to(torch.bfloat16)
         self.layers = nn.ModuleList(Layer(i, a, dev, rank, world, ops) for i in range(a.layers))
-        self.head = Int8Linear(a.hidden, (a.vocab,), (99,), dev, "col", rank, world, a.block, ops)
+        self.head = Int8Linear(a.hidden, (a.vocab,), (99,), dev, "col", rank, world, a.block, ops, getattr(a, "weights", "int8"))
+        self.int4_cache = getattr(a, "cache", "bf16") == "int4"
         self.world, self.vocab, self.block = world, a.vocab, a.block
         self.cis = rope_table(a.prompt + a.decode + 16, a.head_dim, dev)
         self.positions = torch.arange(a.prompt + a.decode + 16, device=dev)
 
     def positions_of(self, ids, pos0, max_len, pos_dev):
+        if self.int4_cache:
+            return self.cis, None                                  # the kernels look up their positions themselves
         if pos_dev is None:
             return self.cis[pos0:pos0 + ids.shape[1]], None
         # an additive mask in the activation type, built once per step: given a boolean mask, every layer's attention call
@@ -494,7 +513,9 @@ def run(a, rank, world, dev, eager=False):
         _lib.device_status()                                      # raises if a bounded flag wait gave up
         PEER = PEER_LARGE = None
     return {
-        "model": f"llama-arch {a.layers}x{a.hidden} ffn {a.ffn} vocab {a.vocab}, random init N(0,0.02), BlockInt8Linear block {a.block}",
+        "model": f"llama-arch {a.layers}x{a.hidden} ffn {a.ffn} vocab {a.vocab}, random init N(0,0.02), "
+                 f"Block{'Int4' if getattr(a, 'weights', 'int8') == 'int4' else 'Int8'}Linear block {a.block}",
+        "weights": getattr(a, "weights", "int8"), "cache": getattr(a, "cache", "bf16"),
         "n_gpus": world, "batch": a.batch, "prompt": a.prompt, "decode": a.decode,
         "prefill_tokens_per_s": a.batch * a.prompt / t_prefill, "prefill_s": t_prefill, "first_prefill_s": t_first,
         "decode_tokens_per_s": a.batch * (a.decode - 1) / t_decode, "decode_ms_per_step": 1e3 * t_decode / max(1, a.decode - 1),
@@ -522,6 +543,8 @@ def main():
                     help="tensor-parallel decode: the library's peer-memory reduction inside one CUDA graph, or NCCL between graphs")
     ap.add_argument("--no-fuse", dest="no_fuse", action="store_true",
                     help="run the normalisations, the gated activation and the residual sums as separate torch kernels")
+    ap.add_argument("--weights", choices=["int8", "int4"], default="int8", help="hold the weights in 8-bit or in 4-bit blocks")
+    ap.add_argument("--cache", choices=["bf16", "int4"], default="bf16", help="hold keys and values in bf16 or in 4-bit blocks")
     ap.add_argument("--out", default=None, help="also append the JSON line to this file")
     a = ap.parse_args()
     a.head_dim = a.hidden // a.heads

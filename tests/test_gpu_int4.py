@@ -473,6 +473,33 @@ def test_two_graphs_and_threads_share_nothing():
     assert wrong == [0, 0]
 
 
+@pytest.mark.parametrize("weights,cache", [("int4", "int4"), ("int8", "int4"), ("int4", "bf16")])
+def test_llama_driver_in_4_bits(weights, cache):
+    """The inference driver at toy size with weights, cache or both in 4 bits: a captured decode step gives the eager step's tokens, and the
+    prompt's logits those of the same model on the values that its 4-bit weights stand for (and a bf16 cache: keys and values within a
+    14th of their block's largest, so the logits of two layers are compared loosely)."""
+    import argparse
+
+    from tests.test_gpu_models import _load
+    L = _load("llama_infer")
+    a = argparse.Namespace(layers=2, hidden=256, heads=4, head_dim=64, ffn=704, vocab=512, batch=2, prompt=24, decode=6, block=64,
+                           weights=weights, cache=cache)
+    r1, r2 = (L.run(a, rank=0, world=1, dev=torch.device(DEV), eager=e) for e in (False, True))
+    assert r1["tokens"] == r2["tokens"] and len(r1["tokens"][0]) == a.decode and r1["cache"] == cache and r1["weights"] == weights
+    model = L.Llama(a, torch.device(DEV), 0, 1)
+    ids = torch.randint(0, a.vocab, (a.batch, a.prompt), generator=torch.Generator().manual_seed(4000)).to(DEV)
+    got = model(ids, 0, 32).float()
+    plain = L.Llama(argparse.Namespace(**{**vars(a), "cache": "bf16"}), torch.device(DEV), 0, 1)
+    if weights == "int4":
+        for m in plain.modules():
+            if isinstance(m, L.Int8Linear):
+                w = m.lin.dequantized_weight()
+                m.lin.infer = lambda x, residual=None, w=w: torch.nn.functional.linear(x, w) + (0 if residual is None else residual)
+    want = plain(ids, 0, 32).float()
+    assert (got - want).norm() <= (0.02 if cache == "bf16" else 0.3) * want.norm()
+    assert_clean_device()
+
+
 def test_linear_module_and_checkpoints():
     from blockwise_int8_linear_b200 import BlockInt4Linear, replace_linear_with_blockwise_int4
     set_config(64, BF)
