@@ -635,7 +635,7 @@ int bi8_matmul_int4(const void* x, int x_dtype, int64_t ldx, const uint8_t* Wq, 
                     void* stream) {
     DeviceOfCall call;
     if (int rc = check_int4("matmul_int4", x_dtype, M, K, block)) return rc;
-    if (N < 0 || M > 0x400000 || N > 0x7fffff00 || K > 0x7fffff00)
+    if (N < 0 || M > 65535 * 64 || N > 0x7fffff00 || K > 0x7fffff00)
         return fail(BI8_ERR_SHAPE, "matmul_int4: bad shape M %lld N %lld K %lld", (long long)M, (long long)N, (long long)K);
     if (!dtype_ok(out_dtype) || (bias && !dtype_ok(bias_dtype))) return fail(BI8_ERR_DTYPE, "matmul_int4: unknown dtype code");
     if (M == 0 || N == 0) return BI8_OK;

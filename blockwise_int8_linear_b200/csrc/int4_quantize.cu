@@ -39,6 +39,31 @@ struct Rows {
 template <bool FLAT>
 constexpr int kUnits = FLAT ? 4 : 1;                 // of a thread
 
+// Eight 16-bit values from any address, those from `count` (below 1: all) on as zeros: from the two aligned 16 bytes that hold them, each read
+// only where it holds one of them.
+__device__ __forceinline__ uint4 load8(const unsigned short* p, int count) {
+    if (count < 1) return make_uint4(0u, 0u, 0u, 0u);
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), base = a & ~(uintptr_t)15;
+    const uint4 lo = __ldg(reinterpret_cast<const uint4*>(base));
+    uint4 hi = make_uint4(0u, 0u, 0u, 0u);
+    if (base + 16 < a + 2 * count) hi = __ldg(reinterpret_cast<const uint4*>(base + 16));
+    const uint32_t r[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    const uint32_t words = (uint32_t)(a & 15u) >> 2, bits = (uint32_t)(a & 2u) * 8u;
+    uint32_t w[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = words & 2u ? (j + 2 < 8 ? r[j + 2] : 0u) : r[j];
+    const uint32_t next = words & 2u ? r[7] : r[5];
+    uint32_t v[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) v[j] = words & 1u ? (j + 1 < 5 ? w[j + 1] : next) : w[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[j] = __funnelshift_r(v[j], v[j + 1], bits);
+        v[j] = 2 * j + 1 < count ? v[j] : 2 * j < count ? v[j] & 0xffffu : 0u;
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
 template <typename T, bool FLAT>
 __global__ void __launch_bounds__(kThreads) quantize_int4_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq,
                                                                  T* __restrict__ s, int64_t K, Rows rows) {
@@ -56,11 +81,7 @@ __global__ void __launch_bounds__(kThreads) quantize_int4_kernel(const T* __rest
         if (FLAT) {
             if (live) v[n] = ld_nc_v4(x + u[n].k);
         } else if (live) {
-            const unsigned short* p = reinterpret_cast<const unsigned short*>(x) + u[n].row * ldx + u[n].k;
-            uint32_t e[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = u[n].k + j < K ? p[j] : 0u;
-            v[n] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+            v[n] = load8(reinterpret_cast<const unsigned short*>(x) + u[n].row * ldx + u[n].k, (int)min((int64_t)8, K - u[n].k));
         }
     }
 #pragma unroll
@@ -105,47 +126,57 @@ __device__ __forceinline__ __half to_out<__half>(float y) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 to_out<__nv_bfloat16>(float y) { return __float2bfloat16_rn(y); }
 
-template <typename T, typename O, bool FLAT>
-__global__ void __launch_bounds__(kThreads) dequantize_int4_kernel(const uint8_t* __restrict__ q, int64_t ldq, const T* __restrict__ s,
-                                                                   O* __restrict__ out, int64_t K, Rows rows) {
-    constexpr int N = kUnits<FLAT>;
+template <typename T, typename O>
+__global__ void __launch_bounds__(kThreads) dequantize_int4_kernel(const uint8_t* __restrict__ q, const T* __restrict__ s, O* __restrict__ out, Rows rows) {
+    constexpr int N = kUnits<true>;
     after_predecessor();
     const int64_t first = (int64_t)blockIdx.x * (N * kThreads) + threadIdx.x;
     uint32_t w[N];
     float sc[N];
-    Unit u[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int64_t i = first + n * kThreads;
         w[n] = kZeroCodes;
         sc[n] = 0.0f;
         if (i >= rows.units) continue;
-        u[n] = rows.unit<FLAT>(i);
         sc[n] = F16Bits<T>::one(__ldg(reinterpret_cast<const unsigned short*>(s) + (i >> rows.shift)));
-        if (FLAT) {
-            w[n] = __ldg(reinterpret_cast<const uint32_t*>(q + u[n].k / 2));
-        } else {
-            const uint8_t* p = q + u[n].row * ldq + u[n].k / 2;
-            w[n] = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (u[n].k + 2 * j < K) w[n] |= (uint32_t)p[j] << (8 * j);
-        }
+        w[n] = __ldg(reinterpret_cast<const uint32_t*>(q) + i);
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        if (first + n * kThreads >= rows.units) continue;
+        const int64_t i = first + n * kThreads;
+        if (i >= rows.units) continue;
         float y[8];
         values8(sc[n], w[n], y);
-        if (FLAT) {
-            store8(out + u[n].k, y);
-        } else {
-            O* p = out + u[n].row * K + u[n].k;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (u[n].k + j < K) p[j] = to_out<O>(y[j]);
-        }
+        store8(out + i * 8, y);
     }
+}
+
+// Rows of any length and alignment: a warp takes 256 neighbouring values of a row, a lane every 32nd, so that what the lanes store at a time
+// lies together.
+template <typename T, typename O>
+__global__ void __launch_bounds__(kThreads) dequantize_int4_rows_kernel(const uint8_t* __restrict__ q, int64_t ldq, const T* __restrict__ s, O* __restrict__ out,
+                                                                        int64_t K, int64_t blocks, Rows rows) {
+    after_predecessor();
+    const int64_t warp = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    if (warp >= rows.units) return;
+    const Unit u = rows.unit<false>(warp);                      // a unit of 256 values
+    const int64_t k0 = u.k * 32 + (threadIdx.x & 31), left = K - k0;
+    const uint8_t* const codes = q + u.row * ldq + k0 / 2;
+    const unsigned short* const scales = reinterpret_cast<const unsigned short*>(s) + u.row * blocks + (k0 >> rows.shift);
+    O* const to = out + u.row * K + k0;
+    const uint32_t nibble = k0 & 1 ? 4u : 0u;
+    uint32_t byte[8], bits[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (32 * j < left) byte[j] = __ldg(codes + 16 * j), bits[j] = __ldg(scales + ((32 * j) >> rows.shift));      // k0 - lane is a multiple of 256
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (32 * j < left) {
+            float y[8];
+            values8(F16Bits<T>::one(bits[j]), byte[j] >> nibble, y);        // the first one counts
+            to[32 * j] = to_out<O>(y[0]);
+        }
 }
 
 int grid_of(int64_t units, bool flat, unsigned* grid) {
@@ -177,15 +208,21 @@ int launch_dequantize_int4(const uint8_t* q, int64_t ldq, const void* s, int s_d
     if (M == 0 || K == 0) return BI8_OK;
     const Rows rows(M, K, block);
     const bool flat = K % block == 0 && (M == 1 || ldq == K / 2) && aligned(q, 4) && aligned(out, 16);
+    Rows pieces = rows;                                     // of 256 values, for a warp each
+    pieces.per_row = (K + 255) / 256;
+    pieces.units = M * pieces.per_row;
+    pieces.small = pieces.units < 0x7fffffffll;
+    pieces.shift = rows.shift + 3;                          // a block in values
+    if (pieces.small) pieces.div = FastDiv(pieces.per_row);
     unsigned grid;
-    if (int rc = grid_of(rows.units, flat, &grid)) return rc;
-    auto go = [&](auto* tag, auto* out_tag, auto is_flat) {
+    if (int rc = grid_of(flat ? rows.units : pieces.units * 32, flat, &grid)) return rc;
+    auto by_layout = [&](auto* tag, auto* out_tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         using O = std::remove_pointer_t<decltype(out_tag)>;
-        return launch_chained(dequantize_int4_kernel<T, O, decltype(is_flat)::value>, grid, kThreads, 0, st, q, ldq, static_cast<const T*>(s),
-                              static_cast<O*>(out), K, rows);
+        if (flat) return launch_chained(dequantize_int4_kernel<T, O>, grid, kThreads, 0, st, q, static_cast<const T*>(s), static_cast<O*>(out), rows);
+        return launch_chained(dequantize_int4_rows_kernel<T, O>, grid, kThreads, 0, st, q, ldq, static_cast<const T*>(s), static_cast<O*>(out), K,
+                              (K + block - 1) / block, pieces);
     };
-    auto by_layout = [&](auto* tag, auto* o) { return flat ? go(tag, o, std::true_type{}) : go(tag, o, std::false_type{}); };
     auto by_out = [&](auto* tag) {
         if (out_dt == BI8_BF16) return by_layout(tag, static_cast<__nv_bfloat16*>(nullptr));
         if (out_dt == BI8_F16) return by_layout(tag, static_cast<__half*>(nullptr));

@@ -125,7 +125,8 @@ def _check_product(got, x, w, s, block, extra=None):
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("block", [32, 64, 128])
 @pytest.mark.parametrize("m,k,n", [(1, 64, 1), (1, 1, 5), (2, 33, 17), (1, 4096, 512), (3, 256, 16), (8, 768, 2304), (9, 1001, 777), (16, 2048, 40),
-                                   (17, 640, 129), (33, 4096, 130), (64, 520, 100), (65, 300, 70), (200, 96, 48), (1, 12000, 24)])
+                                   (17, 640, 129), (33, 4096, 130), (64, 520, 100), (65, 300, 70), (200, 96, 48), (1, 12000, 24),
+                                   (48, 9000, 65), (12, 30000, 33), (5, 11008, 3000)])
 def test_matmul(m, k, n, block, dtype):
     f = _f()
     codes, state, w = _weights(n, k, block, dtype, m + k + n)
