@@ -16,7 +16,7 @@ constexpr int kThreads = 256;
 struct AppendArgs {
     const void* qkv;             // [B, T, Hq + 2 Hkv, D]
     const float2* cis;           // [cis_rows, D / 2]
-    int64_t cis_rows;
+    int64_t rows;                // positions that the table and the cache have
     const long long* pos;
     int64_t pos_step;
     void* q_out;                 // [B, Hq, T, D]
@@ -36,13 +36,14 @@ __global__ void __launch_bounds__(kThreads) rope_cache_append_int4_kernel(const 
     const unsigned tok = a.heads.div(hd), head = hd - tok * a.heads.d;
     const unsigned b = a.tokens.div(tok), t = tok - b * a.tokens.d;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    const long long row = a.pos[b * a.pos_step] + t;
+    const long long position = a.pos[b * a.pos_step] + t;
     // a position outside the table or the cache: its key and value are not written, its query is zero
-    const bool inside = row >= 0 && row < a.cache.max_len && row < a.cis_rows;
+    const bool inside = position >= 0 && position < a.rows;
+    const int row = inside ? (int)position : 0;
     if (live && inside) {
         v = ld_nc_v4(static_cast<const T*>(a.qkv) + (int64_t)unit * 8);
         if (head < (unsigned)(a.Hq + a.Hkv)) {
-            const float4* cs = reinterpret_cast<const float4*>(a.cis + row * (a.D / 2) + 4 * p);
+            const float4* cs = reinterpret_cast<const float4*>(a.cis + (int64_t)row * (a.D / 2) + 4 * p);
             const float4 c01 = cs[0], c23 = cs[1];
             const float c[4] = {c01.x, c01.z, c23.x, c23.z}, s[4] = {c01.y, c01.w, c23.y, c23.w};
             uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -54,22 +55,23 @@ __global__ void __launch_bounds__(kThreads) rope_cache_append_int4_kernel(const 
             v = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
-    uint32_t scale;
-    const uint32_t codes = quantize8<T>(v, kCacheBlock / 8, &scale);     // every lane takes part
-    if (!live) return;
+    if (!live) return;                                    // units come in whole blocks, and the lanes of a block take the same way
     if (head < (unsigned)a.Hq) {
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (((int64_t)b * a.Hq + head) * a.T + t) * a.D + 8 * p) = v;
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (int64_t)((b * a.Hq + head) * a.T + t) * a.D + 8 * p) = v;
         return;
     }
     if (!inside) return;
+    uint32_t scale;
+    const uint32_t codes = quantize8<T, kCacheBlock / 8>(v, 0xffu << (threadIdx.x & 24u), &scale);
     const bool key = head < (unsigned)(a.Hq + a.Hkv);
-    const int64_t h = head - a.Hq - (key ? 0 : a.Hkv);
+    const int h = (int)head - a.Hq - (key ? 0 : a.Hkv);
     const bi8_int4_cache& c = a.cache;
-    uint8_t* q = key ? c.k + b * c.k_batch + h * c.k_head : c.v + b * c.v_batch + h * c.v_head;
-    unsigned short* s = key ? static_cast<unsigned short*>(c.k_state) + b * c.ks_batch + h * c.ks_head
-                            : static_cast<unsigned short*>(c.v_state) + b * c.vs_batch + h * c.vs_head;
-    *reinterpret_cast<uint32_t*>(q + row * (a.D / 2) + 4 * p) = codes;
-    if ((p & 7u) == 0u) s[row * (a.D / kCacheBlock) + (p >> 3)] = (unsigned short)scale;
+    uint8_t* const q = (key ? c.k : c.v) + (int)b * (key ? c.k_batch : c.v_batch) + h * (key ? c.k_head : c.v_head);
+    *reinterpret_cast<uint32_t*>(q + (int64_t)row * (a.D / 2) + 4 * p) = codes;
+    if ((p & 7u) == 0u) {
+        unsigned short* const s = static_cast<unsigned short*>(key ? c.k_state : c.v_state) + (int)b * (key ? c.ks_batch : c.vs_batch) + h * (key ? c.ks_head : c.vs_head);
+        s[(int64_t)row * (a.D / kCacheBlock) + (p >> 3)] = (unsigned short)scale;
+    }
 }
 
 }  // namespace
@@ -81,7 +83,7 @@ int launch_rope_cache_append_int4(const void* qkv, int dt, const float* cis, int
     AppendArgs a{};
     a.qkv = qkv;
     a.cis = reinterpret_cast<const float2*>(cis);
-    a.cis_rows = cis_rows;
+    a.rows = cis_rows < cache->max_len ? cis_rows : cache->max_len;
     a.pos = pos;
     a.pos_step = pos_step;
     a.q_out = q_out;

@@ -67,11 +67,13 @@ __device__ __forceinline__ uint32_t codes8(const uint4& v, float s) {
 }
 constexpr uint32_t kZeroCodes = 0x88888888u;
 
-// Quantizes a block that lies in `lanes` neighbouring lanes, eight values each: codes of this lane, the scale's bits in all of them.
-template <typename T>
-__device__ __forceinline__ uint32_t quantize8(const uint4& v, int lanes, uint32_t* scale_bits) {
+// Quantizes a block that lies in LANES neighbouring lanes, eight values each: codes of this lane, the scale's bits in all of them.  `lanes` are
+// those that call together, whole blocks.
+template <typename T, int LANES>
+__device__ __forceinline__ uint32_t quantize8(const uint4& v, uint32_t lanes, uint32_t* scale_bits) {
     uint32_t m = absmax8(v);
-    for (int d = lanes / 2; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(lanes, m, d));
     const bool bad = m >= F16Bits<T>::kInf;
     *scale_bits = bad ? F16Bits<T>::kNaN : m;
     return bad ? kZeroCodes : codes8<T>(v, F16Bits<T>::one(m));
@@ -81,6 +83,7 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& v, int lanes, uint32_
 // s q / 7 = q a + q (e + s l): the first product is exact inside a multiply-add, the second is 2^-24 of it and its rounding harmless.
 // Scales outside the range in which e is exact take the division itself, the largest a factor of 2^20 lower, where 7 s does not overflow.
 __device__ __forceinline__ void values8(float s, uint32_t w, float (&y)[8]);
+
 // ---- tensor-core operands -----------------------------------------------------------------------------------------------------
 // Codes become the matrix instruction's operands in pairs, as the numbers -7 to 7 in the other operand's type.  Four bits c + 8 under the
 // exponent of 1024 are the fp16 number 1024 + 8 + c, four bits further up 1024 + 16 (8 + c); a packed subtraction or multiply-add
@@ -93,43 +96,34 @@ __device__ __forceinline__ void values8(float s, uint32_t w, float (&y)[8]);
 struct Codes4 {
     uint32_t p04, p15, p26, p37;
 };
-// The constants of the unpacking that have to be in registers (an instruction holds one of its two).  They come as kernel arguments: a
-// value that the compiler sees it moves into a register again for each use, which made three instructions of one.
-struct CodeBits {
-    uint32_t exponent, high;
-};
-template <typename T>
-inline CodeBits code_bits() {
-    return std::is_same<T, __half>::value ? CodeBits{0x64006400u, 0xd480d480u} : CodeBits{0x43004300u, 0u};      // 1024 and -72; 128
-}
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t set) {      // (w & mask) | set, as one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t set) {      // (w & mask) | set, as one instruction: the compiler makes two of it
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(set));
     return r;
 }
-__device__ __forceinline__ uint32_t half2_low(uint32_t w, const CodeBits& c) {
-    const uint32_t v = and_or(w, 0x000f000fu, c.exponent), k = 0x64086408u;              // 1024 + 8 + c, 1032
+__device__ __forceinline__ uint32_t half2_low(uint32_t w) {
+    const uint32_t v = and_or(w, 0x000f000fu, 0x64006400u), k = 0x64086408u;              // 1024 + 8 + c, 1032
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&k));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t half2_high(uint32_t w, const CodeBits& c) {
-    const uint32_t v = and_or(w, 0x00f000f0u, c.exponent), m = 0x2c002c00u;               // 1024 + 16 (8 + c), 1/16
-    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&c.high));
+__device__ __forceinline__ uint32_t half2_high(uint32_t w) {
+    const uint32_t v = and_or(w, 0x00f000f0u, 0x64006400u), m = 0x2c002c00u, k = 0xd480d480u;      // 1024 + 16 (8 + c), 1/16, -72
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&k));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t bf162_low(uint32_t w, const CodeBits& c) {
-    const uint32_t v = and_or(w, 0x000f000fu, c.exponent), k = 0x43084308u;              // 128 + 8 + c, 136
+__device__ __forceinline__ uint32_t bf162_low(uint32_t w) {
+    const uint32_t v = and_or(w, 0x000f000fu, 0x43004300u), k = 0x43084308u;              // 128 + 8 + c, 136
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&k));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 template <typename T>
-__device__ __forceinline__ Codes4 unpack8(uint32_t w, const CodeBits& c) {
-    if (std::is_same<T, __half>::value) return {half2_low(w, c), half2_high(w, c), half2_low(w >> 8, c), half2_high(w >> 8, c)};
-    return {bf162_low(w, c), bf162_low(w >> 4, c), bf162_low(w >> 8, c), bf162_low(w >> 12, c)};
+__device__ __forceinline__ Codes4 unpack8(uint32_t w) {
+    if (std::is_same<T, __half>::value) return {half2_low(w), half2_high(w), half2_low(w >> 8), half2_high(w >> 8)};
+    return {bf162_low(w), bf162_low(w >> 4), bf162_low(w >> 8), bf162_low(w >> 12)};
 }
 __device__ __forceinline__ void values8(float s, uint32_t w, float (&y)[8]) {
     constexpr float H = 1.0f / 7.0f, L = (float)(1.0 / 7.0 - (double)H);
-    const Codes4 c = unpack8<__half>(w, {0x64006400u, 0xd480d480u});
+    const Codes4 c = unpack8<__half>(w);
     const uint32_t pairs[4] = {c.p04, c.p15, c.p26, c.p37};
     if ((s > 0x1p-90f && s < 0x1p127f) || s == 0.0f) {
         const float a = s * H, b = __fmaf_rn(s, L, __fmaf_rn(s, H, -a));

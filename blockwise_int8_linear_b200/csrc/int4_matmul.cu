@@ -6,10 +6,14 @@
 // columns that few rows of x leave empty cost nothing that counts.  (On the CUDA cores a weight takes an unpack, a conversion and a multiply-add per row of x: at 6.5 TB/s, 12 weights per
 // ns, the SMs have three instructions for each.)
 //
-// A warp takes 16 rows of W and strides over K in pieces of 256 (128 bytes a row; lane 4g + c reads 8 bytes of rows g and g + 8 for every 64
-// values), the next piece's loads in flight while this one is multiplied.  A CTA is eight warps, over rows and over K; CTAs of a
-// cluster share the rows and divide K once more, and add what they have over distributed shared memory in rank order: no
-// workspace, no atomics, the same bits on every call.  x comes through shared memory, in the order of the codes.
+// A CTA of 16 warps, one an SM, keeps its share of x in shared memory, in the order of the codes, and goes through tiles of W: its warps are
+// over rows (16 each) and over K, in pieces of 256 values (128 bytes a row), which come into the warp's ring of shared memory by
+// asynchronous copies while an earlier one is multiplied.  CTAs of a cluster share the rows and divide K once more.  The sums of
+// several tiles are collected before they are added, over the warps and over the cluster, in a fixed order: no workspace, no atomics, the
+// same bits on every call.
+//
+// Measured: one row through 4096 x 4096 5.9 us, 4096 -> 32000 19 us (3.65 TB/s); 8 rows through 4096 -> 11008 12 us, 32 29 us, 64 50 us.  Few
+// rows are bound by what the SMs issue (410 instructions a piece, 180 of them unpacking), small layers by latency.
 #include "int4_common.cuh"
 
 #include <cooperative_groups.h>
@@ -40,7 +44,6 @@ struct MatmulArgs {
     int64_t ldc;
     int bias_dtype, out_dtype;
     int M, N, K;
-    CodeBits bits;
     int tiles;               // of 16 * warps_n rows of W
     int group;               // tiles whose sums a CTA collects before they are added
     int warps_n;             // warps of a CTA over rows of W; the others divide K
@@ -174,7 +177,6 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
         });
     };
 
-    const CodeBits bits = a.bits;
     after_predecessor();
     const bool once = a.pieces_cta <= a.pieces_stage;         // all of this CTA's x fits
     if (once) fetch_x(first, last);
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
                             w0 = *reinterpret_cast<const uint2*>(lo + 32 * u);
                             w1 = *reinterpret_cast<const uint2*>(hi + 32 * u);
                         }
-                        const Codes4 r0a = unpack8<T>(w0.x, bits), r0b = unpack8<T>(w0.y, bits), r1a = unpack8<T>(w1.x, bits), r1b = unpack8<T>(w1.y, bits);
+                        const Codes4 r0a = unpack8<T>(w0.x), r0b = unpack8<T>(w0.y), r1a = unpack8<T>(w1.x), r1b = unpack8<T>(w1.y);
                         const int AFTER = BLOCK == 32 ? 2 * u + 1 : u * PER / 4;         // the scale of (the second half of) these 64 values
                         // eight columns, or twice eight, whose sums do not wait for one another
                         constexpr int PAIR = NT == 1 ? 1 : 2;
@@ -396,7 +398,6 @@ int launch(MatmulArgs a, cudaStream_t st) {
     static SmemOptIn opt_in;
     const int m_tiles = (a.M + COLS - 1) / COLS, rows_x = a.M < COLS ? a.M : COLS, sms = sm_count();
     a.pieces = (a.K + kPiece - 1) / kPiece;
-    a.bits = code_bits<T>();
     // The division with the shortest estimate, in cycles.  An SM has one CTA, which goes through its tiles one after the other: its warps
     // take a piece in the time that their matrix and other instructions need, or, if it is their only one, in one piece's latency.
     // clusters of 1, 2, 4 and 8 such CTAs that the device runs at once: fewer than its SMs would hold, which come in groups

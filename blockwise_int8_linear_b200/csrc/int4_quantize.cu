@@ -64,7 +64,7 @@ __device__ __forceinline__ uint4 load8(const unsigned short* p, int count) {
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-template <typename T, bool FLAT>
+template <typename T, bool FLAT, int LANES>
 __global__ void __launch_bounds__(kThreads) quantize_int4_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq,
                                                                  T* __restrict__ s, int64_t K, Rows rows) {
     constexpr int N = kUnits<FLAT>;
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads) quantize_int4_kernel(const T* __rest
     for (int n = 0; n < N; ++n) {
         const int64_t i = first + n * kThreads;
         uint32_t bits;
-        const uint32_t w = quantize8<T>(v[n], 1 << rows.shift, &bits);
+        const uint32_t w = quantize8<T, LANES>(v[n], 0xffffffffu, &bits);
         if (i >= rows.units) continue;
         if (FLAT) {
             *reinterpret_cast<uint32_t*>(q + u[n].k / 2) = w;
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kThreads) quantize_int4_kernel(const T* __rest
             for (int j = 0; j < 4; ++j)
                 if (u[n].k + 2 * j < K) p[j] = (uint8_t)(w >> (8 * j));
         }
-        if ((threadIdx.x & ((1 << rows.shift) - 1)) == 0) reinterpret_cast<unsigned short*>(s)[i >> rows.shift] = (unsigned short)bits;
+        if (threadIdx.x % LANES == 0) reinterpret_cast<unsigned short*>(s)[i / LANES] = (unsigned short)bits;
     }
 }
 
@@ -194,12 +194,17 @@ int launch_quantize_int4(const void* x, int dt, int64_t ldx, uint8_t* q, int64_t
     const bool flat = K % block == 0 && (M == 1 || (ldx == K && ldq == K / 2)) && aligned(x, 16) && aligned(q, 4);
     unsigned grid;
     if (int rc = grid_of(rows.units, flat, &grid)) return rc;
-    auto go = [&](auto* tag, auto is_flat) {
+    auto go = [&](auto* tag, auto is_flat, auto lanes) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        return launch_chained(quantize_int4_kernel<T, decltype(is_flat)::value>, grid, kThreads, 0, st, static_cast<const T*>(x), ldx, q, ldq,
+        return launch_chained(quantize_int4_kernel<T, decltype(is_flat)::value, decltype(lanes)::value>, grid, kThreads, 0, st, static_cast<const T*>(x), ldx, q, ldq,
                               static_cast<T*>(s), K, rows);
     };
-    auto by_layout = [&](auto* tag) { return flat ? go(tag, std::true_type{}) : go(tag, std::false_type{}); };
+    auto by_block = [&](auto* tag, auto is_flat) {
+        if (block == 32) return go(tag, is_flat, std::integral_constant<int, 4>{});
+        if (block == 64) return go(tag, is_flat, std::integral_constant<int, 8>{});
+        return go(tag, is_flat, std::integral_constant<int, 16>{});
+    };
+    auto by_layout = [&](auto* tag) { return flat ? by_block(tag, std::true_type{}) : by_block(tag, std::false_type{}); };
     return dt == BI8_BF16 ? by_layout(static_cast<__nv_bfloat16*>(nullptr)) : by_layout(static_cast<__half*>(nullptr));
 }
 
