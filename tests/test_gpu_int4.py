@@ -126,7 +126,8 @@ def _check_product(got, x, w, s, block, extra=None):
 @pytest.mark.parametrize("block", [32, 64, 128])
 @pytest.mark.parametrize("m,k,n", [(1, 64, 1), (1, 1, 5), (2, 33, 17), (1, 4096, 512), (3, 256, 16), (8, 768, 2304), (9, 1001, 777), (16, 2048, 40),
                                    (17, 640, 129), (33, 4096, 130), (64, 520, 100), (65, 300, 70), (200, 96, 48), (1, 12000, 24),
-                                   (48, 9000, 65), (12, 30000, 33), (5, 11008, 3000)])
+                                   (48, 9000, 65), (12, 30000, 33), (5, 11008, 3000),
+                                   (3, 832, 100), (8, 7712, 601), (20, 3904, 64)])
 def test_matmul(m, k, n, block, dtype):
     f = _f()
     codes, state, w = _weights(n, k, block, dtype, m + k + n)
@@ -153,6 +154,8 @@ def test_matmul_shapes_strides_and_order():
     for off in (1, 2, 8):
         wide[:, off:off + 256] = codes
         assert torch.equal(f.int4_matmul(x, wide[:, off:off + 256], state), y)
+    odd = torch.zeros(300 * 8 + 1, dtype=BF, device=DEV)[1:].view(300, 8).copy_(state)        # scales that begin in a word's upper half
+    assert torch.equal(f.int4_matmul(x, codes, odd), y)
     xs = torch.full((4, 5, 520), float("nan"), dtype=BF, device=DEV)
     xs[..., 3:515] = x
     assert torch.equal(f.int4_matmul(xs[..., 3:515], codes, state), y)
