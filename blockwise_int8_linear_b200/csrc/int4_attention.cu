@@ -10,15 +10,16 @@
 //   S[row, query]  = sum_d k[row, d] q[query, d]
 //   O[d, query]    = sum_row v[row, d] P[row, query]  two rows' words interleaved by byte permutes
 // v's scales differ by row, so they go into P: p * vs in fp16 (11 bits, for bf16 results of 8) or, for fp16 results, as a sum of two fp16
-// numbers, normalised by a power of two that follows the largest scale met, like the running maximum of the softmax.  P leaves the first product with its rows along the lanes and
-// enters the second transposed (movmatrix).  Sums, statistics and scales are fp32.
+// numbers, normalised by a power of two that follows the largest scale met, like the running maximum of the softmax.  P leaves the first
+// product with its rows along the lanes and enters the second transposed (movmatrix).  Sums, statistics and scales are fp32.
 //
 // With that, 650 instructions a step of 32 rows of 128 values, what bounds long caches is what the SMs issue: 127000 rows of 8 heads
 // in 38 us, 3.6 TB/s (IPC 2.5).  Short ones are latency: 4 us for the smallest call, 0.75 us a step.
 //
-// A warp takes steps of 16, 32 or 64 rows (4 KB), the next one on its way into shared memory while one is multiplied.  The warps of a CTA and the CTAs of a cluster divide the rows of one cache head
-// (each reads the lengths and takes its share of what there really is) and are joined over distributed shared memory; more than eight
-// shares go through a workspace and a second kernel.  Every sum has a fixed order.
+// A warp takes steps of 16, 32 or 64 rows (4 KB), the next one on its way into shared memory while one is multiplied.  The warps of a CTA
+// and the CTAs of a cluster divide the rows of one cache head (each reads the lengths and takes its share of what there really is) and
+// are joined over distributed shared memory; more than eight shares go through a workspace and a second kernel.  Every sum has a
+// fixed order.
 #include "int4_common.cuh"
 
 #include <cooperative_groups.h>

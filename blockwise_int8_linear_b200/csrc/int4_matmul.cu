@@ -12,8 +12,8 @@
 // several tiles are collected before they are added, over the warps and over the cluster, in a fixed order: no workspace, no atomics, the
 // same bits on every call.
 //
-// Measured: one row through 4096 x 4096 5.9 us, 4096 -> 32000 19 us (3.65 TB/s); 8 rows through 4096 -> 11008 12 us, 32 29 us, 64 50 us.  Few
-// rows are bound by what the SMs issue (410 instructions a piece, 180 of them unpacking), small layers by latency.
+// Measured: one row through 4096 x 4096 5.9 us, 4096 -> 32000 19 us (3.65 TB/s); 8 rows through 4096 -> 11008 12 us, 16 17 us, 32 28 us,
+// 64 50 us.  Few rows are bound by what the SMs issue (410 instructions a piece, 180 of them unpacking), small layers by latency.
 #include "int4_common.cuh"
 
 #include <cooperative_groups.h>
@@ -264,43 +264,28 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
                         }
                         const Codes4 r0a = unpack8<T>(w0.x), r0b = unpack8<T>(w0.y), r1a = unpack8<T>(w1.x), r1b = unpack8<T>(w1.y);
                         const int AFTER = BLOCK == 32 ? 2 * u + 1 : u * PER / 4;         // the scale of (the second half of) these 64 values
-                        // eight columns, or twice eight, whose sums do not wait for one another
-                        constexpr int PAIR = NT == 1 ? 1 : 2;
 #pragma unroll
-                        for (int t = 0; t < NT; t += PAIR) {
-                            uint4 xa[PAIR], xb[PAIR];
-                            float d[PAIR][4];
-#pragma unroll
-                            for (int h = 0; h < PAIR; ++h) {
-                                // columns behind the last row of x read that row again and are not stored
-                                const uint4* p = reinterpret_cast<const uint4*>(xp + min(8 * (t + h) + g, rows_x - 1) * pitch + u * 128);
-                                xa[h] = p[0];
-                                xb[h] = p[1];
-                            }
-                            auto scaled = [&](int h, int i) {
-                                float (&y4)[4] = y[t + h];
-                                y4[0] = fmaf(d[h][0], scale(0, i), y4[0]);
-                                y4[1] = fmaf(d[h][1], scale(0, i), y4[1]);
-                                y4[2] = fmaf(d[h][2], scale(1, i), y4[2]);
-                                y4[3] = fmaf(d[h][3], scale(1, i), y4[3]);
+                        for (int t = 0; t < NT; ++t) {
+                            // columns behind the last row of x read that row again and are not stored
+                            const uint4* p = reinterpret_cast<const uint4*>(xp + min(8 * t + g, rows_x - 1) * pitch + u * 128);
+                            const uint4 xa = p[0], xb = p[1];
+                            float d[4];
+                            auto scaled = [&](int i) {
+                                y[t][0] = fmaf(d[0], scale(0, i), y[t][0]);
+                                y[t][1] = fmaf(d[1], scale(0, i), y[t][1]);
+                                y[t][2] = fmaf(d[2], scale(1, i), y[t][2]);
+                                y[t][3] = fmaf(d[3], scale(1, i), y[t][3]);
                             };
-#pragma unroll
-                            for (int h = 0; h < PAIR; ++h) mma16_first<T>(d[h], r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa[h].x, xa[h].y);
-#pragma unroll
-                            for (int h = 0; h < PAIR; ++h) mma16<T>(d[h], r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa[h].z, xa[h].w);
-#pragma unroll
-                            for (int h = 0; h < PAIR; ++h) {
-                                if (BLOCK == 32) {
-                                    scaled(h, 2 * u);
-                                    mma16_first<T>(d[h], r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb[h].x, xb[h].y);
-                                } else {
-                                    mma16<T>(d[h], r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb[h].x, xb[h].y);
-                                }
+                            mma16_first<T>(d, r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa.x, xa.y);
+                            mma16<T>(d, r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa.z, xa.w);
+                            if (BLOCK == 32) {
+                                scaled(2 * u);
+                                mma16_first<T>(d, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
+                            } else {
+                                mma16<T>(d, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
                             }
-#pragma unroll
-                            for (int h = 0; h < PAIR; ++h) mma16<T>(d[h], r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb[h].z, xb[h].w);
-#pragma unroll
-                            for (int h = 0; h < PAIR; ++h) scaled(h, AFTER);
+                            mma16<T>(d, r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb.z, xb.w);
+                            scaled(AFTER);
                         }
                     }
                     out = out + 1 == RING ? 0 : out + 1;
@@ -442,10 +427,11 @@ int launch(MatmulArgs a, cudaStream_t st) {
         group = (rounds + (rounds + group - 1) / group - 1) / ((rounds + group - 1) / group);
         bytes += (group - 1) * sums;
         const double waves = ((int64_t)clusters * m_tiles + room - 1) / room, pieces = (cta + wk - 1) / wk;
-        // a tile: its pieces on all warps, x again where it does not stay, what is left of the loop; a group's sums; x, once
+        // a tile: its pieces on all warps, x again where it does not stay, what is left of the loop; x, once; a group's sums, over
+        // the warps and then over the cluster, each of whose CTAs stores its share (taking 16 rows through 4096 -> 11008 from 21 us to 17)
         const double tile = pieces * kWarps * (110.0 + 50.0 * NT) + (stage < cta ? 30.0 * rows_x * cta + 2000.0 * ((cta + stage - 1) / stage) : 0.0) + 450.0;
         const double quads = (double)group * rows_x * wn * 4 / kThreads;
-        const double reduction = 600.0 + quads * (1800.0 + 80.0 * wk) + (ranks > 1 ? 1800.0 : 0.0);
+        const double reduction = 600.0 + (wk > 1 ? quads * (300.0 + 80.0 * wk) : 0.0) + quads / ranks * 1500.0 + (ranks > 1 ? 600.0 + 700.0 * ranks : 0.0);
         const double cost = waves * (4000.0 + 30.0 * rows_x * cta + rounds * tile + (rounds + group - 1) / group * reduction);
         if (cost < best.cost) best = {wn, ranks, cta, stage, tiles, group, clusters * ranks, bytes, cost};
     };

@@ -316,7 +316,7 @@ def test_attention_starts_scale_and_empty_rows():
 
 
 @pytest.mark.parametrize("rows,t", [(96, 1), (96, 20), (20000, 1)])
-def test_attention_never_reads_what_nobody_sees(rows, t):
+def test_attention_ignores_what_nobody_sees(rows, t):
     """NaN scales in every row behind the length, before the start, and (for the earlier of several queries) in the later ones' rows."""
     o = _d()
     cache, k, v = _cache(1, 2, rows, 128, BF, 3)
