@@ -9,12 +9,12 @@
 // them, eight at a time, the columns:
 //   S[row, query]  = sum_d k[row, d] q[query, d]
 //   O[d, query]    = sum_row v[row, d] P[row, query]  two rows' words interleaved by byte permutes
-// v's scales differ by row, so they go into P: p * vs in fp16 (11 bits, for bf16 results of 8) or, for fp16 results, as a sum of two fp16
-// numbers, normalised by a power of two that follows the largest scale met, like the running maximum of the softmax.  P leaves the first
+// v's scales differ by row, so they go into P: p * vs as a sum of two fp16 numbers (22 bits: one alone, 11 bits, is 9 % faster over long caches,
+// but its roundings do not cancel where the values do, and leave a difference of nearly equal weights with two or three bits),
+// normalised by a power of two that follows the largest scale met, like the running maximum of the softmax.  P leaves the first
 // product with its rows along the lanes and enters the second transposed (movmatrix).  Sums, statistics and scales are fp32.
 //
-// With that, 650 instructions a step of 32 rows of 128 values, what bounds long caches is what the SMs issue: 127000 rows of 8 heads
-// in 38 us, 3.6 TB/s (IPC 2.5).  Short ones are latency: 4 us for the smallest call, 0.75 us a step.
+// What bounds long caches is the length of a step in instructions and their waits for one another: 127000 rows of 8 heads in 43 us, 3.2 TB/s.  Short ones are latency: 4 us for the smallest call, 0.75 us a step.
 //
 // A warp takes steps of 16, 32 or 64 rows (4 KB), the next one on its way into shared memory while one is multiplied.  The warps of a CTA
 // and the CTAs of a cluster divide the rows of one cache head (each reads the lengths and takes its share of what there really is) and
@@ -114,7 +114,6 @@ struct Smem {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(const AttnArgs a) {
-    constexpr bool FINE = std::is_same<T, __half>::value;
     constexpr int U = D / 64, TT = kStepTiles<D>, STEP = 16 * TT, COLS = kCols, PITCH = Smem<D>::kPitch, BUF = Smem<D>::kBuf;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* const xs = smem;                                                    // [COLS] rows of PITCH bytes
@@ -322,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
                     const uint32_t hi = pack_f16x2(x0, x1);
                     using H = F16Bits<__half>;
                     bh[r] = transpose8x8(hi);
-                    if (FINE) bl[r] = transpose8x8(pack_f16x2(x0 - H::lo(hi), x1 - H::hi(hi)));
+                    bl[r] = transpose8x8(pack_f16x2(x0 - H::lo(hi), x1 - H::hi(hi)));
                 }
                 const uint8_t* const even = slot + (at_v ^ (32 * u)) + Slot::kV + 16 * i * (D / 2);
                 const uint8_t* const odd = slot + ((at_v ^ (32 * u)) ^ Slot::kOdd) + Slot::kOddAdd + Slot::kV + 16 * i * (D / 2);
@@ -339,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
                         const uint32_t x = w01 >> (8 * j), y = w23 >> (8 * j);
                         const uint32_t a0 = half2_low(x), a1 = half2_high(x), a2 = half2_low(y), a3 = half2_high(y);
                         mma16<__half>(o[4 * u + 2 * half + j], a0, a1, a2, a3, bh[0], bh[1]);
-                        if (FINE) mma16<__half>(o[4 * u + 2 * half + j], a0, a1, a2, a3, bl[0], bl[1]);
+                        mma16<__half>(o[4 * u + 2 * half + j], a0, a1, a2, a3, bl[0], bl[1]);
                     }
                 }
             }
