@@ -11,10 +11,12 @@
 //   O[d, query]    = sum_row v[row, d] P[row, query]  two rows' words interleaved by byte permutes
 // v's scales differ by row, so they go into P: p * vs as a sum of two fp16 numbers (22 bits: one alone, 11 bits, is 9 % faster over long caches,
 // but its roundings do not cancel where the values do, and leave a difference of nearly equal weights with two or three bits),
-// normalised by a power of two that follows the largest scale met, like the running maximum of the softmax.  P leaves the first
+// normalised by a power of two that follows the largest p * vs that the query has met, like the running maximum of the softmax: a
+// query's own, so that rows which it does not see have no part in its result, and of the products, so that large values of no weight
+// take no bits from the others.  P leaves the first
 // product with its rows along the lanes and enters the second transposed (movmatrix).  Sums, statistics and scales are fp32.
 //
-// What bounds long caches is the length of a step in instructions and their waits for one another: 127000 rows of 8 heads in 43 us, 3.2 TB/s.  Short ones are latency: 4 us for the smallest call, 0.75 us a step.
+// What bounds long caches is the length of a step in instructions and their waits for one another: 127000 rows of 8 heads in 45 us, 3.1 TB/s.  Short ones are latency: 4 us for the smallest call, 0.75 us a step.
 //
 // A warp takes steps of 16, 32 or 64 rows (4 KB), the next one on its way into shared memory while one is multiplied.  The warps of a CTA
 // and the CTAs of a cluster divide the rows of one cache head (each reads the lengths and takes its share of what there really is) and
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
     float* const cta_l = cta_m + COLS;                                           // [COLS]
     float* const weight = cta_l + COLS;                                          // [kClusterShares][COLS]
     float* const factor = weight + kClusterShares * COLS;                        // [COLS]
-    float* const buf = reinterpret_cast<float*>(rings);                          // [kWarps][8][BUF], when the rings are done with
+    float* const buf = reinterpret_cast<float*>(rings);                          // [kWarps][8][BUF], when every warp has left its ring
     float* const sums = buf + kWarps * 8 * BUF;                                  // [COLS][D]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -162,7 +164,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
     }
     const int unmasked = min(last, fewest);
     float o[4 * U][4] = {};
-    float vmax = 0x1p-110f, vscale = 0x1p124f;            // power of two, no smaller than the scales of v so far (up to 2^127); 2^14 over it
+    float vtop[2] = {0.0f, 0.0f}, vmax[2] = {0x1p-110f, 0x1p-110f};      // a column's largest p * vs, and a power of two that is no smaller (2^127 at most)
+    auto over = [](float pow2) { return __uint_as_float(((127u + 14u + 127u) << 23) - __float_as_uint(pow2)); };      // 2^14 / pow2
 
     const uint8_t* const kp = a.cache.k + b * a.cache.k_batch + h * a.cache.k_head;
     const uint8_t* const vp = a.cache.v + b * a.cache.v_batch + h * a.cache.v_head;
@@ -275,49 +278,50 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
                 }
             l[j] = fmaf(l[j], alpha[j], sum);
         }
-        // ---- v's scales: a larger one than any before moves the normalisation
-        float vs[TT][2][U], big = 0.0f;
+        // ---- times v's scales: a larger product than any before moves the column's normalisation
+        float pv[TT][2][U][2], big[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < TT; ++i)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                scales_of(slot + Slot::kScalesV, 16 * i + g + 8 * r, vs[i][r]);
+                float vs[U];
+                scales_of(slot + Slot::kScalesV, 16 * i + g + 8 * r, vs);
+                const int row = base + 16 * i + g + 8 * r;
 #pragma unroll
-                for (int u = 0; u < U; ++u) big = fmaxf(big, vs[i][r][u]);       // passes over the NaN of blocks that hold one
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const bool unseen = MASKED && (row >= limit[j] || row < start);          // its scale may be anything
+                        pv[i][r][u][j] = unseen ? 0.0f : p[i][2 * r + j] * vs[u];
+                        big[j] = fmaxf(big[j], fabsf(pv[i][r][u][j]));                            // passes over the NaN of blocks that hold one
+                    }
             }
-        if (__any_sync(0xffffffffu, grown || big > vmax)) {
-            float top = big;
+        if (__any_sync(0xffffffffu, grown || big[0] > vmax[0] || big[1] > vmax[1])) {
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            float shrink = 1.0f;
-            if (top > vmax && vmax < 0x1p127f) {
-                const uint32_t e = min((__float_as_uint(top) >> 23) + 1u, 254u);
-                const float next = __uint_as_float(e << 23);
-                shrink = vmax / next;
-                vmax = next;
-                vscale = 0x1p14f / next;
+            for (int j = 0; j < 2; ++j) {
+                float top = big[j];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                vtop[j] = fmaxf(vtop[j] * alpha[j], top);
+                const float next = __uint_as_float(min(max((__float_as_uint(vtop[j]) + 0x7fffffu) >> 23, 127u - 110u), 254u) << 23);
+                alpha[j] = alpha[j] * vmax[j] * over(next) * 0x1p-14f;      // vmax is the smallest number, or below twice what vtop was: at most 2^15 on the way
+                vmax[j] = next;
             }
 #pragma unroll
             for (int w = 0; w < 4 * U; ++w)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[w][j] *= alpha[j & 1] * shrink;
+                for (int j = 0; j < 4; ++j) o[w][j] *= alpha[j & 1];
         }
         // ---- O += V^T P
+        const float vscale[2] = {over(vmax[0]), over(vmax[1])};
 #pragma unroll
         for (int i = 0; i < TT; ++i)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float s0 = vs[i][0][u] * vscale, s1 = vs[i][1][u] * vscale;
                 uint32_t bh[2], bl[2];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const float sc = r ? s1 : s0;
-                    float x0 = p[i][2 * r] * sc, x1 = p[i][2 * r + 1] * sc;
-                    if (MASKED) {                     // a masked row's scale may be anything
-                        const int row = base + 16 * i + g + 8 * r;
-                        if (row >= limit[0] || row < start) x0 = 0.0f;
-                        if (row >= limit[1] || row < start) x1 = 0.0f;
-                    }
+                    const float x0 = pv[i][r][u][0] * vscale[0], x1 = pv[i][r][u][1] * vscale[1];
                     const uint32_t hi = pack_f16x2(x0, x1);
                     using H = F16Bits<__half>;
                     bh[r] = transpose8x8(hi);
@@ -403,11 +407,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
         cta_l[col] = total;
     }
     __syncthreads();
-    const float unit = vmax * (0x1p-14f / 7.0f);          // (every warp has left its ring)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int col = 2 * c + j;
-        const float w = m[j] == -INFINITY ? 0.0f : exp2_fast(m[j] * fac[j] - cta_m[col]) * unit;
+        const float w = m[j] == -INFINITY ? 0.0f : exp2_fast(m[j] * fac[j] - cta_m[col]) * (vmax[j] * (0x1p-14f / 7.0f));
         float* dst = buf + (warp * 8 + col) * BUF + 8 * g;
 #pragma unroll
         for (int u = 0; u < U; ++u) {

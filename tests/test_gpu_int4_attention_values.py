@@ -39,3 +39,60 @@ def test_weights_that_cancel(d, rows, dtype):
     err = (got.double() - want).abs()
     assert bool((err <= tol).all()), (err / tol).max().item()
     assert_clean_device()
+
+
+def _bits(dtype, seed, shape):
+    """Any 16 bits as a number of the type, and among them its largest, infinities and NaN."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(-32768, 32768, shape, generator=g, dtype=torch.int32).to(torch.int16).view(dtype)
+    special = torch.tensor([torch.finfo(dtype).max, float("inf"), -float("inf"), float("nan")], dtype=dtype)
+    return torch.where(torch.rand(shape, generator=g) < 0.5, special[torch.randint(0, 4, shape, generator=g)], x).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("what", ["max", "inf", "far", "bits"])
+@pytest.mark.parametrize("d,rows,t", [(64, 150, 1), (128, 96, 1), (128, 96, 20), (256, 70, 3), (128, 20000, 1)])
+def test_unseen_rows_may_hold_anything(d, rows, t, what, dtype):
+    """Rows before the start, behind the length, and for each query those of the later ones, with the type's largest number, an infinity, 2^40
+    times the visible scales (2^15 in fp16, which has no more) or any bits as scales and any codes: the same bits as without them."""
+    o = _d()
+    cache, k, v = _cache(1, 2, rows, d, dtype, 3)
+    q = _randn((1, 4, t, d), 4, dtype)
+    last, first = rows - 30, 21
+    n, s = torch.tensor([last], device=DEV), torch.tensor([first], device=DEV)
+    clean = o.attention_int4_cache(q, cache, n, starts=s)
+    _check_attention(clean, q, k, v, [last], [first])
+    fill = {"max": torch.finfo(dtype).max, "inf": float("inf"), "far": 2.0 ** 40 if dtype == BF else 2.0 ** 15}
+
+    def spoil(rows_of):
+        for codes, state in ((cache.k, cache.k_state), (cache.v, cache.v_state)):
+            part = state[:, :, rows_of]
+            state[:, :, rows_of] = _bits(dtype, 7, part.shape) if what == "bits" else fill[what]
+            codes[:, :, rows_of] = torch.randint(0, 256, codes[:, :, rows_of].shape, dtype=torch.uint8).to(DEV)
+
+    spoil(slice(0, first))
+    spoil(slice(last, None))
+    assert torch.equal(o.attention_int4_cache(q, cache, n, starts=s), clean)
+    for later in range(t - 1, 0, -1):                       # the row that query `later` is the first to see
+        spoil(slice(last - t + later, last - t + later + 1))
+        assert torch.equal(o.attention_int4_cache(q, cache, n, starts=s)[:, :, :later], clean[:, :, :later])
+    assert_clean_device()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("at", [0, 40, 299])
+def test_large_values_of_no_weight(at, dtype):
+    """A row whose weight is e^-60 and whose values are 2^30 (2^15 in fp16) times the others': 8e-18 of the result, wherever it lies."""
+    o = _d()
+    rows, d = 300, 128
+    g = torch.Generator().manual_seed(1)
+    k, v = torch.randn((1, 1, rows, d), generator=g) * 0.05, torch.randn((1, 1, rows, d), generator=g)
+    q = torch.ones((1, 1, 1, d))
+    k[0, 0, at] = -60.0 / d ** 0.5
+    v[0, 0, at] *= 2.0 ** 30 if dtype == BF else 2.0 ** 13
+    kc, ks, kv = _held(k, dtype)
+    vc, vs, vv = _held(v, dtype)
+    q = q.to(dtype).to(DEV)
+    got = o.attention_int4_cache(q, o.Int4KVCache(kc, ks, vc, vs), torch.tensor([rows], device=DEV))
+    rest = [i for i in range(rows) if i != at]
+    _check_attention(got, q, kv[:, :, rest], vv[:, :, rest], [rows - 1])
