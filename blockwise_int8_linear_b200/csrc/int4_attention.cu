@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
     const int chunk = (n_rows + a.shares * STEP - 1) / (a.shares * STEP) * STEP;
     const int first = origin + min(n_rows, share * chunk), last = min(origin + n_rows, first + chunk);
     int limit[2];
-    float m[2], l[2], fac[2];
+    float m[2], l[2], fac[2];                              // running maximum (in powers of two) and total of a column, its factor
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int col = 2 * c + j;
@@ -261,10 +261,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
                 }
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float now = fmaxf(m[j], top);
-            // scores are the products without the column's factor, which is not negative; a column may have seen nothing yet
-            const float ref = MASKED && now == -INFINITY ? 0.0f : now * fac[j];
-            alpha[j] = exp2_fast(fmaf(m[j], fac[j], -ref));
+            // The running maximum is kept as it is subtracted: times the column's factor (not negative) and rounded.  So what it was and what it is
+            // differ by nothing where it has not grown, and total and sums are rescaled alike.  A column may have seen nothing yet.
+            const float now = fmaxf(m[j], top * fac[j]), ref = now == -INFINITY ? 0.0f : now;
+            alpha[j] = exp2_fast(m[j] - ref);
             grown = grown || now != m[j];
             m[j] = now;
             float sum = 0.0f;
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], d);
         if (g == 0) {
-            warp_m[warp * COLS + 2 * c + j] = m[j] == -INFINITY ? -INFINITY : m[j] * fac[j];      // log2 units
+            warp_m[warp * COLS + 2 * c + j] = m[j];
             warp_l[warp * COLS + 2 * c + j] = l[j];
         }
     }
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int col = 2 * c + j;
-        const float w = m[j] == -INFINITY ? 0.0f : exp2_fast(m[j] * fac[j] - cta_m[col]) * (vmax[j] * (0x1p-14f / 7.0f));
+        const float w = m[j] == -INFINITY ? 0.0f : exp2_fast(m[j] - cta_m[col]) * (vmax[j] * (0x1p-14f / 7.0f));
         float* dst = buf + (warp * 8 + col) * BUF + 8 * g;
 #pragma unroll
         for (int u = 0; u < U; ++u) {

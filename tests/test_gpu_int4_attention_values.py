@@ -96,3 +96,22 @@ def test_large_values_of_no_weight(at, dtype):
     got = o.attention_int4_cache(q, o.Int4KVCache(kc, ks, vc, vs), torch.tensor([rows], device=DEV))
     rest = [i for i in range(rows) if i != at]
     _check_attention(got, q, kv[:, :, rest], vv[:, :, rest], [rows - 1])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_large_scores_over_many_rows(d, dtype):
+    """Equal keys and values of 1 over 65536 rows, 600 sequences with scores of 60 to 3000: the result is 1.  Weights and total differ by 2^-22
+    (two fp16 numbers), their sums by a step in 2^23 for every 16 of a warp's 2048 rows: 2^-15, an eighth of half a step below 1 in fp16."""
+    o = _d()
+    rows, b = 65536, 600
+    k = torch.zeros((1, 1, 1, d))
+    k[..., 0] = 1.0
+    kc, ks, _ = _held(k, dtype)
+    vc, vs, _ = _held(torch.ones((1, 1, 1, d)), dtype)
+    cache = o.Int4KVCache(*(x.expand(-1, -1, rows, -1).contiguous().expand(b, -1, -1, -1) for x in (kc, ks, vc, vs)))
+    q = torch.zeros((b, 1, 1, d), dtype=dtype, device=DEV)
+    q[:, 0, 0, 0] = torch.logspace(1.78, 3.47, b).to(dtype).to(DEV)
+    got = o.attention_int4_cache(q, cache, torch.tensor([rows - 5], device=DEV), scale=1.0)
+    assert bool((got == 1).all()), (got.double() - 1).abs().max().item()
+    assert_clean_device()
