@@ -2,6 +2,7 @@
 #include "bi8_common.cuh"
 #include "peer_common.cuh"
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
@@ -675,6 +676,7 @@ int bi8_attention_int4(const void* q, int dtype, int64_t q_batch, int64_t q_head
     DeviceOfCall call;
     if (int rc = check_int4_cache("attention_int4", dtype, cache, B, T, Hq, Hkv, D)) return rc;
     if (lengths_step < 0 || starts_step < 0) return fail(BI8_ERR_SHAPE, "attention_int4: negative step");
+    if (!(std::fabs(scale) <= 2e38f)) return fail(BI8_ERR_LIMIT, "attention_int4: scale %g is not a number of at most 2e38", (double)scale);
     if (B == 0 || T == 0 || Hq == 0) return BI8_OK;
     if (!q || !lengths || !out) return fail(BI8_ERR_NULL, "attention_int4: null pointer");
     if (!aligned(q, 16) || q_batch % 8 || q_head % 8 || q_tok % 8 || !aligned(out, 16) || !aligned(lengths, 8) || !aligned(starts, 8))

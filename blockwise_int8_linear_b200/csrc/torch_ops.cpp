@@ -25,6 +25,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <optional>
 #include <string>
@@ -1035,6 +1036,7 @@ Tensor attention_int4(const Tensor& q_in, const Tensor& k, const Tensor& k_state
     if (hkv < 1 || hq < 1 || hq % hkv != 0) value_error(std::to_string(hq) + " query heads do not divide over " + std::to_string(hkv) + " cache heads");
     OnDevice on(q_in);
     const PerSequence len(lengths, q_in, b, "lengths"), start(starts, q_in, b, "starts");
+    if (!(std::abs(scale) <= 2e38)) value_error("scale must be a number of at most 2e38, got " + std::to_string(scale));
     Tensor out = empty_on(q_in, {b, hq, t, d}, q_in.scalar_type());
     if (out.numel() == 0) return out;
     Tensor q = q_in;

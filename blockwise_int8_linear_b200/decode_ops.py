@@ -62,7 +62,8 @@ def attention_int4_cache(q: torch.Tensor, cache: Int4KVCache, lengths: torch.Ten
     ``lengths`` (int64 on the device, one element or ``[B]``): how many rows a sequence has, the last T of which are the queries' own:
     query t sees the rows up to ``lengths - T + t`` (T = 1: all of them).  ``starts`` (the same form): the first row that is seen, for
     batches padded on the left or a window.  A query that sees no row gives zeros; rows that nobody sees may hold anything.  ``scale``
-    defaults to ``1 / sqrt(D)``.  Both are read by the kernel, so the call can be replayed from a CUDA graph while they change."""
+    is a number of at most 2e38, by default ``1 / sqrt(D)``.  Lengths and starts are read by the kernel, so the call can be replayed from a
+    CUDA graph while they change."""
     if scale is None:
         scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     return _lib.native().attention_int4(q, cache.k, cache.k_state, cache.v, cache.v_state, lengths, starts, scale)

@@ -319,6 +319,7 @@ BI8_API int bi8_rope_cache_append_int4(const void* qkv, int dtype, const float* 
  *   lengths  device address (int64): sequence b has lengths[b * lengths_step] rows, the last T of which are the queries' own: query t sees
  *            rows up to lengths - T + t.  Lengths beyond max_len see max_len rows
  *   starts   the first row that is seen (rows before it belong to nobody, as in a batch padded on the left), or NULL for 0
+ *   scale    a number of at most 2e38 (BI8_ERR_LIMIT for infinities and NaN)
  * A query that sees no row gives zeros.  Rows that no query sees may hold anything.  Hq is a multiple of Hkv; query head h reads cache head
  * h / (Hq / Hkv).  workspace: bi8_attention_int4_workspace_bytes bytes, 16-byte aligned, scratch of this call. */
 BI8_API size_t bi8_attention_int4_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len);
