@@ -851,10 +851,13 @@ Tensor rope_cache_append(const Tensor& qkv_in, const Tensor& cis_in, const Tenso
 }
 
 // ---- weights and key/value caches in 4-bit blocks ---------------------------------------------------------------------------
-// These have no backward pass: a tensor that wants a gradient would lose it silently.
+// These have no derivatives: a tensor that wants a gradient, or brings a tangent, would lose it silently.
 void no_gradient(const Tensor& t, const char* what) {
-    if (t.defined() && at::GradMode::is_enabled() && t.requires_grad())
+    if (!t.defined()) return;
+    if (at::GradMode::is_enabled() && t.requires_grad())
         throw PyFail{PyExc_RuntimeError, std::string(what) + " has no backward pass: call it under torch.no_grad() or on detached tensors"};
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+        throw PyFail{PyExc_RuntimeError, std::string(what) + " has no forward-mode derivative: call it on tensors without tangents"};
 }
 int dtype_code16(at::ScalarType t, const char* what) {
     if (t != at::kBFloat16 && t != at::kHalf) value_error(std::string(what) + " must be bfloat16 or float16, got " + c10::toString(t));
@@ -900,6 +903,7 @@ void check_scales4(const Tensor& state, const Tensor& codes, int64_t blocks, int
 
 Tensor dequantize_int4(const Tensor& codes, const Tensor& state, int64_t block, int64_t features, at::ScalarType out_type) {
     need_cuda(codes);
+    no_gradient(state, "dequantize_block_int4");
     if (codes.dim() == 0 || codes.scalar_type() != at::kByte) value_error(std::string("codes must be uint8 with a feature dimension, got ") + c10::toString(codes.scalar_type()));
     const int code = dtype_code16(state.scalar_type(), "state");
     check_block4(block);
@@ -919,8 +923,7 @@ Tensor dequantize_int4(const Tensor& codes, const Tensor& state, int64_t block, 
 Tensor matmul_int4(const Tensor& x_in, const Tensor& codes, const Tensor& state, const Tensor& bias_in, const Tensor& residual, int64_t block,
                    at::ScalarType out_type) {
     need_cuda(x_in);
-    no_gradient(x_in, "int4_matmul");
-    no_gradient(residual, "int4_matmul");
+    for (const Tensor* t : {&x_in, &state, &bias_in, &residual}) no_gradient(*t, "int4_matmul");
     if (x_in.dim() == 0) value_error("expected a tensor with a feature dimension, got a scalar");
     const int code = dtype_code16(x_in.scalar_type(), "activations");
     check_block4(block);
@@ -997,7 +1000,7 @@ bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr(
 Tensor rope_cache_append_int4(const Tensor& qkv_in, const Tensor& cis_in, const Tensor& pos, const Tensor& k, const Tensor& k_state, const Tensor& v,
                               const Tensor& v_state) {
     need_cuda(qkv_in);
-    no_gradient(qkv_in, "rope_cache_append_int4");
+    for (const Tensor* t : {&qkv_in, &cis_in, &k_state, &v_state}) no_gradient(*t, "rope_cache_append_int4");
     if (qkv_in.dim() != 4) value_error("expected [B, T, Hq + 2 Hkv, D], got " + shape_of(qkv_in));
     const int code = dtype_code16(qkv_in.scalar_type(), "activations");
     const int64_t b = qkv_in.size(0), t = qkv_in.size(1), d = qkv_in.size(3);
@@ -1026,7 +1029,7 @@ Tensor rope_cache_append_int4(const Tensor& qkv_in, const Tensor& cis_in, const 
 Tensor attention_int4(const Tensor& q_in, const Tensor& k, const Tensor& k_state, const Tensor& v, const Tensor& v_state, const Tensor& lengths,
                       const Tensor& starts, double scale) {
     need_cuda(q_in);
-    no_gradient(q_in, "attention_int4_cache");
+    for (const Tensor* t : {&q_in, &k_state, &v_state}) no_gradient(*t, "attention_int4_cache");
     if (q_in.dim() != 4) value_error("expected queries [B, Hq, T, D], got " + shape_of(q_in));
     const int code = dtype_code16(q_in.scalar_type(), "queries");
     const int64_t b = q_in.size(0), hq = q_in.size(1), t = q_in.size(2), d = q_in.size(3);

@@ -7,7 +7,8 @@ Scales ("state") are ``[..., ceil(K/block)]`` in x's type, row by row (not trans
 scale 0; one that holds an infinity or a NaN has the scale NaN and reads as NaN throughout.
 
 Blocks have 32, 64 or 128 values: ``block_linear_config.GROUP_SIZE`` read at call time unless ``fblock_size`` is given.  The functions
-run on the current CUDA stream of their operands' device; they have no backward pass and refuse tensors that want a gradient.
+run on the current CUDA stream of their operands' device; they have no derivatives and refuse tensors that want a gradient (outside
+``torch.no_grad()``) or bring a forward-mode tangent: biases, scales and rotary tables as much as activations.
 """
 from __future__ import annotations
 
