@@ -247,7 +247,10 @@ class BlockInt4Linear(nn.Linear):
 
     The weight is quantized on the first forward in eval mode (buffers ``W_int4`` uint8 ``[out, ceil(in/2)]`` and ``state_W4``
     ``[out, ceil(in/block)]``, part of ``state_dict()``); a float32 weight is rounded to ``INPUT_OUTPUT_TORCH_TYPE`` first (to bfloat16
-    where that is float32 too), and activations have the type of the scales.  Training mode refuses to run."""
+    where that is float32 too), and activations have the type of the scales.  Training mode refuses to run.
+
+    Loading a checkpoint that brings 4-bit buffers replaces the layer's, and one that brings a floating-point weight without them drops
+    them.  A weight that is changed in any other way after the first forward counts from the next ``prepare_for_eval()`` on."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None, dtype=None,
                  _skip_init: bool = False):
@@ -291,7 +294,25 @@ class BlockInt4Linear(nn.Linear):
         return self.infer(x)
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
-        _make_room_for_buffers(self, ("W_int4", "state_W4"), state_dict, prefix)
+        weight, codes, state = (state_dict.get(prefix + name) for name in ("weight", "W_int4", "state_W4"))
+        if (codes is None) != (state is None):
+            error_msgs.append(f"{prefix}W_int4 and {prefix}state_W4 belong together: the checkpoint has one of them")
+            return
+        if codes is not None:
+            want = (self.out_features, (self.in_features + 1) // 2)
+            if tuple(codes.shape) != want or state.dim() != 2 or state.shape[0] != self.out_features:
+                error_msgs.append(f"size mismatch for {prefix}W_int4 / {prefix}state_W4: {tuple(codes.shape)} / {tuple(state.shape)} for codes {want}")
+                return
+            # buffers as the checkpoint has them: scales copied into another type would be rounded under codes that stay
+            for name, held in (("W_int4", codes), ("state_W4", state)):
+                mine = self._buffers.get(name)
+                if mine is None or mine.shape != held.shape or mine.dtype != held.dtype:
+                    self.register_buffer(name, torch.empty_like(held, device=self.weight.device))
+        elif weight is not None and weight.numel() > 0 and hasattr(self, "W_int4"):
+            del self.W_int4, self.state_W4                 # another floating-point weight: quantized anew on the next forward
+        # a weight that has been dropped, here or in the checkpoint, has no elements
+        if weight is not None and weight.shape != self.weight.shape and (weight.numel() == 0 or tuple(weight.shape) == (self.out_features, self.in_features)):
+            self.weight.data = torch.empty_like(weight, device=self.weight.device, dtype=self.weight.dtype)
         super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
 
