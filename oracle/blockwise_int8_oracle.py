@@ -85,7 +85,9 @@ def rmsnorm(x: torch.Tensor, eps: float = 1e-5, weight: torch.Tensor = None) -> 
 def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """``F.silu(gate) * up`` as two stored elementwise steps: ``cast(gate / (1 + exp(-gate)))``, then ``cast(. * up)``."""
     gf = gate.to(torch.float32)
-    s = (gf / (1.0 + torch.exp(-gf))).to(gate.dtype)
+    # on the CPU the exponential is taken in 64 bits: torch's 32-bit one now and then has a stretch of a tensor with half its bits
+    e = torch.exp(-gf) if gf.is_cuda else torch.exp(-gf.double()).float()
+    s = (gf / (1.0 + e)).to(gate.dtype)
     return (s.to(torch.float32) * up.to(torch.float32)).to(gate.dtype)
 
 
