@@ -247,7 +247,12 @@ class BlockInt4Linear(nn.Linear):
 
     The weight is quantized on the first forward in eval mode (buffers ``W_int4`` uint8 ``[out, ceil(in/2)]`` and ``state_W4``
     ``[out, ceil(in/block)]``, part of ``state_dict()``); a float32 weight is rounded to ``INPUT_OUTPUT_TORCH_TYPE`` first (to bfloat16
-    where that is float32 too), and activations have the type of the scales.  Training mode refuses to run.
+    where that is float32 too).  Activations are multiplied in the type of the scales: float32 ones are rounded to it, bfloat16 ones become
+    float16 where the scales are (beyond 65504 infinite), float16 ones are refused where the scales are bfloat16.  Results have
+    ``INPUT_OUTPUT_TORCH_TYPE``.  Training mode refuses to run.
+
+    ``model.float()``, ``.half()`` and ``.bfloat16()`` leave the codes alone, so the scales follow only into a 16-bit type that holds
+    each of them exactly.
 
     Loading a checkpoint that brings 4-bit buffers replaces the layer's, and one that brings a floating-point weight without them drops
     them.  A weight that is changed in any other way after the first forward counts from the next ``prepare_for_eval()`` on."""
@@ -285,13 +290,27 @@ class BlockInt4Linear(nn.Linear):
         """``x @ W^T (+ bias) (+ residual)``; ``residual`` has the output's shape and type."""
         if self._buffers.get("W_int4") is None:
             self.prepare_for_eval()
-        bias = self.bias
-        return int4_matmul(x, self._buffers["W_int4"], self._buffers["state_W4"], None if bias is None else bias.detach(), residual=residual)
+        bias, state = self.bias, self._buffers["state_W4"]
+        if x.dtype != state.dtype and (x.dtype == torch.float32 or (x.dtype, state.dtype) == (torch.bfloat16, torch.float16)):
+            x = x.to(state.dtype)
+        return int4_matmul(x, self._buffers["W_int4"], state, None if bias is None else bias.detach(), residual=residual)
 
     def forward(self, x):
         if self.training:
             raise RuntimeError("BlockInt4Linear is for inference: call eval() first")
         return self.infer(x)
+
+    def _apply(self, fn, recurse=True):
+        state = self._buffers.get("state_W4")
+        super()._apply(fn, recurse)
+        if state is not None:
+            cast = self._buffers["state_W4"]
+            if cast.dtype != state.dtype:
+                kept = state.to(cast.device)
+                if (cast.is_meta or cast.dtype not in (torch.bfloat16, torch.float16)
+                        or not torch.allclose(cast.to(kept.dtype), kept, rtol=0, atol=0, equal_nan=True)):
+                    self._buffers["state_W4"] = kept
+        return self
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
         weight, codes, state = (state_dict.get(prefix + name) for name in ("weight", "W_int4", "state_W4"))

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from tests.gpu_util import DEV, assert_clean_device, set_config
-from tests.test_gpu_int4 import BF, HF, _f, _randn
+from tests.test_gpu_int4 import BF, FF, HF, _f, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -33,4 +33,36 @@ def test_loading_another_weight_after_the_first_forward(drop):
     # parameters are copied into the layer's type, as nn.Linear's are: the bias is half's in bf16
     assert torch.equal(a(x.to(HF)), _f().int4_matmul(x.to(HF), half.W_int4, half.state_W4, half.bias.detach().to(BF)))
     set_config(64, BF)
+    assert_clean_device()
+
+
+def test_types_of_model_and_activations():
+    """A chain of layers runs in a float32 model, an fp16 model under results in bf16, and after a cast of the model; results are the functional
+    product's on activations in the scales' type."""
+    f = _f()
+
+    def chain(dtype, out):
+        set_config(64, out)
+        net = torch.nn.Sequential(_layer(dtype, 1, 200, 130), _layer(dtype, 3, 130, 64)).eval()
+        return net, _randn((5, 200), 9, dtype)
+
+    def want(net, x):
+        for m in net:
+            x = f.int4_matmul(x.to(m.state_W4.dtype), m.W_int4, m.state_W4, m.bias.detach())
+        return x
+
+    for dtype, out in ((FF, BF), (FF, HF), (FF, FF), (HF, BF), (HF, FF), (BF, FF), (BF, BF), (HF, HF)):
+        net, x = chain(dtype, out)
+        y = net(x)
+        assert y.dtype == out and torch.equal(y, want(net, x))
+        state = [m.state_W4.clone() for m in net]
+        net.float()
+        assert all(torch.equal(m.state_W4, s) and m.state_W4.dtype == s.dtype for m, s in zip(net, state))
+        got = net(x.float())
+        assert torch.equal(got, want(net, x.float()))
+    net, x = chain(HF, BF)
+    assert bool(net[0](torch.full((1, 200), 1e5, dtype=BF, device=DEV)).isfinite().logical_not().all())      # loudly, beyond fp16
+    net, x = chain(BF, BF)
+    with pytest.raises(ValueError, match="one type"):
+        net(x.to(HF))
     assert_clean_device()

@@ -57,3 +57,23 @@ def test_what_does_not_fit_is_refused():
     nothing = _quantized(0)
     nothing.load_state_dict({"bias": torch.zeros(16)}, strict=False)         # no weight of either kind: the buffers stay
     assert hasattr(nothing, "W_int4")
+
+
+def test_casting_a_model_changes_no_weight():
+    """Scales follow into a type that holds them exactly and stay what they are otherwise, NaN included; devices and everything else follow."""
+    for dtype, cast in ((torch.bfloat16, "half"), (torch.bfloat16, "float"), (torch.float16, "float"), (torch.float16, "bfloat16"), (torch.float16, "double")):
+        m = _quantized(0, dtype)
+        m.state_W4[0, 0] = float("nan")
+        want = m.state_W4.float()
+        getattr(nn.Sequential(m), cast)()
+        assert m.state_W4.dtype == (torch.float16 if cast == "half" else dtype) and torch.equal(m.state_W4.float().nan_to_num(), want.nan_to_num())
+        assert bool(m.state_W4[0, 0].isnan()) and m.W_int4.dtype == torch.uint8 and m.weight.dtype != dtype
+    for s in (1e6, 1e-7):                                  # what fp16 does not hold
+        m = _quantized(0)
+        m.state_W4[3, 1] = s
+        want = m.state_W4.clone()
+        assert torch.equal(m.half().state_W4, want)
+    exact = _quantized(0, torch.float16)
+    exact.state_W4.copy_(exact.state_W4.bfloat16())
+    assert exact.bfloat16().state_W4.dtype == torch.bfloat16
+    assert _quantized(0).to("meta").state_W4.is_meta and _quantized(0).to("meta", torch.float16).state_W4.dtype == torch.bfloat16
