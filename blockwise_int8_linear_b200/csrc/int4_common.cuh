@@ -85,10 +85,11 @@ __device__ __forceinline__ uint32_t quantize8(const uint4& v, uint32_t lanes, ui
 __device__ __forceinline__ void values8(float s, uint32_t w, float (&y)[8]);
 
 // ---- tensor-core operands -----------------------------------------------------------------------------------------------------
-// Codes become the matrix instruction's operands in pairs, as the numbers -7 to 7 in the other operand's type.  Four bits c + 8 under the
+// Codes become the matrix instruction's operands in pairs, as numbers in the other operand's type: -7 to 7 in fp16, and 2^-10 of that in bf16
+// (kCodeUnit), where a block's sum of codes times values as large as the type has would overflow otherwise.  Four bits c + 8 under the
 // exponent of 1024 are the fp16 number 1024 + 8 + c, four bits further up 1024 + 16 (8 + c); a packed subtraction or multiply-add
-// makes c of them, exactly: eight codes are one shift, four AND-ORs and four packed operations.  bf16 has 128 + 8 + c, and no room for four
-// bits further up: two shifts more.  (The four bits alone are fp16 denormals, (8 + c) 2^-24, and the offset could be left to the
+// makes c of them, exactly: eight codes are one shift, four AND-ORs and four packed operations.  bf16 has (128 + 8 + c) 2^-10, and no room for
+// four bits further up: two shifts more.  (This way of unpacking is the usual one of kernels with 4-bit weights.  The four bits alone are fp16 denormals, (8 + c) 2^-24, and the offset could be left to the
 // accumulator's start value, which saves half of that.  But the instruction aligns its sums by the operands' exponent fields, and ten
 // leading zeros in one operand cost the sum as many bits: measured, 2^-16 of the largest term.)
 //
@@ -112,10 +113,12 @@ __device__ __forceinline__ uint32_t half2_high(uint32_t w) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t bf162_low(uint32_t w) {
-    const uint32_t v = and_or(w, 0x000f000fu, 0x43004300u), k = 0x43084308u;              // 128 + 8 + c, 136
+    const uint32_t v = and_or(w, 0x000f000fu, 0x3e003e00u), k = 0x3e083e08u;              // (128 + 8 + c) 2^-10, 136 * 2^-10
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&k));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
+template <typename T>
+constexpr float kCodeUnit = std::is_same<T, __half>::value ? 1.0f : 0x1p-10f;           // what a code of 1 becomes
 template <typename T>
 __device__ __forceinline__ Codes4 unpack8(uint32_t w) {
     if (std::is_same<T, __half>::value) return {half2_low(w), half2_high(w), half2_low(w >> 8), half2_high(w >> 8)};

@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (n + j >= a.N) return;
-                float v = y[j] * (1.0f / 7.0f);
+                float v = y[j] * (1.0f / 7.0f / kCodeUnit<T>);
                 if (a.bias) v += load_as_float(a.bias, a.bias_dtype, n + j);
                 if (a.residual) v += load_as_float(a.residual, a.out_dtype, (int64_t)m * a.ldr + n + j);
                 store_from_float(a.C, a.out_dtype, (int64_t)m * a.ldc + n + j, v);
