@@ -29,6 +29,7 @@
 #include <mutex>
 #include <optional>
 #include <string>
+#include <vector>
 
 #include "../../include/bi8.h"
 
@@ -957,7 +958,42 @@ Tensor matmul_int4(const Tensor& x_in, const Tensor& codes, const Tensor& state,
     return out;
 }
 
-// The cache's tensors as the library takes them.  `written`: heads and sequences must not share memory.
+// Whether heads, sequences, or keys and values of a cache [B, H, rows, width] with dense rows share memory.  Nested steps and tensors that lie
+// apart, as nearly every cache has them, are told by a few comparisons; anything else (keys and values interleaved in one tensor, steps
+// that interlock) by all of its parts in order.
+bool parts_overlap(const Tensor& k, const Tensor& v) {
+    struct Part {
+        uintptr_t begin, end;
+    };
+    Part whole[2];
+    bool nested = true;
+    for (const Tensor* t : {&k, &v}) {
+        if (t->numel() == 0) return false;
+        const int64_t part = t->size(2) * t->size(3);
+        int64_t n[2] = {t->size(0), t->size(1)}, step[2] = {t->stride(0), t->stride(1)};
+        for (int i = 0; i < 2; ++i)
+            if (n[i] == 1) step[i] = 0;
+        if (step[0] > step[1]) std::swap(n[0], n[1]), std::swap(step[0], step[1]);
+        const int64_t inner = (n[0] - 1) * step[0] + part;
+        nested = nested && (n[0] == 1 || step[0] >= part) && (n[1] == 1 || step[1] >= inner);
+        const uintptr_t at = reinterpret_cast<uintptr_t>(t->data_ptr());
+        whole[t == &v] = {at, at + (uintptr_t)(((n[1] - 1) * step[1] + inner) * t->element_size())};
+    }
+    if (nested && (whole[0].end <= whole[1].begin || whole[1].end <= whole[0].begin)) return false;
+    std::vector<Part> parts;
+    for (const Tensor* t : {&k, &v})
+        for (int64_t i = 0; i < t->size(0); ++i)
+            for (int64_t j = 0; j < t->size(1); ++j) {
+                const uintptr_t at = reinterpret_cast<uintptr_t>(t->data_ptr()) + (uintptr_t)((i * t->stride(0) + j * t->stride(1)) * t->element_size());
+                parts.push_back({at, at + (uintptr_t)(t->size(2) * t->size(3) * t->element_size())});
+            }
+    std::sort(parts.begin(), parts.end(), [](const Part& a, const Part& b) { return a.begin < b.begin; });
+    for (size_t i = 1; i < parts.size(); ++i)
+        if (parts[i].begin < parts[i - 1].end) return true;
+    return false;
+}
+
+// The cache's tensors as the library takes them.  `written`: its parts must not share memory.
 bi8_int4_cache cache4(const Tensor& k, const Tensor& k_state, const Tensor& v, const Tensor& v_state, const Tensor& like, int64_t b, int64_t d, bool written) {
     if (k.dim() != 4) value_error("cache codes must be 4-D, got " + shape_of(k));
     const int64_t h = k.size(1), rows = k.size(2);
@@ -973,11 +1009,10 @@ bi8_int4_cache cache4(const Tensor& k, const Tensor& k_state, const Tensor& v, c
             value_error(std::string("cache ") + (codes ? "codes" : "scales") + " must be " + c10::toString(type) + " [" + std::to_string(b) + ", " +
                         std::to_string(h) + ", " + std::to_string(rows) + ", " + std::to_string(width) + "] with dense rows on " + like.device().str() + ", got " +
                         c10::toString(t->scalar_type()) + " " + shape_of(*t));
-        for (int dim = 0; dim < 2; ++dim) {
-            steps[at++] = t->size(dim) > 1 ? t->stride(dim) : 0;
-            if (written && t->size(dim) > 1 && t->stride(dim) < rows * width) value_error("a cache that is written must not share memory between sequences or heads");
-        }
+        for (int dim = 0; dim < 2; ++dim) steps[at++] = t->size(dim) > 1 ? t->stride(dim) : 0;
     }
+    if (written && (parts_overlap(k, v) || parts_overlap(k_state, v_state)))
+        value_error("a cache that is written must not share memory between sequences, heads, or keys and values");
     return {static_cast<uint8_t*>(k.data_ptr()), static_cast<uint8_t*>(v.data_ptr()), k_state.data_ptr(), v_state.data_ptr(),
             steps[0], steps[1], steps[2], steps[3], steps[4], steps[5], steps[6], steps[7], rows};
 }

@@ -291,7 +291,8 @@ BI8_API int bi8_matmul_int4(const void* x, int x_dtype, int64_t ldx, const uint8
 
 /* A key/value cache in 4 bits: codes [batch, head, max_len, D/2] and scales [batch, head, max_len, D/64] (blocks of 64) of k and of v.  Rows
  * of a head are dense; steps between batches and heads are free: bytes for the codes (multiples of 16), elements for the scales
- * (multiples of D/64).  Codes begin on 16-byte boundaries, scales on boundaries of a row's scales. */
+ * (multiples of D/64).  Codes begin on 16-byte boundaries, scales on boundaries of a row's scales.  Sequences and heads may share memory
+ * (steps of 0) in a cache that is read, not in one that is written. */
 typedef struct {
     uint8_t* k;
     uint8_t* v;
