@@ -7,6 +7,7 @@
 
 #include "bi8_common.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 namespace bi8 {
@@ -188,15 +189,15 @@ __device__ __forceinline__ void wait_copies() {
 
 // SMs of the current device.
 inline int sm_count() {
-    static int sms[64] = {0};
+    static std::atomic<int> sms[64];             // calls come from several threads
     int dev = 0;
     if (current_device(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (sms[dev] == 0) {
-        int n = 0;
+    int n = sms[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
-        sms[dev] = n;
+        sms[dev].store(n, std::memory_order_relaxed);
     }
-    return sms[dev];
+    return n;
 }
 
 }  // namespace bi8
