@@ -269,23 +269,23 @@ __global__ void __launch_bounds__(kThreads, 1) matmul_int4_kernel(const MatmulAr
                             // columns behind the last row of x read that row again and are not stored
                             const uint4* p = reinterpret_cast<const uint4*>(xp + min(8 * t + g, rows_x - 1) * pitch + u * 128);
                             const uint4 xa = p[0], xb = p[1];
-                            float d[4];
-                            auto scaled = [&](int i) {
+                            auto scaled = [&](const float (&d)[4], int i) {
                                 y[t][0] = fmaf(d[0], scale(0, i), y[t][0]);
                                 y[t][1] = fmaf(d[1], scale(0, i), y[t][1]);
                                 y[t][2] = fmaf(d[2], scale(1, i), y[t][2]);
                                 y[t][3] = fmaf(d[3], scale(1, i), y[t][3]);
                             };
+                            float d[4];
                             mma16_first<T>(d, r0a.p04, r1a.p04, r0a.p15, r1a.p15, xa.x, xa.y);
                             mma16<T>(d, r0a.p26, r1a.p26, r0a.p37, r1a.p37, xa.z, xa.w);
                             if (BLOCK == 32) {
-                                scaled(2 * u);
+                                scaled(d, 2 * u);
                                 mma16_first<T>(d, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
                             } else {
                                 mma16<T>(d, r0b.p04, r1b.p04, r0b.p15, r1b.p15, xb.x, xb.y);
                             }
                             mma16<T>(d, r0b.p26, r1b.p26, r0b.p37, r1b.p37, xb.z, xb.w);
-                            scaled(AFTER);
+                            scaled(d, AFTER);
                         }
                     }
                     out = out + 1 == RING ? 0 : out + 1;
