@@ -16,7 +16,7 @@
 // take no bits from the others.  P leaves the first
 // product with its rows along the lanes and enters the second transposed (movmatrix).  Sums, statistics and scales are fp32.
 //
-// What bounds long caches is the length of a step in instructions and their waits for one another: 127000 rows of 8 heads in 45 us, 3.1 TB/s.  Short ones are latency: 4 us for the smallest call, 0.75 us a step.
+// What bounds long caches is the length of a step in instructions and their waits for one another: 127000 rows of 8 heads in 45.5 us, 3.0 TB/s.  Short ones are latency: 4 us for the smallest call, 0.75 us a step.
 //
 // A warp takes steps of 16, 32 or 64 rows (4 KB), the next one on its way into shared memory while one is multiplied.  The warps of a CTA
 // and the CTAs of a cluster divide the rows of one cache head (each reads the lengths and takes its share of what there really is) and
@@ -256,14 +256,16 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     float& x = p[i][2 * r + j];
+                    x = __fmul_rn(x, fac[j]);             // the column's factor is not negative
                     if (MASKED && (base + 16 * i + g + 8 * r >= limit[j] || base + 16 * i + g + 8 * r < start)) x = -INFINITY;
                     top = fmaxf(top, x);
                 }
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            // The running maximum is kept as it is subtracted: times the column's factor (not negative) and rounded.  So what it was and what it is
-            // differ by nothing where it has not grown, and total and sums are rescaled alike.  A column may have seen nothing yet.
-            const float now = fmaxf(m[j], top * fac[j]), ref = now == -INFINITY ? 0.0f : now;
+            // The running maximum is one of the rounded products that it is subtracted from.  So nothing is above it, however large the scores (the
+            // product's rounding error alone may be: in one multiply-add of 1e20 it would be 2^40 to the exponential), and where it has not
+            // grown, total and sums are rescaled by 1.  A column may have seen nothing yet.
+            const float now = fmaxf(m[j], top), ref = now == -INFINITY ? 0.0f : now;
             alpha[j] = exp2_fast(m[j] - ref);
             grown = grown || now != m[j];
             m[j] = now;
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) attention_int4_kernel(
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
                     float& x = p[i][2 * r + j];
-                    x = exp2_fast(fmaf(x, fac[j], -ref));
+                    x = exp2_fast(x - ref);
                     sum += x;
                 }
             l[j] = fmaf(l[j], alpha[j], sum);

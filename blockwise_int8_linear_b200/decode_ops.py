@@ -61,7 +61,8 @@ def attention_int4_cache(q: torch.Tensor, cache: Int4KVCache, lengths: torch.Ten
 
     ``lengths`` (int64 on the device, one element or ``[B]``): how many rows a sequence has, the last T of which are the queries' own:
     query t sees the rows up to ``lengths - T + t`` (T = 1: all of them).  ``starts`` (the same form): the first row that is seen, for
-    batches padded on the left or a window.  A query that sees no row gives zeros; rows that nobody sees may hold anything.  ``scale``
+    batches padded on the left or a window.  A query that sees no row gives zeros; rows that it does not see may hold anything.  Keys of
+    2^100 and more may overflow in the scores, which are fp32.  ``scale``
     is a number of at most 2e38, by default ``1 / sqrt(D)``.  Lengths and starts are read by the kernel, so the call can be replayed from a
     CUDA graph while they change."""
     if scale is None:

@@ -115,3 +115,24 @@ def test_large_scores_over_many_rows(d, dtype):
     got = o.attention_int4_cache(q, cache, torch.tensor([rows - 5], device=DEV), scale=1.0)
     assert bool((got == 1).all()), (got.double() - 1).abs().max().item()
     assert_clean_device()
+
+
+@pytest.mark.parametrize("d,rows", [(64, 600), (128, 300), (256, 100)])
+def test_queries_near_the_ends_of_the_range(d, rows):
+    """Queries of 1e20 let one row decide, queries of 1e-30 none; values grow by eight powers of ten along the cache."""
+    o = _d()
+    g = torch.Generator().manual_seed(5)
+    k = torch.randn((1, 2, rows, d), generator=g)
+    v = torch.randn((1, 2, rows, d), generator=g) * torch.logspace(-4, 4, rows)[:, None]
+    kc, ks, kv = _held(k, BF)
+    vc, vs, vv = _held(v, BF)
+    q = _randn((1, 2, 1, d), 2, BF)
+    q[:, 0] *= 1e20
+    q[:, 1] *= 1e-30
+    got = o.attention_int4_cache(q, o.Int4KVCache(kc, ks, vc, vs), torch.tensor([rows], device=DEV))
+    scores = (kv[0, 0] @ q[0, 0, 0].double()) * d ** -0.5
+    first, second = scores.topk(2).values.tolist()
+    assert first - second > 1e-3 * first                    # far more than fp32 sums are off by
+    want = vv[0, 0, scores.argmax()]
+    assert bool(((got[0, 0, 0].double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20)).all())
+    _check_attention(got[:, 1:], q[:, 1:], kv[:, 1:], vv[:, 1:], [rows])
