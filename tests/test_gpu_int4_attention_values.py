@@ -136,3 +136,23 @@ def test_queries_near_the_ends_of_the_range(d, rows):
     want = vv[0, 0, scores.argmax()]
     assert bool(((got[0, 0, 0].double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20)).all())
     _check_attention(got[:, 1:], q[:, 1:], kv[:, 1:], vv[:, 1:], [rows])
+
+
+def test_rows_beyond_2_to_the_31_bytes():
+    """One sequence with 2.5e9 bytes of codes: its last 300 rows are those of a short cache."""
+    o = _d()
+    rows, d, seen = 40_000_000, 128, 300
+    short, k, v = _cache(1, 1, seen, d, BF, 12)
+    big = o.int4_kv_cache(1, 1, rows, d, BF, DEV)
+    for x, y in zip(big, short):
+        x[:, :, rows - seen:] = y
+    q = _randn((1, 4, 2, d), 13, BF)
+    at = lambda n: torch.tensor([n], device=DEV)
+    got = o.attention_int4_cache(q, big, at(rows), starts=at(rows - seen))
+    _check_attention(got, q, k, v, [seen])
+    # and with every row in sight: keys and values of 0, so that a row counts by exp(0 - its score alone)
+    one = o.attention_int4_cache(q[:, :, :1], big, at(rows))
+    total = torch.exp((k[0, 0] @ q[0, :, 0].double().t()) * d ** -0.5)                    # [seen, heads]
+    want = torch.einsum("rh,rd->hd", total, v[0, 0]) / (total.sum(0) + rows - seen)[:, None]
+    # the values that count are 300 of 4e7: sums of weights in fp32 over 128 shares, 1 part in 2^13 at the worst
+    assert bool(((one[0, :, 0].double() - want).abs() <= want.abs() * 2.0 ** -8 + total.sum(0)[:, None] / rows * 2.0 ** -13).all())
