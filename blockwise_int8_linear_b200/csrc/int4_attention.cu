@@ -13,10 +13,12 @@
 // but its roundings do not cancel where the values do, and leave a difference of nearly equal weights with two or three bits),
 // normalised by a power of two that follows the largest p * vs that the query has met, like the running maximum of the softmax: a
 // query's own, so that rows which it does not see have no part in its result, and of the products, so that large values of no weight
-// take no bits from the others.  P leaves the first
-// product with its rows along the lanes and enters the second transposed (movmatrix).  Sums, statistics and scales are fp32.
+// take no bits from the others.  P leaves the first product with its rows along the lanes and enters the second transposed (movmatrix).
+// Sums, statistics and scales are fp32.
 //
-// What bounds long caches is the length of a step in instructions and their waits for one another: 127000 rows of 8 heads in 45.5 us, 3.0 TB/s.  Short ones are latency: 4 us for the smallest call, 0.75 us a step.
+// What bounds long caches: 815 instructions a step of 32 rows of 128 values, at an IPC of 2.4 of 4 (with 3.5 warps a scheduler, waits for the
+// instruction before and for the integer pipe take the rest): 127000 rows of 8 heads in 45.5 us, 3.0 TB/s.  Short ones are latency: 4 us for the
+// smallest call, 0.75 us a step.
 //
 // A warp takes steps of 16, 32 or 64 rows (4 KB), the next one on its way into shared memory while one is multiplied.  The warps of a CTA
 // and the CTAs of a cluster divide the rows of one cache head (each reads the lengths and takes its share of what there really is) and
@@ -557,11 +559,11 @@ Plan plan_of(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     Plan p;
     p.col_tiles = (int)((R + kCols - 1) / kCols);
     p.tiles = B * Hkv * p.col_tiles;
-    // As many CTAs as the device holds at once.  Few tiles are divided down to a step for each warp (one sequence of 2048 rows, 8 heads: 16 us in
-    // 1 share, 8 in 4, 6 in 16), beyond two CTAs an SM into 512 rows and more (16384 rows: 13.1 us in 16 shares, 11.5 in 32, 13.5 in 74), more
-    // tiles than SMs only into 1024 rows and more (256 tiles of 576 rows: 10.6 us in 1, 11.7 in 2).  Long
-    // caches, whose sequences may differ much in length, have shares of 2048 rows (32 sequences of 1 to 8192 rows, 8 heads: 65 us in 2, 55
-    // in 4, 61 in 8; 64 of 4096 rows each: 71 us in 1, 68 in 2, 82 in 4).  The clusters' sizes are powers of two.
+    // As many CTAs as the device holds at once.  Few tiles are divided down to a step for each warp (one sequence of 2048 rows, 8 heads: 19 us in
+    // 1 share, 8.6 in 4, 6.2 in 16), beyond two CTAs an SM into 512 rows and more (16384 rows: 14.2 us in 16 shares, 12.3 in 32, 13.9 in 74), more
+    // tiles than SMs only into 1024 rows and more (256 tiles of 576 rows: 11.5 us in 1, 12.4 in 2).  Long
+    // caches, whose sequences may differ much in length, have shares of 2048 rows (32 sequences of 1 to 8192 rows, 8 heads: 79 us in 2, 62
+    // in 4, 66 in 8; 64 of 4096 rows each: 88 us in 1, 80 in 2, 92 in 4).  The clusters' sizes are powers of two.
     const int64_t step = 16 * (D == 64 ? kStepTiles<64> : D == 128 ? kStepTiles<128> : kStepTiles<256>), sms = sm_count();
     const int64_t useful = p.tiles < sms ? (max_len + kWarps * step - 1) / (kWarps * step) : max_len / 1024, long_ones = max_len / 2048;
     int64_t want = (D == 256 ? kResident<256> : kResident<128>) * sms / p.tiles;

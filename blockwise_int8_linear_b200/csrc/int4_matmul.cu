@@ -12,8 +12,10 @@
 // several tiles are collected before they are added, over the warps and over the cluster, in a fixed order: no workspace, no atomics, the
 // same bits on every call.
 //
-// Measured: one row through 4096 x 4096 5.9 us, 4096 -> 32000 19 us (3.65 TB/s); 8 rows through 4096 -> 11008 12 us, 16 17 us, 32 28 us,
-// 64 50 us.  Few rows are bound by what the SMs issue (410 instructions a piece, 180 of them unpacking), small layers by latency.
+// Measured, launched from a graph: one row through 4096 x 4096 6.0 us, 4096 -> 32000 19 us (3.65 TB/s); 8 rows through 4096 -> 11008 12 us,
+// 16 17 us, 32 28 us, 64 50 us.  Few rows are bound by a warp's 580 instructions a piece (180 unpack, 230 more are the rest of the loop, the
+// others fills, x and sums; IPC 2.1), small layers by latency.  Instances of 16 and more columns spill (12 to 92 bytes a thread at 16, 60 to 128 at
+// 32, 220 to 460 at 64): 128 registers are what 512 threads have.
 #include "int4_common.cuh"
 
 #include <cooperative_groups.h>
