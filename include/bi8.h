@@ -322,7 +322,8 @@ BI8_API int bi8_rope_cache_append_int4(const void* qkv, int dtype, const float* 
  *   starts   the first row that is seen (rows before it belong to nobody, as in a batch padded on the left), or NULL for 0
  *   scale    a number of at most 2e38 (BI8_ERR_LIMIT for infinities and NaN)
  * A query that sees no row gives zeros.  Rows that a query does not see may hold anything.  Keys of 2^100 and more may overflow in the
- * scores, which are fp32.  Hq is a multiple of Hkv; query head h reads cache head h / (Hq / Hkv).  workspace: bi8_attention_int4_workspace_bytes bytes, 16-byte aligned, scratch of this call. */
+ * scores, which are fp32.  Hq is a multiple of Hkv; query head h reads cache head h / (Hq / Hkv).  workspace:
+ * bi8_attention_int4_workspace_bytes bytes, 16-byte aligned, scratch of this call. */
 BI8_API size_t bi8_attention_int4_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len);
 BI8_API int bi8_attention_int4(const void* q, int dtype, int64_t q_batch, int64_t q_head, int64_t q_tok, const bi8_int4_cache* cache,
                                const long long* lengths, int64_t lengths_step, const long long* starts, int64_t starts_step, float scale,
