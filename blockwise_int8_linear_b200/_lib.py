@@ -31,10 +31,11 @@ EXPORTS = [
     "bi8_gemm_dequant_residual", "bi8_quantize_rowwise_pitched", "bi8_quantize_colwise_pitched", "bi8_quantize_dual_pitched",
     "bi8_quantize_rowwise_pre_pitched", "bi8_dequantize_rowwise_pitched", "bi8_column_sum", "bi8_column_sum_workspace_bytes",
     "bi8_copy_rows", "bi8_quantize_int4", "bi8_dequantize_int4", "bi8_matmul_int4", "bi8_rope_cache_append_int4", "bi8_attention_int4",
-    "bi8_attention_int4_workspace_bytes",
+    "bi8_attention_int4_workspace_bytes", "bi8_rope", "bi8_rope_cache_append_paged", "bi8_attention_paged", "bi8_attention_paged_workspace_bytes",
 ]
 ADDEND_FULL = 0x100
 PRE_NONE, PRE_RMSNORM, PRE_SILU_MUL = 0, 1, 2
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 
 
 
@@ -42,6 +43,18 @@ class Int4Cache(ctypes.Structure):
     """``bi8_int4_cache``: a key/value cache in 4-bit blocks."""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "k_state", "v_state")]
                 + [(n, ctypes.c_int64) for n in ("k_batch", "k_head", "v_batch", "v_head", "ks_batch", "ks_head", "vs_batch", "vs_head", "max_len")])
+
+
+class PagedCache(ctypes.Structure):
+    """``bi8_paged_cache``: a key/value cache in pages."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v")]
+                + [(n, ctypes.c_int64) for n in ("k_page", "k_head", "k_row", "v_page", "v_head", "v_row", "pages", "heads", "page_rows", "head_dim")])
+
+
+class Sequences(ctypes.Structure):
+    """``bi8_sequences``: the sequences of a batch of new tokens."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("lengths", "cu_tokens", "starts", "page_table")]
+                + [(n, ctypes.c_int64) for n in ("lengths_step", "starts_step", "table_step", "width", "B", "N")])
 
 
 _lib = None
@@ -121,11 +134,17 @@ def lib() -> ctypes.CDLL:
         L.bi8_attention_int4_workspace_bytes.restype = sz
         L.bi8_attention_int4.argtypes = [vp, i32, i64, i64, i64, c.POINTER(Int4Cache), vp, i64, vp, i64, c.c_float, vp, i64, i64, i64, i64, i64,
                                          vp, sz, vp]
+        L.bi8_rope.argtypes = [vp, i32, i64, i64, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, i64, i64, i32, i32, vp]
+        L.bi8_rope_cache_append_paged.argtypes = [vp, i32, i64, i64, vp, i64, i64, i32, vp, c.POINTER(PagedCache), c.POINTER(Sequences), i64, vp]
+        L.bi8_attention_paged_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64, i32]
+        L.bi8_attention_paged_workspace_bytes.restype = sz
+        L.bi8_attention_paged.argtypes = [vp, i32, i64, i64, c.POINTER(PagedCache), c.POINTER(Sequences), c.c_float, vp, i64, vp, sz, vp]
         for name in EXPORTS:
             fn = getattr(L, name)
             if name not in ("bi8_last_error_string", "bi8_gemm_workspace_bytes", "bi8_gemm_workspace_used", "bi8_quantize_dual_sum_workspace_bytes", "bi8_gemm_static_scratch_bytes",
                             "bi8_peer_allreduce_buffer_bytes", "bi8_peer_allreduce_large_buffer_bytes", "bi8_column_sum_workspace_bytes",
-                            "bi8_peer_allreduce_large_partial_offset", "bi8_peer_allreduce_large_out_offset", "bi8_attention_int4_workspace_bytes"):
+                            "bi8_peer_allreduce_large_partial_offset", "bi8_peer_allreduce_large_out_offset", "bi8_attention_int4_workspace_bytes",
+                            "bi8_attention_paged_workspace_bytes"):
                 fn.restype = i32
         _lib = L
     return _lib

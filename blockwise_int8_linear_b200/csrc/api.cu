@@ -1,5 +1,6 @@
 // extern "C" surface of libbi8.so: argument validation, dispatch, error text.  See include/bi8.h.
 #include "bi8_common.cuh"
+#include "paged_common.cuh"
 #include "peer_common.cuh"
 
 #include <cmath>
@@ -686,6 +687,107 @@ int bi8_attention_int4(const void* q, int dtype, int64_t q_batch, int64_t q_head
         return fail(BI8_ERR_WORKSPACE, "attention_int4: %zu bytes of workspace needed, got %zu", want, workspace ? workspace_bytes : (size_t)0);
     return launch_attention_int4(q, dtype, q_batch, q_head, q_tok, cache, lengths, lengths_step, starts, starts_step, scale, out, B, T, Hq, Hkv, D,
                                  workspace, static_cast<cudaStream_t>(stream));
+}
+
+// ---- rotary positions and a paged key/value cache ---------------------------------------------------------------------------
+int bi8_rope(const void* x, int dtype, int64_t x_batch, int64_t x_tok, int64_t x_head, const float* cis, int64_t rows, int64_t R, const long long* pos,
+             int64_t pos_batch, int64_t pos_tok, void* out, int64_t B, int64_t T, int64_t H, int64_t D, int layout, int conjugate, void* stream) {
+    DeviceOfCall call;
+    if (!dtype_ok(dtype)) return fail(BI8_ERR_DTYPE, "rope: unknown dtype code %d", dtype);
+    if (layout != BI8_ROPE_INTERLEAVED && layout != BI8_ROPE_HALF) return fail(BI8_ERR_SHAPE, "rope: unknown layout %d", layout);
+    if (B < 0 || T < 0 || H < 0 || D < 2 || rows < 0 || H > 0x7fffffff / D || (T > 0 && B > (1ll << 40) / T))
+        return fail(BI8_ERR_SHAPE, "rope: bad shape B %lld T %lld H %lld D %lld", (long long)B, (long long)T, (long long)H, (long long)D);
+    if (R < 2 || R > D || R % 2 != 0) return fail(BI8_ERR_SHAPE, "rope: %lld rotated features of %lld, expected an even number from 2", (long long)R, (long long)D);
+    if (x_batch < 0 || x_tok < 0 || x_head < 0 || pos_batch < 0 || pos_tok < 0) return fail(BI8_ERR_SHAPE, "rope: negative step");
+    if (B == 0 || T == 0 || H == 0) return BI8_OK;
+    if (!x || !out || (rows > 0 && !cis)) return fail(BI8_ERR_NULL, "rope: null pointer");
+    if (!aligned(x, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)) || !aligned(cis, 16) || !aligned(pos, 8))
+        return fail(BI8_ERR_ALIGN, "rope: pointer not aligned");
+    return launch_rope(x, dtype, x_batch, x_tok, x_head, cis, rows, R, pos, pos_batch, pos_tok, out, B, T, H, D, layout == BI8_ROPE_HALF, conjugate != 0,
+                       static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+
+// The shape of a step with a paged cache, the cache's layout and the batch's.
+int check_paged(const char* what, int dtype, const bi8_paged_cache* c, const bi8_sequences* q, int64_t Hq, Sequences* s) {
+    if (dtype != BI8_BF16 && dtype != BI8_F16) return fail(BI8_ERR_DTYPE, "%s: bf16 or fp16 activations (got code %d)", what, dtype);
+    if (!c || !q) return fail(BI8_ERR_NULL, "%s: null cache or sequences", what);
+    if (q->B < 0 || q->N < 0 || Hq < 0 || c->heads < 1 || c->pages < 0 || q->width < 0 || q->B > 0x7ffffffe || q->N > 0x7fffffff || Hq > 0xffff ||
+        c->heads > 0xffff || c->pages > 0x7fffffff || c->page_rows < 1 || c->page_rows > (1 << 20) || q->width > 0x7fff0000 / c->page_rows)
+        return fail(BI8_ERR_SHAPE, "%s: bad shape B %lld N %lld Hq %lld heads %lld pages %lld of %lld rows, %lld a sequence", what, (long long)q->B, (long long)q->N,
+                    (long long)Hq, (long long)c->heads, (long long)c->pages, (long long)c->page_rows, (long long)q->width);
+    if (c->page_rows % 16 != 0) return fail(BI8_ERR_SHAPE, "%s: pages of %lld rows, expected a multiple of 16", what, (long long)c->page_rows);
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(BI8_ERR_SHAPE, "%s: head size %lld, expected 64, 128 or 256", what, (long long)c->head_dim);
+    if (Hq % c->heads != 0) return fail(BI8_ERR_SHAPE, "%s: %lld query heads do not divide over %lld cache heads", what, (long long)Hq, (long long)c->heads);
+    if (q->N > 0 && q->B == 0) return fail(BI8_ERR_SHAPE, "%s: tokens without a sequence", what);
+    if (!q->cu_tokens && q->B > 0 && q->N % q->B != 0)
+        return fail(BI8_ERR_SHAPE, "%s: %lld tokens do not divide over %lld sequences", what, (long long)q->N, (long long)q->B);
+    if (q->N * Hq > 0x7fffffff) return fail(BI8_ERR_LIMIT, "%s: too many queries", what);
+    if (q->lengths_step < 0 || q->starts_step < 0 || q->table_step < 0) return fail(BI8_ERR_SHAPE, "%s: negative step", what);
+    if (q->N == 0 || Hq == 0) return BI8_OK;
+    if (!q->lengths || (q->width > 0 && !q->page_table) || (c->pages > 0 && (!c->k || !c->v))) return fail(BI8_ERR_NULL, "%s: null pointer", what);
+    if (!aligned(q->lengths, 8) || !aligned(q->cu_tokens, 8) || !aligned(q->starts, 8) || !aligned(q->page_table, 4))
+        return fail(BI8_ERR_ALIGN, "%s: numbers of the sequences not aligned", what);
+    const int64_t steps[6] = {c->k_page, c->k_head, c->k_row, c->v_page, c->v_head, c->v_row};
+    for (int64_t step : steps)
+        if (step < 0 || step % 8 != 0) return fail(BI8_ERR_ALIGN, "%s: steps of the cache must be multiples of 8", what);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(BI8_ERR_ALIGN, "%s: cache not on 16-byte boundaries", what);
+    s->lengths = q->lengths;
+    s->cu = q->cu_tokens;
+    s->starts = q->starts;
+    s->pages = q->page_table;
+    s->lengths_step = q->lengths_step;
+    s->starts_step = q->starts_step;
+    s->pages_step = q->table_step;
+    s->B = (int)q->B;
+    s->N = (int)q->N;
+    s->T = (int)(q->cu_tokens ? 0 : q->N / q->B);
+    s->max_len = (int)(q->width * c->page_rows);
+    s->page = FastDiv(c->page_rows);
+    s->tokens = FastDiv(q->cu_tokens ? 1 : s->T);
+    return BI8_OK;
+}
+
+}  // namespace
+
+int bi8_rope_cache_append_paged(const void* qkv, int dtype, int64_t qkv_tok, int64_t qkv_head, const float* cis, int64_t cis_rows, int64_t R, int layout,
+                                void* q_out, const bi8_paged_cache* cache, const bi8_sequences* seq, int64_t Hq, void* stream) {
+    DeviceOfCall call;
+    Sequences s{};
+    if (int rc = check_paged("rope_cache_append_paged", dtype, cache, seq, Hq, &s)) return rc;
+    if (layout != BI8_ROPE_INTERLEAVED && layout != BI8_ROPE_HALF) return fail(BI8_ERR_SHAPE, "rope_cache_append_paged: unknown layout %d", layout);
+    if (R < 16 || R > cache->head_dim || R % 16 != 0 || cis_rows < 0)
+        return fail(BI8_ERR_SHAPE, "rope_cache_append_paged: %lld rotated features of %lld, expected a multiple of 16", (long long)R, (long long)cache->head_dim);
+    if (qkv_tok < 0 || qkv_head < 0 || qkv_tok % 8 || qkv_head % 8) return fail(BI8_ERR_ALIGN, "rope_cache_append_paged: steps must be multiples of 8");
+    if (seq->N == 0 || Hq == 0) return BI8_OK;
+    if (!qkv || !q_out || (cis_rows > 0 && !cis)) return fail(BI8_ERR_NULL, "rope_cache_append_paged: null pointer");
+    if (!aligned(qkv, 16) || !aligned(q_out, 16) || !aligned(cis, 16)) return fail(BI8_ERR_ALIGN, "rope_cache_append_paged: pointer not aligned");
+    return launch_rope_cache_append_paged(qkv, dtype, qkv_tok, qkv_head, cis, cis_rows, R, layout == BI8_ROPE_HALF, q_out, cache, s, Hq, cache->head_dim,
+                                          static_cast<cudaStream_t>(stream));
+}
+
+size_t bi8_attention_paged_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t heads, int64_t D, int64_t max_len, int packed) {
+    if (B <= 0 || N <= 0 || Hq <= 0 || heads <= 0 || Hq % heads != 0 || (D != 64 && D != 128 && D != 256) || max_len < 0 || (!packed && N % B != 0)) return 0;
+    DeviceOfCall call;
+    return attention_paged_workspace_bytes(B, N, Hq, heads, D, max_len, packed != 0);
+}
+
+int bi8_attention_paged(const void* q, int dtype, int64_t q_tok, int64_t q_head, const bi8_paged_cache* cache, const bi8_sequences* seq, float scale, void* out,
+                        int64_t Hq, void* workspace, size_t workspace_bytes, void* stream) {
+    DeviceOfCall call;
+    Sequences s{};
+    if (int rc = check_paged("attention_paged", dtype, cache, seq, Hq, &s)) return rc;
+    if (!(std::fabs(scale) <= 2e38f)) return fail(BI8_ERR_LIMIT, "attention_paged: scale %g is not a number of at most 2e38", (double)scale);
+    if (q_tok < 0 || q_head < 0 || q_tok % 8 || q_head % 8) return fail(BI8_ERR_ALIGN, "attention_paged: steps must be multiples of 8");
+    if (seq->N == 0 || Hq == 0) return BI8_OK;
+    if (!q || !out) return fail(BI8_ERR_NULL, "attention_paged: null pointer");
+    if (!aligned(q, 16) || !aligned(out, 16)) return fail(BI8_ERR_ALIGN, "attention_paged: pointer not aligned");
+    const size_t want = attention_paged_workspace_bytes(s.B, s.N, Hq, cache->heads, cache->head_dim, s.max_len, s.cu != nullptr);
+    if (want > 0 && (!workspace || workspace_bytes < want || !aligned(workspace, 16)))
+        return fail(BI8_ERR_WORKSPACE, "attention_paged: %zu bytes of workspace needed, got %zu", want, workspace ? workspace_bytes : (size_t)0);
+    return launch_attention_paged(q, dtype, q_tok, q_head, cache, s, scale, out, Hq, cache->head_dim, workspace, static_cast<cudaStream_t>(stream));
 }
 
 int bi8_stream_capture_id(void* stream, unsigned long long* id) {

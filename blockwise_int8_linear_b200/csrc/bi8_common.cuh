@@ -169,6 +169,15 @@ size_t attention_int4_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t 
 int launch_attention_int4(const void* q, int dt, int64_t q_batch, int64_t q_head, int64_t q_tok, const bi8_int4_cache* cache, const long long* lengths,
                           int64_t lengths_step, const long long* starts, int64_t starts_step, float scale, void* out, int64_t B, int64_t T, int64_t Hq,
                           int64_t Hkv, int64_t D, void* workspace, cudaStream_t st);
+// rotary positions and a paged key/value cache (rope.cu, paged_cache.cu, paged_attention.cu)
+struct Sequences;
+int launch_rope(const void* x, int dt, int64_t x_batch, int64_t x_tok, int64_t x_head, const float* cis, int64_t rows, int64_t R, const long long* pos,
+                int64_t pos_batch, int64_t pos_tok, void* out, int64_t B, int64_t T, int64_t H, int64_t D, int half_layout, int conj, cudaStream_t st);
+int launch_rope_cache_append_paged(const void* qkv, int dt, int64_t x_tok, int64_t x_head, const float* cis, int64_t cis_rows, int64_t R, int half_layout,
+                                   void* q_out, const bi8_paged_cache* cache, const Sequences& seq, int64_t Hq, int64_t D, cudaStream_t st);
+size_t attention_paged_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len, bool packed);
+int launch_attention_paged(const void* q, int dt, int64_t q_tok, int64_t q_head, const bi8_paged_cache* cache, const Sequences& seq, float scale, void* out,
+                           int64_t Hq, int64_t D, void* workspace, cudaStream_t st);
 // int8 rows of any alignment to rows on 16-byte boundaries (copy_rows.cu)
 int launch_copy_rows(const int8_t* src, int64_t lds, int8_t* dst, int64_t ldd, int64_t rows, int64_t cols, cudaStream_t st);
 // column sums in fp32 (column_sum.cu)

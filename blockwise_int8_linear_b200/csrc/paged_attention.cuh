@@ -1,0 +1,37 @@
+// What both attention kernels over a paged cache take (paged_attention.cu for a few queries of a cache head, paged_attention_tc.cu for many).
+#pragma once
+
+#include "paged_common.cuh"
+
+namespace bi8 {
+
+struct PagedAttnArgs {
+    const void* q;               // [N, Hq, D]
+    int64_t q_tok, q_head;       // steps in elements
+    bi8_paged_cache cache;
+    Sequences seq;
+    void* out;                   // [N, Hq, D]
+    Partials part;
+    int Hq, Hkv, G;
+    int shares, tiles;
+    float scale_log2;            // |scale| * log2(e), not 0
+    uint32_t q_keep, q_flip;     // of two packed queries: bits to keep (none where the scale is 0) and signs to change
+    FastDiv group, heads, per_share, per_sequence;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// The number of rows that query t of a sequence's n sees, counted from the cache's first.
+__device__ __forceinline__ int rows_seen(const Sequences& s, int b, int n, int t) {
+    const long long r = s.first_position(b, n) + t + 1;
+    return b < s.B ? (int)(r < 0 ? 0 : r > s.max_len ? s.max_len : r) : 0;
+}
+
+int launch_paged_few(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st);
+int launch_paged_many(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st);
+
+}  // namespace bi8

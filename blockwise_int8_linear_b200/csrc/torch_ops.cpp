@@ -1096,6 +1096,256 @@ Tensor attention_int4(const Tensor& q_in, const Tensor& k, const Tensor& k_state
     return out;
 }
 
+// ---- rotary positions and a paged key/value cache -----------------------------------------------------------------------------
+// A table of angles: complex64 [rows, R/2] or float32 [rows, R/2, 2] (cos, sin), the same bytes.  Dense and on a 16-byte boundary.
+struct Angles {
+    Tensor owner;
+    const float* ptr = nullptr;
+    int64_t rows = 0, features = 0;
+    Angles(const Tensor& cis, const Tensor& like) {
+        const bool cplx = cis.scalar_type() == at::kComplexFloat;
+        if ((!cplx && cis.scalar_type() != at::kFloat) || cis.dim() != (cplx ? 2 : 3) || (!cplx && cis.size(2) != 2))
+            value_error(std::string("cis must hold [rows, pairs] (cos, sin) float32 pairs, got ") + c10::toString(cis.scalar_type()) + " " + shape_of(cis));
+        same_device(cis, like, "cis");
+        owner = cis.is_conj() ? cis.resolve_conj().contiguous() : cis.contiguous();
+        if (owner.numel() > 0 && !aligned16(owner)) owner = owner.clone();
+        ptr = static_cast<const float*>(owner.data_ptr());
+        rows = cis.size(0);
+        features = 2 * cis.size(1);
+    }
+};
+
+Tensor rope(const Tensor& x, const Tensor& cis, const Tensor& positions, int64_t layout, bool conjugate);
+
+// The rotation is linear and its transpose is the rotation the other way, so its gradient can be differentiated again.
+struct RopeBackward : public Node {
+    SavedVariable cis, positions;
+    int64_t layout = 0;
+    bool conjugate = false;
+    std::string name() const override { return "ropeBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        cis.reset_data();
+        positions.reset_data();
+    }
+    variable_list apply(variable_list&& grads) override {
+        variable_list out(1);
+        if (!grads[0].defined() || !task_should_compute_output(0)) return out;
+        Tensor table, at;
+        {
+            std::lock_guard<std::mutex> lock(mutex_);
+            table = cis.unpack(getptr());
+            at = positions.unpack(getptr());
+        }
+        try {
+            out[0] = rope(grads[0], table, at, layout, conjugate);
+        } catch (const PyFail& e) {
+            throw std::runtime_error(e.text);
+        }
+        return out;
+    }
+};
+
+Tensor rope_values(const Tensor& x_in, const Tensor& cis, const Tensor& positions, int64_t layout, bool conjugate) {
+    at::AutoDispatchBelowADInplaceOrView below_autograd;
+    OnDevice on(x_in);
+    const Angles angles(cis, x_in);
+    const Tensor x = x_in.size(-1) > 1 && x_in.stride(-1) != 1 ? x_in.contiguous() : x_in;
+    const int lead = (int)x.dim() - 3;
+    const int64_t b = lead ? x.size(0) : 1, t = x.size(lead), h = x.size(lead + 1), d = x.size(lead + 2);
+    const int64_t pos_tok = positions.defined() && t > 1 ? positions.stride(-1) : 0;
+    const int64_t pos_batch = positions.defined() && positions.dim() == 2 && positions.size(0) > 1 ? positions.stride(0) : 0;
+    Tensor out = empty_on(x, x.sizes(), x.scalar_type());
+    check(bi8_rope(x.data_ptr(), dtype_code(x.scalar_type()), lead && b > 1 ? x.stride(0) : 0, t > 1 ? x.stride(lead) : 0, h > 1 ? x.stride(lead + 1) : 0, angles.ptr,
+                   angles.rows, angles.features, positions.defined() ? static_cast<const long long*>(positions.data_ptr()) : nullptr, pos_batch, pos_tok,
+                   out.data_ptr(), b, t, h, d, (int)layout, conjugate, on.raw()),
+          "bi8_rope");
+    return out;
+}
+
+Tensor rope(const Tensor& x, const Tensor& cis, const Tensor& positions, int64_t layout, bool conjugate) {
+    need_cuda(x);
+    if (x.dim() != 3 && x.dim() != 4) value_error("expected [B, T, H, D] or [T, H, D], got " + shape_of(x));
+    (void)dtype_code(x.scalar_type());
+    const int64_t pairs = cis.dim() > 1 ? cis.size(1) : 0;
+    if (pairs < 1 || 2 * pairs > x.size(-1))
+        value_error("a table of " + std::to_string(pairs) + " pairs does not fit heads of " + std::to_string(x.size(-1)) + " features");
+    if (at::GradMode::is_enabled() && cis.requires_grad())
+        throw PyFail{PyExc_RuntimeError, "rope has no backward pass for its table: call it with a detached one"};
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && (x._fw_grad(0).defined() || cis._fw_grad(0).defined()))
+        throw PyFail{PyExc_RuntimeError, "rope has no forward-mode derivative: call it on tensors without tangents"};
+    if (positions.defined()) {
+        const int64_t t = x.size(-3);
+        const bool fits = positions.dim() == 1 ? positions.size(0) == t
+                                               : positions.dim() == 2 && x.dim() == 4 && positions.size(1) == t && (positions.size(0) == x.size(0) || positions.size(0) == 1);
+        if (positions.scalar_type() != at::kLong || !fits)
+            value_error("positions must be int64 [T] or [B, T] for activations " + shape_of(x) + ", got " + c10::toString(positions.scalar_type()) + " " +
+                        shape_of(positions));
+        same_device(positions, x, "positions");
+    }
+    Tensor out = rope_values(x, cis, positions, layout, conjugate);
+    if (at::GradMode::is_enabled() && x.requires_grad()) {
+        auto node = std::shared_ptr<RopeBackward>(new RopeBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x));
+        node->cis = SavedVariable(cis, false);
+        node->positions = SavedVariable(positions, false);
+        node->layout = layout;
+        node->conjugate = !conjugate;
+        torch::autograd::set_history(out, node);
+    }
+    return out;
+}
+
+// Whether no two values of k and v [pages, heads, rows, D], features dense, share memory, as far as nested steps show it: every step reaches past
+// what is inside it, and keys and values lie apart, or have the same steps and their distance is one more such step.
+bool values_apart(const Tensor& k, const Tensor& v) {
+    if (k.numel() == 0 || v.numel() == 0) return true;
+    auto nested = [](const Tensor& t, int64_t other, int64_t* extent) {
+        std::vector<std::pair<int64_t, int64_t>> dims;       // step, count
+        for (int i = 0; i < 3; ++i)
+            if (t.size(i) > 1) dims.push_back({t.stride(i), t.size(i)});
+        if (other > 0) dims.push_back({other, 2});
+        std::sort(dims.begin(), dims.end());
+        int64_t reach = t.size(3);
+        for (const auto& [step, n] : dims) {
+            if (step < reach) return false;
+            reach += step * (n - 1);
+        }
+        *extent = reach;
+        return true;
+    };
+    int64_t k_reach = 0, v_reach = 0;
+    if (!nested(k, 0, &k_reach) || !nested(v, 0, &v_reach)) return false;
+    const int64_t size = k.element_size(), at = (int64_t)reinterpret_cast<uintptr_t>(k.data_ptr()), bt = (int64_t)reinterpret_cast<uintptr_t>(v.data_ptr());
+    if (at + k_reach * size <= bt || bt + v_reach * size <= at) return true;
+    for (int i = 0; i < 3; ++i)
+        if (k.size(i) > 1 && k.stride(i) != v.stride(i)) return false;
+    const int64_t apart = at < bt ? bt - at : at - bt;
+    return apart > 0 && apart % size == 0 && nested(k, apart / size, &k_reach);
+}
+
+bi8_paged_cache paged_cache(const Tensor& k, const Tensor& v, const Tensor& like, int64_t d) {
+    if (k.dim() != 4) value_error("cache pages must be 4-D, got " + shape_of(k));
+    for (const Tensor* t : {&k, &v})
+        if (t->dim() != 4 || t->sizes() != k.sizes() || t->size(3) != d || t->scalar_type() != like.scalar_type() || t->device() != like.device() ||
+            (d > 1 && t->stride(3) != 1))
+            value_error(std::string("cache pages must be ") + c10::toString(like.scalar_type()) + " [pages, heads, rows, " + std::to_string(d) +
+                        "] with dense features on " + like.device().str() + ", keys and values alike, got " + c10::toString(t->scalar_type()) + " " + shape_of(*t));
+    if (k.size(1) < 1) value_error("a cache needs a head, got " + shape_of(k));
+    if (k.size(2) < 1 || k.size(2) % 16 != 0) value_error("pages must have a multiple of 16 rows, got " + std::to_string(k.size(2)));
+    int64_t steps[6];
+    for (int i = 0; i < 6; ++i) {
+        const Tensor& t = i < 3 ? k : v;
+        steps[i] = t.size(i % 3) > 1 ? t.stride(i % 3) : 0;
+        if (steps[i] % 8 != 0) value_error("steps of a cache must be multiples of 8 values");
+    }
+    if (k.numel() > 0 && (!aligned16(k) || !aligned16(v))) value_error("a cache must begin on a 16-byte boundary");
+    if (!values_apart(k, v)) value_error("pages, heads, rows, keys and values of a cache must not share memory");
+    return {k.data_ptr(), v.data_ptr(), steps[0], steps[1], steps[2], steps[3], steps[4], steps[5], k.size(0), k.size(1), k.size(2), d};
+}
+
+// The sequences of a batch of n tokens.  The struct's tensors live as long as this does.
+struct Batch {
+    Tensor pages_owner, cu_owner;
+    bi8_sequences s{};
+    Batch(const Tensor& pages, const Tensor& lengths, const Tensor& cu_tokens, const Tensor& starts, const Tensor& like, int64_t n) {
+        if (pages.dim() != 2 || pages.scalar_type() != at::kInt)
+            value_error(std::string("pages must be int32 [B, width], got ") + c10::toString(pages.scalar_type()) + " " + shape_of(pages));
+        same_device(pages, like, "pages");
+        pages_owner = pages.size(1) > 1 && pages.stride(1) != 1 ? pages.contiguous() : pages;
+        const int64_t b = pages.size(0);
+        const PerSequence len(lengths, like, b, "lengths"), start(starts, like, b, "starts");
+        if (cu_tokens.defined()) {
+            if (cu_tokens.scalar_type() != at::kLong || cu_tokens.dim() != 1 || cu_tokens.size(0) != b + 1)
+                value_error("cu_tokens must be int64 [" + std::to_string(b + 1) + "], got " + c10::toString(cu_tokens.scalar_type()) + " " + shape_of(cu_tokens));
+            same_device(cu_tokens, like, "cu_tokens");
+            cu_owner = cu_tokens.contiguous();
+        } else if (b == 0 ? n != 0 : n % b != 0) {
+            value_error(std::to_string(n) + " tokens do not divide over " + std::to_string(b) + " sequences: give cu_tokens");
+        }
+        if (b == 0 && n != 0) value_error("tokens without a sequence");
+        s.lengths = len.ptr;
+        s.lengths_step = len.step;
+        s.starts = start.ptr;
+        s.starts_step = start.step;
+        s.cu_tokens = cu_owner.defined() ? static_cast<const long long*>(cu_owner.data_ptr()) : nullptr;
+        s.page_table = static_cast<const int*>(pages_owner.data_ptr());
+        s.table_step = b > 1 ? pages_owner.stride(0) : 0;
+        s.width = pages.size(1);
+        s.B = b;
+        s.N = n;
+    }
+};
+
+// [N, heads, D] with dense features, steps that are multiples of 8 and a 16-byte boundary: the tensor itself or a copy
+Tensor packed_tokens(const Tensor& t, int64_t (&steps)[2]) {
+    bool ok = t.stride(2) == 1 && aligned16(t);
+    for (int i = 0; i < 2; ++i) {
+        steps[i] = t.size(i) > 1 ? t.stride(i) : 0;
+        ok = ok && steps[i] % 8 == 0;
+    }
+    if (ok) return t;
+    steps[0] = t.size(1) * t.size(2), steps[1] = t.size(2);
+    return t.clone(at::MemoryFormat::Contiguous);
+}
+
+int64_t head_size(const Tensor& t) {
+    const int64_t d = t.size(2);
+    if (d != 64 && d != 128 && d != 256) value_error("head size must be 64, 128 or 256, got " + std::to_string(d));
+    return d;
+}
+
+Tensor rope_cache_append_paged(const Tensor& qkv_in, const Tensor& cis_in, const Tensor& k, const Tensor& v, const Tensor& pages, const Tensor& lengths,
+                               const Tensor& cu_tokens, int64_t layout) {
+    need_cuda(qkv_in);
+    for (const Tensor* t : {&qkv_in, &cis_in, &k, &v}) no_gradient(*t, "rope_cache_append_paged");
+    if (qkv_in.dim() != 3) value_error("expected [N, Hq + 2 Hkv, D], got " + shape_of(qkv_in));
+    const int code = dtype_code16(qkv_in.scalar_type(), "activations");
+    const int64_t n = qkv_in.size(0), d = head_size(qkv_in);
+    const bi8_paged_cache cache = paged_cache(k, v, qkv_in, d);
+    const int64_t hkv = k.size(1), hq = qkv_in.size(1) - 2 * hkv;
+    if (hq < hkv || hq % hkv != 0)
+        value_error(std::to_string(qkv_in.size(1)) + " heads are not Hq + 2 * " + std::to_string(hkv) + " with Hq a multiple of " + std::to_string(hkv));
+    OnDevice on(qkv_in);
+    const Angles angles(cis_in, qkv_in);
+    if (angles.features < 16 || angles.features > d || angles.features % 16 != 0)
+        value_error("rotated features must be a multiple of 16 of the " + std::to_string(d) + ", got " + std::to_string(angles.features));
+    const Batch batch(pages, lengths, cu_tokens, Tensor(), qkv_in, n);
+    Tensor q = empty_on(qkv_in, {n, hq, d}, qkv_in.scalar_type());
+    if (q.numel() == 0) return q;
+    int64_t steps[2];
+    const Tensor qkv = packed_tokens(qkv_in, steps);
+    check(bi8_rope_cache_append_paged(qkv.data_ptr(), code, steps[0], steps[1], angles.ptr, angles.rows, angles.features, (int)layout, q.data_ptr(), &cache, &batch.s,
+                                      hq, on.raw()),
+          "bi8_rope_cache_append_paged");
+    return q;
+}
+
+Tensor attention_paged(const Tensor& q_in, const Tensor& k, const Tensor& v, const Tensor& pages, const Tensor& lengths, const Tensor& cu_tokens,
+                       const Tensor& starts, double scale) {
+    need_cuda(q_in);
+    for (const Tensor* t : {&q_in, &k, &v}) no_gradient(*t, "attention_paged_cache");
+    if (q_in.dim() != 3) value_error("expected queries [N, Hq, D], got " + shape_of(q_in));
+    const int code = dtype_code16(q_in.scalar_type(), "queries");
+    const int64_t n = q_in.size(0), hq = q_in.size(1), d = head_size(q_in);
+    const bi8_paged_cache cache = paged_cache(k, v, q_in, d);
+    const int64_t hkv = k.size(1);
+    if (hq < 1 || hq % hkv != 0) value_error(std::to_string(hq) + " query heads do not divide over " + std::to_string(hkv) + " cache heads");
+    if (!(std::abs(scale) <= 2e38)) value_error("scale must be a number of at most 2e38, got " + std::to_string(scale));
+    OnDevice on(q_in);
+    const Batch batch(pages, lengths, cu_tokens, starts, q_in, n);
+    Tensor out = empty_on(q_in, {n, hq, d}, q_in.scalar_type());
+    if (out.numel() == 0) return out;
+    int64_t steps[2];
+    const Tensor q = packed_tokens(q_in, steps);
+    const size_t bytes = bi8_attention_paged_workspace_bytes(batch.s.B, n, hq, hkv, d, batch.s.width * cache.page_rows, cu_tokens.defined());
+    const Tensor ws = scratch(q, (int64_t)bytes);
+    check(bi8_attention_paged(q.data_ptr(), code, steps[0], steps[1], &cache, &batch.s, (float)scale, out.data_ptr(), hq, ws.defined() ? ws.data_ptr() : nullptr, bytes,
+                              on.raw()),
+          "bi8_attention_paged");
+    return out;
+}
+
 // ---- bindings -----------------------------------------------------------------------------------------------------------
 struct Args {
     PyObject* const* a;
@@ -1266,6 +1516,24 @@ BI8_METHOD(attention_int4) {     // q, k, k_state, v, v_state, lengths, starts, 
                 scale = g.number(7)] { return attention_int4(q, k, ks, v, vs, len, start, scale); };
     });
 }
+BI8_METHOD(rope) {               // x, cis, positions, layout
+    return call("rope", {a, n}, 4, [](const Args& g) {
+        return [x = g.tensor(0), c = g.tensor(1), p = g.optional(2), l = g.integer(3)] { return rope(x, c, p, l, false); };
+    }, true);
+}
+BI8_METHOD(rope_cache_append_paged) {  // qkv, cis, k, v, pages, lengths, cu_tokens, layout
+    return call("rope_cache_append_paged", {a, n}, 8, [](const Args& g) {
+        return [x = g.tensor(0), c = g.tensor(1), k = g.tensor(2), v = g.tensor(3), p = g.tensor(4), len = g.tensor(5), cu = g.optional(6), l = g.integer(7)] {
+            return rope_cache_append_paged(x, c, k, v, p, len, cu, l);
+        };
+    });
+}
+BI8_METHOD(attention_paged) {    // q, k, v, pages, lengths, cu_tokens, starts, scale
+    return call("attention_paged", {a, n}, 8, [](const Args& g) {
+        return [q = g.tensor(0), k = g.tensor(1), v = g.tensor(2), p = g.tensor(3), len = g.tensor(4), cu = g.optional(5), start = g.optional(6),
+                scale = g.number(7)] { return attention_paged(q, k, v, p, len, cu, start, scale); };
+    });
+}
 BI8_METHOD(bind) {               // the exception class of failed library calls, the configuration module
     if (n != 2) {
         PyErr_SetString(PyExc_TypeError, "bind takes 2 arguments");
@@ -1280,7 +1548,8 @@ BI8_METHOD(bind) {               // the exception class of failed library calls,
 PyMethodDef methods[] = {BI8_ENTRY(quantize_rowwise), BI8_ENTRY(quantize_colwise), BI8_ENTRY(quantize_dual), BI8_ENTRY(quantize_pre),
                          BI8_ENTRY(dequantize), BI8_ENTRY(gemm), BI8_ENTRY(block_partials), BI8_ENTRY(matmul), BI8_ENTRY(linear),
                          BI8_ENTRY(train_linear), BI8_ENTRY(rope_cache_append), BI8_ENTRY(quantize_int4), BI8_ENTRY(dequantize_int4),
-                         BI8_ENTRY(matmul_int4), BI8_ENTRY(rope_cache_append_int4), BI8_ENTRY(attention_int4), BI8_ENTRY(bind),
+                         BI8_ENTRY(matmul_int4), BI8_ENTRY(rope_cache_append_int4), BI8_ENTRY(attention_int4), BI8_ENTRY(rope),
+                         BI8_ENTRY(rope_cache_append_paged), BI8_ENTRY(attention_paged), BI8_ENTRY(bind),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Host path of the blockwise-int8 operations.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

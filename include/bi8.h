@@ -330,6 +330,67 @@ BI8_API int bi8_attention_int4(const void* q, int dtype, int64_t q_batch, int64_
                                void* out, int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, void* workspace, size_t workspace_bytes,
                                void* stream);
 
+/* ---- rotary positions and a paged key/value cache (no counterpart in the reference, which has no model code) -----------------
+ * Rotation: of the D features of a head the first R are turned in R/2 pairs, (x + i y) * (cos + i sin) of the token's position, fp32 products and
+ * sums each rounded on their own, the result rounded to dtype; the others are copied.  BI8_ROPE_INTERLEAVED: pairs are neighbours (2j, 2j+1);
+ * BI8_ROPE_HALF: they lie R/2 apart (j, j + R/2). */
+#define BI8_ROPE_INTERLEAVED 0
+#define BI8_ROPE_HALF 1
+
+/* out [B, T, H, D] contiguous = the rotation of x [B, T, H, D] of dtype (any of the three), steps in elements, features contiguous.
+ *   cis      [rows, R/2] pairs (cos, sin) fp32, 16-byte aligned; R even, 2 to D
+ *   pos      device address (int64): the position of token t of batch b is pos[b * pos_batch + t * pos_tok]; NULL: t.  Tokens whose position the
+ *            table does not have are zeros
+ *   conjugate  1: turned the other way, which is the gradient of the rotation */
+BI8_API int bi8_rope(const void* x, int dtype, int64_t x_batch, int64_t x_tok, int64_t x_head, const float* cis, int64_t rows, int64_t R,
+                     const long long* pos, int64_t pos_batch, int64_t pos_tok, void* out, int64_t B, int64_t T, int64_t H, int64_t D, int layout,
+                     int conjugate, void* stream);
+
+/* A key/value cache in pages: k and v [pages, heads, page_rows, head_dim], 16-bit values, features contiguous, 16-byte aligned; all other steps
+ * are free (elements, multiples of 8), but no two values share memory.  page_rows is a multiple of 16, head_dim 64, 128 or 256. */
+typedef struct {
+    void* k;
+    void* v;
+    int64_t k_page, k_head, k_row;
+    int64_t v_page, v_head, v_row;
+    int64_t pages, heads, page_rows, head_dim;
+} bi8_paged_cache;
+
+/* The sequences of a batch of N new tokens, which lie one behind the other.
+ *   lengths    device address (int64): sequence b has lengths[b * lengths_step] rows in the cache, the last of which are its new tokens'
+ *   cu_tokens  device address (int64) of B + 1 numbers: the tokens of sequence b are cu_tokens[b] to cu_tokens[b + 1] - 1.  The first is 0; tokens from
+ *              cu_tokens[B] on belong to nobody.  NULL: N / B each (N a multiple of B)
+ *   starts     device address (int64): the first row that is seen, or NULL for 0 (attention only)
+ *   page_table device address (int32) [B, width], row step table_step: row r of a sequence is row r % page_rows of page
+ *              page_table[b * table_step + r / page_rows]
+ * All of these are read by the kernels, so that a launch can be replayed while they change. */
+typedef struct {
+    const long long* lengths;
+    const long long* cu_tokens;
+    const long long* starts;
+    const int* page_table;
+    int64_t lengths_step, starts_step, table_step, width;
+    int64_t B, N;
+} bi8_sequences;
+
+/* Rotation of q and k and the append of k and v.
+ *   qkv      [N, Hq + 2 heads, D] of dtype (bf16 or fp16), steps in elements (multiples of 8), 16-byte aligned
+ *   cis      [cis_rows, R/2] as above, R a multiple of 16.  Token i of a sequence's n has position and row lengths - n + i
+ *   q_out    [N, Hq, D] contiguous, 16-byte aligned
+ * A token whose position is outside the table of angles or the sequence's row of the page table, or whose page number is none of the cache's, writes
+ * nothing, and its query is zero; so are those of tokens that belong to nobody. */
+BI8_API int bi8_rope_cache_append_paged(const void* qkv, int dtype, int64_t qkv_tok, int64_t qkv_head, const float* cis, int64_t cis_rows, int64_t R,
+                                        int layout, void* q_out, const bi8_paged_cache* cache, const bi8_sequences* seq, int64_t Hq, void* stream);
+
+/* out [N, Hq, D] contiguous = softmax(scale * q k^T) v for q [N, Hq, D], steps in elements (multiples of 8), 16-byte aligned.  The query of a sequence's
+ * token i of n sees the rows from its start up to lengths - n + i (at most width * page_rows rows).  A query that sees no row gives zeros, as do tokens
+ * that belong to nobody.  Rows that no query of a sequence sees may hold anything; pages whose number is none of the cache's read as
+ * zeros.  Keys of 2^100 and more may overflow in the scores, which are fp32.  Query head h reads cache head h / (Hq / heads).  scale: a number of at
+ * most 2e38.  workspace: bi8_attention_paged_workspace_bytes bytes (`packed`: whether cu_tokens is given), 16-byte aligned, scratch of this call. */
+BI8_API size_t bi8_attention_paged_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t heads, int64_t D, int64_t max_len, int packed);
+BI8_API int bi8_attention_paged(const void* q, int dtype, int64_t q_tok, int64_t q_head, const bi8_paged_cache* cache, const bi8_sequences* seq, float scale,
+                                void* out, int64_t Hq, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Capture sequence number of `stream` if it is being captured into a CUDA graph, 0 otherwise (no counterpart in the
  * reference).  A host layer that caches workspaces uses it to give every captured graph a scratch buffer of its own:
  * an address baked into a graph must not be shared with another graph that may be replayed on a different stream. */
