@@ -23,7 +23,7 @@ NATIVE = os.path.join(HERE, "_native.so")
 NATIVE_SOURCE = "torch_ops.cpp"
 SOURCES = ["api.cu", "quantize.cu", "quantize_tile.cu", "gemm_generic.cu", "gemm_tc.cu", "gemm_tc_skinny.cu", "gemm_smallm.cu", "no_alloc.cu", "peer_reduce.cu", "peer_reduce_large.cu", "quantize_pre.cu", "column_sum.cu", "rope_cache.cu", "copy_rows.cu",
            "int4_quantize.cu", "int4_matmul.cu", "int4_cache.cu", "int4_attention.cu",
-           "rope.cu", "paged_cache.cu", "paged_attention.cu"]
+           "rope.cu", "paged_cache.cu", "paged_attention.cu", "paged_attention_tc.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

@@ -425,15 +425,24 @@ __global__ void __launch_bounds__(4 * D) paged_join_kernel(const Partials p, int
 }
 
 struct Plan {
-    int kind;                    // 0: few queries a tile, 1: many
+    bool many;
+    int rows;                    // queries of a tile
     int64_t tiles, shares;
 };
 Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len, bool packed) {
     const int64_t G = Hq / Hkv, sms = sm_count();
     Plan p{};
-    p.kind = 0;
-    p.tiles = tile_count(B, N, G, kCols, packed);
-    const int64_t step = 16 * (D == 64 ? kSubSteps<64> : D == 128 ? kSubSteps<128> : kSubSteps<256>), ctas = p.tiles * Hkv;
+    p.many = packed ? N > B && N * G > kCols * B : N / B * G > kCols;
+    p.rows = p.many ? paged_many_tile(D) : kCols;
+    p.tiles = tile_count(B, N, G, p.rows, packed);
+    const int64_t ctas = p.tiles * Hkv;
+    if (p.many) {
+        int64_t s = max_len / kShareRows, want = (2 * sms + ctas - 1) / ctas;
+        if (s > want) s = want;
+        p.shares = s < 1 ? 1 : s > kMaxShares ? kMaxShares : s;
+        return p;
+    }
+    const int64_t step = 16 * (D == 64 ? kSubSteps<64> : D == 128 ? kSubSteps<128> : kSubSteps<256>);
     const int64_t useful = (max_len + kWarps * step - 1) / (kWarps * step), long_ones = max_len / 2048;
     int64_t want = (D == 256 ? kResident<256> : kResident<128>) * sms / ctas;
     if (want < kClusterShares && want < long_ones) want = long_ones < kClusterShares ? long_ones : kClusterShares;
@@ -447,6 +456,7 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     p.shares = s < 1 ? 1 : s;
     return p;
 }
+bool through_workspace(const Plan& p) { return p.many ? p.shares > 1 : p.shares > kClusterShares; }
 
 template <typename T, int D>
 int launch(const PagedAttnArgs& a, cudaStream_t st) {
@@ -496,8 +506,7 @@ int launch_paged_few(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st)
 
 size_t attention_paged_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len, bool packed) {
     const Plan p = plan_of(B, N, Hq, Hkv, D, max_len, packed);
-    const bool through = p.kind == 1 ? p.shares > 1 : p.shares > kClusterShares;
-    return through ? (size_t)(p.shares * N * Hq) * (D + 2) * 4 : 0;
+    return through_workspace(p) ? (size_t)(p.shares * N * Hq) * (D + 2) * 4 : 0;
 }
 
 int launch_attention_paged(const void* q, int dt, int64_t q_tok, int64_t q_head, const bi8_paged_cache* cache, const Sequences& seq, float scale, void* out,
@@ -506,6 +515,10 @@ int launch_attention_paged(const void* q, int dt, int64_t q_tok, int64_t q_head,
     const Plan p = plan_of(seq.B, seq.N, Hq, Hkv, D, seq.max_len, seq.cu != nullptr);
     if (p.tiles * Hkv * p.shares > 0x7fffffff || (int64_t)seq.N * Hq > 0x7fffffff)
         return fail(BI8_ERR_LIMIT, "attention_paged: %lld queries exceed one launch", (long long)seq.N * Hq);
+    if (cache->pages == 0) {                                  // whatever a query sees reads as zeros
+        BI8_CUDA_TRY(cudaMemsetAsync(out, 0, (size_t)seq.N * Hq * D * 2, st));
+        return BI8_OK;
+    }
     PagedAttnArgs a{};
     a.q = q;
     a.q_tok = q_tok;
@@ -527,9 +540,9 @@ int launch_attention_paged(const void* q, int dt, int64_t q_tok, int64_t q_head,
     a.group = FastDiv(G);
     a.heads = FastDiv(Hkv);
     a.per_share = FastDiv(p.shares);
-    a.per_sequence = FastDiv(seq.cu ? 1 : ((int64_t)seq.T * G + kCols - 1) / kCols);
-    int rc = launch_paged_few(a, dt, D, st);
-    if (rc == BI8_OK && p.shares > kClusterShares) rc = launch_paged_join(a.part, a.shares, out, dt, D, st);
+    a.per_sequence = FastDiv(seq.cu ? 1 : ((int64_t)seq.T * G + p.rows - 1) / p.rows);
+    int rc = p.many ? launch_paged_many(a, dt, D, st) : launch_paged_few(a, dt, D, st);
+    if (rc == BI8_OK && through_workspace(p)) rc = launch_paged_join(a.part, a.shares, out, dt, D, st);
     return rc;
 }
 

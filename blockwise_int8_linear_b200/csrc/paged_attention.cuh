@@ -31,6 +31,9 @@ __device__ __forceinline__ int rows_seen(const Sequences& s, int b, int n, int t
     return b < s.B ? (int)(r < 0 ? 0 : r > s.max_len ? s.max_len : r) : 0;
 }
 
+// The kernel for many queries gives a tile one share for as many rows of the cache.
+constexpr int kShareRows = 1024;
+int paged_many_tile(int64_t D);          // queries of one of its CTAs
 int launch_paged_few(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st);
 int launch_paged_many(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st);
 

@@ -1,0 +1,442 @@
+// Attention of many queries of each cache head over a paged 16-bit cache: parts of prompts, alone or among single tokens.  The same mathematics as
+// in paged_attention.cu, on tcgen05.
+//
+// A CTA takes up to two tiles of 128 queries (tokens and the G heads that share a cache head, in that order) of one sequence and streams the sequence's
+// rows past them, kRows at a time.  One warp fetches k and v by TMA (boxes of as many rows as surely lie in one page, 128-byte swizzle), one
+// issues the products, and four warps a tile, one thread a query, do the softmax between them:
+//   S = Q K^T    queries and keys from shared memory, scores in tensor memory
+//   P = 2^(c S - m)  by the query's thread, back into the scores' own tensor memory as 16-bit numbers
+//   O += P V     weights from tensor memory, values from shared memory as they lie (the contraction runs over their rows)
+// While one tile's weights are computed the other's products run.  With heads of 256 features there is room for one tile, whose scores have two
+// places instead.
+//
+// The maximum m that a query subtracts follows its scores only when they have grown by 2^8 (fp32 sums and 16-bit weights lose nothing by
+// being that much larger), so that O is hardly ever rescaled; that is done by the query's own thread.  m is a rounded number, subtracted inside one
+// multiply-add: all weights are relative to the same power of two, whatever it is.  Only where scores are so large (2^20) that its rounding is
+// a power of two of its own the differences of scores are taken first; the scores' own rounding is no smaller then.
+//
+// Weights are 16-bit numbers: a rounding of half a step each, at random, which leaves the result about as much error again as its own rounding.
+// (A second product with what they lose would cost half of the time again.)
+//
+// What a row holds that no query sees must not count: scores are masked, and v's rows before the start and behind the last one are
+// overwritten by zeros in shared memory before the product, since 0 times an infinity is none.
+#include "paged_attention.cuh"
+#include "tc_common.cuh"
+
+#include <type_traits>
+
+namespace bi8 {
+namespace {
+
+using namespace ptx;
+
+constexpr int kTileRows = 128;
+
+template <int D>
+struct Shape {
+    static constexpr int kTiles = D == 256 ? 1 : 2;                  // of queries
+    static constexpr int kRows = D == 256 ? 64 : 128;                // of the cache at a time
+    static constexpr int kStages = D == 64 ? 8 : 5;
+    static constexpr int kAhead = kTiles == 1 ? 2 : 1;               // scores that are under way before the first weights are used
+    static constexpr int kWarps = 4 * kTiles + 2, kThreads = 32 * kWarps;
+    static constexpr int kQTile = kTileRows * D * 2, kStage = kRows * D * 2;
+    static constexpr int kScores = 0, kOut = 2 * kRows;              // columns of tensor memory
+    static constexpr int kColumns = 512;
+    static_assert(kOut + kTiles * D <= kColumns, "tensor memory");
+    // barriers
+    static constexpr int kFull = 0, kEmpty = kStages, kScoresFull = 2 * kStages, kWeightsFull = kScoresFull + 2, kProductDone = kWeightsFull + 2,
+                         kQueries = kProductDone + 2, kEnd = kQueries + 2, kBarriers = kEnd + 1;
+    static constexpr int kStagesAt = kTiles * kQTile, kBarriersAt = kStagesAt + kStages * kStage, kMisc = kBarriersAt + 8 * kBarriers;
+    static constexpr int kBytes = kMisc + 16 + 1024;                 // tensor memory's address, abort flag, a word that stays zero; alignment
+};
+
+struct Shares {
+    int first, last, count;      // this share's rows; how many shares there are
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Shape<D>::kThreads, 1)
+    paged_many_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PagedAttnArgs a, const int box_rows, const int share_rows,
+                      int* status, const long long wait_limit) {
+    using Z = Shape<D>;
+    constexpr int KT = Z::kRows, TILES = Z::kTiles, CHUNKS = D / 64;
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* const smem = smem_raw + (base - smem_u32(smem_raw));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int MMA_WARP = 4 * TILES, LOAD_WARP = MMA_WARP + 1;
+    auto bar = [&](int i) { return base + (uint32_t)(Z::kBarriersAt + 8 * i); };
+    const uint32_t holder = base + Z::kMisc, abort_flag = holder + 4, zero_word = holder + 8;
+
+    const int tile_head = (int)a.per_share.div(blockIdx.x), share = (int)blockIdx.x - tile_head * a.shares;
+    const int tile_index = (int)a.heads.div((unsigned)tile_head), h = tile_head - tile_index * a.Hkv;
+    after_predecessor();
+    const Sequences& s = a.seq;
+    const QueryTile qt = find_tile(s, tile_index, a.G, TILES * kTileRows, a.per_sequence);
+    if (qt.rows == 0) return;
+    auto token_of = [&](int r) { return (int)a.group.div((unsigned)(qt.row0 + r)); };
+    auto query_at = [&](int r) {                              // token * Hq + head
+        const int t = token_of(r);
+        return (int64_t)(qt.token0 + t) * a.Hq + h * a.G + (qt.row0 + r - t * a.G);
+    };
+
+    // ---- rows of this share.  A tile takes as many shares as its rows fill.
+    const int fewest = rows_seen(s, qt.b, qt.n, token_of(0)), most = rows_seen(s, qt.b, qt.n, token_of(qt.rows - 1));
+    const int start = s.start(qt.b), origin = start & -box_rows, n_rows = most > start ? most - origin : 0;
+    const int count = max(1, min(a.shares, n_rows / share_rows));
+    const int chunk = (n_rows + count * KT - 1) / (count * KT) * KT;
+    const int first = origin + min(n_rows, share * chunk), last = share < count ? min(origin + n_rows, first + chunk) : first;
+    const int steps = (last - first + KT - 1) / KT, tiles = qt.rows > kTileRows ? 2 : 1;
+    if (steps == 0) {                                         // nothing to see, or no such share
+        for (int r = threadIdx.x; r < qt.rows; r += Z::kThreads) {
+            if (a.shares > 1) a.part.stats[share * a.part.rows + query_at(r)] = make_float2(-INFINITY, count == 1 && share == 0 ? kWritten : 0.0f);
+            if (count == 1 && share == 0) {
+                uint4* const dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + query_at(r) * D);
+                for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+        return;
+    }
+
+    // ---- set-up
+    if (warp == MMA_WARP) {
+        tmem_alloc(holder, Z::kColumns);
+        tmem_relinquish();
+        if (lane == 0) {
+            sts_u32(abort_flag, 0u);
+            sts_u32(zero_word, 0u);
+            for (int i = 0; i < Z::kStages; ++i) {
+                mbar_init(bar(Z::kFull + i), 1);
+                mbar_init(bar(Z::kEmpty + i), 1);
+            }
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(bar(Z::kScoresFull + i), 1);
+                mbar_init(bar(Z::kWeightsFull + i), 128);
+                mbar_init(bar(Z::kProductDone + i), 1);
+                mbar_init(bar(Z::kQueries + i), 128);
+            }
+            mbar_init(bar(Z::kEnd), 1);
+            mbar_fence_init();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = lds_u32(holder);
+    auto stage_at = [&](int stage) { return base + (uint32_t)(Z::kStagesAt + stage * Z::kStage); };
+    // where k and v of a step come in the order of the copies
+    auto order_v = [&](int j) { return min(steps, j + Z::kAhead) + j; };
+    auto order_k = [&](int j) { return j < Z::kAhead ? j : order_v(j - Z::kAhead) + 1; };
+
+    if (warp == LOAD_WARP) {
+        // ---- copies: a box of box_rows rows and 64 features at a time, a lane for every box_rows rows of the step
+        const int boxes = KT / box_rows;
+        const int* const table = s.pages + (qt.b < s.B ? qt.b : 0) * s.pages_step;
+        bool ok = true;
+        int order = 0;
+        auto fetch = [&](const CUtensorMap& map, int j) {
+            const int stage = order % Z::kStages, parity = (order / Z::kStages) & 1;
+            const int row = first + j * KT + lane * box_rows;
+            const bool mine = lane < boxes && row < last;
+            const int in_table = mine ? (int)s.page.div((unsigned)row) : 0;
+            const int page = mine ? table[in_table] : 0;
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kEmpty + stage), (uint32_t)parity ^ 1u, abort_flag, wait_limit));
+            if (!ok) {
+                if (lane == 0) report_timeout(status, abort_flag, W_EMPTY_AB);
+                return;
+            }
+            const int copied = __popc(__ballot_sync(0xffffffffu, mine));
+            if (lane == 0) mbar_expect_tx(bar(Z::kFull + stage), (uint32_t)(copied * box_rows * D * 2));
+            __syncwarp();
+            if (mine) {
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c)
+                    tma_load_4d(stage_at(stage) + (uint32_t)((c * KT + lane * box_rows) * 128), &map, bar(Z::kFull + stage), 64 * c, row - in_table * (int)s.page.d, h, page);
+            }
+            __syncwarp();
+            ++order;
+        };
+        for (int j = 0; j < min(Z::kAhead, steps) && ok; ++j) fetch(k_map, j);
+        for (int j = 0; j < steps && ok; ++j) {
+            fetch(v_map, j);
+            if (ok && j + Z::kAhead < steps) fetch(k_map, j + Z::kAhead);
+        }
+        // after an abort: the copies that are still on their way
+        if (!ok)
+            for (int i = max(0, order - Z::kStages); i < order; ++i) (void)mbar_wait(bar(Z::kFull + i % Z::kStages), (uint32_t)(i / Z::kStages) & 1u, zero_word, wait_limit);
+    } else if (warp == MMA_WARP) {
+        // ---- products, issued by one thread
+        if (elect_one()) {
+            constexpr uint32_t S_DESC = umma_idesc_16bit(kTileRows, KT, BF16, false), O_DESC = umma_idesc_16bit(kTileRows, D, BF16, true);
+            bool ok = true;
+            auto wait = [&](int b, int parity, int code) {
+                if (!ok) return;
+                ok = mbar_wait(bar(b), (uint32_t)parity, abort_flag, wait_limit);
+                if (!ok) report_timeout(status, abort_flag, code);
+            };
+            auto wait_stage = [&](int order) { wait(Z::kFull + order % Z::kStages, (order / Z::kStages) & 1, W_FULL_AB); };
+            auto scores = [&](int t, int buf, int order) {
+                const uint32_t q = base + (uint32_t)(t * Z::kQTile), k = stage_at(order % Z::kStages);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    mma_f16(tmem + (uint32_t)(Z::kScores + buf * KT), umma_desc_k_sw128(q + (uint32_t)((i / 4) * kTileRows * 128 + (i % 4) * 32)),
+                            umma_desc_k_sw128(k + (uint32_t)((i / 4) * KT * 128 + (i % 4) * 32)), S_DESC, i > 0);
+                tc_commit(bar(Z::kScoresFull + buf));
+            };
+            for (int t = 0; t < tiles; ++t) wait(Z::kQueries + t, 0, W_FULL_AB);
+            for (int j = 0; j < min(Z::kAhead, steps) && ok; ++j) {
+                wait_stage(order_k(j));
+                if (!ok) break;
+                tc_fence_after();
+                for (int t = 0; t < tiles; ++t) scores(t, TILES == 2 ? t : j & 1, order_k(j));
+                tc_commit(bar(Z::kEmpty + order_k(j) % Z::kStages));
+            }
+            for (int j = 0; j < steps && ok; ++j) {
+                const int ov = order_v(j), ahead = j + Z::kAhead, ok_order = order_k(ahead);
+                wait_stage(ov);
+                for (int t = 0; t < tiles && ok; ++t) {
+                    const int buf = TILES == 2 ? t : j & 1;
+                    wait(Z::kWeightsFull + buf, TILES == 2 ? j & 1 : (j >> 1) & 1, W_ACC_FULL);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t v = stage_at(ov % Z::kStages);
+#pragma unroll
+                    for (int i = 0; i < KT / 16; ++i)
+                        mma_f16_ta(tmem + (uint32_t)(Z::kOut + t * D), tmem + (uint32_t)(Z::kScores + buf * KT + 8 * i), umma_desc_mn_sw128(v + (uint32_t)(2048 * i), KT * 128),
+                                   O_DESC, j > 0 || i > 0);
+                    tc_commit(bar(Z::kProductDone + t));
+                    if (ahead < steps) {
+                        if (t == 0) wait_stage(ok_order);
+                        if (ok) scores(t, buf, ok_order);
+                    }
+                }
+                if (!ok) break;
+                tc_commit(bar(Z::kEmpty + ov % Z::kStages));
+                if (ahead < steps) tc_commit(bar(Z::kEmpty + ok_order % Z::kStages));
+            }
+            if (!ok) {                                        // products that are still under way
+                tc_commit(bar(Z::kEnd));
+                (void)mbar_wait(bar(Z::kEnd), 0u, zero_word, wait_limit);
+            }
+        }
+        __syncwarp();
+    } else if (warp / 4 < tiles) {
+        // ---- softmax: a thread is a query
+        const int t = warp / 4, r = t * kTileRows + (threadIdx.x & 127);
+        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), out = lanes + (uint32_t)(Z::kOut + t * D);
+        {
+            // the tile's queries, neighbouring threads neighbouring pieces
+            constexpr int PIECES = D / 8;
+            for (int i = threadIdx.x & 127; i < kTileRows * PIECES; i += 128) {
+                const int row = i / PIECES, p = i % PIECES;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (t * kTileRows + row < qt.rows) {
+                    const int tok = token_of(t * kTileRows + row), head = h * a.G + (qt.row0 + t * kTileRows + row - tok * a.G);
+                    v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(qt.token0 + tok) * a.q_tok + head * a.q_head + 8 * p);
+                    v = make_uint4((v.x & a.q_keep) ^ a.q_flip, (v.y & a.q_keep) ^ a.q_flip, (v.z & a.q_keep) ^ a.q_flip, (v.w & a.q_keep) ^ a.q_flip);
+                }
+                *reinterpret_cast<uint4*>(smem + t * Z::kQTile + (p / 8) * kTileRows * 128 + row * 128 + (((p % 8) ^ (row & 7)) << 4)) = v;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(bar(Z::kQueries + t));
+        }
+        const bool live = r < qt.rows;
+        const int limit = live ? min(last, rows_seen(s, qt.b, qt.n, token_of(r))) : last, unmasked = min(last, fewest);
+        const float c = a.scale_log2;
+        constexpr float kGrowth = 8.0f, kLift = BF16 ? 0.0f : 6.0f;      // fp16 weights: 2^-20 of the largest is still a normal number
+        float m = -INFINITY, shift = -INFINITY;                // the score that weights are relative to; c m - kLift as it is subtracted
+        float total = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < steps; ++j) {
+            const int buf = TILES == 2 ? t : j & 1, at = first + j * KT;
+            const uint32_t scores = lanes + (uint32_t)(Z::kScores + buf * KT);
+            const bool edge = at < start || at + KT > last;
+            if (edge) {                                       // v's rows that nobody sees
+                const int order = order_v(j);
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kFull + order % Z::kStages), (uint32_t)(order / Z::kStages) & 1u, abort_flag, wait_limit));
+                if (ok) {
+                    uint8_t* const v = smem + Z::kStagesAt + (order % Z::kStages) * Z::kStage;
+                    for (int i = threadIdx.x & 127; i < KT * CHUNKS * 8; i += 128) {
+                        const int row = (i >> 3) % KT;
+                        if (at + row < start || at + row >= last) *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async_smem();
+                }
+            }
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kScoresFull + buf), TILES == 2 ? j & 1 : (j >> 1) & 1, abort_flag, wait_limit));
+            if (!ok) {
+                if (lane == 0) report_timeout(status, abort_flag, W_ACC_FULL);
+                break;
+            }
+            tc_fence_after();
+            uint32_t x[KT];
+#pragma unroll
+            for (int i = 0; i < KT; i += 32) tmem_ld32(scores + (uint32_t)i, *reinterpret_cast<uint32_t(*)[32]>(x + i));
+            tmem_wait_ld();
+            if (at < start || at + KT > unmasked) {
+#pragma unroll
+                for (int i = 0; i < KT; ++i)
+                    if (at + i >= limit || at + i < start) x[i] = 0xff800000u;
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < KT; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
+            const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+            const bool need = (now - m) * c > kGrowth;         // a first score always is
+            // O is at rest when the product before is done.  With two tiles these scores came after it; with one it is waited for in every step, which also
+            // keeps the barrier's phases in sight: a wait for one phase may be one behind, not two.
+            if (TILES == 1 && j > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kProductDone), (uint32_t)(j - 1) & 1u, abort_flag, wait_limit));
+                if (!ok) {
+                    if (lane == 0) report_timeout(status, abort_flag, W_ACC_EMPTY);
+                    break;
+                }
+                tc_fence_after();
+            }
+            if (__any_sync(0xffffffffu, need)) {
+                float alpha = 1.0f;
+                if (need) {
+                    m = now;
+                    const float next = __fmaf_rn(m, c, -kLift);
+                    alpha = exp2_fast(shift - next);
+                    shift = next;
+                    total *= alpha;
+                }
+                if (j > 0) {
+                    const uint64_t both = pack_f32x2(alpha, alpha);
+#pragma unroll
+                    for (int d = 0; d < D; d += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(out + (uint32_t)d, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            float y, z;
+                            unpack_f32x2(mul_f32x2(pack_u32x2(o[i], o[i + 1]), both), y, z);
+                            o[i] = __float_as_uint(y), o[i + 1] = __float_as_uint(z);
+                        }
+                        tmem_st16(out + (uint32_t)d, o);
+                    }
+                }
+            }
+            const float zero = m == -INFINITY ? 0.0f : m, ref = m == -INFINITY ? 0.0f : shift;
+            const uint64_t cc = pack_f32x2(c, c), less = pack_f32x2(-ref, -ref);
+            uint64_t sums[2] = {0ull, 0ull};
+            auto weights = [&](auto far) {
+#pragma unroll
+                for (int i0 = 0; i0 < KT; i0 += 64) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        float y, z;
+                        if (decltype(far)::value) {
+                            y = __fmaf_rn(__uint_as_float(x[i0 + i]) - zero, c, -kLift);
+                            z = __fmaf_rn(__uint_as_float(x[i0 + i + 1]) - zero, c, -kLift);
+                        } else {
+                            unpack_f32x2(fma_f32x2(pack_u32x2(x[i0 + i], x[i0 + i + 1]), cc, less), y, z);
+                        }
+                        y = exp2_fast(y);
+                        z = exp2_fast(z);
+                        sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(y, z));
+                        p[i / 2] = F16Bits<T>::pack(y, z);
+                    }
+                    tmem_st32(scores + (uint32_t)(i0 / 2), p);
+                }
+            };
+            if (__any_sync(0xffffffffu, fabsf(ref) >= 0x1p20f)) weights(std::true_type{});
+            else weights(std::false_type{});
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar(Z::kWeightsFull + buf));
+            float y, z;
+            unpack_f32x2(add_f32x2(sums[0], sums[1]), y, z);
+            total += y + z;
+        }
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kProductDone + t), (uint32_t)(steps - 1) & 1u, abort_flag, wait_limit));
+        if (!ok) {
+            if (lane == 0) report_timeout(status, abort_flag, W_ACC_FULL);
+        } else {
+            // ---- results
+            tc_fence_after();
+            const int64_t query = live ? query_at(r) : 0;
+            const bool whole = count == 1;
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            if (live && a.shares > 1) a.part.stats[share * a.part.rows + query] = whole ? make_float2(0.0f, kWritten) : make_float2(m == -INFINITY ? m : shift, total);
+#pragma unroll
+            for (int d = 0; d < D; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(out + (uint32_t)d, o);
+                tmem_wait_ld();
+                if (!live) continue;
+                if (whole) {
+                    uint4* const dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + query * D + d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = F16Bits<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                        dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else {
+                    uint4* const dst = reinterpret_cast<uint4*>(a.part.sums + (share * a.part.rows + query) * D + d);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, Z::kColumns);
+    }
+}
+
+int make_page_map(CUtensorMap* map, const void* ptr, int dt, const bi8_paged_cache& c, int64_t page, int64_t head, int64_t row, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(BI8_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    ensure_current_context();
+    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_rows, (cuuint64_t)c.heads, (cuuint64_t)c.pages};
+    // a dimension of one element needs no step, but the encoder wants one
+    const cuuint64_t dense = (cuuint64_t)c.head_dim * 2;
+    const cuuint64_t steps[3] = {(cuuint64_t)row * 2, c.heads > 1 ? (cuuint64_t)head * 2 : dense, c.pages > 1 ? (cuuint64_t)page * 2 : dense};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, dt == BI8_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(ptr), dims, steps, box, one,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(BI8_ERR_CUDA, "cuTensorMapEncodeTiled (pages) failed with CUresult %d", (int)r);
+    return BI8_OK;
+}
+
+template <typename T, int D>
+int launch(const PagedAttnArgs& a, int dt, cudaStream_t st) {
+    using Z = Shape<D>;
+    int box_rows = 16;                                        // the largest power of two that divides a page, up to a step
+    while (box_rows < Z::kRows && a.cache.page_rows % (2 * box_rows) == 0) box_rows *= 2;
+    CUtensorMap k_map, v_map;
+    if (int rc = make_page_map(&k_map, a.cache.k, dt, a.cache, a.cache.k_page, a.cache.k_head, a.cache.k_row, box_rows)) return rc;
+    if (int rc = make_page_map(&v_map, a.cache.v, dt, a.cache, a.cache.v_page, a.cache.v_head, a.cache.v_row, box_rows)) return rc;
+    int* const status = device_status_ptr();
+    if (!status) return fail(BI8_ERR_CUDA, "attention_paged: the device's status word cannot be reached");
+    static SmemOptIn opt_in;
+    if (int rc = opt_in.ensure(paged_many_kernel<T, D>, Z::kBytes)) return rc;
+    return launch_chained(paged_many_kernel<T, D>, (unsigned)((int64_t)a.tiles * a.Hkv * a.shares), Z::kThreads, Z::kBytes, st, k_map, v_map, a, box_rows, kShareRows, status,
+                          4000000000ll);
+}
+
+}  // namespace
+
+int paged_many_tile(int64_t D) { return D == 256 ? Shape<256>::kTiles * kTileRows : Shape<128>::kTiles * kTileRows; }
+
+int launch_paged_many(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st) {
+    auto go = [&](auto* tag) {
+        using E = std::remove_pointer_t<decltype(tag)>;
+        if (D == 64) return launch<E, 64>(a, dt, st);
+        if (D == 128) return launch<E, 128>(a, dt, st);
+        return launch<E, 256>(a, dt, st);
+    };
+    return dt == BI8_BF16 ? go(static_cast<__nv_bfloat16*>(nullptr)) : go(static_cast<__half*>(nullptr));
+}
+
+}  // namespace bi8
