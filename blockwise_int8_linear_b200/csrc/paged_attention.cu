@@ -424,6 +424,53 @@ __global__ void __launch_bounds__(4 * D) paged_join_kernel(const Partials p, int
     reinterpret_cast<unsigned short*>(out)[row * D + d] = (unsigned short)F16Bits<T>::pack((sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d]), 0.0f);
 }
 
+// The same for few shares and any number of queries: a warp each, whose lanes know a share's weight and have 4 or 8 features.
+constexpr int kFewShares = 16, kJoinWarps = 4;
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kJoinWarps) paged_join_few_kernel(const Partials p, int shares, T* out) {
+    constexpr int V = D / 32;
+    after_predecessor();
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * kJoinWarps + (threadIdx.x >> 5);
+    if (row >= p.rows) return;
+    const float2 mine = lane < shares ? p.stats[lane * p.rows + row] : make_float2(-INFINITY, 0.0f);
+    if (__shfl_sync(0xffffffffu, mine.y, 0) == kWritten) return;
+    float top = mine.x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float w = mine.y != 0.0f ? exp2_fast(mine.x - top) : 0.0f;
+    float total = w * mine.y;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+    const float weight = mine.y != 0.0f ? w * (total == 0.0f ? 0.0f : 1.0f / total) : -1.0f;
+    float x[V] = {};
+    const float* const src = p.sums + row * D + lane * V;
+#pragma unroll 4
+    for (int k = 0; k < shares; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, weight, k);
+        if (wk == -1.0f) continue;                        // a share that saw nothing may have left no sums
+        float v[V];
+        if constexpr (V == 2) {
+            const float2 y = *reinterpret_cast<const float2*>(src + k * p.rows * D);
+            v[0] = y.x, v[1] = y.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(src + k * p.rows * D + i);
+                v[i] = y.x, v[i + 1] = y.y, v[i + 2] = y.z, v[i + 3] = y.w;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = fmaf(v[i], wk, x[i]);
+    }
+    uint32_t* const dst = reinterpret_cast<uint32_t*>(out + row * D + lane * V);
+#pragma unroll
+    for (int i = 0; i < V; i += 2) dst[i / 2] = F16Bits<T>::pack(x[i], x[i + 1]);
+}
+
+// (A row past two tiles takes 13 ns.)
+constexpr int64_t kSetUpRows = 600, kJoinRows = 80, kJoinRows0 = 200;
+
 struct Plan {
     bool many;
     int rows;                    // queries of a tile
@@ -437,9 +484,16 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     p.tiles = tile_count(B, N, G, p.rows, packed);
     const int64_t ctas = p.tiles * Hkv;
     if (p.many) {
-        int64_t s = max_len / kShareRows, want = (2 * sms + ctas - 1) / ctas;
-        if (s > want) s = want;
-        p.shares = s < 1 ? 1 : s > kMaxShares ? kMaxShares : s;
+        // A CTA an SM: the number of shares for which as many rounds of CTAs as it takes are shortest, a CTA's set-up counted as kSetUpRows and what
+        // the shares write and the join reads as rows that go by meanwhile.
+        const int64_t most = max_len / kShareRows < kFewShares ? max_len / kShareRows : kFewShares;
+        int64_t best = 0;
+        p.shares = 1;
+        for (int64_t s = 1; s <= most || s == 1; ++s) {
+            const int64_t rounds = (ctas * s + sms - 1) / sms, join = s > 1 ? s * N * Hq / kJoinRows + kJoinRows0 : 0;
+            const int64_t cost = rounds * (max_len / s + kSetUpRows) + join;
+            if (s == 1 || cost < best) best = cost, p.shares = s;
+        }
         return p;
     }
     const int64_t step = 16 * (D == 64 ? kSubSteps<64> : D == 128 ? kSubSteps<128> : kSubSteps<256>);
@@ -483,6 +537,12 @@ int launch(const PagedAttnArgs& a, cudaStream_t st) {
 template <typename T>
 int join(const Partials& p, int shares, void* out, int64_t D, cudaStream_t st) {
     T* const o = static_cast<T*>(out);
+    if (shares <= kFewShares) {
+        const unsigned grid = (unsigned)((p.rows + kJoinWarps - 1) / kJoinWarps);
+        if (D == 64) return launch_chained(paged_join_few_kernel<T, 64>, grid, 32 * kJoinWarps, 0, st, p, shares, o);
+        if (D == 128) return launch_chained(paged_join_few_kernel<T, 128>, grid, 32 * kJoinWarps, 0, st, p, shares, o);
+        return launch_chained(paged_join_few_kernel<T, 256>, grid, 32 * kJoinWarps, 0, st, p, shares, o);
+    }
     if (D == 64) return launch_chained(paged_join_kernel<T, 64>, (unsigned)p.rows, 256, 0, st, p, shares, o);
     if (D == 128) return launch_chained(paged_join_kernel<T, 128>, (unsigned)p.rows, 512, 0, st, p, shares, o);
     return launch_chained(paged_join_kernel<T, 256>, (unsigned)p.rows, 1024, 0, st, p, shares, o);

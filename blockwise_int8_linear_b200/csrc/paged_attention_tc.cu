@@ -23,6 +23,7 @@
 #include "paged_attention.cuh"
 #include "tc_common.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 namespace bi8 {
@@ -31,6 +32,7 @@ namespace {
 using namespace ptx;
 
 constexpr int kTileRows = 128;
+constexpr int kSoftmaxRegisters = 208, kOtherRegisters = 80;       // of two tiles' warps and of the four others
 
 template <int D>
 struct Shape {
@@ -38,13 +40,13 @@ struct Shape {
     static constexpr int kRows = D == 256 ? 64 : 128;                // of the cache at a time
     static constexpr int kStages = D == 64 ? 8 : 5;
     static constexpr int kAhead = kTiles == 1 ? 2 : 1;               // scores that are under way before the first weights are used
-    static constexpr int kWarps = 4 * kTiles + 2, kThreads = 32 * kWarps;
+    static constexpr int kWarps = kTiles == 2 ? 12 : 6, kThreads = 32 * kWarps;
     static constexpr int kQTile = kTileRows * D * 2, kStage = kRows * D * 2;
     static constexpr int kScores = 0, kOut = 2 * kRows;              // columns of tensor memory
     static constexpr int kColumns = 512;
     static_assert(kOut + kTiles * D <= kColumns, "tensor memory");
     // barriers
-    static constexpr int kFull = 0, kEmpty = kStages, kScoresFull = 2 * kStages, kWeightsFull = kScoresFull + 2, kProductDone = kWeightsFull + 2,
+    static constexpr int kFull = 0, kEmpty = kStages, kScoresFull = 2 * kStages, kWeightsFull = kScoresFull + 2, kProductDone = kWeightsFull + 4,
                          kQueries = kProductDone + 2, kEnd = kQueries + 2, kBarriers = kEnd + 1;
     static constexpr int kStagesAt = kTiles * kQTile, kBarriersAt = kStagesAt + kStages * kStage, kMisc = kBarriersAt + 8 * kBarriers;
     static constexpr int kBytes = kMisc + 16 + 1024;                 // tensor memory's address, abort flag, a word that stays zero; alignment
@@ -113,6 +115,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
             for (int i = 0; i < 2; ++i) {
                 mbar_init(bar(Z::kScoresFull + i), 1);
                 mbar_init(bar(Z::kWeightsFull + i), 128);
+                mbar_init(bar(Z::kWeightsFull + 2 + i), 128);
                 mbar_init(bar(Z::kProductDone + i), 1);
                 mbar_init(bar(Z::kQueries + i), 128);
             }
@@ -129,6 +132,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
     auto order_v = [&](int j) { return min(steps, j + Z::kAhead) + j; };
     auto order_k = [&](int j) { return j < Z::kAhead ? j : order_v(j - Z::kAhead) + 1; };
 
+    if (warp >= MMA_WARP) {
+    if constexpr (TILES == 2) setmaxnreg_dec<kOtherRegisters>();
     if (warp == LOAD_WARP) {
         // ---- copies: a box of box_rows rows and 64 features at a time, a lane for every box_rows rows of the step
         const int boxes = KT / box_rows;
@@ -197,14 +202,18 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                 wait_stage(ov);
                 for (int t = 0; t < tiles && ok; ++t) {
                     const int buf = TILES == 2 ? t : j & 1;
-                    wait(Z::kWeightsFull + buf, TILES == 2 ? j & 1 : (j >> 1) & 1, W_ACC_FULL);
-                    if (!ok) break;
-                    tc_fence_after();
                     const uint32_t v = stage_at(ov % Z::kStages);
 #pragma unroll
-                    for (int i = 0; i < KT / 16; ++i)
-                        mma_f16_ta(tmem + (uint32_t)(Z::kOut + t * D), tmem + (uint32_t)(Z::kScores + buf * KT + 8 * i), umma_desc_mn_sw128(v + (uint32_t)(2048 * i), KT * 128),
-                                   O_DESC, j > 0 || i > 0);
+                    for (int half = 0; half < 2; ++half) {
+                        wait(Z::kWeightsFull + 2 * half + buf, TILES == 2 ? j & 1 : (j >> 1) & 1, W_ACC_FULL);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int i = half * (KT / 32); i < (half + 1) * (KT / 32); ++i)
+                            mma_f16_ta(tmem + (uint32_t)(Z::kOut + t * D), tmem + (uint32_t)(Z::kScores + buf * KT + 8 * i), umma_desc_mn_sw128(v + (uint32_t)(2048 * i), KT * 128),
+                                       O_DESC, j > 0 || i > 0);
+                    }
+                    if (!ok) break;
                     tc_commit(bar(Z::kProductDone + t));
                     if (ahead < steps) {
                         if (t == 0) wait_stage(ok_order);
@@ -221,22 +230,32 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp / 4 < tiles) {
+    }
+    } else {
+        if constexpr (TILES == 2) setmaxnreg_inc<kSoftmaxRegisters>();
+        if (warp / 4 < tiles) {
         // ---- softmax: a thread is a query
         const int t = warp / 4, r = t * kTileRows + (threadIdx.x & 127);
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), out = lanes + (uint32_t)(Z::kOut + t * D);
         {
-            // the tile's queries, neighbouring threads neighbouring pieces
-            constexpr int PIECES = D / 8;
-            for (int i = threadIdx.x & 127; i < kTileRows * PIECES; i += 128) {
-                const int row = i / PIECES, p = i % PIECES;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (t * kTileRows + row < qt.rows) {
-                    const int tok = token_of(t * kTileRows + row), head = h * a.G + (qt.row0 + t * kTileRows + row - tok * a.G);
-                    v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(qt.token0 + tok) * a.q_tok + head * a.q_head + 8 * p);
-                    v = make_uint4((v.x & a.q_keep) ^ a.q_flip, (v.y & a.q_keep) ^ a.q_flip, (v.z & a.q_keep) ^ a.q_flip, (v.w & a.q_keep) ^ a.q_flip);
+            // the tile's queries, neighbouring threads neighbouring pieces, eight loads under way
+            constexpr int PIECES = D / 8, ROWS = 128 / PIECES;
+            const int row0 = (threadIdx.x & 127) / PIECES, p = threadIdx.x % PIECES;
+#pragma unroll
+            for (int i0 = 0; i0 < PIECES; i0 += 8) {
+                uint4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = t * kTileRows + row0 + (i0 + i) * ROWS, tok = token_of(row), head = h * a.G + (qt.row0 + row - tok * a.G);
+                    v[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (row < qt.rows) v[i] = ld_nc_v4(static_cast<const T*>(a.q) + (int64_t)(qt.token0 + tok) * a.q_tok + head * a.q_head + 8 * p);
                 }
-                *reinterpret_cast<uint4*>(smem + t * Z::kQTile + (p / 8) * kTileRows * 128 + row * 128 + (((p % 8) ^ (row & 7)) << 4)) = v;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = row0 + (i0 + i) * ROWS;
+                    const uint4 w = make_uint4((v[i].x & a.q_keep) ^ a.q_flip, (v[i].y & a.q_keep) ^ a.q_flip, (v[i].z & a.q_keep) ^ a.q_flip, (v[i].w & a.q_keep) ^ a.q_flip);
+                    *reinterpret_cast<uint4*>(smem + t * Z::kQTile + (p / 8) * kTileRows * 128 + row * 128 + (((p % 8) ^ (row & 7)) << 4)) = w;
+                }
             }
             fence_proxy_async_smem();
             mbar_arrive(bar(Z::kQueries + t));
@@ -325,10 +344,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
             uint64_t sums[2] = {0ull, 0ull};
             auto weights = [&](auto far) {
 #pragma unroll
-                for (int i0 = 0; i0 < KT; i0 += 64) {
-                    uint32_t p[32];
+                for (int i0 = 0; i0 < KT; i0 += KT / 4) {
+                    uint32_t p[KT / 8];
 #pragma unroll
-                    for (int i = 0; i < 64; i += 2) {
+                    for (int i = 0; i < KT / 4; i += 2) {
                         float y, z;
                         if (decltype(far)::value) {
                             y = __fmaf_rn(__uint_as_float(x[i0 + i]) - zero, c, -kLift);
@@ -341,14 +360,20 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                         sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(y, z));
                         p[i / 2] = F16Bits<T>::pack(y, z);
                     }
-                    tmem_st32(scores + (uint32_t)(i0 / 2), p);
+                    if (i0 == KT / 2) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(bar(Z::kWeightsFull + buf));
+                    }
+                    if constexpr (KT == 128) tmem_st16(scores + (uint32_t)(i0 / 2), p);
+                    else tmem_st8(scores + (uint32_t)(i0 / 2), p);
                 }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(bar(Z::kWeightsFull + 2 + buf));
             };
             if (__any_sync(0xffffffffu, fabsf(ref) >= 0x1p20f)) weights(std::true_type{});
             else weights(std::false_type{});
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(bar(Z::kWeightsFull + buf));
             float y, z;
             unpack_f32x2(add_f32x2(sums[0], sums[1]), y, z);
             total += y + z;
@@ -359,31 +384,58 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
         } else {
             // ---- results
             tc_fence_after();
-            const int64_t query = live ? query_at(r) : 0;
             const bool whole = count == 1;
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            if (live && a.shares > 1) a.part.stats[share * a.part.rows + query] = whole ? make_float2(0.0f, kWritten) : make_float2(m == -INFINITY ? m : shift, total);
-#pragma unroll
-            for (int d = 0; d < D; d += 32) {
-                uint32_t o[32];
-                tmem_ld32(out + (uint32_t)d, o);
-                tmem_wait_ld();
-                if (!live) continue;
-                if (whole) {
-                    uint4* const dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + query * D + d);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = F16Bits<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                        dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            if (live && a.shares > 1)
+                a.part.stats[share * a.part.rows + query_at(r)] = whole ? make_float2(0.0f, kWritten) : make_float2(m == -INFINITY ? m : shift, total);
+            // by way of the queries' place, 256 bytes of a row at a time (128 with 64 features), so that rows are written whole
+            constexpr int PASS = D == 64 ? 128 : 256, LANES = PASS / 16, ROWS = 128 / LANES;
+            uint8_t* const place = smem + t * Z::kQTile;
+            const int mine = threadIdx.x & 127;
+            auto through = [&](auto fill, char* to, int64_t row_bytes, int passes) {
+                for (int pass = 0; pass < passes; ++pass) {
+                    fill(pass, place + mine * PASS);
+                    asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
+                    const int piece = mine % LANES;
+#pragma unroll 8
+                    for (int i = 0; i < 128 / ROWS; ++i) {
+                        const int row = mine / LANES + i * ROWS;
+                        if (t * kTileRows + row >= qt.rows) break;
+                        const uint4 v = *reinterpret_cast<const uint4*>(place + row * PASS + ((piece ^ (row & 7)) << 4));
+                        *reinterpret_cast<uint4*>(to + query_at(t * kTileRows + row) * row_bytes + pass * PASS + piece * 16) = v;
                     }
-                } else {
-                    uint4* const dst = reinterpret_cast<uint4*>(a.part.sums + (share * a.part.rows + query) * D + d);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
                 }
+            };
+            if (whole) {
+                through([&](int pass, uint8_t* row) {
+#pragma unroll
+                    for (int d = 0; d < PASS / 2; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(out + (uint32_t)(pass * (PASS / 2) + d), o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) w[e] = F16Bits<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                            *reinterpret_cast<uint4*>(row + (((d / 8 + i) ^ (mine & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }, static_cast<char*>(a.out), D * 2, D * 2 / PASS);
+            } else {
+                through([&](int pass, uint8_t* row) {
+#pragma unroll
+                    for (int d = 0; d < PASS / 4; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(out + (uint32_t)(pass * (PASS / 4) + d), o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(row + (((d / 4 + i) ^ (mine & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                }, reinterpret_cast<char*>(a.part.sums + share * a.part.rows * D), D * 4, D * 4 / PASS);
             }
+        }
         }
     }
     tc_fence_before();
@@ -417,6 +469,18 @@ int launch(const PagedAttnArgs& a, int dt, cudaStream_t st) {
     CUtensorMap k_map, v_map;
     if (int rc = make_page_map(&k_map, a.cache.k, dt, a.cache, a.cache.k_page, a.cache.k_head, a.cache.k_row, box_rows)) return rc;
     if (int rc = make_page_map(&v_map, a.cache.v, dt, a.cache, a.cache.v_page, a.cache.v_head, a.cache.v_row, box_rows)) return rc;
+    if constexpr (Z::kTiles == 2) {
+        // The roles' shares of the registers come out of what the block was launched with; were that less, their wait for it would not end.
+        static std::atomic<int> registers{0};
+        int n = registers.load(std::memory_order_relaxed);
+        if (n == 0) {
+            cudaFuncAttributes at;
+            BI8_CUDA_TRY(cudaFuncGetAttributes(&at, paged_many_kernel<T, D>));
+            registers.store(n = at.numRegs, std::memory_order_relaxed);
+        }
+        if (n * Z::kThreads < 128 * (2 * kSoftmaxRegisters + kOtherRegisters))
+            return fail(BI8_ERR_CUDA, "attention_paged: built with %d registers a thread, too few for the kernel's roles", n);
+    }
     int* const status = device_status_ptr();
     if (!status) return fail(BI8_ERR_CUDA, "attention_paged: the device's status word cannot be reached");
     static SmemOptIn opt_in;

@@ -7,10 +7,12 @@
 #include "paged_common.cuh"
 #include "rope.cuh"
 
+#include <type_traits>
+
 namespace bi8 {
 namespace {
 
-constexpr int kThreads = 256, kHeads = 4, kMaxTokens = 64, P = 8;
+constexpr int kThreads = 256, kHeads = 2, kMaxTokens = 64, P = 8;
 
 struct PagedAppendArgs {
     const void* qkv;             // [N, Hq + 2 Hkv, D]
@@ -20,13 +22,13 @@ struct PagedAppendArgs {
     void* q_out;                 // [N, Hq, D]
     bi8_paged_cache cache;
     Sequences seq;
-    int Hq, Hkv, D, R, half_layout;
+    int Hq, Hkv, D, R;
     int slices, units, tokens;   // tokens of a block
     FastDiv per_unit, per_token;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) rope_cache_append_paged_kernel(const PagedAppendArgs a) {
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(kThreads, 4) rope_cache_append_paged_kernel(const PagedAppendArgs a) {
     __shared__ int sequence[kMaxTokens];
     after_predecessor();
     const Sequences& s = a.seq;
@@ -57,24 +59,23 @@ __global__ void __launch_bounds__(kThreads) rope_cache_append_paged_kernel(const
         int off_a, off_b;
         piece_offsets<P>(u, a.R, a.D, off_a, off_b);
         const T* const src = static_cast<const T*>(a.qkv) + token * a.x_tok;
-        using V = Piece<T, P>;
-        V x[kHeads], y[kHeads];
+        Piece<T, P> x[kHeads], y[kHeads];
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) {
             const int h = slice + j * a.slices;
-            if (h < H && inside) {
-                x[j] = *reinterpret_cast<const V*>(src + h * a.x_head + off_a);
-                y[j] = *reinterpret_cast<const V*>(src + h * a.x_head + off_b);
-            } else {
-#pragma unroll
-                for (int e = 0; e < P; ++e) x[j].v[e] = y[j].v[e] = RopeType<T>::set(0.0f);
+            if (h < H) {
+                x[j].load(src + h * a.x_head + off_a);
+                y[j].load(src + h * a.x_head + off_b);
             }
         }
-        if (u < a.R / (2 * P) && inside) {
-            const Angles<P> g = load_angles<P>(a.cis + position * (a.R / 2), u, a.R, a.half_layout != 0);
+        if (!inside) {
+#pragma unroll
+            for (int j = 0; j < kHeads; ++j) x[j].clear(), y[j].clear();
+        } else if (u < a.R / (2 * P)) {
+            const Angles<P> g = load_angles<P>(a.cis + position * (a.R / 2), u, a.R, HALF);
 #pragma unroll
             for (int j = 0; j < kHeads; ++j)
-                if (slice + j * a.slices < a.Hq + a.Hkv) turn_pieces<T, P>(x[j], y[j], g, a.half_layout != 0);
+                if (slice + j * a.slices < a.Hq + a.Hkv) turn_pieces<T, P>(x[j], y[j], g, HALF);
         }
         const bi8_paged_cache& c = a.cache;
 #pragma unroll
@@ -90,8 +91,8 @@ __global__ void __launch_bounds__(kThreads) rope_cache_append_paged_kernel(const
             } else {
                 continue;
             }
-            *reinterpret_cast<V*>(dst + off_a) = x[j];
-            *reinterpret_cast<V*>(dst + off_b) = y[j];
+            x[j].store(dst + off_a);
+            y[j].store(dst + off_b);
         }
     }
 }
@@ -113,7 +114,6 @@ int launch_rope_cache_append_paged(const void* qkv, int dt, int64_t x_tok, int64
     a.Hkv = (int)cache->heads;
     a.D = (int)D;
     a.R = (int)R;
-    a.half_layout = half_layout;
     a.units = (int)D / (2 * P);
     a.slices = (int)((Hq + 2 * cache->heads + kHeads - 1) / kHeads);
     const int64_t per_token = (int64_t)a.slices * a.units;
@@ -122,8 +122,12 @@ int launch_rope_cache_append_paged(const void* qkv, int dt, int64_t x_tok, int64
     a.per_unit = FastDiv(a.units);
     a.per_token = FastDiv(per_token);
     const unsigned grid = (unsigned)(((int64_t)seq.N + a.tokens - 1) / a.tokens);
-    return dt == BI8_BF16 ? launch_chained(rope_cache_append_paged_kernel<__nv_bfloat16>, grid, kThreads, 0, st, a)
-                          : launch_chained(rope_cache_append_paged_kernel<__half>, grid, kThreads, 0, st, a);
+    auto go = [&](auto* tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        return half_layout ? launch_chained(rope_cache_append_paged_kernel<T, true>, grid, kThreads, 0, st, a)
+                           : launch_chained(rope_cache_append_paged_kernel<T, false>, grid, kThreads, 0, st, a);
+    };
+    return dt == BI8_BF16 ? go(static_cast<__nv_bfloat16*>(nullptr)) : go(static_cast<__half*>(nullptr));
 }
 
 }  // namespace bi8

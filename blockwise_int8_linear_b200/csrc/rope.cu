@@ -10,7 +10,7 @@
 namespace bi8 {
 namespace {
 
-constexpr int kThreads = 256, kHeads = 4;
+constexpr int kThreads = 256, kHeads = 2;
 
 struct RopeArgs {
     const void* x;
@@ -20,82 +20,74 @@ struct RopeArgs {
     const long long* pos;                // of token t of batch b at pos[b * pos_batch + t * pos_tok], or null: t
     int64_t pos_batch, pos_tok;
     void* out;                           // [B, T, H, D]
-    int64_t items;                       // B * T * slices * units
-    int H, D, R, slices, units;
+    int N, H, D, R;                      // N = B * T
+    int slices, units, tokens;           // of heads, of a head, of a block
     int half_layout, conj;
-    FastDiv per_unit, per_slice;
-    int64_t T;
+    FastDiv per_unit, per_token, per_batch;
 };
 
-template <typename T, int P>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
+template <typename T, int P, bool HALF>
+__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
     after_predecessor();
-    const int64_t tokens_per_block = a.items;                              // tokens that this launch has
-    // a block has kThreads items of consecutive tokens: item = (token, slice of heads, unit)
-    const int per_token = a.slices * a.units;
-    const int64_t block_first = (int64_t)blockIdx.x * kThreads;
-    const int64_t token0 = block_first / per_token;
-    const unsigned rest = (unsigned)(block_first - token0 * per_token) + threadIdx.x;
-    const unsigned tok_in = a.per_slice.div(rest);
-    const int64_t token = token0 + tok_in;
-    if (token >= tokens_per_block) return;
-    const unsigned item = rest - tok_in * a.per_slice.d;
-    const int slice = (int)a.per_unit.div(item), u = (int)item - slice * a.units;
-    const int64_t b = token / a.T, t = token - b * a.T;
-    const long long p = a.pos ? a.pos[b * a.pos_batch + t * a.pos_tok] : t;
-    const bool inside = p >= 0 && p < a.rows;
-
-    int off_a, off_b;
-    piece_offsets<P>(u, a.R, a.D, off_a, off_b);
-    const bool turned = u < a.R / (2 * P);
-    const T* const src = static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_tok;
-    T* const dst = static_cast<T*>(a.out) + token * a.H * a.D;
-    using V = Piece<T, P>;
-    V x[kHeads], y[kHeads];
+    // item = (token, slice of heads, unit)
+    const unsigned token0 = blockIdx.x * (unsigned)a.tokens, tokens = min((unsigned)a.tokens, (unsigned)a.N - token0);
+    for (unsigned i = threadIdx.x; i < tokens * a.per_token.d; i += kThreads) {
+        const unsigned in = a.per_token.div(i), item = i - in * a.per_token.d, token = token0 + in;
+        const int slice = (int)a.per_unit.div(item), u = (int)item - slice * a.units;
+        const unsigned b = a.per_batch.div(token), t = token - b * a.per_batch.d;
+        const long long p = a.pos ? a.pos[b * a.pos_batch + t * a.pos_tok] : (long long)t;
+        int off_a, off_b;
+        piece_offsets<P>(u, a.R, a.D, off_a, off_b);
+        const T* const src = static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_tok;
+        Piece<T, P> x[kHeads], y[kHeads];
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        const int h = slice + i * a.slices;
-        if (h < a.H && inside) {
-            x[i] = *reinterpret_cast<const V*>(src + h * a.x_head + off_a);
-            y[i] = *reinterpret_cast<const V*>(src + h * a.x_head + off_b);
-        } else {
-#pragma unroll
-            for (int j = 0; j < P; ++j) x[i].v[j] = y[i].v[j] = RopeType<T>::set(0.0f);      // a position outside the table: zeros
+        for (int j = 0; j < kHeads; ++j) {
+            const int h = slice + j * a.slices;
+            if (h < a.H) {
+                x[j].load(src + h * a.x_head + off_a);
+                y[j].load(src + h * a.x_head + off_b);
+            }
         }
-    }
-    if (turned && inside) {
-        Angles<P> g = load_angles<P>(a.cis + p * (a.R / 2), u, a.R, a.half_layout != 0);
-        if (a.conj) {
+        const bool inside = p >= 0 && p < a.rows;             // a position outside the table: zeros
+        if (!inside) {
 #pragma unroll
-            for (int j = 0; j < P; ++j) g.s[j] = -g.s[j];
+            for (int j = 0; j < kHeads; ++j) x[j].clear(), y[j].clear();
+        } else if (u < a.R / (2 * P)) {
+            Angles<P> g = load_angles<P>(a.cis + p * (a.R / 2), u, a.R, HALF);
+            if (a.conj) {
+#pragma unroll
+                for (int e = 0; e < P; ++e) g.s[e] = -g.s[e];
+            }
+#pragma unroll
+            for (int j = 0; j < kHeads; ++j) turn_pieces<T, P>(x[j], y[j], g, HALF);
         }
+        T* const dst = static_cast<T*>(a.out) + (int64_t)token * a.H * a.D;
 #pragma unroll
-        for (int i = 0; i < kHeads; ++i)
-            if (slice + i * a.slices < a.H) turn_pieces<T, P>(x[i], y[i], g, a.half_layout != 0);
-    }
-#pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        const int h = slice + i * a.slices;
-        if (h < a.H) {
-            *reinterpret_cast<V*>(dst + (int64_t)h * a.D + off_a) = x[i];
-            *reinterpret_cast<V*>(dst + (int64_t)h * a.D + off_b) = y[i];
+        for (int j = 0; j < kHeads; ++j) {
+            const int h = slice + j * a.slices;
+            if (h < a.H) {
+                x[j].store(dst + (int64_t)h * a.D + off_a);
+                y[j].store(dst + (int64_t)h * a.D + off_b);
+            }
         }
     }
 }
 
 // Any even R and any D, of any alignment: one feature a thread.
 template <typename T>
+__device__ __forceinline__ float to_float(T v) { return static_cast<float>(v); }
+template <typename T>
 __global__ void __launch_bounds__(kThreads) rope_single_kernel(const RopeArgs a) {
     after_predecessor();
     const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, per_token = (int64_t)a.H * a.D;
     const int64_t token = i / per_token;
-    if (token >= a.items) return;
+    if (token >= a.N) return;
     const int hd = (int)(i - token * per_token), h = hd / a.D, d = hd - h * a.D;
-    const int64_t b = token / a.T, t = token - b * a.T;
-    const long long p = a.pos ? a.pos[b * a.pos_batch + t * a.pos_tok] : t;
+    const unsigned b = a.per_batch.div((unsigned)token), t = (unsigned)token - b * a.per_batch.d;
+    const long long p = a.pos ? a.pos[b * a.pos_batch + t * a.pos_tok] : (long long)t;
     T* const dst = static_cast<T*>(a.out) + i;
     if (p < 0 || p >= a.rows) {
-        *dst = RopeType<T>::set(0.0f);
+        *dst = static_cast<T>(0.0f);
         return;
     }
     const T* const src = static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_tok + h * a.x_head;
@@ -107,25 +99,25 @@ __global__ void __launch_bounds__(kThreads) rope_single_kernel(const RopeArgs a)
     const bool second = a.half_layout ? d >= half : (d & 1) != 0;
     const int first = a.half_layout ? pair : 2 * pair, other = a.half_layout ? pair + half : first + 1;
     const float2 cs = __ldg(a.cis + p * half + pair);
-    float x = RopeType<T>::get(src[first]), y = RopeType<T>::get(src[other]);
+    float x = to_float(src[first]), y = to_float(src[other]);
     turn(x, y, cs.x, a.conj ? -cs.y : cs.y);
-    *dst = RopeType<T>::set(second ? y : x);
+    *dst = static_cast<T>(second ? y : x);
 }
 
 template <typename T, int P>
-int launch(RopeArgs a, int64_t tokens, cudaStream_t st) {
+int launch(RopeArgs a, cudaStream_t st) {
     a.units = a.D / (2 * P);
     a.slices = (a.H + kHeads - 1) / kHeads;
-    a.items = tokens;
+    const int64_t per_token = (int64_t)a.slices * a.units;
+    a.tokens = (int)(per_token >= kThreads ? 1 : kThreads / per_token);
     a.per_unit = FastDiv(a.units);
-    a.per_slice = FastDiv((int64_t)a.slices * a.units);
-    const int64_t blocks = (tokens * a.slices * a.units + kThreads - 1) / kThreads;
-    if (blocks > 0x7fffffff) return fail(BI8_ERR_LIMIT, "rope: %lld tokens exceed one launch", (long long)tokens);
-    return launch_chained(rope_kernel<T, P>, (unsigned)blocks, kThreads, 0, st, a);
+    a.per_token = FastDiv(per_token);
+    const unsigned grid = (unsigned)(((int64_t)a.N + a.tokens - 1) / a.tokens);
+    return a.half_layout ? launch_chained(rope_kernel<T, P, true>, grid, kThreads, 0, st, a) : launch_chained(rope_kernel<T, P, false>, grid, kThreads, 0, st, a);
 }
 
 template <typename T>
-int launch_type(const RopeArgs& a, int64_t tokens, cudaStream_t st) {
+int launch_type(const RopeArgs& a, cudaStream_t st) {
     // pieces of 8, 4 or 2 features: the widest that divides both parts of a head and begins on its boundaries everywhere
     auto fits = [&](int P) {
         const size_t bytes = sizeof(T) * P > 16 ? 16 : sizeof(T) * P;
@@ -134,14 +126,13 @@ int launch_type(const RopeArgs& a, int64_t tokens, cudaStream_t st) {
         for (int64_t s : steps) ok = ok && s * (int64_t)sizeof(T) % (int64_t)bytes == 0;
         return ok && (int64_t)((a.H + kHeads - 1) / kHeads) * (a.D / (2 * P)) < (1 << 30);
     };
-    if (fits(8)) return launch<T, 8>(a, tokens, st);
-    if (fits(4)) return launch<T, 4>(a, tokens, st);
-    if (fits(2)) return launch<T, 2>(a, tokens, st);
-    RopeArgs s = a;
-    s.items = tokens;
-    const int64_t per_block = kThreads, values = tokens * a.H * a.D, blocks = (values + per_block - 1) / per_block;
-    if (blocks > 0x7fffffff) return fail(BI8_ERR_LIMIT, "rope: %lld tokens exceed one launch", (long long)tokens);
-    return launch_chained(rope_single_kernel<T>, (unsigned)blocks, kThreads, 0, st, s);
+    if constexpr (sizeof(T) == 2)
+        if (fits(8)) return launch<T, 8>(a, st);
+    if (fits(4)) return launch<T, 4>(a, st);
+    if (fits(2)) return launch<T, 2>(a, st);
+    const int64_t blocks = ((int64_t)a.N * a.H * a.D + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffff) return fail(BI8_ERR_LIMIT, "rope: %d tokens exceed one launch", a.N);
+    return launch_chained(rope_single_kernel<T>, (unsigned)blocks, kThreads, 0, st, a);
 }
 
 }  // namespace
@@ -164,9 +155,11 @@ int launch_rope(const void* x, int dt, int64_t x_batch, int64_t x_tok, int64_t x
     a.R = (int)R;
     a.half_layout = half_layout;
     a.conj = conj;
-    a.T = T;
-    if (dt == BI8_F32) return launch_type<float>(a, B * T, st);
-    return dt == BI8_BF16 ? launch_type<__nv_bfloat16>(a, B * T, st) : launch_type<__half>(a, B * T, st);
+    if (B * T > 0x7fffffff) return fail(BI8_ERR_LIMIT, "rope: %lld tokens exceed one launch", (long long)(B * T));
+    a.N = (int)(B * T);
+    a.per_batch = FastDiv(T);
+    if (dt == BI8_F32) return launch_type<float>(a, st);
+    return dt == BI8_BF16 ? launch_type<__nv_bfloat16>(a, st) : launch_type<__half>(a, st);
 }
 
 }  // namespace bi8

@@ -8,32 +8,56 @@
 // has P / 2 pairs of its own.  Neighbouring threads read neighbouring pieces.  Features that are not rotated come in two pieces as well.
 #pragma once
 
-#include "bi8_common.cuh"
+#include "int4_common.cuh"
 
 namespace bi8 {
 
-// P values of a type as floats, and back with one rounding.  P * sizeof(T) bytes are read at a time, up to 16.
 template <typename T>
-struct RopeType;
+struct RopeType {                        // the two 16-bit types: two values to a word
+    static constexpr int kPerWord = 2;
+    static __device__ __forceinline__ float get(uint32_t w, int i) { return i ? F16Bits<T>::hi(w) : F16Bits<T>::lo(w); }
+    static __device__ __forceinline__ uint32_t set(float a, float b) { return F16Bits<T>::pack(a, b); }
+};
 template <>
 struct RopeType<float> {
-    static __device__ __forceinline__ float get(float v) { return v; }
-    static __device__ __forceinline__ float set(float v) { return v; }
-};
-template <>
-struct RopeType<__nv_bfloat16> {
-    static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
-    static __device__ __forceinline__ __nv_bfloat16 set(float v) { return __float2bfloat16_rn(v); }
-};
-template <>
-struct RopeType<__half> {
-    static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
-    static __device__ __forceinline__ __half set(float v) { return __float2half_rn(v); }
+    static constexpr int kPerWord = 1;
+    static __device__ __forceinline__ float get(uint32_t w, int) { return __uint_as_float(w); }
+    static __device__ __forceinline__ uint32_t set(float a, float) { return __float_as_uint(a); }
 };
 
+// P values as they lie in memory, read and written 16 bytes at a time where they have as many.
 template <typename T, int P>
-struct alignas(sizeof(T) * P > 16 ? 16 : sizeof(T) * P) Piece {
-    T v[P];
+struct Piece {
+    static constexpr int kWords = P / RopeType<T>::kPerWord;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (kWords == 1) {
+            w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+        } else if constexpr (kWords == 2) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+            w[0] = v.x, w[1] = v.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 v = ld_nc_v4(p + i * RopeType<T>::kPerWord);
+                w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (kWords == 1) {
+            *reinterpret_cast<uint32_t*>(p) = w[0];
+        } else if constexpr (kWords == 2) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) *reinterpret_cast<uint4*>(p + i * RopeType<T>::kPerWord) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0u;
+    }
 };
 
 template <int P>
@@ -77,26 +101,33 @@ __device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
 
 template <typename T, int P>
 __device__ __forceinline__ void turn_pieces(Piece<T, P>& a, Piece<T, P>& b, const Angles<P>& g, bool half_layout) {
-    float x[P], y[P];
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-        x[j] = RopeType<T>::get(a.v[j]);
-        y[j] = RopeType<T>::get(b.v[j]);
-    }
+    using R = RopeType<T>;
+    constexpr int N = R::kPerWord;
     if (half_layout) {
 #pragma unroll
-        for (int j = 0; j < P; ++j) turn(x[j], y[j], g.c[j], g.s[j]);
+        for (int k = 0; k < P / N; ++k) {
+            float x[2] = {}, y[2] = {};
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                x[i] = R::get(a.w[k], i), y[i] = R::get(b.w[k], i);
+                turn(x[i], y[i], g.c[N * k + i], g.s[N * k + i]);
+            }
+            a.w[k] = R::set(x[0], x[1]);
+            b.w[k] = R::set(y[0], y[1]);
+        }
     } else {
 #pragma unroll
-        for (int j = 0; j < P / 2; ++j) {
-            turn(x[2 * j], x[2 * j + 1], g.c[j], g.s[j]);
-            turn(y[2 * j], y[2 * j + 1], g.c[P / 2 + j], g.s[P / 2 + j]);
-        }
-    }
+        for (int k = 0; k < P / 2; ++k) {                     // a pair of either piece
+            constexpr int STEP = 2 / N;
 #pragma unroll
-    for (int j = 0; j < P; ++j) {
-        a.v[j] = RopeType<T>::set(x[j]);
-        b.v[j] = RopeType<T>::set(y[j]);
+            for (int side = 0; side < 2; ++side) {
+                Piece<T, P>& p = side ? b : a;
+                float x = R::get(p.w[k * STEP], 0), y = R::get(p.w[k * STEP + STEP - 1], 1);
+                turn(x, y, g.c[side * (P / 2) + k], g.s[side * (P / 2) + k]);
+                p.w[k * STEP] = R::set(x, y);
+                if (N == 1) p.w[k * STEP + STEP - 1] = R::set(y, y);
+            }
+        }
     }
 }
 
