@@ -600,6 +600,7 @@ int launch_attention_paged(const void* q, int dt, int64_t q_tok, int64_t q_head,
     a.group = FastDiv(G);
     a.heads = FastDiv(Hkv);
     a.per_share = FastDiv(p.shares);
+    a.sequences = FastDiv(seq.B);
     a.per_sequence = FastDiv(seq.cu ? 1 : ((int64_t)seq.T * G + p.rows - 1) / p.rows);
     int rc = p.many ? launch_paged_many(a, dt, D, st) : launch_paged_few(a, dt, D, st);
     if (rc == BI8_OK && through_workspace(p)) rc = launch_paged_join(a.part, a.shares, out, dt, D, st);

@@ -16,7 +16,7 @@ struct PagedAttnArgs {
     int shares, tiles;
     float scale_log2;            // |scale| * log2(e), not 0
     uint32_t q_keep, q_flip;     // of two packed queries: bits to keep (none where the scale is 0) and signs to change
-    FastDiv group, heads, per_share, per_sequence;
+    FastDiv group, heads, per_share, per_sequence, sequences;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {

@@ -72,9 +72,15 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
     const uint32_t holder = base + Z::kMisc, abort_flag = holder + 4, zero_word = holder + 8;
 
     const int tile_head = (int)a.per_share.div(blockIdx.x), share = (int)blockIdx.x - tile_head * a.shares;
-    const int tile_index = (int)a.heads.div((unsigned)tile_head), h = tile_head - tile_index * a.Hkv;
+    const int turn = (int)a.heads.div((unsigned)tile_head), h = tile_head - turn * a.Hkv;
     after_predecessor();
     const Sequences& s = a.seq;
+    // A sequence's last tiles see the most rows: they go first, so that short ones fill what is left at the end.
+    int tile_index = a.tiles - 1 - turn;
+    if (!s.cu) {
+        const int before = (int)a.sequences.div((unsigned)turn);
+        tile_index = (turn - before * s.B) * (int)a.per_sequence.d + ((int)a.per_sequence.d - 1 - before);
+    }
     const QueryTile qt = find_tile(s, tile_index, a.G, TILES * kTileRows, a.per_sequence);
     if (qt.rows == 0) return;
     auto token_of = [&](int r) { return (int)a.group.div((unsigned)(qt.row0 + r)); };
@@ -83,13 +89,31 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
         return (int64_t)(qt.token0 + t) * a.Hq + h * a.G + (qt.row0 + r - t * a.G);
     };
 
+    // ---- the tiles' queries are on their way while the rest is found out: neighbouring threads have neighbouring pieces
+    constexpr int PIECES = D / 8, Q_ROWS = 128 / PIECES, Q_LOADS = PIECES < 16 ? PIECES : 16;
+    const int tiles = qt.rows > kTileRows ? 2 : 1, my_tile = warp / 4, q_row = (threadIdx.x & 127) / PIECES, q_piece = threadIdx.x % PIECES;
+    auto load_query = [&](int row) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        const int r = my_tile * kTileRows + row;
+        if (r < qt.rows) {
+            const int tok = token_of(r), head = h * a.G + (qt.row0 + r - tok * a.G);
+            v = ld_nc_v4(static_cast<const T*>(a.q) + (int64_t)(qt.token0 + tok) * a.q_tok + head * a.q_head + 8 * q_piece);
+        }
+        return v;
+    };
+    uint4 query[Q_LOADS];
+    if (my_tile < tiles && warp < MMA_WARP) {
+#pragma unroll
+        for (int i = 0; i < Q_LOADS; ++i) query[i] = load_query(q_row + i * Q_ROWS);
+    }
+
     // ---- rows of this share.  A tile takes as many shares as its rows fill.
     const int fewest = rows_seen(s, qt.b, qt.n, token_of(0)), most = rows_seen(s, qt.b, qt.n, token_of(qt.rows - 1));
     const int start = s.start(qt.b), origin = start & -box_rows, n_rows = most > start ? most - origin : 0;
     const int count = max(1, min(a.shares, n_rows / share_rows));
     const int chunk = (n_rows + count * KT - 1) / (count * KT) * KT;
     const int first = origin + min(n_rows, share * chunk), last = share < count ? min(origin + n_rows, first + chunk) : first;
-    const int steps = (last - first + KT - 1) / KT, tiles = qt.rows > kTileRows ? 2 : 1;
+    const int steps = (last - first + KT - 1) / KT;
     if (steps == 0) {                                         // nothing to see, or no such share
         for (int r = threadIdx.x; r < qt.rows; r += Z::kThreads) {
             if (a.shares > 1) a.part.stats[share * a.part.rows + query_at(r)] = make_float2(-INFINITY, count == 1 && share == 0 ? kWritten : 0.0f);
@@ -238,24 +262,17 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
         const int t = warp / 4, r = t * kTileRows + (threadIdx.x & 127);
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), out = lanes + (uint32_t)(Z::kOut + t * D);
         {
-            // the tile's queries, neighbouring threads neighbouring pieces, eight loads under way
-            constexpr int PIECES = D / 8, ROWS = 128 / PIECES;
-            const int row0 = (threadIdx.x & 127) / PIECES, p = threadIdx.x % PIECES;
+            auto store_query = [&](int row, const uint4& v) {
+                *reinterpret_cast<uint4*>(smem + t * Z::kQTile + (q_piece / 8) * kTileRows * 128 + row * 128 + (((q_piece % 8) ^ (row & 7)) << 4)) =
+                    make_uint4((v.x & a.q_keep) ^ a.q_flip, (v.y & a.q_keep) ^ a.q_flip, (v.z & a.q_keep) ^ a.q_flip, (v.w & a.q_keep) ^ a.q_flip);
+            };
 #pragma unroll
-            for (int i0 = 0; i0 < PIECES; i0 += 8) {
-                uint4 v[8];
+            for (int i = 0; i < Q_LOADS; ++i) store_query(q_row + i * Q_ROWS, query[i]);
+            if constexpr (PIECES > Q_LOADS) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int row = t * kTileRows + row0 + (i0 + i) * ROWS, tok = token_of(row), head = h * a.G + (qt.row0 + row - tok * a.G);
-                    v[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (row < qt.rows) v[i] = ld_nc_v4(static_cast<const T*>(a.q) + (int64_t)(qt.token0 + tok) * a.q_tok + head * a.q_head + 8 * p);
-                }
+                for (int i = 0; i < Q_LOADS; ++i) query[i] = load_query(q_row + (Q_LOADS + i) * Q_ROWS);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int row = row0 + (i0 + i) * ROWS;
-                    const uint4 w = make_uint4((v[i].x & a.q_keep) ^ a.q_flip, (v[i].y & a.q_keep) ^ a.q_flip, (v[i].z & a.q_keep) ^ a.q_flip, (v[i].w & a.q_keep) ^ a.q_flip);
-                    *reinterpret_cast<uint4*>(smem + t * Z::kQTile + (p / 8) * kTileRows * 128 + row * 128 + (((p % 8) ^ (row & 7)) << 4)) = w;
-                }
+                for (int i = 0; i < Q_LOADS; ++i) store_query(q_row + (Q_LOADS + i) * Q_ROWS, query[i]);
             }
             fence_proxy_async_smem();
             mbar_arrive(bar(Z::kQueries + t));
