@@ -29,7 +29,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kCols = 16;                // queries of a CTA
+constexpr int kCols = kFewQueries;       // queries of a CTA
 constexpr int kClusterShares = 8, kMaxShares = 128;
 constexpr int kSlots = 3;
 
@@ -73,10 +73,21 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int tile_head = (int)a.per_share.div(blockIdx.x), share = (int)blockIdx.x - tile_head * a.shares;
     const int tile = (int)a.heads.div((unsigned)tile_head), h = tile_head - tile * a.Hkv;
-    after_predecessor();
     const Sequences& s = a.seq;
-    const QueryTile qt = find_tile(s, tile, a.G, kCols, a.per_sequence);
-    if (qt.rows == 0) return;                                                    // the whole cluster's tile
+    QueryTile qt;
+    if (a.by_length) {
+        // Behind the kernel for many queries, which waits for what came before it when it begins: this one reads and writes nothing of that kernel's,
+        // takes the SMs that it leaves, and waits for it at its end.
+        const int first = s.first_token(tile), n = max(s.first_token(tile + 1) - first, 0);
+        qt = {tile, n, first, 0, (int64_t)n * a.G <= kCols ? n * a.G : 0};
+    } else {
+        after_predecessor();
+        qt = find_tile(s, tile, a.G, kCols, a.per_sequence);
+    }
+    if (qt.rows == 0) {                                                          // the whole cluster's tile
+        if (a.by_length) wait_predecessor();
+        return;
+    }
     auto token_of = [&](int r) { return (int)a.group.div((unsigned)(qt.row0 + r)); };
 
     // ---- rows of this share
@@ -309,6 +320,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
         const int t = token_of(col);
         return (int64_t)(qt.token0 + t) * a.Hq + h * a.G + (qt.row0 + col - t * a.G);
     };
+    if (a.mark && share == 0 && threadIdx.x < (unsigned)qt.rows) a.part.stats[query_at(threadIdx.x)] = make_float2(0.0f, kWritten);
     auto store = [&](int col, int d, float x, float y) {
         *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + query_at(col) * D + d) = F16Bits<T>::pack(x, y);
     };
@@ -318,6 +330,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
             const float total = cta_l[col], inv = total == 0.0f ? 0.0f : 1.0f / total;
             store(col, d, sums[col * D + d] * inv, sums[col * D + d + 1] * inv);
         }
+        if (a.by_length) wait_predecessor();
         return;
     }
     if (a.shares > kClusterShares) {
@@ -371,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
         store(col, d, x, y);
     }
     cluster.sync();                                       // the others read this CTA's sums
+    if (a.by_length) wait_predecessor();
 }
 
 // Joins the shares of one query: a CTA of four times D threads, a quarter of the shares each.
@@ -468,46 +482,46 @@ __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_few_kernel(const P
     for (int i = 0; i < V; i += 2) dst[i / 2] = F16Bits<T>::pack(x[i], x[i + 1]);
 }
 
-// (A row past two tiles takes 13 ns.)
-constexpr int64_t kSetUpRows = 600, kJoinRows = 80, kJoinRows0 = 200;
-
 struct Plan {
     bool many;
+    bool both;                   // sequences of few and of many queries in one batch: a kernel for each
     int rows;                    // queries of a tile
-    int64_t tiles, shares;
+    int64_t tiles, shares, few_shares;
 };
-Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len, bool packed) {
-    const int64_t G = Hq / Hkv, sms = sm_count();
-    Plan p{};
-    p.many = packed ? N > B && N * G > kCols * B : N / B * G > kCols;
-    p.rows = p.many ? paged_many_tile(D) : kCols;
-    p.tiles = tile_count(B, N, G, p.rows, packed);
-    const int64_t ctas = p.tiles * Hkv;
-    if (p.many) {
-        // A CTA an SM: the number of shares for which as many rounds of CTAs as it takes are shortest, a CTA's set-up counted as kSetUpRows and what
-        // the shares write and the join reads as rows that go by meanwhile.
-        const int64_t most = max_len / kShareRows < kFewShares ? max_len / kShareRows : kFewShares;
-        int64_t best = 0;
-        p.shares = 1;
-        for (int64_t s = 1; s <= most || s == 1; ++s) {
-            const int64_t rounds = (ctas * s + sms - 1) / sms, join = s > 1 ? s * N * Hq / kJoinRows + kJoinRows0 : 0;
-            const int64_t cost = rounds * (max_len / s + kSetUpRows) + join;
-            if (s == 1 || cost < best) best = cost, p.shares = s;
-        }
-        return p;
-    }
-    const int64_t step = 16 * (D == 64 ? kSubSteps<64> : D == 128 ? kSubSteps<128> : kSubSteps<256>);
+int64_t few_shares(int64_t ctas, int64_t D, int64_t max_len, int64_t most) {
+    const int64_t sms = sm_count(), step = 16 * (D == 64 ? kSubSteps<64> : D == 128 ? kSubSteps<128> : kSubSteps<256>);
     const int64_t useful = (max_len + kWarps * step - 1) / (kWarps * step), long_ones = max_len / 2048;
     int64_t want = (D == 256 ? kResident<256> : kResident<128>) * sms / ctas;
     if (want < kClusterShares && want < long_ones) want = long_ones < kClusterShares ? long_ones : kClusterShares;
     int64_t s = useful < want ? useful : want;
-    if (s > kMaxShares) s = kMaxShares;
-    if (s <= kClusterShares) {
+    if (s > most) s = most;
+    if (s < 2 * kClusterShares) {
         int64_t pow = 1;
-        while (pow * 2 <= s) pow *= 2;
+        while (pow * 2 <= s && pow < kClusterShares) pow *= 2;
         s = pow;
     }
-    p.shares = s < 1 ? 1 : s;
+    return s < 1 ? 1 : s;
+}
+Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len, bool packed) {
+    const int64_t G = Hq / Hkv;
+    Plan p{};
+    p.many = packed ? N > B && N * G > kCols * B : N / B * G > kCols;
+    p.both = packed && N > B && G <= kCols;
+    p.many = p.many || p.both;
+    p.rows = p.many ? paged_many_tile(D) : kCols;
+    p.tiles = tile_count(B, N, G, p.rows, packed);
+    p.few_shares = few_shares(p.both ? (B + 1) * Hkv : p.tiles * Hkv, D, max_len, p.both ? kClusterShares : kMaxShares);
+    p.shares = p.few_shares;
+    if (p.many) {
+        // A CTA an SM.  Rounds of CTAs that do not come out even cost little, since the SMs at work clock higher meanwhile; a share costs what it
+        // writes and the join reads.  (2048 tokens of 32 heads, D 128: 256 CTAs of 32768 rows 891 us in 1 share, 936 in 2, 946 in 4; 256 of 8192
+        // rows 227, 270, 287.  Heads of 256, 64 CTAs of 8192 rows: 149 us in 1, 90 in 2, 98 in 4.)  What may be tiles of few queries is not
+        // counted where those have a kernel of their own.
+        const int64_t ctas = (p.both ? N * G / p.rows + 1 : p.tiles) * Hkv, rows = max_len / kShareRows;
+        int64_t s = sm_count() / ctas;
+        if (s > rows) s = rows;
+        p.shares = s < 1 ? 1 : s > kMaxShares ? kMaxShares : s;
+    }
     return p;
 }
 bool through_workspace(const Plan& p) { return p.many ? p.shares > 1 : p.shares > kClusterShares; }
@@ -573,7 +587,7 @@ int launch_attention_paged(const void* q, int dt, int64_t q_tok, int64_t q_head,
                            int64_t Hq, int64_t D, void* workspace, cudaStream_t st) {
     const int64_t Hkv = cache->heads, G = Hq / Hkv;
     const Plan p = plan_of(seq.B, seq.N, Hq, Hkv, D, seq.max_len, seq.cu != nullptr);
-    if (p.tiles * Hkv * p.shares > 0x7fffffff || (int64_t)seq.N * Hq > 0x7fffffff)
+    if (p.tiles * Hkv * p.shares > 0x7fffffff || ((int64_t)seq.B + 1) * Hkv * p.few_shares > 0x7fffffff || (int64_t)seq.N * Hq > 0x7fffffff)
         return fail(BI8_ERR_LIMIT, "attention_paged: %lld queries exceed one launch", (long long)seq.N * Hq);
     if (cache->pages == 0) {                                  // whatever a query sees reads as zeros
         BI8_CUDA_TRY(cudaMemsetAsync(out, 0, (size_t)seq.N * Hq * D * 2, st));
@@ -592,19 +606,31 @@ int launch_attention_paged(const void* q, int dt, int64_t q_tok, int64_t q_head,
     a.Hq = (int)Hq;
     a.Hkv = (int)Hkv;
     a.G = (int)G;
-    a.shares = (int)p.shares;
-    a.tiles = (int)p.tiles;
     a.scale_log2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 0x1p-126f);       // never 0, which the infinities of unseen rows do not bear
     a.q_keep = scale == 0.0f ? 0u : 0xffffffffu;
     a.q_flip = scale < 0.0f ? 0x80008000u : 0u;
     a.group = FastDiv(G);
     a.heads = FastDiv(Hkv);
-    a.per_share = FastDiv(p.shares);
     a.sequences = FastDiv(seq.B);
-    a.per_sequence = FastDiv(seq.cu ? 1 : ((int64_t)seq.T * G + p.rows - 1) / p.rows);
-    int rc = p.many ? launch_paged_many(a, dt, D, st) : launch_paged_few(a, dt, D, st);
-    if (rc == BI8_OK && through_workspace(p)) rc = launch_paged_join(a.part, a.shares, out, dt, D, st);
-    return rc;
+    a.by_length = p.both;
+    const bool joined = through_workspace(p);
+    if (p.many) {
+        a.shares = (int)p.shares;
+        a.tiles = (int)p.tiles;
+        a.per_share = FastDiv(p.shares);
+        a.per_sequence = FastDiv(seq.cu ? 1 : ((int64_t)seq.T * G + p.rows - 1) / p.rows);
+        if (int rc = launch_paged_many(a, dt, D, st)) return rc;
+    }
+    if (!p.many || p.both) {
+        PagedAttnArgs f = a;
+        f.shares = (int)p.few_shares;
+        f.tiles = (int)(p.both ? seq.B + 1 : p.tiles);
+        f.mark = p.both && joined;
+        f.per_share = FastDiv(p.few_shares);
+        f.per_sequence = FastDiv(seq.cu ? 1 : ((int64_t)seq.T * G + kCols - 1) / kCols);
+        if (int rc = launch_paged_few(f, dt, D, st)) return rc;
+    }
+    return joined ? launch_paged_join(a.part, (int)p.shares, out, dt, D, st) : BI8_OK;
 }
 
 }  // namespace bi8

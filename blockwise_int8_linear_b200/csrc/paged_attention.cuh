@@ -14,6 +14,8 @@ struct PagedAttnArgs {
     Partials part;
     int Hq, Hkv, G;
     int shares, tiles;
+    bool by_length;              // both kernels run, each for its sequences: those of at most kFewQueries queries a cache head, and the others
+    bool mark;                   // the kernel for few queries tells the join that its results are in place
     float scale_log2;            // |scale| * log2(e), not 0
     uint32_t q_keep, q_flip;     // of two packed queries: bits to keep (none where the scale is 0) and signs to change
     FastDiv group, heads, per_share, per_sequence, sequences;
@@ -34,6 +36,7 @@ __device__ __forceinline__ int rows_seen(const Sequences& s, int b, int n, int t
 // The kernel for many queries gives a tile one share for as many rows of the cache.
 constexpr int kShareRows = 1024;
 int paged_many_tile(int64_t D);          // queries of one of its CTAs
+constexpr int kFewQueries = 16;
 int launch_paged_few(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st);
 int launch_paged_many(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st);
 

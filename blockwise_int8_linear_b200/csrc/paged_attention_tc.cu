@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
         tile_index = (turn - before * s.B) * (int)a.per_sequence.d + ((int)a.per_sequence.d - 1 - before);
     }
     const QueryTile qt = find_tile(s, tile_index, a.G, TILES * kTileRows, a.per_sequence);
-    if (qt.rows == 0) return;
+    if (qt.rows == 0 || (a.by_length && (int64_t)qt.n * a.G <= kFewQueries)) return;
     auto token_of = [&](int r) { return (int)a.group.div((unsigned)(qt.row0 + r)); };
     auto query_at = [&](int r) {                              // token * Hq + head
         const int t = token_of(r);
