@@ -15,7 +15,8 @@
 // memory; more than eight shares go through a workspace and a second kernel.  Every sum has a fixed order.
 //
 // Rows that a sequence does not have, or that come before its start, are not read: they are zeros in shared memory, so that whatever is in the
-// cache there, infinities and NaN among it, has no part in the products.
+// cache there, infinities and NaN among it, has no part in the products.  Those of rows that only some of the queries see take a way of their own
+// (paged_attention.cuh).
 #include "paged_attention.cuh"
 
 #include <cooperative_groups.h>
@@ -47,7 +48,7 @@ struct Smem {
     static constexpr int kRingBytes = kWarps * kSlots * kSlot, kSumBytes = (kWarps * kCols * kBuf + kCols * D) * 4;
     static constexpr int kQueries = kRingBytes > kSumBytes ? kRingBytes : kSumBytes;
     static constexpr int kStats = kQueries + kCols * kRow;
-    static constexpr int kBytes = kStats + (2 * kWarps + 2 + kClusterShares) * kCols * 4;
+    static constexpr int kNoted = kStats + (2 * kWarps + 2 + kClusterShares) * kCols * 4, kBytes = kNoted + 16;
 };
 
 __device__ __forceinline__ void load_matrices(uint32_t at, uint32_t (&r)[4]) {
@@ -142,6 +143,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
     };
 
     // ---- queries
+    unsigned* const noted = reinterpret_cast<unsigned*>(smem + L::kNoted);      // rows from `fewest` on with values that are not finite
+    if (threadIdx.x == 0) *noted = 0u;
     const uint32_t queries = (uint32_t)__cvta_generic_to_shared(smem + L::kQueries);
     for (int i = threadIdx.x; i < kCols * PIECES; i += kThreads) {
         const int r = i / PIECES, p = i % PIECES;
@@ -250,6 +253,19 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
             for (int d = 0; d < CHUNKS; ++d) {
                 uint32_t v[4];
                 load_matrices_transposed(at(slot + L::kV, 16 * i + mr + 8 * (mi & 1), 2 * d + (mi >> 1)), v);
+                if (MASKED && fewest < most) {            // this lane's values of rows 2c, 2c + 1 and 8 more
+                    constexpr uint32_t E = F16Bits<T>::kInf;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int row = step_base + 16 * i + 8 * (w & 1) + 2 * c + e;
+                            if (row >= fewest && ((v[w] >> (16 * e)) & 0x7fffu) >= E) {
+                                atomicOr(noted, 1u << (row - fewest));
+                                v[w] &= e ? 0x0000ffffu : 0xffff0000u;
+                            }
+                        }
+                }
                 mma16<T>(o[2 * d], hi[0], hi[1], hi[2], hi[3], v[0], v[1]);
                 mma16<T>(o[2 * d + 1], hi[0], hi[1], hi[2], hi[3], v[2], v[3]);
                 mma16<T>(o[2 * d], lo[0], lo[1], lo[2], lo[3], v[0], v[1]);
@@ -311,6 +327,12 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
         for (int w = 1; w < kWarps; ++w) {
             const float4 y = *reinterpret_cast<const float4*>(buf + (w * kCols + col) * BUF + d);
             x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        }
+        for (unsigned w = *noted; w; w &= w - 1) {
+            const int row = fewest + __ffs(w) - 1;
+            if (row >= rows_seen(s, qt.b, qt.n, token_of(col)) || row < start) continue;
+            float* const e = reinterpret_cast<float*>(&x);
+            for (int k = 0; k < 4; ++k) e[k] += not_finite<T>(a, pages, row, h, d + k);
         }
         *reinterpret_cast<float4*>(sums + col * D + d) = x;
     }

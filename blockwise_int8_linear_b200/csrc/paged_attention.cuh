@@ -37,6 +37,18 @@ __device__ __forceinline__ int rows_seen(const Sequences& s, int b, int n, int t
 constexpr int kShareRows = 1024;
 int paged_many_tile(int64_t D);          // queries of one of its CTAs
 constexpr int kFewQueries = 16;
+// Rows of the newest tokens are seen by some queries of a tile and not by others, and in a matrix product a weight of 0 times an infinity is none.  So
+// values that are not finite are taken out of those rows before the product (the row is noted, counted from the first that not all
+// queries see) and given to the queries that see them when the sums are done: what an infinite value times a positive weight adds is itself.
+template <typename T>
+__device__ __forceinline__ float not_finite(const PagedAttnArgs& a, const int* pages, int row, int h, int d) {      // that value, 0 for a finite one
+    const int in_table = (int)a.seq.page.div((unsigned)row), page = pages[in_table];
+    if (page < 0 || page >= a.cache.pages) return 0.0f;
+    const unsigned short* const v =
+        static_cast<const unsigned short*>(a.cache.v) + page * a.cache.v_page + h * a.cache.v_head + (int64_t)(row - in_table * (int)a.seq.page.d) * a.cache.v_row;
+    return (v[d] & 0x7fffu) >= F16Bits<T>::kInf ? F16Bits<T>::one(v[d]) : 0.0f;
+}
+
 int launch_paged_few(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st);
 int launch_paged_many(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st);
 

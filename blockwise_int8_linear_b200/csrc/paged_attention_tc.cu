@@ -3,7 +3,7 @@
 //
 // A CTA takes up to two tiles of 128 queries (tokens and the G heads that share a cache head, in that order) of one sequence and streams the sequence's
 // rows past them, kRows at a time.  One warp fetches k and v by TMA (boxes of as many rows as surely lie in one page, 128-byte swizzle), one
-// issues the products, and four warps a tile, one thread a query, do the softmax between them:
+// issues the products, two look after what v holds where it must not count, and four warps a tile, one thread a query, do the softmax:
 //   S = Q K^T    queries and keys from shared memory, scores in tensor memory
 //   P = 2^(c S - m)  by the query's thread, back into the scores' own tensor memory as 16-bit numbers
 //   O += P V     weights from tensor memory, values from shared memory as they lie (the contraction runs over their rows)
@@ -18,8 +18,9 @@
 // Weights are 16-bit numbers: a rounding of half a step each, at random, which leaves the result about as much error again as its own rounding.
 // (A second product with what they lose would cost half of the time again.)
 //
-// What a row holds that no query sees must not count: scores are masked, and v's rows before the start and behind the last one are
-// overwritten by zeros in shared memory before the product, since 0 times an infinity is none.
+// What a query does not see must not count: scores are masked, and v's rows before the start and behind the last one are overwritten by zeros in
+// shared memory before the product, since 0 times an infinity is none.  Infinities and NaN of rows that only some queries see take a way of
+// their own (paged_attention.cuh).
 #include "paged_attention.cuh"
 #include "tc_common.cuh"
 
@@ -40,16 +41,16 @@ struct Shape {
     static constexpr int kRows = D == 256 ? 64 : 128;                // of the cache at a time
     static constexpr int kStages = D == 64 ? 8 : 5;
     static constexpr int kAhead = kTiles == 1 ? 2 : 1;               // scores that are under way before the first weights are used
-    static constexpr int kWarps = kTiles == 2 ? 12 : 6, kThreads = 32 * kWarps;
+    static constexpr int kWarps = 4 * kTiles + 4, kThreads = 32 * kWarps;
     static constexpr int kQTile = kTileRows * D * 2, kStage = kRows * D * 2;
     static constexpr int kScores = 0, kOut = 2 * kRows;              // columns of tensor memory
     static constexpr int kColumns = 512;
     static_assert(kOut + kTiles * D <= kColumns, "tensor memory");
     // barriers
     static constexpr int kFull = 0, kEmpty = kStages, kScoresFull = 2 * kStages, kWeightsFull = kScoresFull + 2, kProductDone = kWeightsFull + 4,
-                         kQueries = kProductDone + 2, kEnd = kQueries + 2, kBarriers = kEnd + 1;
+                         kQueries = kProductDone + 2, kClean = kQueries + 2, kEnd = kClean + kStages, kBarriers = kEnd + 1;
     static constexpr int kStagesAt = kTiles * kQTile, kBarriersAt = kStagesAt + kStages * kStage, kMisc = kBarriersAt + 8 * kBarriers;
-    static constexpr int kBytes = kMisc + 16 + 1024;                 // tensor memory's address, abort flag, a word that stays zero; alignment
+    static constexpr int kNoted = kMisc + 16, kBytes = kNoted + 32 + 1024;     // tensor memory's address, abort flag, a word that stays zero; rows noted; alignment
 };
 
 struct Shares {
@@ -135,6 +136,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
             for (int i = 0; i < Z::kStages; ++i) {
                 mbar_init(bar(Z::kFull + i), 1);
                 mbar_init(bar(Z::kEmpty + i), 1);
+                mbar_init(bar(Z::kClean + i), 2);
             }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(bar(Z::kScoresFull + i), 1);
@@ -146,6 +148,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
             mbar_init(bar(Z::kEnd), 1);
             mbar_fence_init();
         }
+        if (lane < 8) sts_u32(base + Z::kNoted + 4 * lane, 0u);
     }
     tc_fence_before();
     __syncthreads();
@@ -224,6 +227,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
             for (int j = 0; j < steps && ok; ++j) {
                 const int ov = order_v(j), ahead = j + Z::kAhead, ok_order = order_k(ahead);
                 wait_stage(ov);
+                const int at = first + j * KT;
+                if (at < start || at + KT > min(last, fewest)) wait(Z::kClean + j % Z::kStages, (j / Z::kStages) & 1, W_FULL_AB);
                 for (int t = 0; t < tiles && ok; ++t) {
                     const int buf = TILES == 2 ? t : j & 1;
                     const uint32_t v = stage_at(ov % Z::kStages);
@@ -254,6 +259,46 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
             }
         }
         __syncwarp();
+    } else {
+        // ---- v's rows that nobody sees become zeros, and those that only some of the queries see are looked through
+        const int me = threadIdx.x - 32 * (LOAD_WARP + 1), row0 = me >> 3;
+        bool ok = true;
+        for (int j = 0; j < steps && ok; ++j) {
+            const int order = order_v(j), stage = order % Z::kStages, at = first + j * KT;
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kFull + stage), (uint32_t)(order / Z::kStages) & 1u, abort_flag, wait_limit));
+            if (!ok) {
+                if (lane == 0) report_timeout(status, abort_flag, W_FULL_AB);
+                break;
+            }
+            if (at < start || at + KT > min(last, fewest)) {
+                uint8_t* const v = smem + Z::kStagesAt + stage * Z::kStage;
+                constexpr int LOOKS = 8 * KT / 64;
+                uint32_t largest = 0u;
+#pragma unroll
+                for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll 8
+                    for (int i = 0; i < LOOKS; ++i) {
+                        uint4* const piece = reinterpret_cast<uint4*>(v + c * KT * 128 + (me + 64 * i) * 16);
+                        const int row = at + row0 + 8 * i;
+                        if (row < start || row >= last) *piece = make_uint4(0u, 0u, 0u, 0u);
+                        else if (row >= fewest) largest = max(largest, absmax8(*piece));
+                    }
+                if (__any_sync(0xffffffffu, largest >= F16Bits<T>::kInf)) {
+                    for (int i = me; i < CHUNKS * 8 * KT; i += 64) {
+                        uint4* const piece = reinterpret_cast<uint4*>(v + i * 16);
+                        const int row = at + (i >> 3) % KT;
+                        if (row < fewest || absmax8(*piece) < F16Bits<T>::kInf) continue;
+                        atomicOr(reinterpret_cast<unsigned*>(smem + Z::kNoted) + ((row - fewest) >> 5), 1u << ((row - fewest) & 31));
+                        unsigned short* const value = reinterpret_cast<unsigned short*>(piece);
+                        for (int e = 0; e < 8; ++e)
+                            if ((value[e] & 0x7fffu) >= F16Bits<T>::kInf) value[e] = 0;
+                    }
+                }
+                fence_proxy_async_smem();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(Z::kClean + j % Z::kStages));      // v may be in any place, so these go by steps
+        }
     }
     } else {
         if constexpr (TILES == 2) setmaxnreg_inc<kSoftmaxRegisters>();
@@ -287,19 +332,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
         for (int j = 0; j < steps; ++j) {
             const int buf = TILES == 2 ? t : j & 1, at = first + j * KT;
             const uint32_t scores = lanes + (uint32_t)(Z::kScores + buf * KT);
-            const bool edge = at < start || at + KT > last;
-            if (edge) {                                       // v's rows that nobody sees
-                const int order = order_v(j);
-                ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kFull + order % Z::kStages), (uint32_t)(order / Z::kStages) & 1u, abort_flag, wait_limit));
-                if (ok) {
-                    uint8_t* const v = smem + Z::kStagesAt + (order % Z::kStages) * Z::kStage;
-                    for (int i = threadIdx.x & 127; i < KT * CHUNKS * 8; i += 128) {
-                        const int row = (i >> 3) % KT;
-                        if (at + row < start || at + row >= last) *reinterpret_cast<uint4*>(v + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async_smem();
-                }
-            }
+            const bool masked = at < start || at + KT > unmasked;
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kScoresFull + buf), TILES == 2 ? j & 1 : (j >> 1) & 1, abort_flag, wait_limit));
             if (!ok) {
                 if (lane == 0) report_timeout(status, abort_flag, W_ACC_FULL);
@@ -310,7 +343,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
 #pragma unroll
             for (int i = 0; i < KT; i += 32) tmem_ld32(scores + (uint32_t)i, *reinterpret_cast<uint32_t(*)[32]>(x + i));
             tmem_wait_ld();
-            if (at < start || at + KT > unmasked) {
+            if (masked) {
 #pragma unroll
                 for (int i = 0; i < KT; ++i)
                     if (at + i >= limit || at + i < start) x[i] = 0xff800000u;
@@ -405,6 +438,18 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
             if (live && a.shares > 1)
                 a.part.stats[share * a.part.rows + query_at(r)] = whole ? make_float2(0.0f, kWritten) : make_float2(m == -INFINITY ? m : shift, total);
+            unsigned noted[8], any = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) any |= noted[i] = lds_volatile_u32(base + Z::kNoted + 4 * i);
+            auto add_noted = [&](uint32_t (&o)[32], int d) {
+                const int* const table = s.pages + (qt.b < s.B ? qt.b : 0) * s.pages_step;
+                for (int i = 0; i < 8; ++i)
+                    for (unsigned w = noted[i]; w; w &= w - 1) {
+                        const int row = fewest + 32 * i + __ffs(w) - 1;
+                        if (!live || row >= limit || row < start) continue;
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + not_finite<T>(a, table, row, h, d + e));
+                    }
+            };
             // by way of the queries' place, 256 bytes of a row at a time (128 with 64 features), so that rows are written whole
             constexpr int PASS = D == 64 ? 128 : 256, LANES = PASS / 16, ROWS = 128 / LANES;
             uint8_t* const place = smem + t * Z::kQTile;
@@ -431,6 +476,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                         uint32_t o[32];
                         tmem_ld32(out + (uint32_t)(pass * (PASS / 2) + d), o);
                         tmem_wait_ld();
+                        if (any) add_noted(o, pass * (PASS / 2) + d);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             uint32_t w[4];
@@ -447,6 +493,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                         uint32_t o[32];
                         tmem_ld32(out + (uint32_t)(pass * (PASS / 4) + d), o);
                         tmem_wait_ld();
+                        if (any) add_noted(o, pass * (PASS / 4) + d);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(row + (((d / 4 + i) ^ (mine & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }

@@ -169,9 +169,9 @@ def attention_paged_cache(q: torch.Tensor, cache: PagedKVCache, pages: torch.Ten
     its prompt and another a single token.
 
     The query of a sequence's token i of n sees the rows up to ``lengths - n + i``, its own.  ``starts`` (as ``lengths``): the first row that is seen.  A
-    query that sees no row gives zeros, as do tokens that belong to nobody; rows that no query of a sequence sees may hold anything.  A page number that
-    is none of the cache's reads as a page of zeros.  Keys of 2^100 and more may overflow in the scores, which are fp32.  ``scale`` is a number of at most
-    2e38, by default ``1 / sqrt(D)``."""
+    query that sees no row gives zeros, as do tokens that belong to nobody; rows that it does not see may hold anything.  Infinite values that it sees
+    give nothing finite in their feature.  A page number that is none of the cache's reads as a page of zeros.  Keys of 2^100 and more may overflow in the
+    scores, which are fp32.  ``scale`` is a number of at most 2e38, by default ``1 / sqrt(D)``."""
     if scale is None:
         scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     return _lib.native().attention_paged(q, cache.k, cache.v, pages, lengths, cu_tokens, starts, scale)

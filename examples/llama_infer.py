@@ -42,8 +42,9 @@ if ROOT not in sys.path:
 
 import block_linear_config as cfg  # noqa: E402
 from block_linear import BlockInt4Linear, BlockInt8Linear  # noqa: E402
-from blockwise_int8_linear_b200.decode_ops import (attention_int4_cache, int4_kv_cache, rope_cache_append,  # noqa: E402
-                                                   rope_cache_append_int4)
+from blockwise_int8_linear_b200.decode_ops import (attention_int4_cache, attention_paged_cache, int4_kv_cache,  # noqa: E402
+                                                   paged_kv_cache, rope_cache_append, rope_cache_append_int4,
+                                                   rope_cache_append_paged)
 from blockwise_int8_linear_b200.parallel import block_aligned_bounds  # noqa: E402
 from triton_functions import pre_quantize_matmul_block_rowwise_dequantize  # noqa: E402
 
@@ -174,6 +175,7 @@ class Int8Linear(nn.Module):
 
 
 NORM_EPS = 1e-5
+PAGE = 64        # rows of a page of the paged cache
 FUSE = True      # producer steps and residual sums inside the library's calls (Int8Linear.fused); --no-fuse runs them as torch kernels
 
 
@@ -207,7 +209,7 @@ class Layer(nn.Module):
         self.heads_local = self.qkv.widths[0] // a.head_dim
         self.head_dim = a.head_dim
         self.kcache = self.vcache = None
-        self.int4_cache, self.cache = getattr(a, "cache", "bf16") == "int4", None
+        self.cache_kind, self.cache, self.pages = getattr(a, "cache", "bf16"), None, None
 
     def attn_partial(self, x, pos0, max_len, cis, mask=None, pos_dev=None, summed=False, residual=None):
         """Attention half of the layer up to the output projection; without `residual` also without the sum over ranks
@@ -218,7 +220,17 @@ class Layer(nn.Module):
         B, T, _ = x.shape
         hl, hd = self.heads_local, self.head_dim
         qkv = self.qkv.fused(x, "rmsnorm").view(B, T, 3, hl, hd)
-        if self.int4_cache:
+        if self.cache_kind == "paged":
+            # prompt and decode alike: the new tokens of all sequences, packed, are rotated and go to their pages, and see what those have
+            if self.cache is None:
+                width = -(-max_len // PAGE)
+                self.cache = paged_kv_cache(B * width, hl, PAGE, hd, x.dtype, x.device)
+                self.pages = torch.arange(B * width, device=x.device, dtype=torch.int32).view(B, width)
+            lengths = torch.full((1,), pos0 + T, device=x.device, dtype=torch.long) if pos_dev is None else pos_dev + T
+            q = rope_cache_append_paged(qkv.view(B * T, 3 * hl, hd), cis, self.cache, self.pages, lengths)
+            att = attention_paged_cache(q, self.cache, self.pages, lengths).view(B, T, hl * hd)
+            return self.project(att, summed, residual)
+        if self.cache_kind == "int4":
             # prompt and decode alike: rotation, quantization and append in one launch, attention over what the cache then has; `cis`
             # holds the factors of all positions
             if self.cache is None:
@@ -294,13 +306,13 @@ class Llama(nn.Module):
         self.emb = (torch.randn((a.vocab, a.hidden), device=dev, generator=g) * 0.02).to(torch.bfloat16)
         self.layers = nn.ModuleList(Layer(i, a, dev, rank, world, ops) for i in range(a.layers))
         self.head = Int8Linear(a.hidden, (a.vocab,), (99,), dev, "col", rank, world, a.block, ops, getattr(a, "weights", "int8"))
-        self.int4_cache = getattr(a, "cache", "bf16") == "int4"
+        self.all_angles = getattr(a, "cache", "bf16") in ("int4", "paged")
         self.world, self.vocab, self.block = world, a.vocab, a.block
         self.cis = rope_table(a.prompt + a.decode + 16, a.head_dim, dev)
         self.positions = torch.arange(a.prompt + a.decode + 16, device=dev)
 
     def positions_of(self, ids, pos0, max_len, pos_dev):
-        if self.int4_cache:
+        if self.all_angles:
             return self.cis, None                                  # the kernels look up their positions themselves
         if pos_dev is None:
             return self.cis[pos0:pos0 + ids.shape[1]], None
@@ -545,7 +557,8 @@ def main():
     ap.add_argument("--no-fuse", dest="no_fuse", action="store_true",
                     help="run the normalisations, the gated activation and the residual sums as separate torch kernels")
     ap.add_argument("--weights", choices=["int8", "int4"], default="int8", help="hold the weights in 8-bit or in 4-bit blocks")
-    ap.add_argument("--cache", choices=["bf16", "int4"], default="bf16", help="hold keys and values in bf16 or in 4-bit blocks")
+    ap.add_argument("--cache", choices=["bf16", "int4", "paged"], default="bf16",
+                    help="hold keys and values in bf16, in 4-bit blocks, or in bf16 pages")
     ap.add_argument("--out", default=None, help="also append the JSON line to this file")
     a = ap.parse_args()
     a.head_dim = a.hidden // a.heads

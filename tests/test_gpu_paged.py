@@ -216,6 +216,29 @@ def test_infinities_and_nan_of_a_sequence_are_its_own(tokens):
     assert torch.equal(last[..., others], clean[2 * tokens:][..., others])
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d, tokens, length", [(64, 3, 40), (128, 2, 5), (256, 4, 1000), (64, 40, 40), (128, 300, 300), (128, 90, 4000), (256, 70, 200), (64, 16, 3000)])
+def test_infinities_and_nan_of_later_tokens_reach_no_earlier_query(d, tokens, length, dtype):
+    """Keys and values of some of the new tokens are infinite or NaN: queries before them notice nothing, those that see them do."""
+    b = Batch([length, length], [tokens, tokens], 1, d, 16, dtype, 51)
+    q = _randn((b.n, 2, d), 52, dtype)
+    clean = b.attend(q)
+    at = lambda seq, row: (b.pages[seq, row // 16], 0, row % 16)
+    first = length - tokens
+    bad = {first + tokens // 2: (3, math.inf), first + tokens - 1: (d - 1, math.nan), first + tokens // 3: (17, -math.inf)}
+    for row, (feature, value) in bad.items():
+        b.cache.v[at(0, row)][feature] = value
+    b.cache.k[at(1, length - 1)][5] = math.nan
+    got = b.attend(q)
+    for i in range(tokens):
+        hit = [f for row, (f, _) in bad.items() if row <= first + i]
+        others = [f for f in range(d) if f not in hit]
+        assert torch.equal(got[i][:, others], clean[i][:, others])
+        assert not got[i][:, hit].isfinite().any()
+    assert torch.equal(got[tokens:-1], clean[tokens:-1]) and got[-1].isnan().all()
+    assert_clean_device()
+
+
 LAYOUTS = {
     "rows before heads": lambda p, h, r, d: tuple(torch.empty((p, r, h, d), device=DEV, dtype=BF).transpose(1, 2) for _ in range(2)),
     "one tensor": lambda p, h, r, d: torch.empty((p, 2, h, r, d), device=DEV, dtype=BF).unbind(1),
