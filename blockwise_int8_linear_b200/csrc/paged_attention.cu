@@ -91,6 +91,20 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
     }
     auto token_of = [&](int r) { return (int)a.group.div((unsigned)(qt.row0 + r)); };
 
+    // ---- queries, on their way while the rest is found out
+    constexpr int Q_LOADS = kCols * PIECES / kThreads;
+    const int q_piece = threadIdx.x % PIECES;
+    uint4 query[Q_LOADS];
+#pragma unroll
+    for (int i = 0; i < Q_LOADS; ++i) {
+        const int r = (int)threadIdx.x / PIECES + i * (kThreads / PIECES);
+        query[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < qt.rows) {
+            const int t = token_of(r), head = h * a.G + (qt.row0 + r - t * a.G);
+            query[i] = ld_nc_v4(static_cast<const T*>(a.q) + (int64_t)(qt.token0 + t) * a.q_tok + head * a.q_head + 8 * q_piece);
+        }
+    }
+
     // ---- rows of this share
     const int fewest = rows_seen(s, qt.b, qt.n, token_of(0)), most = rows_seen(s, qt.b, qt.n, token_of(qt.rows - 1));
     const int start = s.start(qt.b), origin = start & ~15, n_rows = most > start ? most - origin : 0;
@@ -114,6 +128,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kSlots * L::kSlot);
     constexpr int AT_ONCE = 32 / PIECES == 0 ? 1 : 32 / PIECES;                 // rows of a warp's access
     const int row0 = lane / PIECES, piece = lane % PIECES;
+    constexpr int AHEAD = kWarps * STEP;
     struct Pages {
         int number[TT];
     };
@@ -142,28 +157,23 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
         }
     };
 
-    // ---- queries
     unsigned* const noted = reinterpret_cast<unsigned*>(smem + L::kNoted);      // rows from `fewest` on with values that are not finite
     if (threadIdx.x == 0) *noted = 0u;
     const uint32_t queries = (uint32_t)__cvta_generic_to_shared(smem + L::kQueries);
-    for (int i = threadIdx.x; i < kCols * PIECES; i += kThreads) {
-        const int r = i / PIECES, p = i % PIECES;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < qt.rows) {
-            const int t = token_of(r), head = h * a.G + (qt.row0 + r - t * a.G);
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(qt.token0 + t) * a.q_tok + head * a.q_head + 8 * p);
-            v = make_uint4((v.x & a.q_keep) ^ a.q_flip, (v.y & a.q_keep) ^ a.q_flip, (v.z & a.q_keep) ^ a.q_flip, (v.w & a.q_keep) ^ a.q_flip);
-        }
-        *reinterpret_cast<uint4*>(smem + L::kQueries + r * L::kRow + 16 * (p ^ (r & 7))) = v;
-    }
     int base = first + warp * STEP;
-    constexpr int AHEAD = kWarps * STEP;
 #pragma unroll
     for (int i = 0; i < kSlots - 1; ++i) {
         if (base + i * AHEAD < last) fill(ring + i * L::kSlot, base + i * AHEAD, pages_of(base + i * AHEAD));
         commit_copies();
     }
     Pages next = pages_of(base + (kSlots - 1) * AHEAD);
+#pragma unroll
+    for (int i = 0; i < Q_LOADS; ++i) {
+        const int r = (int)threadIdx.x / PIECES + i * (kThreads / PIECES);
+        const uint4 v = query[i];
+        *reinterpret_cast<uint4*>(smem + L::kQueries + r * L::kRow + 16 * (q_piece ^ (r & 7))) =
+            make_uint4((v.x & a.q_keep) ^ a.q_flip, (v.y & a.q_keep) ^ a.q_flip, (v.z & a.q_keep) ^ a.q_flip, (v.w & a.q_keep) ^ a.q_flip);
+    }
     __syncthreads();
 
     // lane's row and piece of the matrices that it gives the address of: queries (16 rows, 2 pieces), k (16 rows, 2 pieces, rows first), v
@@ -316,8 +326,9 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
         const int col = g + 8 * r;
         const float w = m[r] == -INFINITY ? 0.0f : exp2_fast(m[r] - cta_m[col]);
         float* const dst = buf + (warp * kCols + col) * BUF + 2 * c;
+        if (col < qt.rows)
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(dst + 8 * d) = make_float2(o[d][2 * r] * w, o[d][2 * r + 1] * w);
+            for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(dst + 8 * d) = make_float2(o[d][2 * r] * w, o[d][2 * r + 1] * w);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < qt.rows * (D / 4); i += kThreads) {
