@@ -32,16 +32,16 @@ namespace cg = cooperative_groups;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kCols = kFewQueries;       // queries of a CTA
 constexpr int kClusterShares = 8, kMaxShares = 128;
-constexpr int kSlots = 3;
+constexpr int kSingleRound = 2;          // CTAs of an SM where more shares than a cluster's make one round of CTAs (few_shares): with a step more on its way in each warp
 
 template <int D>
 constexpr int kSubSteps = D == 64 ? 2 : 1;          // 16 rows each
 template <int D>
-constexpr int kResident = D == 256 ? 1 : 2;         // CTAs of an SM
+constexpr int kResident = D == 256 ? 1 : 3;         // CTAs of an SM
 
 // Shared memory: the warps' rings (k and v of a step in each slot), afterwards the warps' sums and the CTA's; queries; statistics.  The 16-byte
 // pieces of a row are permuted by the row's number, so that the eight rows of a matrix lie in different banks.
-template <int D>
+template <int D, int kSlots>
 struct Smem {
     static constexpr int kStep = 16 * kSubSteps<D>, kRow = 2 * D, kV = kStep * kRow, kSlot = 2 * kV;
     static constexpr int kBuf = D + 4;                                   // a sum's row in floats
@@ -58,9 +58,9 @@ __device__ __forceinline__ void load_matrices_transposed(uint32_t at, uint32_t (
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const PagedAttnArgs a) {
-    using L = Smem<D>;
+template <typename T, int D, int kSlots>
+__global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kResident<D>) paged_few_kernel(const PagedAttnArgs a) {
+    using L = Smem<D, kSlots>;
     constexpr int TT = kSubSteps<D>, STEP = L::kStep, PIECES = D / 8, CHUNKS = D / 16, BUF = L::kBuf;
     extern __shared__ __align__(128) uint8_t smem[];
     float* const warp_m = reinterpret_cast<float*>(smem + L::kStats);            // [kWarps][kCols]
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) paged_few_kernel(const
     // lane's row and piece of the matrices that it gives the address of: queries (16 rows, 2 pieces), k (16 rows, 2 pieces, rows first), v
     const int mi = lane >> 3, mr = lane & 7;
     auto at = [&](uint32_t from, int row, int p) { return from + row * L::kRow + 16 * (p ^ (row & 7)); };
-    constexpr bool KEEP_Q = D <= 128;
+    constexpr bool KEEP_Q = D == 64 || (D == 128 && kSlots == 3);      // else they are read again in every step: three CTAs an SM have 168 registers a thread
     uint32_t q[KEEP_Q ? CHUNKS : 1][4];
     if (KEEP_Q) {
 #pragma unroll
@@ -521,19 +521,27 @@ struct Plan {
     int rows;                    // queries of a tile
     int64_t tiles, shares, few_shares;
 };
+// How many shares the rows are divided into, for the kernel of few queries.  Time is counted in rows of a CTA among as many as the SMs hold (36 ns at
+// D 128): a round of CTAs takes a share's rows and kSetUp more (latency until the first rows are there, and the join), a last round that is not full its part, but
+// no less than kAlone, because few CTAs cannot draw all of the memory's bandwidth.  (D 128, us: 16 sequences of 8192 rows on 8 heads in 1, 2, 3, 4, 5, 6
+// shares: 124, 107, 111, 133, 117, 111; 32 of 4096: 104, 134, 105, 117, 122, 118; 100 of 1000: 87, 94, 103.)  Long tables, whose sequences may
+// differ much in length, have shares of 2048 rows at most (32 sequences of 1 to 8192 rows: 174, 109, 107, 101, 100, 101), more than a cluster's eight a
+// second kernel.  Those are few sequences, one round of CTAs at most: two an SM, which come out even (131072 rows, 8 heads: 296 CTAs 88 to 90 us, 440 of
+// three an SM 93 to 104).
 int64_t few_shares(int64_t ctas, int64_t D, int64_t max_len, int64_t most) {
-    const int64_t sms = sm_count(), step = 16 * (D == 64 ? kSubSteps<64> : D == 128 ? kSubSteps<128> : kSubSteps<256>);
-    const int64_t useful = (max_len + kWarps * step - 1) / (kWarps * step), long_ones = max_len / 2048;
-    int64_t want = (D == 256 ? kResident<256> : kResident<128>) * sms / ctas;
-    if (want < kClusterShares && want < long_ones) want = long_ones < kClusterShares ? long_ones : kClusterShares;
-    int64_t s = useful < want ? useful : want;
-    if (s > most) s = most;
-    if (s < 2 * kClusterShares) {
-        int64_t pow = 1;
-        while (pow * 2 <= s && pow < kClusterShares) pow *= 2;
-        s = pow;
+    const int64_t step = kWarps * 16 * (D == 64 ? kSubSteps<64> : D == 128 ? kSubSteps<128> : kSubSteps<256>);
+    const int64_t sms = sm_count(), set_up = 12800 / D;
+    const int64_t useful = (max_len + step - 1) / step, least = max_len / 2048;
+    int64_t best = 1, best_cost = 0;
+    for (int64_t s = least < 1 ? 1 : least > kClusterShares ? kClusterShares : least; s <= most && (s <= useful || s == 1); ++s) {
+        const int64_t slots = sms * (D == 256 ? 1 : s > kClusterShares ? kSingleRound : kResident<128>), alone = (D == 256 ? 80 : 45) * slots / 100;
+        const int64_t n = ctas * s, left = n % slots;
+        const int64_t rounds = n / slots * slots + (left == 0 ? 0 : s > kClusterShares ? slots : left < alone ? alone : left);
+        const int64_t cost = rounds * (max_len / s + set_up) + (s > kClusterShares ? slots * set_up : 0);
+        if (best_cost == 0 || cost < best_cost) best = s, best_cost = cost;
+        if (n > 16 * slots) break;
     }
-    return s < 1 ? 1 : s;
+    return best < most ? best : most;
 }
 Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len, bool packed) {
     const int64_t G = Hq / Hkv;
@@ -559,11 +567,11 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
 }
 bool through_workspace(const Plan& p) { return p.many ? p.shares > 1 : p.shares > kClusterShares; }
 
-template <typename T, int D>
-int launch(const PagedAttnArgs& a, cudaStream_t st) {
-    constexpr int smem = Smem<D>::kBytes;
+template <typename T, int D, int SLOTS>
+int launch_slots(const PagedAttnArgs& a, cudaStream_t st) {
+    constexpr int smem = Smem<D, SLOTS>::kBytes;
     static SmemOptIn opt_in;
-    if (int rc = opt_in.ensure(paged_few_kernel<T, D>, smem)) return rc;
+    if (int rc = opt_in.ensure(paged_few_kernel<T, D, SLOTS>, smem)) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)((int64_t)a.tiles * a.Hkv * a.shares));
     cfg.blockDim = dim3(kThreads);
@@ -577,8 +585,14 @@ int launch(const PagedAttnArgs& a, cudaStream_t st) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    BI8_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_few_kernel<T, D>, a));
+    BI8_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_few_kernel<T, D, SLOTS>, a));
     return BI8_OK;
+}
+template <typename T, int D>
+int launch(const PagedAttnArgs& a, cudaStream_t st) {
+    if constexpr (D != 256)
+        if (a.shares > kClusterShares) return launch_slots<T, D, 3>(a, st);
+    return launch_slots<T, D, 2>(a, st);
 }
 
 template <typename T>

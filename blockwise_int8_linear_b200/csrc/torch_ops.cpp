@@ -1201,15 +1201,16 @@ Tensor rope(const Tensor& x, const Tensor& cis, const Tensor& positions, int64_t
 bool values_apart(const Tensor& k, const Tensor& v) {
     if (k.numel() == 0 || v.numel() == 0) return true;
     auto nested = [](const Tensor& t, int64_t other, int64_t* extent) {
-        std::vector<std::pair<int64_t, int64_t>> dims;       // step, count
+        std::pair<int64_t, int64_t> dims[4];                 // step, count
+        int count = 0;
         for (int i = 0; i < 3; ++i)
-            if (t.size(i) > 1) dims.push_back({t.stride(i), t.size(i)});
-        if (other > 0) dims.push_back({other, 2});
-        std::sort(dims.begin(), dims.end());
+            if (t.size(i) > 1) dims[count++] = {t.stride(i), t.size(i)};
+        if (other > 0) dims[count++] = {other, 2};
+        std::sort(dims, dims + count);
         int64_t reach = t.size(3);
-        for (const auto& [step, n] : dims) {
-            if (step < reach) return false;
-            reach += step * (n - 1);
+        for (int i = 0; i < count; ++i) {
+            if (dims[i].first < reach) return false;
+            reach += dims[i].first * (dims[i].second - 1);
         }
         *extent = reach;
         return true;
