@@ -227,8 +227,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
             for (int j = 0; j < steps && ok; ++j) {
                 const int ov = order_v(j), ahead = j + Z::kAhead, ok_order = order_k(ahead);
                 wait_stage(ov);
-                const int at = first + j * KT;
-                if (at < start || at + KT > min(last, fewest)) wait(Z::kClean + j % Z::kStages, (j / Z::kStages) & 1, W_FULL_AB);
+                // in every step, so that the warps that look after v are never a round of stages behind
+                wait(Z::kClean + j % Z::kStages, (j / Z::kStages) & 1, W_FULL_AB);
                 for (int t = 0; t < tiles && ok; ++t) {
                     const int buf = TILES == 2 ? t : j & 1;
                     const uint32_t v = stage_at(ov % Z::kStages);

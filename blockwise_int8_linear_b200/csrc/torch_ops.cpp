@@ -1107,7 +1107,7 @@ struct Angles {
         if ((!cplx && cis.scalar_type() != at::kFloat) || cis.dim() != (cplx ? 2 : 3) || (!cplx && cis.size(2) != 2))
             value_error(std::string("cis must hold [rows, pairs] (cos, sin) float32 pairs, got ") + c10::toString(cis.scalar_type()) + " " + shape_of(cis));
         same_device(cis, like, "cis");
-        owner = cis.is_conj() ? cis.resolve_conj().contiguous() : cis.contiguous();
+        owner = cis.resolve_conj().resolve_neg().contiguous();
         if (owner.numel() > 0 && !aligned16(owner)) owner = owner.clone();
         ptr = static_cast<const float*>(owner.data_ptr());
         rows = cis.size(0);
@@ -1150,7 +1150,7 @@ Tensor rope_values(const Tensor& x_in, const Tensor& cis, const Tensor& position
     at::AutoDispatchBelowADInplaceOrView below_autograd;
     OnDevice on(x_in);
     const Angles angles(cis, x_in);
-    const Tensor x = x_in.size(-1) > 1 && x_in.stride(-1) != 1 ? x_in.contiguous() : x_in;
+    const Tensor plain = x_in.resolve_neg(), x = plain.size(-1) > 1 && plain.stride(-1) != 1 ? plain.contiguous() : plain;
     const int lead = (int)x.dim() - 3;
     const int64_t b = lead ? x.size(0) : 1, t = x.size(lead), h = x.size(lead + 1), d = x.size(lead + 2);
     const int64_t pos_tok = positions.defined() && t > 1 ? positions.stride(-1) : 0;
@@ -1232,6 +1232,7 @@ bi8_paged_cache paged_cache(const Tensor& k, const Tensor& v, const Tensor& like
             (d > 1 && t->stride(3) != 1))
             value_error(std::string("cache pages must be ") + c10::toString(like.scalar_type()) + " [pages, heads, rows, " + std::to_string(d) +
                         "] with dense features on " + like.device().str() + ", keys and values alike, got " + c10::toString(t->scalar_type()) + " " + shape_of(*t));
+    if (k.is_neg() || v.is_neg()) value_error("a cache must hold its values as they are, not negated ones of another tensor");
     if (k.size(1) < 1) value_error("a cache needs a head, got " + shape_of(k));
     if (k.size(2) < 1 || k.size(2) % 16 != 0) value_error("pages must have a multiple of 16 rows, got " + std::to_string(k.size(2)));
     int64_t steps[6];
@@ -1279,7 +1280,8 @@ struct Batch {
 };
 
 // [N, heads, D] with dense features, steps that are multiples of 8 and a 16-byte boundary: the tensor itself or a copy
-Tensor packed_tokens(const Tensor& t, int64_t (&steps)[2]) {
+Tensor packed_tokens(const Tensor& given, int64_t (&steps)[2]) {
+    const Tensor t = given.resolve_neg();
     bool ok = t.stride(2) == 1 && aligned16(t);
     for (int i = 0; i < 2; ++i) {
         steps[i] = t.size(i) > 1 ? t.stride(i) : 0;

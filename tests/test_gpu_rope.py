@@ -115,6 +115,23 @@ def test_any_strides(dtype):
     assert ((gx.cpu().double() - turned.double().sum(2, keepdim=True)).abs() <= 4 * HALF_STEP[dtype] * turned.double().abs().sum(2, keepdim=True)).all()
 
 
+def test_values_that_another_tensor_holds_negated():
+    """The imaginary part of a conjugated tensor is a view whose memory has the other sign."""
+    o = _d()
+    cis = o.rope_table(6, 16, device=DEV)
+    z = torch.complex(_randn((2, 6, 3, 32), 1, FF), _randn((2, 6, 3, 32), 2, FF))
+    x = z.conj().imag
+    assert x.is_neg()
+    _same(o.rope(x, cis), o.rope(-z.imag, cis))
+    q = _randn((3, 4, 64), 3, BF)
+    cache = o.paged_kv_cache(2, 2, 16, 64, BF, DEV)
+    with pytest.raises(ValueError, match="negated"):
+        o.attention_paged_cache(q, o.PagedKVCache(torch._neg_view(cache.k), cache.v), torch.zeros((3, 1), dtype=torch.int32, device=DEV), torch.tensor([1], device=DEV))
+    cache.k.copy_(_randn(cache.k.shape, 4, BF)), cache.v.copy_(_randn(cache.v.shape, 5, BF))
+    args = cache, torch.zeros((3, 1), dtype=torch.int32, device=DEV), torch.tensor([9], device=DEV)
+    _same(o.attention_paged_cache(torch._neg_view(q), *args), o.attention_paged_cache(-q, *args))
+
+
 def test_tables_of_both_forms_and_any_place():
     o = _d()
     cis = o.rope_table(12, 64, device=DEV)
