@@ -77,8 +77,9 @@ __global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kReside
     const Sequences& s = a.seq;
     QueryTile qt;
     if (a.by_length) {
-        // Behind the kernel for many queries, which waits for what came before it when it begins: this one reads and writes nothing of that kernel's,
-        // takes the SMs that it leaves, and waits for it at its end.
+        // Behind the kernel for many queries, which waits for what came before it when it begins: this one reads and writes nothing of that kernel's and
+        // takes the SMs that it leaves.  Its first CTA waits for that kernel before it ends, so that whoever waits for this one has waited for both;
+        // the others leave their places to the next.
         const int first = s.first_token(tile), n = max(s.first_token(tile + 1) - first, 0);
         qt = {tile, n, first, 0, (int64_t)n * a.G <= kCols ? n * a.G : 0};
     } else {
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kReside
         qt = find_tile(s, tile, a.G, kCols, a.per_sequence);
     }
     if (qt.rows == 0) {                                                          // the whole cluster's tile
-        if (a.by_length) wait_predecessor();
+        if (a.by_length && blockIdx.x == 0) wait_predecessor();
         return;
     }
     auto token_of = [&](int r) { return (int)a.group.div((unsigned)(qt.row0 + r)); };
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kReside
             const float total = cta_l[col], inv = total == 0.0f ? 0.0f : 1.0f / total;
             store(col, d, sums[col * D + d] * inv, sums[col * D + d + 1] * inv);
         }
-        if (a.by_length) wait_predecessor();
+        if (a.by_length && blockIdx.x == 0) wait_predecessor();
         return;
     }
     if (a.shares > kClusterShares) {
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kReside
         store(col, d, x, y);
     }
     cluster.sync();                                       // the others read this CTA's sums
-    if (a.by_length) wait_predecessor();
+    if (a.by_length && blockIdx.x == 0) wait_predecessor();
 }
 
 // Joins the shares of one query: a CTA of four times D threads, a quarter of the shares each.
