@@ -14,6 +14,9 @@
 // a cluster divide the rows (each reads the lengths and takes its share of what there really is) and are joined over distributed shared
 // memory; more than eight shares go through a workspace and a second kernel.  Every sum has a fixed order.
 //
+// One sequence of 131072 rows, 32 heads on 8: 89 us, 92 % of a copy's bandwidth; 32 sequences of 1 to 8192 rows: 103 us, 82 %, because a CTA's first rows
+// come 2 to 3 us after the last ones of the CTA whose place it takes; 600 rows alone: 7.8 us, latency.
+//
 // Rows that a sequence does not have, or that come before its start, are not read: they are zeros in shared memory, so that whatever is in the
 // cache there, infinities and NaN among it, has no part in the products.  Those of rows that only some of the queries see take a way of their own
 // (paged_attention.cuh).
@@ -545,6 +548,8 @@ int64_t few_shares(int64_t ctas, int64_t D, int64_t max_len, int64_t most) {
     return best < most ? best : most;
 }
 Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len, bool packed) {
+    // One tile of few queries reads the cache as fast as it comes; a second one reads it again, and a CTA of the other kernel is no slower for up to 256.  (32
+    // sequences of 4096 rows, 8 heads, few and many: 16 queries of each 112 and 127 us, 20: 160 and 127, 32: 156 and 127.)
     const int64_t G = Hq / Hkv;
     Plan p{};
     p.many = packed ? N > B && N * G > kCols * B : N / B * G > kCols;

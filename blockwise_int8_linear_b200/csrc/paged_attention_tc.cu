@@ -15,6 +15,12 @@
 // multiply-add: all weights are relative to the same power of two, whatever it is.  Only where scores are so large (2^20) that its rounding is
 // a power of two of its own the differences of scores are taken first; the scores' own rounding is no smaller then.
 //
+// What bounds it: the chain of a tile, scores read (545 cycles a step with their maximum), weights (1460 alone, 1900 beside the other tile's: the exponentials'
+// unit has 1024 for each), the rest of the product and the next scores (1080), 3540 cycles in all of which the tensor cores work 2048; and the power cap, since
+// without any exponentials a call takes 7 % less.  2048 tokens behind 30720 rows, 32 heads on 8 of 128 features: 880 us alone, 990 in a loop (1.07 PFLOP/s, 76 % of
+// cuBLAS's sustained rate).  Tried without gain: a part of the exponentials as polynomials on the multiply-add pipe, two threads a query, steps of 64 rows
+// with two places for the scores of heads of 64.
+//
 // Weights are 16-bit numbers: a rounding of half a step each, at random, which leaves the result about as much error again as its own rounding.
 // (A second product with what they lose would cost half of the time again.)
 //
@@ -160,346 +166,350 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
     auto order_k = [&](int j) { return j < Z::kAhead ? j : order_v(j - Z::kAhead) + 1; };
 
     if (warp >= MMA_WARP) {
-    if constexpr (TILES == 2) setmaxnreg_dec<kOtherRegisters>();
-    if (warp == LOAD_WARP) {
-        // ---- copies: a box of box_rows rows and 64 features at a time, a lane for every box_rows rows of the step
-        const int boxes = KT / box_rows;
-        const int* const table = s.pages + (qt.b < s.B ? qt.b : 0) * s.pages_step;
-        bool ok = true;
-        int order = 0;
-        auto fetch = [&](const CUtensorMap& map, int j) {
-            const int stage = order % Z::kStages, parity = (order / Z::kStages) & 1;
-            const int row = first + j * KT + lane * box_rows;
-            const bool mine = lane < boxes && row < last;
-            const int in_table = mine ? (int)s.page.div((unsigned)row) : 0;
-            const int page = mine ? table[in_table] : 0;
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kEmpty + stage), (uint32_t)parity ^ 1u, abort_flag, wait_limit));
-            if (!ok) {
-                if (lane == 0) report_timeout(status, abort_flag, W_EMPTY_AB);
-                return;
-            }
-            const int copied = __popc(__ballot_sync(0xffffffffu, mine));
-            if (lane == 0) mbar_expect_tx(bar(Z::kFull + stage), (uint32_t)(copied * box_rows * D * 2));
-            __syncwarp();
-            if (mine) {
-#pragma unroll
-                for (int c = 0; c < CHUNKS; ++c)
-                    tma_load_4d(stage_at(stage) + (uint32_t)((c * KT + lane * box_rows) * 128), &map, bar(Z::kFull + stage), 64 * c, row - in_table * (int)s.page.d, h, page);
-            }
-            __syncwarp();
-            ++order;
-        };
-        for (int j = 0; j < min(Z::kAhead, steps) && ok; ++j) fetch(k_map, j);
-        for (int j = 0; j < steps && ok; ++j) {
-            fetch(v_map, j);
-            if (ok && j + Z::kAhead < steps) fetch(k_map, j + Z::kAhead);
-        }
-        // after an abort: the copies that are still on their way
-        if (!ok)
-            for (int i = max(0, order - Z::kStages); i < order; ++i) (void)mbar_wait(bar(Z::kFull + i % Z::kStages), (uint32_t)(i / Z::kStages) & 1u, zero_word, wait_limit);
-    } else if (warp == MMA_WARP) {
-        // ---- products, issued by one thread
-        if (elect_one()) {
-            constexpr uint32_t S_DESC = umma_idesc_16bit(kTileRows, KT, BF16, false), O_DESC = umma_idesc_16bit(kTileRows, D, BF16, true);
+        if constexpr (TILES == 2) setmaxnreg_dec<kOtherRegisters>();
+        if (warp == LOAD_WARP) {
+            // ---- copies: a box of box_rows rows and 64 features at a time, a lane for every box_rows rows of the step
+            const int boxes = KT / box_rows;
+            const int* const table = s.pages + (qt.b < s.B ? qt.b : 0) * s.pages_step;
             bool ok = true;
-            auto wait = [&](int b, int parity, int code) {
-                if (!ok) return;
-                ok = mbar_wait(bar(b), (uint32_t)parity, abort_flag, wait_limit);
-                if (!ok) report_timeout(status, abort_flag, code);
-            };
-            auto wait_stage = [&](int order) { wait(Z::kFull + order % Z::kStages, (order / Z::kStages) & 1, W_FULL_AB); };
-            auto scores = [&](int t, int buf, int order) {
-                const uint32_t q = base + (uint32_t)(t * Z::kQTile), k = stage_at(order % Z::kStages);
+            int order = 0;
+            auto fetch = [&](const CUtensorMap& map, int j) {
+                const int stage = order % Z::kStages, parity = (order / Z::kStages) & 1;
+                const int row = first + j * KT + lane * box_rows;
+                const bool mine = lane < boxes && row < last;
+                const int in_table = mine ? (int)s.page.div((unsigned)row) : 0;
+                const int page = mine ? table[in_table] : 0;
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kEmpty + stage), (uint32_t)parity ^ 1u, abort_flag, wait_limit));
+                if (!ok) {
+                    if (lane == 0) report_timeout(status, abort_flag, W_EMPTY_AB);
+                    return;
+                }
+                const int copied = __popc(__ballot_sync(0xffffffffu, mine));
+                if (lane == 0) mbar_expect_tx(bar(Z::kFull + stage), (uint32_t)(copied * box_rows * D * 2));
+                __syncwarp();
+                if (mine) {
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    mma_f16(tmem + (uint32_t)(Z::kScores + buf * KT), umma_desc_k_sw128(q + (uint32_t)((i / 4) * kTileRows * 128 + (i % 4) * 32)),
-                            umma_desc_k_sw128(k + (uint32_t)((i / 4) * KT * 128 + (i % 4) * 32)), S_DESC, i > 0);
-                tc_commit(bar(Z::kScoresFull + buf));
+                    for (int c = 0; c < CHUNKS; ++c)
+                        tma_load_4d(stage_at(stage) + (uint32_t)((c * KT + lane * box_rows) * 128), &map, bar(Z::kFull + stage), 64 * c, row - in_table * (int)s.page.d, h, page);
+                }
+                __syncwarp();
+                ++order;
             };
-            for (int t = 0; t < tiles; ++t) wait(Z::kQueries + t, 0, W_FULL_AB);
-            for (int j = 0; j < min(Z::kAhead, steps) && ok; ++j) {
-                wait_stage(order_k(j));
-                if (!ok) break;
-                tc_fence_after();
-                for (int t = 0; t < tiles; ++t) scores(t, TILES == 2 ? t : j & 1, order_k(j));
-                tc_commit(bar(Z::kEmpty + order_k(j) % Z::kStages));
-            }
+            for (int j = 0; j < min(Z::kAhead, steps) && ok; ++j) fetch(k_map, j);
             for (int j = 0; j < steps && ok; ++j) {
-                const int ov = order_v(j), ahead = j + Z::kAhead, ok_order = order_k(ahead);
-                wait_stage(ov);
-                // in every step, so that the warps that look after v are never a round of stages behind
-                wait(Z::kClean + j % Z::kStages, (j / Z::kStages) & 1, W_FULL_AB);
-                for (int t = 0; t < tiles && ok; ++t) {
-                    const int buf = TILES == 2 ? t : j & 1;
-                    const uint32_t v = stage_at(ov % Z::kStages);
+                fetch(v_map, j);
+                if (ok && j + Z::kAhead < steps) fetch(k_map, j + Z::kAhead);
+            }
+            // after an abort: the copies that are still on their way
+            if (!ok)
+                for (int i = max(0, order - Z::kStages); i < order; ++i) (void)mbar_wait(bar(Z::kFull + i % Z::kStages), (uint32_t)(i / Z::kStages) & 1u, zero_word, wait_limit);
+        } else if (warp == MMA_WARP) {
+            // ---- products, issued by one thread
+            if (elect_one()) {
+                constexpr uint32_t S_DESC = umma_idesc_16bit(kTileRows, KT, BF16, false), O_DESC = umma_idesc_16bit(kTileRows, D, BF16, true);
+                bool ok = true;
+                auto wait = [&](int b, int parity, int code) {
+                    if (!ok) return;
+                    ok = mbar_wait(bar(b), (uint32_t)parity, abort_flag, wait_limit);
+                    if (!ok) report_timeout(status, abort_flag, code);
+                };
+                auto wait_stage = [&](int order) { wait(Z::kFull + order % Z::kStages, (order / Z::kStages) & 1, W_FULL_AB); };
+                auto scores = [&](int t, int buf, int order) {
+                    const uint32_t q = base + (uint32_t)(t * Z::kQTile), k = stage_at(order % Z::kStages);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        wait(Z::kWeightsFull + 2 * half + buf, TILES == 2 ? j & 1 : (j >> 1) & 1, W_ACC_FULL);
+                    for (int i = 0; i < D / 16; ++i)
+                        mma_f16(tmem + (uint32_t)(Z::kScores + buf * KT), umma_desc_k_sw128(q + (uint32_t)((i / 4) * kTileRows * 128 + (i % 4) * 32)),
+                                umma_desc_k_sw128(k + (uint32_t)((i / 4) * KT * 128 + (i % 4) * 32)), S_DESC, i > 0);
+                    tc_commit(bar(Z::kScoresFull + buf));
+                };
+                for (int t = 0; t < tiles; ++t) wait(Z::kQueries + t, 0, W_FULL_AB);
+                for (int j = 0; j < min(Z::kAhead, steps) && ok; ++j) {
+                    wait_stage(order_k(j));
+                    if (!ok) break;
+                    tc_fence_after();
+                    for (int t = 0; t < tiles; ++t) scores(t, TILES == 2 ? t : j & 1, order_k(j));
+                    tc_commit(bar(Z::kEmpty + order_k(j) % Z::kStages));
+                }
+                for (int j = 0; j < steps && ok; ++j) {
+                    const int ov = order_v(j), ahead = j + Z::kAhead, ok_order = order_k(ahead);
+                    wait_stage(ov);
+                    // in every step, so that the warps that look after v are never behind
+                    wait(Z::kClean + j % Z::kStages, (j / Z::kStages) & 1, W_FULL_AB);
+                    for (int t = 0; t < tiles && ok; ++t) {
+                        const int buf = TILES == 2 ? t : j & 1;
+                        const uint32_t v = stage_at(ov % Z::kStages);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            wait(Z::kWeightsFull + 2 * half + buf, TILES == 2 ? j & 1 : (j >> 1) & 1, W_ACC_FULL);
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int i = half * (KT / 32); i < (half + 1) * (KT / 32); ++i)
+                                mma_f16_ta(tmem + (uint32_t)(Z::kOut + t * D), tmem + (uint32_t)(Z::kScores + buf * KT + 8 * i), umma_desc_mn_sw128(v + (uint32_t)(2048 * i), KT * 128),
+                                           O_DESC, j > 0 || i > 0);
+                        }
                         if (!ok) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int i = half * (KT / 32); i < (half + 1) * (KT / 32); ++i)
-                            mma_f16_ta(tmem + (uint32_t)(Z::kOut + t * D), tmem + (uint32_t)(Z::kScores + buf * KT + 8 * i), umma_desc_mn_sw128(v + (uint32_t)(2048 * i), KT * 128),
-                                       O_DESC, j > 0 || i > 0);
+                        tc_commit(bar(Z::kProductDone + t));
+                        if (ahead < steps) {
+                            if (t == 0) wait_stage(ok_order);
+                            if (ok) scores(t, buf, ok_order);
+                        }
                     }
                     if (!ok) break;
-                    tc_commit(bar(Z::kProductDone + t));
-                    if (ahead < steps) {
-                        if (t == 0) wait_stage(ok_order);
-                        if (ok) scores(t, buf, ok_order);
-                    }
+                    tc_commit(bar(Z::kEmpty + ov % Z::kStages));
+                    if (ahead < steps) tc_commit(bar(Z::kEmpty + ok_order % Z::kStages));
                 }
-                if (!ok) break;
-                tc_commit(bar(Z::kEmpty + ov % Z::kStages));
-                if (ahead < steps) tc_commit(bar(Z::kEmpty + ok_order % Z::kStages));
-            }
-            if (!ok) {                                        // products that are still under way
-                tc_commit(bar(Z::kEnd));
-                (void)mbar_wait(bar(Z::kEnd), 0u, zero_word, wait_limit);
-            }
-        }
-        __syncwarp();
-    } else {
-        // ---- v's rows that nobody sees become zeros, and those that only some of the queries see are looked through
-        const int me = threadIdx.x - 32 * (LOAD_WARP + 1), row0 = me >> 3;
-        bool ok = true;
-        for (int j = 0; j < steps && ok; ++j) {
-            const int order = order_v(j), stage = order % Z::kStages, at = first + j * KT;
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kFull + stage), (uint32_t)(order / Z::kStages) & 1u, abort_flag, wait_limit));
-            if (!ok) {
-                if (lane == 0) report_timeout(status, abort_flag, W_FULL_AB);
-                break;
-            }
-            if (at < start || at + KT > min(last, fewest)) {
-                uint8_t* const v = smem + Z::kStagesAt + stage * Z::kStage;
-                constexpr int LOOKS = 8 * KT / 64;
-                uint32_t largest = 0u;
-#pragma unroll
-                for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll 8
-                    for (int i = 0; i < LOOKS; ++i) {
-                        uint4* const piece = reinterpret_cast<uint4*>(v + c * KT * 128 + (me + 64 * i) * 16);
-                        const int row = at + row0 + 8 * i;
-                        if (row < start || row >= last) *piece = make_uint4(0u, 0u, 0u, 0u);
-                        else if (row >= fewest) largest = max(largest, absmax8(*piece));
-                    }
-                if (__any_sync(0xffffffffu, largest >= F16Bits<T>::kInf)) {
-                    for (int i = me; i < CHUNKS * 8 * KT; i += 64) {
-                        uint4* const piece = reinterpret_cast<uint4*>(v + i * 16);
-                        const int row = at + (i >> 3) % KT;
-                        if (row < fewest || absmax8(*piece) < F16Bits<T>::kInf) continue;
-                        atomicOr(reinterpret_cast<unsigned*>(smem + Z::kNoted) + ((row - fewest) >> 5), 1u << ((row - fewest) & 31));
-                        unsigned short* const value = reinterpret_cast<unsigned short*>(piece);
-                        for (int e = 0; e < 8; ++e)
-                            if ((value[e] & 0x7fffu) >= F16Bits<T>::kInf) value[e] = 0;
-                    }
+                if (!ok) {                                        // products that are still under way
+                    tc_commit(bar(Z::kEnd));
+                    (void)mbar_wait(bar(Z::kEnd), 0u, zero_word, wait_limit);
                 }
-                fence_proxy_async_smem();
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(Z::kClean + j % Z::kStages));      // v may be in any place, so these go by steps
+        } else {
+            // ---- v's rows that nobody sees become zeros, and those that only some of the queries see are looked through
+            const int me = threadIdx.x - 32 * (LOAD_WARP + 1), row0 = me >> 3;
+            bool ok = true;
+            for (int j = 0; j < steps && ok; ++j) {
+                const int order = order_v(j), stage = order % Z::kStages, at = first + j * KT;
+                // First the step's scores: they show that whatever the stage held before has come and gone (a wait for a barrier's phase is none while an
+                // older one is under way, and copies may overtake one another).
+                const int buf = TILES == 2 ? 0 : j & 1;
+                ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kScoresFull + buf), (uint32_t)(TILES == 2 ? j & 1 : (j >> 1) & 1), abort_flag, wait_limit) &&
+                                                 mbar_wait(bar(Z::kFull + stage), (uint32_t)(order / Z::kStages) & 1u, abort_flag, wait_limit));
+                if (!ok) {
+                    if (lane == 0) report_timeout(status, abort_flag, W_FULL_AB);
+                    break;
+                }
+                if (at < start || at + KT > min(last, fewest)) {
+                    uint8_t* const v = smem + Z::kStagesAt + stage * Z::kStage;
+                    constexpr int LOOKS = 8 * KT / 64;
+                    uint32_t largest = 0u;
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll 8
+                        for (int i = 0; i < LOOKS; ++i) {
+                            uint4* const piece = reinterpret_cast<uint4*>(v + c * KT * 128 + (me + 64 * i) * 16);
+                            const int row = at + row0 + 8 * i;
+                            if (row < start || row >= last) *piece = make_uint4(0u, 0u, 0u, 0u);
+                            else if (row >= fewest) largest = max(largest, absmax8(*piece));
+                        }
+                    if (__any_sync(0xffffffffu, largest >= F16Bits<T>::kInf)) {
+                        for (int i = me; i < CHUNKS * 8 * KT; i += 64) {
+                            uint4* const piece = reinterpret_cast<uint4*>(v + i * 16);
+                            const int row = at + (i >> 3) % KT;
+                            if (row < fewest || absmax8(*piece) < F16Bits<T>::kInf) continue;
+                            atomicOr(reinterpret_cast<unsigned*>(smem + Z::kNoted) + ((row - fewest) >> 5), 1u << ((row - fewest) & 31));
+                            unsigned short* const value = reinterpret_cast<unsigned short*>(piece);
+                            for (int e = 0; e < 8; ++e)
+                                if ((value[e] & 0x7fffu) >= F16Bits<T>::kInf) value[e] = 0;
+                        }
+                    }
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(Z::kClean + j % Z::kStages));      // v may be in any place, so these go by steps
+            }
         }
-    }
     } else {
         if constexpr (TILES == 2) setmaxnreg_inc<kSoftmaxRegisters>();
         if (warp / 4 < tiles) {
-        // ---- softmax: a thread is a query
-        const int t = warp / 4, r = t * kTileRows + (threadIdx.x & 127);
-        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), out = lanes + (uint32_t)(Z::kOut + t * D);
-        {
-            auto store_query = [&](int row, const uint4& v) {
-                *reinterpret_cast<uint4*>(smem + t * Z::kQTile + (q_piece / 8) * kTileRows * 128 + row * 128 + (((q_piece % 8) ^ (row & 7)) << 4)) =
-                    make_uint4((v.x & a.q_keep) ^ a.q_flip, (v.y & a.q_keep) ^ a.q_flip, (v.z & a.q_keep) ^ a.q_flip, (v.w & a.q_keep) ^ a.q_flip);
-            };
+            // ---- softmax: a thread is a query
+            const int t = warp / 4, r = t * kTileRows + (threadIdx.x & 127);
+            const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21), out = lanes + (uint32_t)(Z::kOut + t * D);
+            {
+                auto store_query = [&](int row, const uint4& v) {
+                    *reinterpret_cast<uint4*>(smem + t * Z::kQTile + (q_piece / 8) * kTileRows * 128 + row * 128 + (((q_piece % 8) ^ (row & 7)) << 4)) =
+                        make_uint4((v.x & a.q_keep) ^ a.q_flip, (v.y & a.q_keep) ^ a.q_flip, (v.z & a.q_keep) ^ a.q_flip, (v.w & a.q_keep) ^ a.q_flip);
+                };
 #pragma unroll
-            for (int i = 0; i < Q_LOADS; ++i) store_query(q_row + i * Q_ROWS, query[i]);
-            if constexpr (PIECES > Q_LOADS) {
+                for (int i = 0; i < Q_LOADS; ++i) store_query(q_row + i * Q_ROWS, query[i]);
+                if constexpr (PIECES > Q_LOADS) {
 #pragma unroll
-                for (int i = 0; i < Q_LOADS; ++i) query[i] = load_query(q_row + (Q_LOADS + i) * Q_ROWS);
+                    for (int i = 0; i < Q_LOADS; ++i) query[i] = load_query(q_row + (Q_LOADS + i) * Q_ROWS);
 #pragma unroll
-                for (int i = 0; i < Q_LOADS; ++i) store_query(q_row + (Q_LOADS + i) * Q_ROWS, query[i]);
+                    for (int i = 0; i < Q_LOADS; ++i) store_query(q_row + (Q_LOADS + i) * Q_ROWS, query[i]);
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(bar(Z::kQueries + t));
             }
-            fence_proxy_async_smem();
-            mbar_arrive(bar(Z::kQueries + t));
-        }
-        const bool live = r < qt.rows;
-        const int limit = live ? min(last, rows_seen(s, qt.b, qt.n, token_of(r))) : last, unmasked = min(last, fewest);
-        const float c = a.scale_log2;
-        constexpr float kGrowth = 8.0f, kLift = BF16 ? 0.0f : 6.0f;      // fp16 weights: 2^-20 of the largest is still a normal number
-        float m = -INFINITY, shift = -INFINITY;                // the score that weights are relative to; c m - kLift as it is subtracted
-        float total = 0.0f;
-        bool ok = true;
-        for (int j = 0; j < steps; ++j) {
-            const int buf = TILES == 2 ? t : j & 1, at = first + j * KT;
-            const uint32_t scores = lanes + (uint32_t)(Z::kScores + buf * KT);
-            const bool masked = at < start || at + KT > unmasked;
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kScoresFull + buf), TILES == 2 ? j & 1 : (j >> 1) & 1, abort_flag, wait_limit));
-            if (!ok) {
-                if (lane == 0) report_timeout(status, abort_flag, W_ACC_FULL);
-                break;
-            }
-            tc_fence_after();
-            uint32_t x[KT];
-#pragma unroll
-            for (int i = 0; i < KT; i += 32) tmem_ld32(scores + (uint32_t)i, *reinterpret_cast<uint32_t(*)[32]>(x + i));
-            tmem_wait_ld();
-            if (masked) {
-#pragma unroll
-                for (int i = 0; i < KT; ++i)
-                    if (at + i >= limit || at + i < start) x[i] = 0xff800000u;
-            }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < KT; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
-            const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-            const bool need = (now - m) * c > kGrowth;         // a first score always is
-            // O is at rest when the product before is done.  With two tiles these scores came after it; with one it is waited for in every step, which also
-            // keeps the barrier's phases in sight: a wait for one phase may be one behind, not two.
-            if (TILES == 1 && j > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kProductDone), (uint32_t)(j - 1) & 1u, abort_flag, wait_limit));
+            const bool live = r < qt.rows;
+            const int limit = live ? min(last, rows_seen(s, qt.b, qt.n, token_of(r))) : last, unmasked = min(last, fewest);
+            const float c = a.scale_log2;
+            constexpr float kGrowth = 8.0f, kLift = BF16 ? 0.0f : 6.0f;      // fp16 weights: 2^-20 of the largest is still a normal number
+            float m = -INFINITY, shift = -INFINITY;                // the score that weights are relative to; c m - kLift as it is subtracted
+            float total = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < steps; ++j) {
+                const int buf = TILES == 2 ? t : j & 1, at = first + j * KT;
+                const uint32_t scores = lanes + (uint32_t)(Z::kScores + buf * KT);
+                const bool masked = at < start || at + KT > unmasked;
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kScoresFull + buf), TILES == 2 ? j & 1 : (j >> 1) & 1, abort_flag, wait_limit));
                 if (!ok) {
-                    if (lane == 0) report_timeout(status, abort_flag, W_ACC_EMPTY);
+                    if (lane == 0) report_timeout(status, abort_flag, W_ACC_FULL);
                     break;
                 }
                 tc_fence_after();
-            }
-            if (__any_sync(0xffffffffu, need)) {
-                float alpha = 1.0f;
-                if (need) {
-                    m = now;
-                    const float next = __fmaf_rn(m, c, -kLift);
-                    alpha = exp2_fast(shift - next);
-                    shift = next;
-                    total *= alpha;
+                uint32_t x[KT];
+#pragma unroll
+                for (int i = 0; i < KT; i += 32) tmem_ld32(scores + (uint32_t)i, *reinterpret_cast<uint32_t(*)[32]>(x + i));
+                tmem_wait_ld();
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < KT; ++i)
+                        if (at + i >= limit || at + i < start) x[i] = 0xff800000u;
                 }
-                if (j > 0) {
-                    const uint64_t both = pack_f32x2(alpha, alpha);
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int d = 0; d < D; d += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(out + (uint32_t)d, o);
-                        tmem_wait_ld();
+                for (int i = 0; i < KT; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i]));
+                const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+                const bool need = (now - m) * c > kGrowth;         // a first score always is
+                // O is at rest when the product before is done.  With two tiles these scores came after it; with one it is waited for in every step, which also
+                // keeps the barrier's phases in sight: a wait for one phase may be one behind, not two.
+                if (TILES == 1 && j > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kProductDone), (uint32_t)(j - 1) & 1u, abort_flag, wait_limit));
+                    if (!ok) {
+                        if (lane == 0) report_timeout(status, abort_flag, W_ACC_EMPTY);
+                        break;
+                    }
+                    tc_fence_after();
+                }
+                if (__any_sync(0xffffffffu, need)) {
+                    float alpha = 1.0f;
+                    if (need) {
+                        m = now;
+                        const float next = __fmaf_rn(m, c, -kLift);
+                        alpha = exp2_fast(shift - next);
+                        shift = next;
+                        total *= alpha;
+                    }
+                    if (j > 0) {
+                        const uint64_t both = pack_f32x2(alpha, alpha);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
+                        for (int d = 0; d < D; d += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(out + (uint32_t)d, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                float y, z;
+                                unpack_f32x2(mul_f32x2(pack_u32x2(o[i], o[i + 1]), both), y, z);
+                                o[i] = __float_as_uint(y), o[i + 1] = __float_as_uint(z);
+                            }
+                            tmem_st16(out + (uint32_t)d, o);
+                        }
+                    }
+                }
+                const float zero = m == -INFINITY ? 0.0f : m, ref = m == -INFINITY ? 0.0f : shift;
+                const uint64_t cc = pack_f32x2(c, c), less = pack_f32x2(-ref, -ref);
+                uint64_t sums[2] = {0ull, 0ull};
+                auto weights = [&](auto far) {
+#pragma unroll
+                    for (int i0 = 0; i0 < KT; i0 += KT / 4) {
+                        uint32_t p[KT / 8];
+#pragma unroll
+                        for (int i = 0; i < KT / 4; i += 2) {
                             float y, z;
-                            unpack_f32x2(mul_f32x2(pack_u32x2(o[i], o[i + 1]), both), y, z);
-                            o[i] = __float_as_uint(y), o[i + 1] = __float_as_uint(z);
+                            if (decltype(far)::value) {
+                                y = __fmaf_rn(__uint_as_float(x[i0 + i]) - zero, c, -kLift);
+                                z = __fmaf_rn(__uint_as_float(x[i0 + i + 1]) - zero, c, -kLift);
+                            } else {
+                                unpack_f32x2(fma_f32x2(pack_u32x2(x[i0 + i], x[i0 + i + 1]), cc, less), y, z);
+                            }
+                            y = exp2_fast(y);
+                            z = exp2_fast(z);
+                            sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(y, z));
+                            p[i / 2] = F16Bits<T>::pack(y, z);
                         }
-                        tmem_st16(out + (uint32_t)d, o);
+                        if (i0 == KT / 2) {
+                            tmem_wait_st();
+                            tc_fence_before();
+                            mbar_arrive(bar(Z::kWeightsFull + buf));
+                        }
+                        if constexpr (KT == 128) tmem_st16(scores + (uint32_t)(i0 / 2), p);
+                        else tmem_st8(scores + (uint32_t)(i0 / 2), p);
                     }
-                }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(bar(Z::kWeightsFull + 2 + buf));
+                };
+                if (__any_sync(0xffffffffu, fabsf(ref) >= 0x1p20f)) weights(std::true_type{});
+                else weights(std::false_type{});
+                float y, z;
+                unpack_f32x2(add_f32x2(sums[0], sums[1]), y, z);
+                total += y + z;
             }
-            const float zero = m == -INFINITY ? 0.0f : m, ref = m == -INFINITY ? 0.0f : shift;
-            const uint64_t cc = pack_f32x2(c, c), less = pack_f32x2(-ref, -ref);
-            uint64_t sums[2] = {0ull, 0ull};
-            auto weights = [&](auto far) {
-#pragma unroll
-                for (int i0 = 0; i0 < KT; i0 += KT / 4) {
-                    uint32_t p[KT / 8];
-#pragma unroll
-                    for (int i = 0; i < KT / 4; i += 2) {
-                        float y, z;
-                        if (decltype(far)::value) {
-                            y = __fmaf_rn(__uint_as_float(x[i0 + i]) - zero, c, -kLift);
-                            z = __fmaf_rn(__uint_as_float(x[i0 + i + 1]) - zero, c, -kLift);
-                        } else {
-                            unpack_f32x2(fma_f32x2(pack_u32x2(x[i0 + i], x[i0 + i + 1]), cc, less), y, z);
-                        }
-                        y = exp2_fast(y);
-                        z = exp2_fast(z);
-                        sums[(i >> 1) & 1] = add_f32x2(sums[(i >> 1) & 1], pack_f32x2(y, z));
-                        p[i / 2] = F16Bits<T>::pack(y, z);
-                    }
-                    if (i0 == KT / 2) {
-                        tmem_wait_st();
-                        tc_fence_before();
-                        mbar_arrive(bar(Z::kWeightsFull + buf));
-                    }
-                    if constexpr (KT == 128) tmem_st16(scores + (uint32_t)(i0 / 2), p);
-                    else tmem_st8(scores + (uint32_t)(i0 / 2), p);
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(bar(Z::kWeightsFull + 2 + buf));
-            };
-            if (__any_sync(0xffffffffu, fabsf(ref) >= 0x1p20f)) weights(std::true_type{});
-            else weights(std::false_type{});
-            float y, z;
-            unpack_f32x2(add_f32x2(sums[0], sums[1]), y, z);
-            total += y + z;
-        }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kProductDone + t), (uint32_t)(steps - 1) & 1u, abort_flag, wait_limit));
-        if (!ok) {
-            if (lane == 0) report_timeout(status, abort_flag, W_ACC_FULL);
-        } else {
-            // ---- results
-            tc_fence_after();
-            const bool whole = count == 1;
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            if (live && a.shares > 1)
-                a.part.stats[share * a.part.rows + query_at(r)] = whole ? make_float2(0.0f, kWritten) : make_float2(m == -INFINITY ? m : shift, total);
-            unsigned noted[8], any = 0u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) any |= noted[i] = lds_volatile_u32(base + Z::kNoted + 4 * i);
-            auto add_noted = [&](uint32_t (&o)[32], int d) {
-                const int* const table = s.pages + (qt.b < s.B ? qt.b : 0) * s.pages_step;
-                for (int i = 0; i < 8; ++i)
-                    for (unsigned w = noted[i]; w; w &= w - 1) {
-                        const int row = fewest + 32 * i + __ffs(w) - 1;
-                        if (!live || row >= limit || row < start) continue;
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + not_finite<T>(a, table, row, h, d + e));
-                    }
-            };
-            // by way of the queries' place, 256 bytes of a row at a time (128 with 64 features), so that rows are written whole
-            constexpr int PASS = D == 64 ? 128 : 256, LANES = PASS / 16, ROWS = 128 / LANES;
-            uint8_t* const place = smem + t * Z::kQTile;
-            const int mine = threadIdx.x & 127;
-            auto through = [&](auto fill, char* to, int64_t row_bytes, int passes) {
-                for (int pass = 0; pass < passes; ++pass) {
-                    fill(pass, place + mine * PASS);
-                    asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
-                    const int piece = mine % LANES;
-#pragma unroll 8
-                    for (int i = 0; i < 128 / ROWS; ++i) {
-                        const int row = mine / LANES + i * ROWS;
-                        if (t * kTileRows + row >= qt.rows) break;
-                        const uint4 v = *reinterpret_cast<const uint4*>(place + row * PASS + ((piece ^ (row & 7)) << 4));
-                        *reinterpret_cast<uint4*>(to + query_at(t * kTileRows + row) * row_bytes + pass * PASS + piece * 16) = v;
-                    }
-                    asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
-                }
-            };
-            if (whole) {
-                through([&](int pass, uint8_t* row) {
-#pragma unroll
-                    for (int d = 0; d < PASS / 2; d += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(out + (uint32_t)(pass * (PASS / 2) + d), o);
-                        tmem_wait_ld();
-                        if (any) add_noted(o, pass * (PASS / 2) + d);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = F16Bits<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-                            *reinterpret_cast<uint4*>(row + (((d / 8 + i) ^ (mine & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    }
-                }, static_cast<char*>(a.out), D * 2, D * 2 / PASS);
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kProductDone + t), (uint32_t)(steps - 1) & 1u, abort_flag, wait_limit));
+            if (!ok) {
+                if (lane == 0) report_timeout(status, abort_flag, W_ACC_FULL);
             } else {
-                through([&](int pass, uint8_t* row) {
+                // ---- results
+                tc_fence_after();
+                const bool whole = count == 1;
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+                if (live && a.shares > 1)
+                    a.part.stats[share * a.part.rows + query_at(r)] = whole ? make_float2(0.0f, kWritten) : make_float2(m == -INFINITY ? m : shift, total);
+                unsigned noted[8], any = 0u;
 #pragma unroll
-                    for (int d = 0; d < PASS / 4; d += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(out + (uint32_t)(pass * (PASS / 4) + d), o);
-                        tmem_wait_ld();
-                        if (any) add_noted(o, pass * (PASS / 4) + d);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(row + (((d / 4 + i) ^ (mine & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                for (int i = 0; i < 8; ++i) any |= noted[i] = lds_volatile_u32(base + Z::kNoted + 4 * i);
+                auto add_noted = [&](uint32_t (&o)[32], int d) {
+                    const int* const table = s.pages + (qt.b < s.B ? qt.b : 0) * s.pages_step;
+                    for (int i = 0; i < 8; ++i)
+                        for (unsigned w = noted[i]; w; w &= w - 1) {
+                            const int row = fewest + 32 * i + __ffs(w) - 1;
+                            if (!live || row >= limit || row < start) continue;
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + not_finite<T>(a, table, row, h, d + e));
+                        }
+                };
+                // by way of the queries' place, 256 bytes of a row at a time (128 with 64 features), so that rows are written whole
+                constexpr int PASS = D == 64 ? 128 : 256, LANES = PASS / 16, ROWS = 128 / LANES;
+                uint8_t* const place = smem + t * Z::kQTile;
+                const int mine = threadIdx.x & 127;
+                auto through = [&](auto fill, char* to, int64_t row_bytes, int passes) {
+                    for (int pass = 0; pass < passes; ++pass) {
+                        fill(pass, place + mine * PASS);
+                        asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
+                        const int piece = mine % LANES;
+#pragma unroll 8
+                        for (int i = 0; i < 128 / ROWS; ++i) {
+                            const int row = mine / LANES + i * ROWS;
+                            if (t * kTileRows + row >= qt.rows) break;
+                            const uint4 v = *reinterpret_cast<const uint4*>(place + row * PASS + ((piece ^ (row & 7)) << 4));
+                            *reinterpret_cast<uint4*>(to + query_at(t * kTileRows + row) * row_bytes + pass * PASS + piece * 16) = v;
+                        }
+                        asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
                     }
-                }, reinterpret_cast<char*>(a.part.sums + share * a.part.rows * D), D * 4, D * 4 / PASS);
+                };
+                if (whole) {
+                    through([&](int pass, uint8_t* row) {
+#pragma unroll
+                        for (int d = 0; d < PASS / 2; d += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(out + (uint32_t)(pass * (PASS / 2) + d), o);
+                            tmem_wait_ld();
+                            if (any) add_noted(o, pass * (PASS / 2) + d);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) w[e] = F16Bits<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+                                *reinterpret_cast<uint4*>(row + (((d / 8 + i) ^ (mine & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }, static_cast<char*>(a.out), D * 2, D * 2 / PASS);
+                } else {
+                    through([&](int pass, uint8_t* row) {
+#pragma unroll
+                        for (int d = 0; d < PASS / 4; d += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(out + (uint32_t)(pass * (PASS / 4) + d), o);
+                            tmem_wait_ld();
+                            if (any) add_noted(o, pass * (PASS / 4) + d);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(row + (((d / 4 + i) ^ (mine & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        }
+                    }, reinterpret_cast<char*>(a.part.sums + share * a.part.rows * D), D * 4, D * 4 / PASS);
+                }
             }
-        }
         }
     }
     tc_fence_before();

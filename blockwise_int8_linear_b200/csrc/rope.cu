@@ -1,8 +1,10 @@
 // Rotary positions of any tensor [B, T, H, D]: the first R features of every head are turned by the angles of the token's position
 // (rope.cuh), the others copied.  The gradient is the same operation with the angles' signs changed (`conj`): the rotation's transpose.
 //
-// Bound by memory: x read once, the result written once, the table's rows from the caches.  A thread has its two pieces in up to kHeads heads
-// of one token, so that a row of the table is read once for those, and as many loads are under way before the first is used.
+// Bound by memory: x read once, the result written once, the table's rows from the caches.  A thread has its two pieces in kHeads heads of one token, so
+// that a row of the table is read once for both, and all of its loads are under way before the first is used.  4 x 4096 tokens of 40 heads of
+// 128 bf16 features: 58 us in a loop, 87 % of a copy's bandwidth.  (Four blocks an SM want 64 registers a thread: with four heads it spilled, 74 us a call
+// alone against 61, and without that bound had too few loads under way, 68.)
 #include "rope.cuh"
 
 #include <type_traits>

@@ -276,6 +276,33 @@ def test_layouts_of_the_cache_and_strided_operands(layout):
     assert_clean_device()
 
 
+@pytest.mark.parametrize("d, heads, rows", [(128, 8, 4096), (64, 12, 4096), (256, 4, 2000)])
+def test_many_sequences_from_cold_memory(d, heads, rows):
+    """More CTAs than SMs, each with few queries of a long sequence, behind a fill of the caches: copies come late and in any order.  The reference
+    is every token by itself, which takes the other kernel, and sum p |v| comes from the same call on |v|.  Tolerance: half a step of each result, half a
+    step of each weight times sum p |v|, and 2^-12 of that for both calls' weights (Batch.check: at most 2^-20 (1 + sum |q k| scale), below 2^-14
+    for normal values of 256 features)."""
+    o = _d()
+    B, T, G, page = 32, 5, 4, 64
+    w = -(-rows // page)
+    cache = o.paged_kv_cache(B * w, heads, page, d, BF, DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for t in cache:
+        t.copy_(torch.randn(t.shape, device=DEV, generator=g))
+    pages = torch.randperm(B * w, generator=torch.Generator().manual_seed(2)).view(B, w).to(torch.int32).to(DEV)
+    fill = torch.empty(64 << 20, device=DEV, dtype=torch.int32)
+    for seed in (3, 4, 5):
+        q = torch.randn((B, T, heads * G, d), device=DEV, generator=g).to(BF)
+        n = torch.randint(rows - 300, rows + 1, (B,), generator=torch.Generator().manual_seed(seed)).to(DEV)
+        alone = lambda c: torch.stack([o.attention_paged_cache(q[:, t].contiguous(), c, pages, n - T + t + 1) for t in range(T)], 1)
+        want, spread = alone(cache), alone(o.PagedKVCache(cache.k, cache.v.abs())).double()
+        fill.zero_()
+        got = o.attention_paged_cache(q.view(B * T, heads * G, d), cache, pages, n).view_as(want)
+        u = HALF_STEP[BF]
+        assert ((got.double() - want.double()).abs() <= 2 * u * want.double().abs() + (u * (1 + 4 * u) + 2.0 ** -12) * spread).all()
+        assert_clean_device()
+
+
 def test_pages_far_apart():
     """A cache of more than 2^32 bytes a tensor whose last pages are in use."""
     o = _d()
