@@ -256,7 +256,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                         }
                     }
                     if (!ok) break;
-                    tc_commit(bar(Z::kEmpty + ov % Z::kStages));
+                    // not behind the last product, whose own barrier is the last that anyone waits for: nothing arrives in memory that the CTA has left
+                    if (j + 1 < steps) tc_commit(bar(Z::kEmpty + ov % Z::kStages));
                     if (ahead < steps) tc_commit(bar(Z::kEmpty + ok_order % Z::kStages));
                 }
                 if (!ok) {                                        // products that are still under way
