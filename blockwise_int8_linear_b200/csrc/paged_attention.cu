@@ -560,14 +560,20 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     p.few_shares = few_shares(p.both ? (B + 1) * Hkv : p.tiles * Hkv, D, max_len, p.both ? kClusterShares : kMaxShares);
     p.shares = p.few_shares;
     if (p.many) {
-        // A CTA an SM.  Rounds of CTAs that do not come out even cost little, since the SMs at work clock higher meanwhile; a share costs what it
-        // writes and the join reads.  (2048 tokens of 32 heads, D 128: 256 CTAs of 32768 rows 891 us in 1 share, 936 in 2, 946 in 4; 256 of 8192
-        // rows 227, 270, 287.  Heads of 256, 64 CTAs of 8192 rows: 149 us in 1, 90 in 2, 98 in 4.)  What may be tiles of few queries is not
-        // counted where those have a kernel of their own.
-        const int64_t ctas = (p.both ? N * G / p.rows + 1 : p.tiles) * Hkv, rows = max_len / kShareRows;
-        int64_t s = sm_count() / ctas;
-        if (s > rows) s = rows;
-        p.shares = s < 1 ? 1 : s > kMaxShares ? kMaxShares : s;
+        // A CTA an SM.  Rounds of CTAs that do not come out even cost little, since the SMs at work clock higher meanwhile, and so do not shares
+        // beyond one round pay.  (2048 tokens of 32 heads, D 128: 256 CTAs of 32768 rows 891 us in 1 share, 936 in 2, 946 in 4; 256 of 8192 rows 227,
+        // 270, 287.)  Within a round a share takes 14 ns a row, and more than one 3 us for the join and what they write and it reads at 6 bytes a
+        // ns.  (64 tokens behind 2000 rows, 32 heads on 8: 36 us in 1 share, 16 in 7; 512 tokens from the first on: 15 in 1, 20 in 2.)  What may be
+        // tiles of few queries is not counted where those have a kernel of their own.
+        const int64_t ctas = (p.both ? N * G / p.rows + 1 : p.tiles) * Hkv;
+        int64_t most = sm_count() / ctas, best = 0;
+        if (most > max_len / kShareRows) most = max_len / kShareRows;
+        if (most > kMaxShares) most = kMaxShares;
+        p.shares = 1;
+        for (int64_t s = 1; s <= most; ++s) {
+            const int64_t ns = 14 * max_len / s + (s > 1 ? 3000 + s * (N * Hq) * D * 8 / 6000 : 0);
+            if (s == 1 || ns < best) best = ns, p.shares = s;
+        }
     }
     return p;
 }

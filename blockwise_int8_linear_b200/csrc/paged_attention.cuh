@@ -33,8 +33,8 @@ __device__ __forceinline__ int rows_seen(const Sequences& s, int b, int n, int t
     return b < s.B ? (int)(r < 0 ? 0 : r > s.max_len ? s.max_len : r) : 0;
 }
 
-// The kernel for many queries gives a tile one share for as many rows of the cache.
-constexpr int kShareRows = 1024;
+// The kernel for many queries gives a tile one share for as many rows of the cache, two of its steps.
+constexpr int kShareRows = 256;
 int paged_many_tile(int64_t D);          // queries of one of its CTAs
 constexpr int kFewQueries = 16;
 // Rows of the newest tokens are seen by some queries of a tile and not by others, and in a matrix product a weight of 0 times an infinity is none.  So

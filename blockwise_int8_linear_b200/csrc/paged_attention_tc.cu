@@ -80,6 +80,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
 
     const int tile_head = (int)a.per_share.div(blockIdx.x), share = (int)blockIdx.x - tile_head * a.shares;
     const int turn = (int)a.heads.div((unsigned)tile_head), h = tile_head - turn * a.Hkv;
+    if (warp == LOAD_WARP && lane == 0) {
+        prefetch_map(&k_map);
+        prefetch_map(&v_map);
+    }
     after_predecessor();
     const Sequences& s = a.seq;
     // A sequence's last tiles see the most rows: they go first, so that short ones fill what is left at the end.
@@ -132,6 +136,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
         return;
     }
 
+    // the pages of the first step's rows, a lane of the loading warp for every box
+    const int* const table = s.pages + (qt.b < s.B ? qt.b : 0) * s.pages_step;
+    int first_page = 0;
+    if (warp == LOAD_WARP && lane < KT / box_rows && first + lane * box_rows < last) first_page = table[s.page.div((unsigned)(first + lane * box_rows))];
+
     // ---- set-up
     if (warp == MMA_WARP) {
         tmem_alloc(holder, Z::kColumns);
@@ -170,7 +179,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
         if (warp == LOAD_WARP) {
             // ---- copies: a box of box_rows rows and 64 features at a time, a lane for every box_rows rows of the step
             const int boxes = KT / box_rows;
-            const int* const table = s.pages + (qt.b < s.B ? qt.b : 0) * s.pages_step;
             bool ok = true;
             int order = 0;
             auto fetch = [&](const CUtensorMap& map, int j) {
@@ -178,7 +186,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                 const int row = first + j * KT + lane * box_rows;
                 const bool mine = lane < boxes && row < last;
                 const int in_table = mine ? (int)s.page.div((unsigned)row) : 0;
-                const int page = mine ? table[in_table] : 0;
+                const int page = j == 0 ? first_page : mine ? table[in_table] : 0;
                 ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kEmpty + stage), (uint32_t)parity ^ 1u, abort_flag, wait_limit));
                 if (!ok) {
                     if (lane == 0) report_timeout(status, abort_flag, W_EMPTY_AB);
@@ -453,7 +461,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) any |= noted[i] = lds_volatile_u32(base + Z::kNoted + 4 * i);
                 auto add_noted = [&](uint32_t (&o)[32], int d) {
-                    const int* const table = s.pages + (qt.b < s.B ? qt.b : 0) * s.pages_step;
                     for (int i = 0; i < 8; ++i)
                         for (unsigned w = noted[i]; w; w &= w - 1) {
                             const int row = fewest + 32 * i + __ffs(w) - 1;

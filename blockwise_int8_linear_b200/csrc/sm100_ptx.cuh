@@ -147,6 +147,7 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const void* tenso
         : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const void* tensor_map) { asm volatile("prefetch.tensormap [%0];" ::"l"(tensor_map) : "memory"); }
 __device__ __forceinline__ void tma_load_4d(uint32_t dst_smem, const void* tensor_map, uint32_t bar, int x, int y, int z, int w) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst_smem),
