@@ -17,7 +17,7 @@
 //
 // What bounds it: the chain of a tile, scores read (545 cycles a step with their maximum), weights (1460 alone, 1900 beside the other tile's: the exponentials'
 // unit has 1024 for each), the rest of the product and the next scores (1080), 3540 cycles in all of which the tensor cores work 2048; and the power cap, since
-// without any exponentials a call takes 7 % less.  2048 tokens behind 30720 rows, 32 heads on 8 of 128 features: 880 us alone, 990 in a loop (1.07 PFLOP/s, 76 % of
+// without any exponentials a call takes 7 % less.  2048 tokens, the last of 32768 rows, 32 heads on 8 of 128 features: 880 us alone, 990 in a loop (1.07 PFLOP/s, 76 % of
 // cuBLAS's sustained rate).  Tried without gain: a part of the exponentials as polynomials on the multiply-add pipe, two threads a query, steps of 64 rows
 // with two places for the scores of heads of 64.
 //
