@@ -27,11 +27,6 @@ struct Sequences {
         const long long v = cu[b];
         return (int)(v < 0 ? 0 : v > N ? N : v);
     }
-    __device__ __forceinline__ int length(int b) const {
-        if (b >= B) return 0;
-        const long long v = lengths[b * lengths_step];
-        return (int)(v < 0 ? 0 : v > max_len ? max_len : v);
-    }
     // position of a sequence's first new token; any number
     __device__ __forceinline__ long long first_position(int b, int n) const { return b < B ? lengths[b * lengths_step] - n : -n; }
     __device__ __forceinline__ int start(int b) const {
