@@ -448,9 +448,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                 total += y + z;
             }
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(Z::kProductDone + t), (uint32_t)(steps - 1) & 1u, abort_flag, wait_limit));
-            if (!ok) {
-                if (lane == 0) report_timeout(status, abort_flag, W_ACC_FULL);
-            } else {
+            if (!ok && lane == 0) report_timeout(status, abort_flag, W_ACC_FULL);
+            // The barriers between the parts of the results have no limit of their own.  So a tile's four warps, all of which get here because every wait before
+            // this one ends, go on to them together or not at all: one may have run out of time, or seen that others did, where the next had what it waited for.
+            if (role_barrier_all(t + 1, 128, ok)) {
                 // ---- results
                 tc_fence_after();
                 const bool whole = count == 1;
@@ -475,7 +476,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                 auto through = [&](auto fill, char* to, int64_t row_bytes, int passes) {
                     for (int pass = 0; pass < passes; ++pass) {
                         fill(pass, place + mine * PASS);
-                        asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
+                        role_barrier(t + 1, 128);
                         const int piece = mine % LANES;
 #pragma unroll 8
                         for (int i = 0; i < 128 / ROWS; ++i) {
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                             const uint4 v = *reinterpret_cast<const uint4*>(place + row * PASS + ((piece ^ (row & 7)) << 4));
                             *reinterpret_cast<uint4*>(to + query_at(t * kTileRows + row) * row_bytes + pass * PASS + piece * 16) = v;
                         }
-                        asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
+                        role_barrier(t + 1, 128);
                     }
                 };
                 if (whole) {

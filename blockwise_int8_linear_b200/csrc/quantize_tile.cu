@@ -154,20 +154,6 @@ struct PairQ {
     }
 };
 
-// Barrier among the `n` threads of one role (named barrier `id`) that also tells every one of them whether all of them
-// came with `ok` set: a wait that ran out in some thread ends the loop in all threads of the role, so that no thread is
-// left waiting at a barrier the others will never reach.
-__device__ __forceinline__ bool role_barrier_all(int id, int n, bool ok) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"(ok ? 1u : 0u), "r"(id), "r"(n)
-        : "memory");
-    return r != 0u;
-}
-__device__ __forceinline__ void role_barrier(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-
 // Persistent CTAs walk over the tiles; the input tile has two or three stages (full / empty mbarriers per stage, the
 // loads of the next tiles are in flight while the current one is quantized, and a stage is released as soon as every thread
 // has its part of it in registers).  256 threads do the column-wise work; in the dual kernel 256 more do the row-wise work on the

@@ -362,6 +362,20 @@ __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.
 template <int N>
 __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// Barrier among the `n` threads of one role (named barrier `id`) that also tells every one of them whether all of them
+// came with `ok` set: a wait that ran out in some thread ends the loop in all threads of the role, so that no thread is
+// left waiting at a barrier the others will never reach.
+__device__ __forceinline__ bool role_barrier_all(int id, int n, bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(ok ? 1u : 0u), "r"(id), "r"(n)
+        : "memory");
+    return r != 0u;
+}
+__device__ __forceinline__ void role_barrier(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
 // K-major operand tile in shared memory written by TMA with 128-byte swizzle: rows of 128 bytes, groups of
 // 8 rows 1024 bytes apart.  Descriptor fields: start address >> 4 (bits 0-13), leading byte offset (bits
 // 16-29, unused for swizzled K-major, set to 1), stride byte offset = 1024 >> 4 (bits 32-45), descriptor
