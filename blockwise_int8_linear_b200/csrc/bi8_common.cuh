@@ -76,7 +76,10 @@ struct SmemOptIn {
 // after the wait, which is for the whole preceding grid.  Two kernels release before their wait: the decode GEMM with early weights, which runs
 // only behind this library's own quantizer (that one releases after its wait and writes neither weights nor their scales), and the
 // reduction over peers behind such a GEMM, which reads nothing early but its own sequence number.  What follows either may start while two or three
-// kernels are incomplete, and waits first thing.  What all this saves is the launch latency and the kernel's set-up, 1-2 us per
+// kernels are incomplete, and waits first thing.  One kernel goes without a wait but for its first block's, before that ends: the paged attention of few
+// queries when it runs beside the one of many, which is always its predecessor.  All of that one's blocks wait before they release, so everything before it
+// has completed when the other begins; neither touches what the other writes; the first block's wait makes "has completed" mean both.  What completed grids
+// wrote is in the L2, but no wait has shown it to this kernel, so it reads by loads and copies that go there.  What all this saves is the launch latency and the kernel's set-up, 1-2 us per
 // kernel of a chain.
 template <typename... P, typename... A>
 int launch_chained_grid(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, A&&... args) {

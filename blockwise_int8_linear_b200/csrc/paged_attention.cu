@@ -82,8 +82,10 @@ __global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kReside
     if (a.by_length) {
         // Behind the kernel for many queries, which waits for what came before it when it begins: this one reads and writes nothing of that kernel's and
         // takes the SMs that it leaves.  Its first CTA waits for that kernel before it ends, so that whoever waits for this one has waited for both;
-        // the others leave their places to the next.
-        const int first = s.first_token(tile), n = max(s.first_token(tile + 1) - first, 0);
+        // the others leave their places to the next.  Without a wait of its own it reads what earlier kernels wrote from the L2 (bi8_common.cuh): numbers and
+        // queries by ld_l2, the cache by copies that pass by the SM's own.  (16 sequences of up to 4096 rows, one with 33 tokens: 101 us, 99 by ordinary loads.  A
+        // fence in each CTA: 106.)
+        const int first = s.first_token<true>(tile), n = max(s.first_token<true>(tile + 1) - first, 0);
         qt = {tile, n, first, 0, (int64_t)n * a.G <= kCols ? n * a.G : 0};
     } else {
         after_predecessor();
@@ -105,20 +107,21 @@ __global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kReside
         query[i] = make_uint4(0u, 0u, 0u, 0u);
         if (r < qt.rows) {
             const int t = token_of(r), head = h * a.G + (qt.row0 + r - t * a.G);
-            query[i] = ld_nc_v4(static_cast<const T*>(a.q) + (int64_t)(qt.token0 + t) * a.q_tok + head * a.q_head + 8 * q_piece);
+            query[i] = ld_l2(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(qt.token0 + t) * a.q_tok + head * a.q_head + 8 * q_piece));
         }
     }
 
     // ---- rows of this share
-    const int fewest = rows_seen(s, qt.b, qt.n, token_of(0)), most = rows_seen(s, qt.b, qt.n, token_of(qt.rows - 1));
-    const int start = s.start(qt.b), origin = start & ~15, n_rows = most > start ? most - origin : 0;
+    const long long position = s.first_position<true>(qt.b, qt.n);
+    const int fewest = rows_seen(s, position, token_of(0)), most = rows_seen(s, position, token_of(qt.rows - 1));
+    const int start = s.start<true>(qt.b), origin = start & ~15, n_rows = most > start ? most - origin : 0;
     const int chunk = (n_rows + a.shares * STEP - 1) / (a.shares * STEP) * STEP;
     const int first = origin + min(n_rows, share * chunk), last = min(origin + n_rows, first + chunk);
     int limit[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int r = g + 8 * i;
-        limit[i] = r < qt.rows ? min(last, rows_seen(s, qt.b, qt.n, token_of(r))) : last;      // a query that is none sees all: it is zero
+        limit[i] = r < qt.rows ? min(last, rows_seen(s, position, token_of(r))) : last;      // a query that is none sees all: it is zero
     }
     const int unmasked = min(last, fewest);
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};             // running maximum (in powers of two) and total of queries g and g + 8
@@ -136,10 +139,12 @@ __global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kReside
     struct Pages {
         int number[TT];
     };
+    // elsewhere from the SM's own cache, since consecutive numbers lie together (8 sequences of 4000 rows, D 256: 68 us, 71 from the L2)
+    auto page_number = [&](const int* p) { return a.by_length ? ld_l2(p) : __ldg(p); };
     auto pages_of = [&](int base) {
         Pages p;
 #pragma unroll
-        for (int i = 0; i < TT; ++i) p.number[i] = base + 16 * i < last ? pages[s.page.div((unsigned)(base + 16 * i))] : -1;
+        for (int i = 0; i < TT; ++i) p.number[i] = base + 16 * i < last ? page_number(pages + s.page.div((unsigned)(base + 16 * i))) : -1;
         return p;
     };
     auto fill = [&](uint32_t slot, int base, const Pages& p) {
@@ -345,9 +350,9 @@ __global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kReside
         }
         for (unsigned w = *noted; w; w &= w - 1) {
             const int row = fewest + __ffs(w) - 1;
-            if (row >= rows_seen(s, qt.b, qt.n, token_of(col)) || row < start) continue;
+            if (row >= rows_seen(s, position, token_of(col)) || row < start) continue;
             float* const e = reinterpret_cast<float*>(&x);
-            for (int k = 0; k < 4; ++k) e[k] += not_finite<T>(a, pages, row, h, d + k);
+            for (int k = 0; k < 4; ++k) e[k] += not_finite<T, true>(a, pages, row, h, d + k);
         }
         *reinterpret_cast<float4*>(sums + col * D + d) = x;
     }

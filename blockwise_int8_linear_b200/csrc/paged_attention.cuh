@@ -27,10 +27,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
-// The number of rows that query t of a sequence's n sees, counted from the cache's first.
-__device__ __forceinline__ int rows_seen(const Sequences& s, int b, int n, int t) {
-    const long long r = s.first_position(b, n) + t + 1;
-    return b < s.B ? (int)(r < 0 ? 0 : r > s.max_len ? s.max_len : r) : 0;
+// The number of rows that query t of a sequence sees, counted from the cache's first, by the position of the sequence's first new token.  (Tokens that belong to
+// nobody have positions below 0.)
+__device__ __forceinline__ int rows_seen(const Sequences& s, long long first_position, int t) {
+    const long long r = first_position + t + 1;
+    return (int)(r < 0 ? 0 : r > s.max_len ? s.max_len : r);
 }
 
 // The kernel for many queries gives a tile one share for as many rows of the cache, two of its steps.
@@ -40,13 +41,14 @@ constexpr int kFewQueries = 16;
 // Rows of the newest tokens are seen by some queries of a tile and not by others, and in a matrix product a weight of 0 times an infinity is none.  So
 // values that are not finite are taken out of those rows before the product (the row is noted, counted from the first that not all
 // queries see) and given to the queries that see them when the sums are done: what an infinite value times a positive weight adds is itself.
-template <typename T>
+template <typename T, bool L2>
 __device__ __forceinline__ float not_finite(const PagedAttnArgs& a, const int* pages, int row, int h, int d) {      // that value, 0 for a finite one
-    const int in_table = (int)a.seq.page.div((unsigned)row), page = pages[in_table];
+    const int in_table = (int)a.seq.page.div((unsigned)row), page = load<L2>(pages + in_table);
     if (page < 0 || page >= a.cache.pages) return 0.0f;
     const unsigned short* const v =
         static_cast<const unsigned short*>(a.cache.v) + page * a.cache.v_page + h * a.cache.v_head + (int64_t)(row - in_table * (int)a.seq.page.d) * a.cache.v_row;
-    return (v[d] & 0x7fffu) >= F16Bits<T>::kInf ? F16Bits<T>::one(v[d]) : 0.0f;
+    const unsigned short x = load<L2>(v + d);
+    return (x & 0x7fffu) >= F16Bits<T>::kInf ? F16Bits<T>::one(x) : 0.0f;
 }
 
 int launch_paged_few(const PagedAttnArgs& a, int dt, int64_t D, cudaStream_t st);

@@ -119,7 +119,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
     }
 
     // ---- rows of this share.  A tile takes as many shares as its rows fill.
-    const int fewest = rows_seen(s, qt.b, qt.n, token_of(0)), most = rows_seen(s, qt.b, qt.n, token_of(qt.rows - 1));
+    const long long position = s.first_position(qt.b, qt.n);
+    const int fewest = rows_seen(s, position, token_of(0)), most = rows_seen(s, position, token_of(qt.rows - 1));
     const int start = s.start(qt.b), origin = start & -box_rows, n_rows = most > start ? most - origin : 0;
     const int count = max(1, min(a.shares, n_rows / share_rows));
     const int chunk = (n_rows + count * KT - 1) / (count * KT) * KT;
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                 mbar_arrive(bar(Z::kQueries + t));
             }
             const bool live = r < qt.rows;
-            const int limit = live ? min(last, rows_seen(s, qt.b, qt.n, token_of(r))) : last, unmasked = min(last, fewest);
+            const int limit = live ? min(last, rows_seen(s, position, token_of(r))) : last, unmasked = min(last, fewest);
             const float c = a.scale_log2;
             constexpr float kGrowth = 8.0f, kLift = BF16 ? 0.0f : 6.0f;      // fp16 weights: 2^-20 of the largest is still a normal number
             float m = -INFINITY, shift = -INFINITY;                // the score that weights are relative to; c m - kLift as it is subtracted
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1)
                         for (unsigned w = noted[i]; w; w &= w - 1) {
                             const int row = fewest + 32 * i + __ffs(w) - 1;
                             if (!live || row >= limit || row < start) continue;
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + not_finite<T>(a, table, row, h, d + e));
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) + not_finite<T, false>(a, table, row, h, d + e));
                         }
                 };
                 // by way of the queries' place, 256 bytes of a row at a time (128 with 64 features), so that rows are written whole

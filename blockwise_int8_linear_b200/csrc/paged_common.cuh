@@ -9,6 +9,33 @@
 
 namespace bi8 {
 
+// Loads from the L2, past the SM's own cache: for a kernel that begins without a wait of its own (bi8_common.cuh).
+__device__ __forceinline__ long long ld_l2(const long long* p) {
+    long long v;
+    asm volatile("ld.relaxed.gpu.global.s64 %0, [%1];" : "=l"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ int ld_l2(const int* p) {
+    int v;
+    asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ unsigned short ld_l2(const unsigned short* p) {
+    unsigned short v;
+    asm volatile("ld.relaxed.gpu.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 ld_l2(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.relaxed.gpu.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+template <bool L2, typename V>
+__device__ __forceinline__ V load(const V* p) {
+    if constexpr (L2) return ld_l2(p);
+    else return *p;
+}
+
 struct Sequences {
     const long long* lengths;
     const long long* cu;         // B + 1 first tokens, or null: T tokens each
@@ -20,18 +47,21 @@ struct Sequences {
     FastDiv page, tokens;        // rows of a page; tokens of a sequence without cu
 
     // cu[0] is 0 whatever it says; tokens behind the last sequence's belong to sequence B, which has no rows
+    template <bool L2 = false>
     __device__ __forceinline__ int first_token(int b) const {
         if (b <= 0) return 0;
         if (b > B) return N;
         if (!cu) return b * T;
-        const long long v = cu[b];
+        const long long v = load<L2>(cu + b);
         return (int)(v < 0 ? 0 : v > N ? N : v);
     }
     // position of a sequence's first new token; any number
-    __device__ __forceinline__ long long first_position(int b, int n) const { return b < B ? lengths[b * lengths_step] - n : -n; }
+    template <bool L2 = false>
+    __device__ __forceinline__ long long first_position(int b, int n) const { return b < B ? load<L2>(lengths + b * lengths_step) - n : -n; }
+    template <bool L2 = false>
     __device__ __forceinline__ int start(int b) const {
         if (!starts || b >= B) return 0;
-        const long long v = starts[b * starts_step];
+        const long long v = load<L2>(starts + b * starts_step);
         return (int)(v < 0 ? 0 : v > max_len ? max_len : v);
     }
 };

@@ -25,3 +25,16 @@ def test_barriers_without_a_limit_stand_behind_a_vote():
     # nothing between the last bounded wait and the vote leaves, so that every warp comes to it
     assert not re.search(r"return|break|else", results[:vote.start()])
 
+
+
+def test_the_kernel_that_begins_without_a_wait_reads_from_the_l2():
+    """Beside the kernel for many queries the one for few has no wait that shows it what earlier kernels wrote, so no load of its own may find something older
+    in the SM's cache.  (The branch of a lone call and its search for the tile come behind a wait.)"""
+    text = re.sub(r"//[^\n]*", "", (CSRC / "paged_attention.cu").read_text())
+    kernel = text[text.index("paged_few_kernel(const PagedAttnArgs a)"):text.index("paged_join_kernel(")]
+    beside = kernel[kernel.index("if (a.by_length) {"):kernel.index("} else {")]
+    assert beside.count("first_token<true>(") == 2 and "wait" not in beside
+    rest = kernel[kernel.index("if (qt.rows == 0)"):]
+    assert not re.search(r"ld_nc|first_token\(|first_position\(|start\(|not_finite<T, false>", rest)
+    assert re.findall(r"a\.by_length \? ld_l2\(p\) : __ldg\(p\)", rest) and rest.count("__ldg") == 1
+    assert "cp.async.cg" in re.search(r"void copy16\(uint32_t dst, const void\* src, int bytes\).*?\n}", (CSRC / "int4_common.cuh").read_text(), re.S).group()
