@@ -670,7 +670,7 @@ int launch_attention_paged(const void* q, int dt, int64_t q_tok, int64_t q_head,
     a.Hq = (int)Hq;
     a.Hkv = (int)Hkv;
     a.G = (int)G;
-    a.scale_log2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 0x1p-126f);       // never 0, which the infinities of unseen rows do not bear
+    a.scale_log2 = std::fmax(std::fabs(scale) * 1.4426950408889634f, 0x1p-149f);       // never 0, which the infinities of unseen rows do not bear
     a.q_keep = scale == 0.0f ? 0u : 0xffffffffu;
     a.q_flip = scale < 0.0f ? 0x80008000u : 0u;
     a.group = FastDiv(G);
