@@ -14,8 +14,9 @@
 // a cluster divide the rows (each reads the lengths and takes its share of what there really is) and are joined over distributed shared
 // memory; more than eight shares go through a workspace and a second kernel.  Every sum has a fixed order.
 //
-// One sequence of 131072 rows, 32 heads on 8: 89 us, 92 % of a copy's bandwidth; 32 sequences of 1 to 8192 rows: 103 us, 82 %, because a CTA's first rows
-// come 2 to 3 us after the last ones of the CTA whose place it takes; 600 rows alone: 7.8 us, latency.
+// One sequence of 131072 rows, 32 heads on 8: 87 to 90 us, 91 to 94 % of a copy's bandwidth; 32 sequences of 1 to 8192 rows: 101 to 111 us from one GPU to another, 76
+// to 84 %, because a CTA's first rows come 2 to 3 us after the last ones of the CTA whose place it takes; 600 rows alone: 7.7 to 8.3 us, latency.  Heads of
+// 256, 32 on 8: 8 sequences of 4000 rows 61 us (40 by the bytes), 32 of them 261 to 276 (160): one CTA an SM.
 //
 // Rows that a sequence does not have, or that come before its start, are not read: they are zeros in shared memory, so that whatever is in the
 // cache there, infinities and NaN among it, has no part in the products.  Those of rows that only some of the queries see take a way of their own
@@ -480,7 +481,7 @@ __global__ void __launch_bounds__(4 * D) paged_join_kernel(const Partials p, int
     reinterpret_cast<unsigned short*>(out)[row * D + d] = (unsigned short)F16Bits<T>::pack((sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d]), 0.0f);
 }
 
-// The same for few shares and any number of queries: a warp each, whose lanes know a share's weight and have 4 or 8 features.
+// The same for few shares and any number of queries: a warp each, whose lanes know a share's weight and have 2, 4 or 8 features.
 constexpr int kFewShares = 16, kJoinWarps = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kJoinWarps) paged_join_few_kernel(const Partials p, int shares, T* out) {
@@ -537,6 +538,8 @@ struct Plan {
 // differ much in length, have shares of 2048 rows at most (32 sequences of 1 to 8192 rows: 174, 109, 107, 101, 100, 101), more than a cluster's eight a
 // second kernel.  Those are few sequences, one round of CTAs at most: two an SM, which come out even (131072 rows, 8 heads: 296 CTAs 88 to 90 us, 440 of
 // three an SM 93 to 104).
+// The table's room is all that the host knows of the lengths.  Sequences much shorter than that have shares of a few rows each (32 sequences of 600 rows on 8
+// heads: 20 us with tables of 600 rows, 22 of 4096, 43 of 32768 and more; 8 of 2000: 18, 29 of 131072).
 int64_t few_shares(int64_t ctas, int64_t D, int64_t max_len, int64_t most) {
     const int64_t step = kWarps * 16 * (D == 64 ? kSubSteps<64> : D == 128 ? kSubSteps<128> : kSubSteps<256>);
     const int64_t sms = sm_count(), set_up = 12800 / D;
@@ -558,6 +561,8 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     const int64_t G = Hq / Hkv;
     Plan p{};
     p.many = packed ? N > B && N * G > kCols * B : N / B * G > kCols;
+    // The host cannot tell tokens that belong to nobody from parts of prompts: they bring the other kernel's launch along (32 sequences of 600 rows 20 us, 28 with
+    // 7 such tokens) and bound the shares of few queries to a cluster's (one sequence of 131072 rows 90 us, 254 to 311).
     p.both = packed && N > B && G <= kCols;
     p.many = p.many || p.both;
     p.rows = p.many ? paged_many_tile(D) : kCols;
@@ -565,9 +570,8 @@ Plan plan_of(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t m
     p.few_shares = few_shares(p.both ? (B + 1) * Hkv : p.tiles * Hkv, D, max_len, p.both ? kClusterShares : kMaxShares);
     p.shares = p.few_shares;
     if (p.many) {
-        // A CTA an SM.  Rounds of CTAs that do not come out even cost little, since the SMs at work clock higher meanwhile, and so do not shares
-        // beyond one round pay.  (2048 tokens of 32 heads, D 128: 256 CTAs of 32768 rows 891 us in 1 share, 936 in 2, 946 in 4; 256 of 8192 rows 227,
-        // 270, 287.)  Within a round a share takes 14 ns a row, and more than one 3 us for the join and what they write and it reads at 6 bytes a
+        // A CTA an SM.  Shares beyond one round of CTAs do not pay for what they write and for the join, even where the rounds do not come out even.  (2048
+        // tokens of 32 heads, D 128: 256 CTAs of 32768 rows 891 us in 1 share, 936 in 2, 946 in 4; 256 of 8192 rows 227, 270, 287.)  Within a round a share takes 14 ns a row, and more than one 3 us for the join and what they write and it reads at 6 bytes a
         // ns.  (64 tokens behind 2000 rows, 32 heads on 8: 36 us in 1 share, 16 in 7; 512 tokens from the first on: 15 in 1, 20 in 2.)  What may be
         // tiles of few queries is not counted where those have a kernel of their own.
         const int64_t ctas = (p.both ? N * G / p.rows + 1 : p.tiles) * Hkv;

@@ -34,10 +34,11 @@ __device__ __forceinline__ int rows_seen(const Sequences& s, long long first_pos
     return (int)(r < 0 ? 0 : r > s.max_len ? s.max_len : r);
 }
 
-// The kernel for many queries gives a tile one share for as many rows of the cache, two of its steps.
+// The kernel for many queries gives a tile one share for as many rows of the cache: two of its steps, four with heads of 256 features.
 constexpr int kShareRows = 256;
 int paged_many_tile(int64_t D);          // queries of one of its CTAs
 constexpr int kFewQueries = 16;
+
 // Rows of the newest tokens are seen by some queries of a tile and not by others, and in a matrix product a weight of 0 times an infinity is none.  So
 // values that are not finite are taken out of those rows before the product (the row is noted, counted from the first that not all
 // queries see) and given to the queries that see them when the sums are done: what an infinite value times a positive weight adds is itself.

@@ -16,13 +16,16 @@
 // a power of two of its own the differences of scores are taken first; the scores' own rounding is no smaller then.
 //
 // What bounds it: the chain of a tile, scores read (545 cycles a step with their maximum), weights (1460 alone, 1900 beside the other tile's: the exponentials'
-// unit has 1024 for each), the rest of the product and the next scores (1080), 3540 cycles in all of which the tensor cores work 2048; and the power cap, since
-// without any exponentials a call takes 7 % less.  2048 tokens, the last of 32768 rows, 32 heads on 8 of 128 features: 880 us alone, 990 in a loop (1.07 PFLOP/s, 76 % of
-// cuBLAS's sustained rate).  Tried without gain: a part of the exponentials as polynomials on the multiply-add pipe, two threads a query, steps of 64 rows
+// unit has 1024 for each), the rest of the product and the next scores (1080), 3540 cycles in all of which the tensor cores work 2048 (without any
+// exponentials a call takes 7 % less); the power cap; and whole rounds of CTAs.  2048 tokens, the last of 32768 rows, 32 heads on 8 of 128 features, are 256 CTAs for
+// 148 SMs: 880 us alone, 990 to 1010 in a loop (1.06 PFLOP/s, 75 % of cuBLAS's sustained rate).  With heads of 64 a step is no shorter, although its products are half: 8 x 512
+// tokens over 2048 rows, 32 heads, 131 us, the exponentials' unit busy half of the time, the tensor cores a quarter.  Heads of 256, one tile a CTA: 2048 tokens, the
+// last of 16384 rows, 32 heads on 8, 1090 to 1170 us for 620 of products.  Tried without gain: a part of the exponentials as polynomials on the multiply-add pipe, two threads a query, steps of 64 rows
 // with two places for the scores of heads of 64.
 //
-// Weights are 16-bit numbers: a rounding of half a step each, at random, which leaves the result about as much error again as its own rounding.
-// (A second product with what they lose would cost half of the time again.)
+// Weights are 16-bit numbers: a rounding of half a step each, at random, which leaves the result about as much error again as its own rounding (against 64
+// bits 0.0023 in the 2-norm for bf16, 0.0017 by its rounding alone).  A second product with what they lose would cost half of the time again.  Their total is
+// summed before they are rounded, in fp32.
 //
 // What a query does not see must not count: scores are masked, and v's rows before the start and behind the last one are overwritten by zeros in
 // shared memory before the product, since 0 times an infinity is none.  Infinities and NaN of rows that only some queries see take a way of
@@ -57,10 +60,6 @@ struct Shape {
                          kQueries = kProductDone + 2, kClean = kQueries + 2, kEnd = kClean + kStages, kBarriers = kEnd + 1;
     static constexpr int kStagesAt = kTiles * kQTile, kBarriersAt = kStagesAt + kStages * kStage, kMisc = kBarriersAt + 8 * kBarriers;
     static constexpr int kNoted = kMisc + 16, kBytes = kNoted + 32 + 1024;     // tensor memory's address, abort flag, a word that stays zero; rows noted; alignment
-};
-
-struct Shares {
-    int first, last, count;      // this share's rows; how many shares there are
 };
 
 template <typename T, int D>

@@ -170,8 +170,16 @@ def attention_paged_cache(q: torch.Tensor, cache: PagedKVCache, pages: torch.Ten
 
     The query of a sequence's token i of n sees the rows up to ``lengths - n + i``, its own.  ``starts`` (as ``lengths``): the first row that is seen.  A
     query that sees no row gives zeros, as do tokens that belong to nobody; rows that it does not see may hold anything.  Infinite values that it sees
-    give nothing finite in their feature.  A page number that is none of the cache's reads as a page of zeros.  Keys of 2^100 and more may overflow in the
-    scores, which are fp32.  ``scale`` is a number of at most 2e38, by default ``1 / sqrt(D)``."""
+    give nothing finite in their feature.  A page number that is none of the cache's reads as a page of zeros.  Scores are fp32 and overflow where
+    ``q k^T`` does, before the scale.  ``scale`` is a number of at most 2e38, by default ``1 / sqrt(D)``.
+
+    Statistics and sums are fp32.  In a sequence with up to 16 queries on a cache head (new tokens times ``Hq / Hkv``) each weight enters the product with v as two
+    numbers of the cache's type, and the result is off by its own rounding; with more queries as one, which adds up to half a step of the type
+    times ``sum p |v|`` and on average 0.7 to 1 times that rounding again.
+
+    A call is planned from its tensors' sizes, since lengths are on the device.  For single tokens, tables much wider than the sequences and tokens that belong to
+    nobody cost time: 32 sequences of 600 rows on 8 heads take 20 us, with tables of 32768 rows 43, with 7 unused tokens 28; one of 131072 rows 90 us, with
+    unused tokens three times that."""
     if scale is None:
         scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     return _lib.native().attention_paged(q, cache.k, cache.v, pages, lengths, cu_tokens, starts, scale)

@@ -385,9 +385,11 @@ BI8_API int bi8_rope_cache_append_paged(const void* qkv, int dtype, int64_t qkv_
 /* out [N, Hq, D] contiguous = softmax(scale * q k^T) v for q [N, Hq, D], steps in elements (multiples of 8), 16-byte aligned.  The query of a sequence's
  * token i of n sees the rows from its start up to lengths - n + i (at most width * page_rows rows).  A query that sees no row gives zeros, as do tokens
  * that belong to nobody.  Rows that a query does not see may hold anything; pages whose number is none of the cache's read as
- * zeros.  Infinite values that it sees give nothing finite in their feature.  Keys of 2^100 and more may overflow in the scores, which are fp32.
- * Query head h reads cache head h / (Hq / heads).  scale: a number of at
- * most 2e38.  workspace: bi8_attention_paged_workspace_bytes bytes (`packed`: whether cu_tokens is given), 16-byte aligned, scratch of this call. */
+ * zeros.  Infinite values that it sees give nothing finite in their feature.  Scores are fp32 and overflow where q k^T does, before the scale.
+ * Weights enter the product with v as two numbers of dtype in sequences of up to 16 queries on a cache head (new tokens * Hq / heads), as one in those with
+ * more: up to half a step of dtype times sum p |v| besides the result's rounding.  Query head h reads cache head h / (Hq / heads).  scale: a number of at
+ * most 2e38.  A call is planned from max_len = width * page_rows, B and N: tables much wider than the sequences and tokens that belong to nobody cost single
+ * tokens time.  workspace: bi8_attention_paged_workspace_bytes bytes (`packed`: whether cu_tokens is given), 16-byte aligned, scratch of this call. */
 BI8_API size_t bi8_attention_paged_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t heads, int64_t D, int64_t max_len, int packed);
 BI8_API int bi8_attention_paged(const void* q, int dtype, int64_t q_tok, int64_t q_head, const bi8_paged_cache* cache, const bi8_sequences* seq, float scale,
                                 void* out, int64_t Hq, void* workspace, size_t workspace_bytes, void* stream);
