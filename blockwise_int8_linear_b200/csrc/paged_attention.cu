@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, kSlots == 3 ? kSingleRound : kReside
         int number[TT];
     };
     // elsewhere from the SM's own cache, since consecutive numbers lie together (8 sequences of 4000 rows, D 256: 68 us, 71 from the L2)
-    auto page_number = [&](const int* p) { return a.by_length ? ld_l2(p) : __ldg(p); };
+    auto page_number = [&](const int* p) { return a.by_length ? ld_l2(p) : *p; };
     auto pages_of = [&](int base) {
         Pages p;
 #pragma unroll
